@@ -63,6 +63,12 @@ SIGNATURES = {
     "dz_group_sumsq_static": (_i32, [_p, _p, _p, _i32, _i32, _p, _p, _p, _p]),
     "dz_project": (_i32, [_p, _p, _i32, _p, _p, _p, _p]),
     "dz_group_dot": (_i32, [_p, _p, _p, _p, _p]),
+    "dz_token_logprobs": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _p, _p, _p, _p,
+                                 _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p]),
+    "dz_topk_distill": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _i32, _f32, _i32, _p, _p, _i64, _i64,
+                               _p, _i64, _i64, _p]),
+    "dz_linear_token_logprobs_workspace": (_i32, [_i32, _i64, _i64, _i64, C.POINTER(_i64)]),
+    "dz_linear_token_logprobs": (_i32, [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p]),
 }
 
 _lock = threading.Lock()

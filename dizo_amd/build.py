@@ -12,8 +12,8 @@ import sys
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libdizo_amd.so")
-SOURCES = ["dz_kernels.hip", "dz_api.hip"]
-HEADERS = ["dz_common.h", "dz_kernels.h"]
+SOURCES = ["dz_kernels.hip", "dz_api.hip", "dz_token_loss.hip", "dz_token_head.hip", "dz_token_api.hip"]
+HEADERS = ["dz_common.h", "dz_internal.h", "dz_kernels.h", "dz_token_loss.h", "dz_token_math.h"]
 
 # -ffp-contract=off: products must not be contracted into FMAs (bit parity with
 # PyTorch's one-rounding-per-op recipe). -packed-fp32-ops: no v_pk_*_f32.

@@ -17,6 +17,7 @@
 
 #include "../../include/dizo_amd.h"
 #include "dz_common.h"
+#include "dz_internal.h"
 #include "dz_kernels.h"
 
 namespace {
@@ -185,6 +186,23 @@ int32_t check_range(uint64_t p, uint64_t bytes, const char* what, int32_t i) {
 }
 
 }  // namespace
+
+namespace dz {
+
+int32_t api_fail(int32_t code, const std::string& msg) { return fail(code, msg); }
+
+int32_t api_check_range(const void* p, uint64_t bytes, const char* what) {
+  hipDeviceptr_t base = nullptr;
+  size_t size = 0;
+  const hipError_t e = hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)(uintptr_t)p);
+  if (e != hipSuccess) return fail(DZ_ERR_RANGE, std::string(what) + " is not device memory: " + hipGetErrorString(e));
+  const uint64_t b = (uint64_t)(uintptr_t)base, q = (uint64_t)(uintptr_t)p;
+  if (q < b || bytes > (uint64_t)size || q - b > (uint64_t)size - bytes)
+    return fail(DZ_ERR_RANGE, std::string(what) + " range exceeds its allocation");
+  return DZ_OK;
+}
+
+}  // namespace dz
 
 // ---------------------------------------------------------------------------
 // Scratch of the allocation-free entry point (dz_group_sumsq_static): device

@@ -1,0 +1,307 @@
+"""What is read of a model's distributions over the vocabulary, on the HIP kernels.
+
+``token_logprobs``        log probabilities of given tokens, the rows' entropies and their largest
+                          alternatives, differentiable in the logits
+``topk_distill``          the distance to a teacher of which the largest logits were kept
+                          (``token_logprobs(..., top=k)`` records them), differentiable in the logits
+``linear_token_logprobs`` log probabilities and entropies straight from the last hidden states and
+                          the language-model head: the logits are never stored
+``token_logprobs_grad``, ``topk_distill_grad``   value and gradient in one call, for callers that
+                          know the rows' weights beforehand (the logits are then read once)
+
+They replace log_softmax, gather and mask of the option loss (trainer.py:1477-1500 and its copy
+:497-520). Leading dimensions are rows: logits (..., vocab) go with tokens (...). The vocabulary
+dimension has to be contiguous; rows may be strided (``logits[:, :-1]`` is read in place). Results are
+fp32: a row's sums are kept in fp32, and rounding them to a 16-bit type would leave a log probability
+of -10 with a step of 1/16 (bf16).
+
+Work goes to the current stream of the logits' device; tensors made on another stream are the
+caller's to order, as with torch's own operators.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+
+from . import _lib as L
+from ._lib import DzError
+from .table import _on, _ptr, dtype_code, stream_handle
+
+IGNORE_INDEX = -100  # the masked label of shift_option_labels
+MAX_TOP = 128
+MAX_TEACHER = 512
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row: the token's log probability, the entropy and, with top > 0, the largest log
+    probabilities with their tokens (else None)."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_tokens: Optional[torch.Tensor]
+
+
+def _fail(what: str, why: str):
+    raise DzError(f"{what}: {why}")
+
+
+def _check_logits(what: str, logits: torch.Tensor) -> int:
+    if not logits.is_cuda:
+        _fail(what, f"logits must live on a GPU, got {logits.device}")
+    code = dtype_code(logits.dtype)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        _fail(what, f"logits must be (..., vocab), got {tuple(logits.shape)}")
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        _fail(what, "the vocabulary dimension of the logits must be contiguous")
+    return code
+
+
+def _check_rows(what: str, name: str, t: torch.Tensor, lead, device, dtypes) -> None:
+    if t.device != device:
+        _fail(what, f"{name} must be on {device}, got {t.device}")
+    if t.dtype not in dtypes:
+        _fail(what, f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.shape != lead:
+        _fail(what, f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+
+
+_INT = (torch.int64, torch.int32)
+_F32 = (torch.float32,)
+
+
+def _two(lead) -> Tuple[int, int]:
+    """Leading dimensions as (batch, length)."""
+    n = len(lead)
+    if n == 2:
+        return lead[0], lead[1]
+    if n == 1:
+        return 1, lead[0]
+    total = 1
+    for d in lead:
+        total *= d
+    return 1, total
+
+
+def _strides(t: torch.Tensor, n: int) -> Tuple[int, int]:
+    """(batch, row) strides of a tensor of n leading dimensions, n <= 2."""
+    if n == 2:
+        return t.stride(0), t.stride(1)
+    return (0, t.stride(0)) if n == 1 else (0, 0)
+
+
+def _flat(t: Optional[torch.Tensor], n: int, inner: int):
+    """More than two leading dimensions as one (a view where the strides allow it, else a copy)."""
+    if t is None or n <= 2:
+        return t
+    return t.reshape(-1, *t.shape[n:]) if inner else t.reshape(-1)
+
+
+def _grad_like(logits: torch.Tensor) -> torch.Tensor:
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+def _score(logits, tokens, top, ignore_index, weights, entropy_weights, grad):
+    """One launch over checked operands. grad: a tensor to write, or None."""
+    lead = logits.shape[:-1]
+    n, (batch, length) = len(lead), _two(lead)
+    dev = logits.device
+    lp = torch.empty(lead, dtype=torch.float32, device=dev)
+    ent = torch.empty(lead, dtype=torch.float32, device=dev)
+    tlp = ttok = None
+    if top:
+        tlp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        ttok = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+    if batch * length:
+        x, t = _flat(logits, n, 1), _flat(tokens, n, 0)
+        w, u, g = _flat(weights, n, 0), _flat(entropy_weights, n, 0), _flat(grad, n, 1)
+        m = min(n, 2) if n <= 2 else 1
+        zero = (0, 0)
+        with _on(dev):
+            L.call("dz_token_logprobs", x.data_ptr(), dtype_code(x.dtype), batch, length, x.shape[-1],
+                   *_strides(x, m), t.data_ptr(), *_strides(t, m), ignore_index, top, lp.data_ptr(), ent.data_ptr(),
+                   _ptr(tlp), _ptr(ttok), _ptr(w), *(zero if w is None else _strides(w, m)), _ptr(u),
+                   *(zero if u is None else _strides(u, m)), _ptr(g), *(zero if g is None else _strides(g, m)),
+                   stream_handle())
+    return lp, ent, tlp, ttok
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, ignore_index):
+        lp, ent, tlp, ttok = _score(logits, tokens, top, ignore_index, None, None, None)
+        ctx.save_for_backward(logits, tokens)
+        ctx.ignore_index = ignore_index
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(tlp, ttok)
+        return lp, ent, tlp, ttok
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_lp, d_ent, _tlp, _ttok):
+        logits, tokens = ctx.saved_tensors
+        if d_lp is None and d_ent is None:
+            return None, None, None, None
+        grad = _grad_like(logits)
+        _score(logits, tokens, 0, ctx.ignore_index, d_lp, d_ent, grad)
+        return grad, None, None, None
+
+
+def _score_checked(what, logits, tokens, top, ignore_index):
+    _check_logits(what, logits)
+    _check_rows(what, "tokens", tokens, logits.shape[:-1], logits.device, _INT)
+    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
+        _fail(what, f"top must be 0 to {min(MAX_TOP, logits.shape[-1])}, got {top}")
+    return tokens if tokens.dtype == torch.int64 else tokens.long()
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
+                   ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
+    """log softmax(logits)[tokens] and the entropy of softmax(logits) for every row, with the `top`
+    largest log probabilities and their tokens, largest first and equal ones by token.
+
+    Rows whose token is ignore_index are not read: 0, 0, -inf and -1. Another token outside the
+    vocabulary gives NaN, and so does a row without a distribution (NaN, +inf, or nothing above -inf).
+    Gradients flow to the logits through logprobs and entropy; the alternatives are a report."""
+    tokens = _score_checked("token_logprobs", logits, tokens, top, ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top, ignore_index))
+    return TokenLogprobs(*_score(logits, tokens, top, ignore_index, None, None, None))
+
+
+def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, weights: Optional[torch.Tensor] = None,
+                        entropy_weights: Optional[torch.Tensor] = None, *,
+                        ignore_index: int = IGNORE_INDEX) -> Tuple[TokenLogprobs, torch.Tensor]:
+    """token_logprobs, and the gradient of sum(weights logprobs) + sum(entropy_weights entropy) with
+    respect to the logits, in their dtype. Weights are fp32, shaped like tokens; None stands for zeros."""
+    what = "token_logprobs_grad"
+    tokens = _score_checked(what, logits, tokens, 0, ignore_index)
+    if weights is None and entropy_weights is None:
+        _fail(what, "weights or entropy_weights are needed")
+    for name, w in (("weights", weights), ("entropy_weights", entropy_weights)):
+        if w is not None:
+            _check_rows(what, name, w, logits.shape[:-1], logits.device, _F32)
+    with torch.no_grad():
+        grad = _grad_like(logits)
+        out = _score(logits, tokens, 0, ignore_index, weights, entropy_weights, grad)
+    return TokenLogprobs(*out), grad
+
+
+def _distill(logits, values, tokens, temperature, normalize, weights, grad):
+    lead = logits.shape[:-1]
+    n, (batch, length) = len(lead), _two(lead)
+    loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    if batch * length:
+        x, w, g = _flat(logits, n, 1), _flat(weights, n, 0), _flat(grad, n, 1)
+        m = min(n, 2) if n <= 2 else 1
+        zero = (0, 0)
+        with _on(logits.device):
+            L.call("dz_topk_distill", x.data_ptr(), dtype_code(x.dtype), batch, length, x.shape[-1], *_strides(x, m),
+                   values.data_ptr(), tokens.data_ptr(), values.shape[-1], temperature, int(normalize),
+                   loss.data_ptr(), _ptr(w), *(zero if w is None else _strides(w, m)), _ptr(g),
+                   *(zero if g is None else _strides(g, m)), stream_handle())
+    return loss
+
+
+class _TopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, tokens, temperature, normalize):
+        ctx.save_for_backward(logits, values, tokens)
+        ctx.how = (temperature, normalize)
+        return _distill(logits, values, tokens, temperature, normalize, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss):
+        logits, values, tokens = ctx.saved_tensors
+        grad = _grad_like(logits)
+        _distill(logits, values, tokens, *ctx.how, d_loss, grad)
+        return grad, None, None, None, None
+
+
+def _distill_checked(what, logits, values, tokens, temperature):
+    _check_logits(what, logits)
+    lead, k = logits.shape[:-1], values.shape[-1] if values.dim() else 0
+    if not 1 <= k <= MAX_TEACHER:
+        _fail(what, f"a teacher has 1 to {MAX_TEACHER} entries a row, got {k}")
+    _check_rows(what, "values", values, (*lead, k), logits.device, (torch.float32, torch.float16, torch.bfloat16))
+    _check_rows(what, "tokens", tokens, (*lead, k), logits.device, _INT)
+    if not (0.0 < temperature < float("inf")):
+        _fail(what, f"temperature must be positive and finite, got {temperature}")
+    if values.requires_grad and torch.is_grad_enabled():
+        _fail(what, "the teacher's values take no gradient (detach them)")
+    return values.detach().float().contiguous(), tokens.long().contiguous()
+
+
+def topk_distill(logits: torch.Tensor, values: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0,
+                 normalize: bool = True) -> torch.Tensor:
+    """The distance of softmax(logits / T) to a teacher of which some entries were kept, per row:
+
+        T^2 sum_j w_j (log w_j - log softmax(logits / T)[tokens_j])
+
+    values, tokens: (..., k), the teacher's entries: logits, or log probabilities (both give the same
+    with normalize=True, where w = softmax(values / T) over the row's entries; with normalize=False
+    w = exp(values), log probabilities at temperature T, and the rest of the teacher's mass is left
+    out). A token of -1 is no entry; a row without entries is not read and gives 0. Entries of weight 0
+    (a value of -inf) add nothing; a token named twice counts twice. A token outside the vocabulary
+    and a value of NaN or +inf give NaN. Gradients flow to the logits."""
+    values, tokens = _distill_checked("topk_distill", logits, values, tokens, temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TopkDistill.apply(logits, values, tokens, temperature, normalize)
+    return _distill(logits, values, tokens, temperature, normalize, None, None)
+
+
+def topk_distill_grad(logits: torch.Tensor, values: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor, *,
+                      temperature: float = 1.0, normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """topk_distill, and the gradient of sum(weights loss) with respect to the logits, in their dtype.
+    weights: fp32, one per row."""
+    what = "topk_distill_grad"
+    values, tokens = _distill_checked(what, logits, values, tokens, temperature)
+    _check_rows(what, "weights", weights, logits.shape[:-1], logits.device, _F32)
+    with torch.no_grad():
+        grad = _grad_like(logits)
+        loss = _distill(logits, values, tokens, temperature, normalize, weights, grad)
+    return loss, grad
+
+
+def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *,
+                          ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
+    """token_logprobs of the logits hidden @ weight.T, which are not stored (and not rounded: products
+    and sums are fp32). hidden (..., width) and weight (vocab, width) of one dtype; the width has to be
+    contiguous. Ignored rows are not computed. Where autograd records (hidden or weight require a
+    gradient), the logits are made by F.linear and scored by token_logprobs instead."""
+    what = "linear_token_logprobs"
+    if not hidden.is_cuda:
+        _fail(what, f"hidden must live on a GPU, got {hidden.device}")
+    code = dtype_code(hidden.dtype)
+    if weight.device != hidden.device or weight.dtype != hidden.dtype:
+        _fail(what, f"weight is {weight.dtype} on {weight.device}, hidden {hidden.dtype} on {hidden.device}")
+    if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or not weight.numel():
+        _fail(what, f"hidden (..., width) and weight (vocab, width) do not fit: {tuple(hidden.shape)}, {tuple(weight.shape)}")
+    _check_rows(what, "tokens", tokens, hidden.shape[:-1], hidden.device, _INT)
+    vocab, width = weight.shape
+    if weight.stride(1) != 1 and width > 1:
+        _fail(what, "the width of the weight must be contiguous")
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return token_logprobs(F.linear(hidden, weight), tokens, ignore_index=ignore_index)
+    lead = tokens.shape
+    h = hidden.reshape(-1, width)
+    if h.stride(1) != 1 and width > 1:
+        h = h.contiguous()
+    t = tokens.reshape(-1).long().contiguous()
+    lp = torch.empty(lead, dtype=torch.float32, device=hidden.device)
+    ent = torch.empty(lead, dtype=torch.float32, device=hidden.device)
+    rows = h.shape[0]
+    if rows:
+        need = C.c_int64()
+        L.call("dz_linear_token_logprobs_workspace", code, rows, width, vocab, C.byref(need))
+        work = torch.empty(need.value, dtype=torch.uint8, device=hidden.device)
+        with _on(hidden.device):
+            L.call("dz_linear_token_logprobs", h.data_ptr(), weight.data_ptr(), code, rows, width, vocab, h.stride(0),
+                   weight.stride(0), t.data_ptr(), ignore_index, lp.data_ptr(), ent.data_ptr(), work.data_ptr(),
+                   need.value, stream_handle())
+    return TokenLogprobs(lp, ent, None, None)

@@ -223,6 +223,58 @@ int32_t dz_project(dz_table* t, const void* d_alpha, int32_t mode, double* d_sum
 int32_t dz_group_dot(dz_table* t, const uint64_t* other_ptrs, double* d_dot, float* d_dot_f32,
                      void* stream);
 
+/* ---- distributions over the vocabulary ----------------------------------- */
+/* Rows of logits: `batch` x `length` rows of `vocab` contiguous elements of
+ * `dtype`, by element strides (sequence, position); at most 4,194,303 rows and
+ * 2^30 tokens. Row r is position r % length of sequence r / length; outputs
+ * without strides are dense over rows. Logits of -inf take no part in a row's
+ * distribution. A row of NaN, +inf or nothing above -inf has none: its results
+ * are NaN (its alternatives -1). Everything is computed in fp32 and rounded
+ * once. Calls allocate nothing and may be captured. They replace log_softmax,
+ * gather and the mask of the option loss (trainer.py:1477-1500). */
+
+/* logprobs[r] = log softmax(logits_r)[tokens_r], entropy[r] = the entropy of
+ * softmax(logits_r), and the `top` (0 to 128) largest entries of log
+ * softmax(logits_r) with their tokens, largest first and equal ones by token.
+ * A row whose token is ignore_index is not read: 0, 0, -inf and -1. Another
+ * token outside the vocabulary gives NaN.
+ * With grad (top = 0 then): grad_r = the gradient of
+ * weights_r logprobs_r + entropy_weights_r entropy_r with respect to logits_r
+ * (either weights may be NULL: zeros), in `dtype`. */
+int32_t dz_token_logprobs(const void* logits, int32_t dtype, int64_t batch, int64_t length, int64_t vocab,
+                          int64_t logits_bs, int64_t logits_ls, const int64_t* tokens, int64_t tokens_bs,
+                          int64_t tokens_ls, int64_t ignore_index, int32_t top, float* logprobs, float* entropy,
+                          float* top_logprobs, int64_t* top_tokens, const float* weights, int64_t weights_bs,
+                          int64_t weights_ls, const float* entropy_weights, int64_t entropy_weights_bs,
+                          int64_t entropy_weights_ls, void* grad, int64_t grad_bs, int64_t grad_ls, void* stream);
+
+/* The distance of softmax(logits_r / T) to a teacher of which k (1 to 512)
+ * entries are known: loss[r] = T^2 sum_j w_j (log w_j - log softmax(logits_r /
+ * T)[i_j]) over the entries i_j = teacher_tokens[r, j] (-1: no entry), with w
+ * = softmax(teacher_values[r] / T) over the row's entries (normalize != 0) or w
+ * = exp(teacher_values[r]) (normalize = 0: log probabilities at temperature T;
+ * the rest of the teacher's mass is left out). Entries of weight 0 add nothing.
+ * A row without entries is not read: 0. A token outside the vocabulary, or a
+ * teacher value of NaN or +inf, gives NaN. With grad: grad_r = weights_r times the
+ * gradient of loss[r] with respect to logits_r, in `dtype`. */
+int32_t dz_topk_distill(const void* logits, int32_t dtype, int64_t batch, int64_t length, int64_t vocab,
+                        int64_t logits_bs, int64_t logits_ls, const float* teacher_values,
+                        const int64_t* teacher_tokens, int32_t k, float temperature, int32_t normalize, float* loss,
+                        const float* weights, int64_t weights_bs, int64_t weights_ls, void* grad, int64_t grad_bs,
+                        int64_t grad_ls, void* stream);
+
+/* dz_token_logprobs' logprobs and entropy of the logits hidden weight^T, which
+ * are not stored: hidden (rows, width) and weight (vocab, width) of `dtype`,
+ * rows hidden_stride and weight_stride elements apart, products and sums in
+ * fp32. Ignored rows are not computed. `workspace` is device memory (16-byte
+ * aligned) of at least the bytes that the first call reports; calls that overlap in
+ * time need one each. */
+int32_t dz_linear_token_logprobs_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, int64_t* bytes);
+int32_t dz_linear_token_logprobs(const void* hidden, const void* weight, int32_t dtype, int64_t rows, int64_t width,
+                                 int64_t vocab, int64_t hidden_stride, int64_t weight_stride, const int64_t* tokens,
+                                 int64_t ignore_index, float* logprobs, float* entropy, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
