@@ -7,10 +7,6 @@
 namespace dz {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
 // 16 bytes of a row's width per lane: lane l holds row l & 15, bytes
 // 16 (l >> 4) .. + 15 of a 64-byte slab. The products of one slab: 16 head
 // rows by 16 tokens; lane l then holds token l & 15, head rows 4 (l >> 4) .. + 3.
@@ -18,17 +14,17 @@ template <class T>
 struct Frag;
 template <>
 struct Frag<TypeF16> {
-  using V = f16x8;
+  using V = TypeF16::V;
   __device__ static f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<TypeBF16> {
-  using V = bf16x8;
+  using V = TypeBF16::V;
   __device__ static f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<TypeF32> {
-  using V = f32x4;
+  using V = TypeF32::V;
   // the slab's 16 columns in the order (0, 4, 8, 12), (1, 5, ...), the same on both sides
   __device__ static f32x4 mma(V a, V b, f32x4 c) {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
@@ -84,7 +80,7 @@ __global__ __launch_bounds__(1024) void live_rows_kernel(HeadRows a, Work w) {
 template <class T>
 __device__ typename Frag<T>::V load16(const typename T::Elem* row, uint32_t col, uint32_t width, bool vec) {
   if (vec && col + T::kPer16 <= width) return *(const typename Frag<T>::V*)(row + col);
-  typename Frag<T>::V v;
+  typename T::V v;
   for (int j = 0; j < T::kPer16; ++j) v[j] = col + j < width ? row[col + j] : (typename T::Elem)0.f;
   return v;
 }

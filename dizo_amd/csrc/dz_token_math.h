@@ -11,23 +11,26 @@ namespace dz {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// An element type, and 16 bytes of it.
 struct TypeF32 {
   using Elem = float;
-  static constexpr int kPer16 = 4;  // elements of 16 bytes
-  __device__ static float load(const Elem* p) { return *p; }
-  __device__ static void store(Elem* p, float v) { *p = v; }
+  using V = f32x4;
+  static constexpr int kPer16 = 4;
 };
 struct TypeF16 {
   using Elem = _Float16;
+  using V = f16x8;
   static constexpr int kPer16 = 8;
-  __device__ static float load(const Elem* p) { return (float)*p; }
-  __device__ static void store(Elem* p, float v) { *p = (_Float16)v; }
 };
 struct TypeBF16 {
   using Elem = __bf16;
+  using V = bf16x8;
   static constexpr int kPer16 = 8;
-  __device__ static float load(const Elem* p) { return (float)*p; }
-  __device__ static void store(Elem* p, float v) { *p = (__bf16)v; }
 };
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -49,11 +52,12 @@ struct SoftStats {
   __device__ float lnq(float x, float inv) const { return __builtin_fmaf(-kLn2, log2_hw(s), (x - m) * inv); }
 
   // 2^y y is 0 where y is -inf; a NaN logit leaves a NaN in s
+  template <bool ENTROPY = true>
   __device__ void add(float x, float c) {
     const float y = y_of(x, c);
     const float e = exp2_hw(y);
     s += e;
-    t = __builtin_fmaf(e, fmaxf(y, -1e30f), t);
+    if (ENTROPY) t = __builtin_fmaf(e, fmaxf(y, -1e30f), t);
   }
 
   // The same statistics against another maximum, m2 >= m.
