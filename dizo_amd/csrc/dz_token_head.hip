@@ -15,16 +15,19 @@ struct Frag;
 template <>
 struct Frag<TypeF16> {
   using V = TypeF16::V;
+  typedef TypeF16::V Loose __attribute__((aligned(2)));  // at any element
   __device__ static f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<TypeBF16> {
   using V = TypeBF16::V;
+  typedef TypeBF16::V Loose __attribute__((aligned(2)));  // at any element
   __device__ static f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<TypeF32> {
   using V = TypeF32::V;
+  typedef TypeF32::V Loose __attribute__((aligned(4)));  // at any element
   // the slab's 16 columns in the order (0, 4, 8, 12), (1, 5, ...), the same on both sides
   __device__ static f32x4 mma(V a, V b, f32x4 c) {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
@@ -39,10 +42,10 @@ struct Work {
   float* token_logit;  // per live row
   float4* partial;     // (live row, head tile)
 };
-constexpr uint32_t kTile = 64;  // head rows of a workgroup
+constexpr uint32_t kStreamTile = 128;  // head rows of a workgroup of the kernel for few rows
 
 __host__ __device__ inline uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
-inline uint32_t head_tiles(uint32_t vocab) { return (vocab + kTile - 1) / kTile; }
+inline uint32_t head_tiles(uint32_t vocab, uint32_t tile) { return (vocab + tile - 1) / tile; }
 inline Work work_of(void* p, uint32_t nrows) {
   const uint64_t n = align256((uint64_t)nrows * 4);
   char* c = (char*)p;
@@ -76,40 +79,44 @@ __global__ __launch_bounds__(1024) void live_rows_kernel(HeadRows a, Work w) {
   if (tid == 0) *w.count = base;
 }
 
-// 16 bytes from column `col` of a row; columns past the width are 0.
+// 16 bytes from column `col` of a row; columns past the width are 0. Rows start at any element.
 template <class T>
-__device__ typename Frag<T>::V load16(const typename T::Elem* row, uint32_t col, uint32_t width, bool vec) {
-  if (vec && col + T::kPer16 <= width) return *(const typename Frag<T>::V*)(row + col);
+__device__ __forceinline__ typename T::V load16(const typename T::Elem* row, uint32_t col, uint32_t width) {
+  if (col + T::kPer16 <= width) return *(const typename Frag<T>::Loose*)(row + col);
   typename T::V v;
   for (int j = 0; j < T::kPer16; ++j) v[j] = col + j < width ? row[col + j] : (typename T::Elem)0.f;
   return v;
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void head_kernel(HeadRows a, Work w, uint32_t tiles, bool vec) {
-  __shared__ SoftStats sh[4][16];
-  const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, count = *w.count;
-  const uint32_t at = blockIdx.y * 16 + (lane & 15);
-  if (blockIdx.y * 16 >= count) return;
-  const uint32_t row = w.row_of[at < count ? at : count - 1];
-  const uint32_t v0 = blockIdx.x * kTile + wv * 16;
-  const uint32_t vr = v0 + (lane & 15) < a.vocab ? v0 + (lane & 15) : a.vocab - 1;
-  const typename T::Elem* h = (const typename T::Elem*)a.hidden + (int64_t)row * a.hidden_stride;
-  const typename T::Elem* e = (const typename T::Elem*)a.weight + (int64_t)vr * a.weight_stride;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t lane_col = (lane >> 4) * T::kPer16;
-  for (uint32_t k = 0; k < a.width; k += 4 * T::kPer16)  // the same trips for the whole wave
-    acc = Frag<T>::mma(load16<T>(e, k + lane_col, a.width, vec), load16<T>(h, k + lane_col, a.width, vec), acc);
-  const int64_t tok = a.tokens[row];
-  SoftStats st = SoftStats::of(-INFINITY);
-  for (int j = 0; j < 4; ++j)
-    if (v0 + 4 * (lane >> 4) + j < a.vocab) st.m = fmaxf(st.m, acc[j]);
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t v = v0 + 4 * (lane >> 4) + j;
-    if (v >= a.vocab) continue;
-    st.add(acc[j], kLog2e);
-    if ((int64_t)v == tok && at < count) w.token_logit[at] = acc[j];
+// A token's logits over a lane's head rows (4 of each of VF slabs of 16) to their statistics: over the
+// four lanes that hold the token's. v0: the first head row of the wave. Leaves the token's own logit.
+template <int VF>
+__device__ __forceinline__ SoftStats lane_stats(f32x4 (&acc)[VF], uint32_t v0, uint32_t vocab, int64_t tok, bool live, float* token_logit) {
+  const uint32_t lane = threadIdx.x & 63, first = v0 + 4 * (lane >> 4);
+  if (v0 + 16 * VF > vocab) {  // head rows past the last one take no part
+#pragma unroll
+    for (int i = 0; i < VF; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (first + 16 * i + j >= vocab) acc[i][j] = -INFINITY;
   }
+  const uint64_t rel = (uint64_t)(tok - (int64_t)first);
+  if (__any(live && rel < 16 * VF)) {
+#pragma unroll
+    for (int i = 0; i < VF; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (rel == (uint64_t)(16 * i + j) && live && first + 16 * i + j < vocab) *token_logit = acc[i][j];
+  }
+  SoftStats st = SoftStats::of(-INFINITY);
+#pragma unroll
+  for (int i = 0; i < VF; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.m = fmaxf(st.m, acc[i][j]);
+#pragma unroll
+  for (int i = 0; i < VF; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.add(acc[i][j], kLog2e);
   for (int off = 16; off <= 32; off *= 2) {
     SoftStats o;
     o.m = __shfl_xor(st.m, off, 64);
@@ -117,23 +124,220 @@ __global__ __launch_bounds__(256) void head_kernel(HeadRows a, Work w, uint32_t 
     o.t = __shfl_xor(st.t, off, 64);
     st.join(o, kLog2e);
   }
-  if (lane < 16) sh[wv][lane] = st;
+  return st;
+}
+
+// Few rows: bound by reading the head once. A wave takes 32 head rows and all tokens of the
+// tile (16 TF) and keeps D slabs of 64 bytes a row on their way, head and hidden states alike,
+// straight to its registers: waves never wait for each other, and 1,571 of them (50,272 tokens)
+// have 8 KB each in flight. The hidden states come from the caches every time.
+template <class T, int TF, int D>
+__global__ __launch_bounds__(256) void head_stream_kernel(HeadRows a, Work w, uint32_t tiles) {
+  constexpr int VF = kStreamTile / 64;
+  constexpr uint32_t E = T::kPer16, K = 4 * E;
+  using V = typename T::V;
+  using Loose = typename Frag<T>::Loose;
+  __shared__ SoftStats sh[4][16 * TF];
+  const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = (lane >> 4) * E;
+  const uint32_t v0 = blockIdx.x * kStreamTile + wv * 16 * VF, r0 = blockIdx.y * 16 * TF;
+  const typename T::Elem* e[VF];
+  const typename T::Elem* h[TF];
+#pragma unroll
+  for (int i = 0; i < VF; ++i) {
+    const uint32_t v = v0 + 16 * i + (lane & 15);
+    e[i] = (const typename T::Elem*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride + col;
+  }
+#pragma unroll
+  for (int i = 0; i < TF; ++i) {
+    const uint32_t r = r0 + 16 * i + (lane & 15);
+    h[i] = (const typename T::Elem*)a.hidden + (int64_t)(r < a.nrows ? r : a.nrows - 1) * a.hidden_stride + col;
+  }
+  f32x4 acc[TF][VF];
+#pragma unroll
+  for (int i = 0; i < TF; ++i)
+#pragma unroll
+    for (int j = 0; j < VF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  V we[D][VF], wh[D][TF];
+  const uint32_t full = a.width / K;
+  auto fetch = [&](int d, uint32_t k) {
+    const uint64_t at = (uint64_t)(k < full ? k : full - 1) * K;
+#pragma unroll
+    for (int i = 0; i < VF; ++i) we[d][i] = __builtin_nontemporal_load((const Loose*)(e[i] + at));
+#pragma unroll
+    for (int i = 0; i < TF; ++i) wh[d][i] = *(const Loose*)(h[i] + at);
+  };
+  auto product = [&](int d) {
+#pragma unroll
+    for (int i = 0; i < TF; ++i)
+#pragma unroll
+      for (int j = 0; j < VF; ++j) acc[i][j] = Frag<T>::mma(we[d][j], wh[d][i], acc[i][j]);
+  };
+  if (full) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) fetch(d, d);
+    uint32_t k = 0;
+    for (; k + D <= full; k += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        product(d);
+        fetch(d, k + d + D);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (k + d < full) product(d);
+  }
+  if (full * K < a.width) {  // columns that do not fill a slab
+    const uint32_t left = a.width - full * K > col ? a.width - full * K - col : 0;
+#pragma unroll
+    for (int i = 0; i < VF; ++i) we[0][i] = load16<T>(e[i] + full * K, 0, left);
+#pragma unroll
+    for (int i = 0; i < TF; ++i) wh[0][i] = load16<T>(h[i] + full * K, 0, left);
+    product(0);
+  }
+#pragma unroll
+  for (int i = 0; i < TF; ++i) {
+    const uint32_t r = r0 + 16 * i + (lane & 15);
+    const bool live = r < a.nrows;
+    const SoftStats st = lane_stats<VF>(acc[i], v0, a.vocab, live ? a.tokens[r] : -1, live, w.token_logit + r);
+    if (lane < 16) sh[wv][16 * i + lane] = st;
+  }
   __syncthreads();
-  if (wv == 0 && lane < 16 && at < count) {
-    for (int i = 1; i < 4; ++i) st.join(sh[i][lane], kLog2e);
-    w.partial[(uint64_t)at * tiles + blockIdx.x] = float4{st.m, st.s, st.t, 0.f};
+  const uint32_t r = r0 + threadIdx.x;
+  if (threadIdx.x < 16 * TF && r < a.nrows) {
+    SoftStats st = sh[0][threadIdx.x];
+    for (int i = 1; i < 4; ++i) st.join(sh[i][threadIdx.x], kLog2e);
+    w.partial[(uint64_t)r * tiles + blockIdx.x] = float4{st.m, st.s, st.t, 0.f};
+  }
+}
+
+// Many rows: bound by the products. A workgroup of WT x WV waves takes 16 TF WT live rows by
+// 16 VF WV head rows, in slabs of 128 bytes a row through LDS, two of them: the next one is on
+// its way while this one's products run.
+//
+// A slab's 16-byte chunk c of row r lies at r * 128 + (c ^ swizzle(r)) * 16.
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r >> 1) & 7; }
+__device__ u32x4 zeros16[1];  // what the columns past the width are read from
+
+template <class T, int TF, int VF, int WT, int WV, bool DIRECT>
+__global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
+  using Elem = typename T::Elem;
+  using V = typename T::V;
+  constexpr uint32_t E = T::kPer16, K = 8 * E, WAVES = WT * WV;
+  constexpr uint32_t MT = 16 * TF * WT, NT = 16 * VF * WV, ROWS = MT + NT, LOADS = ROWS / 8 / WAVES;
+  static_assert(ROWS % (8 * WAVES) == 0, "loads");
+  __shared__ __attribute__((aligned(128))) char buf0[ROWS * 128];
+  __shared__ __attribute__((aligned(128))) char buf1[ROWS * 128];
+  __shared__ SoftStats sh[WV][MT];
+  const uint32_t count = *w.count, mtiles = (count + MT - 1) / MT;
+  // Workgroups go to the 8 XCDs in turn: an XCD takes every eighth of the head's tiles, and all
+  // live rows of one after another, so that its L2 holds the tile's slabs for them.
+  const uint32_t vt = blockIdx.x / 8 / (mtiles ? mtiles : 1) * 8 + blockIdx.x % 8, mt = mtiles ? blockIdx.x / 8 % mtiles : 0;
+  if (vt >= tiles || !mtiles) return;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wt = wave % WT, wv = wave / WT;
+
+  // this lane's rows of the loads, at its chunk
+  const Elem* from[LOADS];
+  uint32_t chunk[LOADS];
+#pragma unroll
+  for (uint32_t i = 0; i < LOADS; ++i) {
+    const uint32_t r = (wave + i * WAVES) * 8 + (lane >> 3);
+    chunk[i] = (lane & 7) ^ swizzle(r);
+    if ((wave + i * WAVES) * 8 < MT) {
+      const uint32_t at = mt * MT + r;
+      from[i] = (const Elem*)a.hidden + (int64_t)w.row_of[at < count ? at : count - 1] * a.hidden_stride;
+    } else {
+      const uint32_t v = vt * NT + r - MT;
+      from[i] = (const Elem*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
+    }
+    from[i] += chunk[i] * E;
+  }
+  f32x4 acc[TF][VF];
+#pragma unroll
+  for (int i = 0; i < TF; ++i)
+#pragma unroll
+    for (int j = 0; j < VF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 held[LOADS];  // !DIRECT: a slab on its way
+  const uint32_t slabs = (a.width + K - 1) / K;
+  auto fetch = [&](uint32_t k, char* buf) {
+    const bool tail = (k + 1) * K > a.width;
+#pragma unroll
+    for (uint32_t i = 0; i < LOADS; ++i) {
+      const Elem* p = from[i] + (uint64_t)k * K;
+      const uint32_t at = k * K + chunk[i] * E;
+      if constexpr (DIRECT) {
+        if (tail && at >= a.width) p = (const Elem*)zeros16;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                         (__attribute__((address_space(3))) void*)(buf + (wave + i * WAVES) * 1024), 16, 0, 0);
+      } else {
+        const V x = tail ? load16<T>(p, 0, at < a.width ? a.width - at : 0) : (V)*(const typename Frag<T>::Loose*)p;
+        held[i] = __builtin_bit_cast(u32x4, x);
+      }
+    }
+  };
+  auto put = [&](char* buf) {
+    if constexpr (!DIRECT)
+#pragma unroll
+      for (uint32_t i = 0; i < LOADS; ++i) *(u32x4*)(buf + (wave + i * WAVES) * 1024 + lane * 16) = held[i];
+  };
+  auto products = [&](const char* buf) {
+    const char* bt = buf + (wt * 16 * TF + (lane & 15)) * 128;
+    const char* bv = buf + (MT + wv * 16 * VF + (lane & 15)) * 128;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const uint32_t at = ((kk * 4 + (lane >> 4)) ^ swizzle(lane & 15)) * 16;
+      V xt[TF], xv[VF];
+#pragma unroll
+      for (int i = 0; i < TF; ++i) xt[i] = *(const V*)(bt + i * 2048 + at);
+#pragma unroll
+      for (int j = 0; j < VF; ++j) xv[j] = *(const V*)(bv + j * 2048 + at);
+#pragma unroll
+      for (int j = 0; j < VF; ++j)
+#pragma unroll
+        for (int i = 0; i < TF; ++i) acc[i][j] = Frag<T>::mma(xv[j], xt[i], acc[i][j]);
+    }
+  };
+  fetch(0, buf0);
+  put(buf0);
+  for (uint32_t k = 0; k < slabs; k += 2) {
+    __syncthreads();  // slab k is there; the products of slab k - 1 are done
+    if (k + 1 < slabs) fetch(k + 1, buf1);
+    products(buf0);
+    if (k + 1 >= slabs) break;
+    put(buf1);
+    __syncthreads();
+    if (k + 2 < slabs) fetch(k + 2, buf0);
+    products(buf1);
+    if (k + 2 < slabs) put(buf0);
+  }
+#pragma unroll
+  for (int i = 0; i < TF; ++i) {
+    const uint32_t r = wt * 16 * TF + 16 * i + (lane & 15), at = mt * MT + r;
+    const bool live = at < count;
+    const int64_t tok = a.tokens[w.row_of[live ? at : count - 1]];
+    const SoftStats st = lane_stats<VF>(acc[i], vt * NT + wv * 16 * VF, a.vocab, tok, live, w.token_logit + at);
+    if (lane < 16) sh[wv][r] = st;
+  }
+  __syncthreads();
+  for (uint32_t r = threadIdx.x; r < MT; r += 64 * WAVES) {
+    const uint32_t at = mt * MT + r;
+    if (at >= count) break;
+    SoftStats st = sh[0][r];
+    for (int i = 1; i < WV; ++i) st.join(sh[i][r], kLog2e);
+    w.partial[(uint64_t)at * tiles + vt] = float4{st.m, st.s, st.t, 0.f};
   }
 }
 
 // One wave joins a row's statistics over the head's tiles.
-__global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint32_t tiles) {
+__global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint32_t tiles, bool all_rows) {
   const uint32_t r = blockIdx.x, lane = threadIdx.x;
   const int64_t tok = a.tokens[r];
   if (tok == a.ignore) {
     if (lane == 0) a.logprobs[r] = a.entropy[r] = 0.f;
     return;
   }
-  const uint32_t at = w.live_of[r];
+  const uint32_t at = all_rows ? r : w.live_of[r];
   SoftStats st = SoftStats::of(-INFINITY);
   for (uint32_t i = lane; i < tiles; i += 64) {
     const float4 p = w.partial[(uint64_t)at * tiles + i];
@@ -158,30 +362,65 @@ __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint3
   }
 }
 
+// Which kernel, by the number of rows: up to 64 rows the head's bytes bound it, from there on the products.
+struct Plan {
+  uint32_t row_tile, head_tile;
+  bool stream;
+};
+Plan plan_of(int dtype, uint32_t nrows) {
+  if (nrows <= 64) return Plan{nrows <= 16 ? 16u : nrows <= 32 ? 32u : 64u, kStreamTile, true};
+  if (dtype == DZ_F32) return Plan{64, 128, false};
+  return Plan{nrows <= 128 ? 128u : 256u, 256, false};
+}
+
+template <class T, int TF, int D>
+void stream(const HeadRows& a, const Work& w, uint32_t tiles, hipStream_t st) {
+  head_stream_kernel<T, TF, D><<<dim3(tiles, (a.nrows + 16 * TF - 1) / (16 * TF)), 256, 0, st>>>(a, w, tiles);
+}
+template <class T, int TF, int VF, int WT, int WV>
+void tile(const HeadRows& a, const Work& w, uint32_t tiles, bool direct, hipStream_t st) {
+  const uint32_t grid = (tiles + 7) / 8 * 8 * ((a.nrows + 16 * TF * WT - 1) / (16 * TF * WT));
+  if (direct) head_tile_kernel<T, TF, VF, WT, WV, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
+  else head_tile_kernel<T, TF, VF, WT, WV, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
+}
+template <class T>
+void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, hipStream_t st) {
+  if (p.stream) {
+    if (p.row_tile == 16) stream<T, 1, 8>(a, w, tiles, st);
+    else if (p.row_tile == 32) stream<T, 2, 6>(a, w, tiles, st);
+    else stream<T, 4, 4>(a, w, tiles, st);
+    return;
+  }
+  // whole 16-byte chunks, which can go to LDS without a stop in registers
+  const uint64_t es = sizeof(typename T::Elem);
+  const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0;
+  if constexpr (sizeof(typename T::Elem) == 4) tile<T, 2, 4, 2, 2>(a, w, tiles, direct, st);
+  else if (p.row_tile == 128) tile<T, 4, 8, 2, 2>(a, w, tiles, direct, st);
+  else tile<T, 4, 8, 4, 2>(a, w, tiles, direct, st);
+}
+
 }  // namespace
 
 int64_t head_workspace(int dtype, uint32_t nrows, uint32_t width, uint32_t vocab) {
-  (void)dtype;
   (void)width;
-  return (int64_t)(256 + 3 * align256((uint64_t)nrows * 4) + (uint64_t)nrows * head_tiles(vocab) * sizeof(float4));
+  return (int64_t)(256 + 3 * align256((uint64_t)nrows * 4) + (uint64_t)nrows * head_tiles(vocab, plan_of(dtype, nrows).head_tile) * sizeof(float4));
 }
 
 hipError_t launch_head(int dtype, const HeadRows& a, void* workspace, hipStream_t st) {
+  const Plan p = plan_of(dtype, a.nrows);
   const Work w = work_of(workspace, a.nrows);
-  const uint32_t tiles = head_tiles(a.vocab);
-  const int64_t es = dtype == DZ_F32 ? 4 : 2;
-  const bool vec = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)(a.hidden_stride * es) |
-                    (uint64_t)(a.weight_stride * es)) % 16 == 0;
-  live_rows_kernel<<<1, 1024, 0, st>>>(a, w);
-  hipError_t e = hipGetLastError();
+  const uint32_t tiles = head_tiles(a.vocab, p.head_tile);
+  if (!p.stream) {
+    live_rows_kernel<<<1, 1024, 0, st>>>(a, w);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (dtype == DZ_F32) products<TypeF32>(a, w, p, tiles, st);
+  else if (dtype == DZ_F16) products<TypeF16>(a, w, p, tiles, st);
+  else products<TypeBF16>(a, w, p, tiles, st);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid(tiles, (a.nrows + 15) / 16);
-  if (dtype == DZ_F32) head_kernel<TypeF32><<<grid, 256, 0, st>>>(a, w, tiles, vec);
-  else if (dtype == DZ_F16) head_kernel<TypeF16><<<grid, 256, 0, st>>>(a, w, tiles, vec);
-  else head_kernel<TypeBF16><<<grid, 256, 0, st>>>(a, w, tiles, vec);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  head_join_kernel<<<a.nrows, 64, 0, st>>>(a, w, tiles);
+  head_join_kernel<<<a.nrows, 64, 0, st>>>(a, w, tiles, p.stream);
   return hipGetLastError();
 }
 
