@@ -36,13 +36,12 @@ struct Frag<TypeF32> {
 };
 
 struct Work {
-  uint32_t* count;   // live rows
+  uint32_t* count;   // live rows; NULL: every row is taken as one, in its order
   uint32_t* row_of;  // live row -> row
   uint32_t* live_of;  // row -> live row
   float* token_logit;  // per live row
   float4* partial;     // (live row, head tile)
 };
-constexpr uint32_t kStreamTile = 128;  // head rows of a workgroup of the kernel for few rows
 
 __host__ __device__ inline uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
 inline uint32_t head_tiles(uint32_t vocab, uint32_t tile) { return (vocab + tile - 1) / tile; }
@@ -127,114 +126,57 @@ __device__ __forceinline__ SoftStats lane_stats(f32x4 (&acc)[VF], uint32_t v0, u
   return st;
 }
 
-// Few rows: bound by reading the head once. A wave takes 32 head rows and all tokens of the
-// tile (16 TF) and keeps D slabs of 64 bytes a row on their way, head and hidden states alike,
-// straight to its registers: waves never wait for each other, and 1,571 of them (50,272 tokens)
-// have 8 KB each in flight. The hidden states come from the caches every time.
-template <class T, int TF, int D>
-__global__ __launch_bounds__(256) void head_stream_kernel(HeadRows a, Work w, uint32_t tiles) {
-  constexpr int VF = kStreamTile / 64;
-  constexpr uint32_t E = T::kPer16, K = 4 * E;
-  using V = typename T::V;
-  using Loose = typename Frag<T>::Loose;
-  __shared__ SoftStats sh[4][16 * TF];
-  const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = (lane >> 4) * E;
-  const uint32_t v0 = blockIdx.x * kStreamTile + wv * 16 * VF, r0 = blockIdx.y * 16 * TF;
-  const typename T::Elem* e[VF];
-  const typename T::Elem* h[TF];
-#pragma unroll
-  for (int i = 0; i < VF; ++i) {
-    const uint32_t v = v0 + 16 * i + (lane & 15);
-    e[i] = (const typename T::Elem*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride + col;
-  }
-#pragma unroll
-  for (int i = 0; i < TF; ++i) {
-    const uint32_t r = r0 + 16 * i + (lane & 15);
-    h[i] = (const typename T::Elem*)a.hidden + (int64_t)(r < a.nrows ? r : a.nrows - 1) * a.hidden_stride + col;
-  }
-  f32x4 acc[TF][VF];
-#pragma unroll
-  for (int i = 0; i < TF; ++i)
-#pragma unroll
-    for (int j = 0; j < VF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  V we[D][VF], wh[D][TF];
-  const uint32_t full = a.width / K;
-  auto fetch = [&](int d, uint32_t k) {
-    const uint64_t at = (uint64_t)(k < full ? k : full - 1) * K;
-#pragma unroll
-    for (int i = 0; i < VF; ++i) we[d][i] = __builtin_nontemporal_load((const Loose*)(e[i] + at));
-#pragma unroll
-    for (int i = 0; i < TF; ++i) wh[d][i] = *(const Loose*)(h[i] + at);
-  };
-  auto product = [&](int d) {
-#pragma unroll
-    for (int i = 0; i < TF; ++i)
-#pragma unroll
-      for (int j = 0; j < VF; ++j) acc[i][j] = Frag<T>::mma(we[d][j], wh[d][i], acc[i][j]);
-  };
-  if (full) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) fetch(d, d);
-    uint32_t k = 0;
-    for (; k + D <= full; k += D) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        product(d);
-        fetch(d, k + d + D);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (k + d < full) product(d);
-  }
-  if (full * K < a.width) {  // columns that do not fill a slab
-    const uint32_t left = a.width - full * K > col ? a.width - full * K - col : 0;
-#pragma unroll
-    for (int i = 0; i < VF; ++i) we[0][i] = load16<T>(e[i] + full * K, 0, left);
-#pragma unroll
-    for (int i = 0; i < TF; ++i) wh[0][i] = load16<T>(h[i] + full * K, 0, left);
-    product(0);
-  }
-#pragma unroll
-  for (int i = 0; i < TF; ++i) {
-    const uint32_t r = r0 + 16 * i + (lane & 15);
-    const bool live = r < a.nrows;
-    const SoftStats st = lane_stats<VF>(acc[i], v0, a.vocab, live ? a.tokens[r] : -1, live, w.token_logit + r);
-    if (lane < 16) sh[wv][16 * i + lane] = st;
-  }
-  __syncthreads();
-  const uint32_t r = r0 + threadIdx.x;
-  if (threadIdx.x < 16 * TF && r < a.nrows) {
-    SoftStats st = sh[0][threadIdx.x];
-    for (int i = 1; i < 4; ++i) st.join(sh[i][threadIdx.x], kLog2e);
-    w.partial[(uint64_t)r * tiles + blockIdx.x] = float4{st.m, st.s, st.t, 0.f};
-  }
-}
-
-// Many rows: bound by the products. A workgroup of WT x WV waves takes 16 TF WT live rows by
-// 16 VF WV head rows, in slabs of 128 bytes a row through LDS, two of them: the next one is on
-// its way while this one's products run.
+// A workgroup of WT x WV waves takes 16 TF WT live rows by 16 VF WV head rows, in slabs of 128
+// bytes a row through LDS, STAGES of them: the next ones are on their way while this one's
+// products run.
 //
 // A slab's 16-byte chunk c of row r lies at r * 128 + (c ^ swizzle(r)) * 16.
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r >> 1) & 7; }
 __device__ u32x4 zeros16[1];  // what the columns past the width are read from
 
-template <class T, int TF, int VF, int WT, int WV, bool DIRECT>
+// 16 bytes a lane from p to LDS, 1,024 consecutive bytes from `lds` on (the same for the whole wave). In
+// assembly, so that the compiler, which cannot tell the slabs' places apart from one round of the
+// loop to the next, does not wait for every load before it reads LDS; arrive() waits. (M0 is not named
+// as overwritten, since it cannot be: nothing else here uses it.)
+template <bool ONCE>
+__device__ __forceinline__ void to_lds(const void* p, char* lds) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
+  if (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(p) : "memory");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
+}
+
+// All but the last N of this wave's loads are done, and every wave of the workgroup is here.
+template <int N>
+__device__ __forceinline__ void arrive() {
+  static_assert(N < 16, "a count of four bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | N);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <class T, int TF, int VF, int WT, int WV, int STAGES, bool DIRECT>
 __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
   using Elem = typename T::Elem;
   using V = typename T::V;
   constexpr uint32_t E = T::kPer16, K = 8 * E, WAVES = WT * WV;
   constexpr uint32_t MT = 16 * TF * WT, NT = 16 * VF * WV, ROWS = MT + NT, LOADS = ROWS / 8 / WAVES;
   static_assert(ROWS % (8 * WAVES) == 0, "loads");
+  static_assert(STAGES == 2 || (STAGES == 3 && DIRECT), "stages");
   __shared__ __attribute__((aligned(128))) char buf0[ROWS * 128];
   __shared__ __attribute__((aligned(128))) char buf1[ROWS * 128];
+  __shared__ __attribute__((aligned(128))) char buf2[STAGES == 3 ? ROWS * 128 : 128];
   __shared__ SoftStats sh[WV][MT];
-  const uint32_t count = *w.count, mtiles = (count + MT - 1) / MT;
+  const uint32_t count = w.count ? *w.count : a.nrows, mtiles = (count + MT - 1) / MT;
   // Workgroups go to the 8 XCDs in turn: an XCD takes every eighth of the head's tiles, and all
   // live rows of one after another, so that its L2 holds the tile's slabs for them.
   const uint32_t vt = blockIdx.x / 8 / (mtiles ? mtiles : 1) * 8 + blockIdx.x % 8, mt = mtiles ? blockIdx.x / 8 % mtiles : 0;
   if (vt >= tiles || !mtiles) return;
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wt = wave % WT, wv = wave / WT;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = wave % WT, wv = wave / WT;
+  auto row_of = [&](uint32_t at) {
+    if (at >= count) at = count - 1;
+    return w.count ? w.row_of[at] : at;
+  };
 
   // this lane's rows of the loads, at its chunk
   const Elem* from[LOADS];
@@ -244,8 +186,7 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
     const uint32_t r = (wave + i * WAVES) * 8 + (lane >> 3);
     chunk[i] = (lane & 7) ^ swizzle(r);
     if ((wave + i * WAVES) * 8 < MT) {
-      const uint32_t at = mt * MT + r;
-      from[i] = (const Elem*)a.hidden + (int64_t)w.row_of[at < count ? at : count - 1] * a.hidden_stride;
+      from[i] = (const Elem*)a.hidden + (int64_t)row_of(mt * MT + r) * a.hidden_stride;
     } else {
       const uint32_t v = vt * NT + r - MT;
       from[i] = (const Elem*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
@@ -258,6 +199,8 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
 #pragma unroll
     for (int j = 0; j < VF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // one tile of rows: nothing reads the head again, and its lines need not stay (6.5 TB/s for 5.9)
+  constexpr bool ONCE = STAGES == 3;
   u32x4 held[LOADS];  // !DIRECT: a slab on its way
   const uint32_t slabs = (a.width + K - 1) / K;
   auto fetch = [&](uint32_t k, char* buf) {
@@ -268,8 +211,7 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
       const uint32_t at = k * K + chunk[i] * E;
       if constexpr (DIRECT) {
         if (tail && at >= a.width) p = (const Elem*)zeros16;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
-                                         (__attribute__((address_space(3))) void*)(buf + (wave + i * WAVES) * 1024), 16, 0, 0);
+        to_lds<ONCE>(p, buf + (wave + i * WAVES) * 1024);
       } else {
         const V x = tail ? load16<T>(p, 0, at < a.width ? a.width - at : 0) : (V)*(const typename Frag<T>::Loose*)p;
         held[i] = __builtin_bit_cast(u32x4, x);
@@ -298,25 +240,47 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
         for (int i = 0; i < TF; ++i) acc[i][j] = Frag<T>::mma(xv[j], xt[i], acc[i][j]);
     }
   };
-  fetch(0, buf0);
-  put(buf0);
-  for (uint32_t k = 0; k < slabs; k += 2) {
-    __syncthreads();  // slab k is there; the products of slab k - 1 are done
-    if (k + 1 < slabs) fetch(k + 1, buf1);
-    products(buf0);
-    if (k + 1 >= slabs) break;
-    put(buf1);
-    __syncthreads();
-    if (k + 2 < slabs) fetch(k + 2, buf0);
-    products(buf1);
-    if (k + 2 < slabs) put(buf0);
+  if constexpr (STAGES == 3) {
+    // Two slabs past the last one are loaded too (zeros), so that the wait is one number.
+    fetch(0, buf0);
+    fetch(1, buf1);
+    // slab k is there, and the products of slab k - 1, whose place slab k + 2 takes, are done
+    auto step = [&](uint32_t k, const char* here, char* next) {
+      arrive<LOADS>();
+      fetch(k + 2, next);
+      products(here);
+    };
+    for (uint32_t k = 0;;) {
+      step(k, buf0, buf2);
+      if (++k >= slabs) break;
+      step(k, buf1, buf0);
+      if (++k >= slabs) break;
+      step(k, buf2, buf1);
+      if (++k >= slabs) break;
+    }
+    arrive<0>();  // a workgroup must not end, and give its LDS away, with loads to it on their way
+  } else {
+    fetch(0, buf0);
+    put(buf0);
+    auto step = [&](uint32_t k, const char* here, char* next) {
+      // slab k is there; the products of slab k - 1 are done
+      if (DIRECT) arrive<0>();
+      else __syncthreads();
+      if (k + 1 < slabs) fetch(k + 1, next);
+      products(here);
+      if (k + 1 < slabs) put(next);
+    };
+    for (uint32_t k = 0; k < slabs; k += 2) {
+      step(k, buf0, buf1);
+      if (k + 1 < slabs) step(k + 1, buf1, buf0);
+    }
   }
 #pragma unroll
   for (int i = 0; i < TF; ++i) {
     const uint32_t r = wt * 16 * TF + 16 * i + (lane & 15), at = mt * MT + r;
     const bool live = at < count;
-    const int64_t tok = a.tokens[w.row_of[live ? at : count - 1]];
-    const SoftStats st = lane_stats<VF>(acc[i], vt * NT + wv * 16 * VF, a.vocab, tok, live, w.token_logit + at);
+    const int64_t tok = a.tokens[row_of(at)];
+    const SoftStats st = lane_stats(acc[i], vt * NT + wv * 16 * VF, a.vocab, tok, live, w.token_logit + at);
     if (lane < 16) sh[wv][r] = st;
   }
   __syncthreads();
@@ -330,14 +294,14 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
 }
 
 // One wave joins a row's statistics over the head's tiles.
-__global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint32_t tiles, bool all_rows) {
+__global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint32_t tiles) {
   const uint32_t r = blockIdx.x, lane = threadIdx.x;
   const int64_t tok = a.tokens[r];
   if (tok == a.ignore) {
     if (lane == 0) a.logprobs[r] = a.entropy[r] = 0.f;
     return;
   }
-  const uint32_t at = all_rows ? r : w.live_of[r];
+  const uint32_t at = w.count ? w.live_of[r] : r;
   SoftStats st = SoftStats::of(-INFINITY);
   for (uint32_t i = lane; i < tiles; i += 64) {
     const float4 p = w.partial[(uint64_t)at * tiles + i];
@@ -362,41 +326,33 @@ __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint3
   }
 }
 
-// Which kernel, by the number of rows: up to 64 rows the head's bytes bound it, from there on the products.
+// A workgroup's rows and head rows, by the number of rows: up to 64 rows the head's bytes bound the
+// kernel, from there on the products.
 struct Plan {
   uint32_t row_tile, head_tile;
-  bool stream;
 };
 Plan plan_of(int dtype, uint32_t nrows) {
-  if (nrows <= 64) return Plan{nrows <= 16 ? 16u : nrows <= 32 ? 32u : 64u, kStreamTile, true};
-  if (dtype == DZ_F32) return Plan{64, 128, false};
-  return Plan{nrows <= 128 ? 128u : 256u, 256, false};
+  if (nrows <= 32) return Plan{32, 128};
+  if (nrows <= 64 || dtype == DZ_F32) return Plan{64, 128};
+  return Plan{nrows <= 128 ? 128u : 256u, 256};
 }
 
-template <class T, int TF, int D>
-void stream(const HeadRows& a, const Work& w, uint32_t tiles, hipStream_t st) {
-  head_stream_kernel<T, TF, D><<<dim3(tiles, (a.nrows + 16 * TF - 1) / (16 * TF)), 256, 0, st>>>(a, w, tiles);
-}
-template <class T, int TF, int VF, int WT, int WV>
+template <class T, int TF, int VF, int WT, int WV, int STAGES>
 void tile(const HeadRows& a, const Work& w, uint32_t tiles, bool direct, hipStream_t st) {
   const uint32_t grid = (tiles + 7) / 8 * 8 * ((a.nrows + 16 * TF * WT - 1) / (16 * TF * WT));
-  if (direct) head_tile_kernel<T, TF, VF, WT, WV, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
-  else head_tile_kernel<T, TF, VF, WT, WV, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
+  if (direct) head_tile_kernel<T, TF, VF, WT, WV, STAGES, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
+  else head_tile_kernel<T, TF, VF, WT, WV, 2, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
 }
 template <class T>
 void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, hipStream_t st) {
-  if (p.stream) {
-    if (p.row_tile == 16) stream<T, 1, 8>(a, w, tiles, st);
-    else if (p.row_tile == 32) stream<T, 2, 6>(a, w, tiles, st);
-    else stream<T, 4, 4>(a, w, tiles, st);
-    return;
-  }
   // whole 16-byte chunks, which can go to LDS without a stop in registers
   const uint64_t es = sizeof(typename T::Elem);
   const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0;
-  if constexpr (sizeof(typename T::Elem) == 4) tile<T, 2, 4, 2, 2>(a, w, tiles, direct, st);
-  else if (p.row_tile == 128) tile<T, 4, 8, 2, 2>(a, w, tiles, direct, st);
-  else tile<T, 4, 8, 4, 2>(a, w, tiles, direct, st);
+  if (p.row_tile == 32) return tile<T, 2, 2, 1, 4, 3>(a, w, tiles, direct, st);
+  if (a.nrows <= 64) return tile<T, 4, 2, 1, 4, 3>(a, w, tiles, direct, st);
+  if constexpr (sizeof(typename T::Elem) == 4) return tile<T, 2, 4, 2, 2, 2>(a, w, tiles, direct, st);
+  else if (p.row_tile == 128) return tile<T, 4, 8, 2, 2, 3>(a, w, tiles, direct, st);
+  else return tile<T, 4, 8, 4, 2, 2>(a, w, tiles, direct, st);
 }
 
 }  // namespace
@@ -408,9 +364,11 @@ int64_t head_workspace(int dtype, uint32_t nrows, uint32_t width, uint32_t vocab
 
 hipError_t launch_head(int dtype, const HeadRows& a, void* workspace, hipStream_t st) {
   const Plan p = plan_of(dtype, a.nrows);
-  const Work w = work_of(workspace, a.nrows);
+  Work w = work_of(workspace, a.nrows);
   const uint32_t tiles = head_tiles(a.vocab, p.head_tile);
-  if (!p.stream) {
+  if (a.nrows <= 64) {  // one tile: all of them
+    w.count = nullptr;
+  } else {
     live_rows_kernel<<<1, 1024, 0, st>>>(a, w);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -420,7 +378,7 @@ hipError_t launch_head(int dtype, const HeadRows& a, void* workspace, hipStream_
   else products<TypeBF16>(a, w, p, tiles, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  head_join_kernel<<<a.nrows, 64, 0, st>>>(a, w, tiles, p.stream);
+  head_join_kernel<<<a.nrows, 64, 0, st>>>(a, w, tiles);
   return hipGetLastError();
 }
 
