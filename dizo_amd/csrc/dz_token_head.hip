@@ -4,6 +4,8 @@
 #include "dz_token_loss.h"
 #include "dz_token_math.h"
 
+#include <type_traits>
+
 namespace dz {
 namespace {
 
@@ -134,15 +136,17 @@ __device__ __forceinline__ SoftStats lane_stats(f32x4 (&acc)[VF], uint32_t v0, u
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r >> 1) & 7; }
 __device__ u32x4 zeros16[1];  // what the columns past the width are read from
 
-// 16 bytes a lane from p to LDS, 1,024 consecutive bytes from `lds` on (the same for the whole wave). In
-// assembly, so that the compiler, which cannot tell the slabs' places apart from one round of the
-// loop to the next, does not wait for every load before it reads LDS; arrive() waits. (M0 is not named
-// as overwritten, since it cannot be: nothing else here uses it.)
+// 16 bytes a lane to LDS, 1,024 consecutive bytes from address `lds` on (the same for the whole wave), from
+// base + offset or from p. In assembly, so that the compiler, which cannot tell the slabs' places apart
+// from one round of the loop to the next, does not wait for every load before it reads LDS; arrive() waits.
+// (M0 is not named as overwritten, since it cannot be: nothing else here uses it.)
 template <bool ONCE>
-__device__ __forceinline__ void to_lds(const void* p, char* lds) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-  if (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(p) : "memory");
-  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
+__device__ __forceinline__ void to_lds(const void* base, uint32_t offset, uint32_t lds) {
+  if (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void to_lds(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
 
 // All but the last N of this wave's loads are done, and every wave of the workgroup is here.
@@ -163,9 +167,7 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
   constexpr uint32_t MT = 16 * TF * WT, NT = 16 * VF * WV, ROWS = MT + NT, LOADS = ROWS / 8 / WAVES;
   static_assert(ROWS % (8 * WAVES) == 0, "loads");
   static_assert(STAGES == 2 || (STAGES == 3 && DIRECT), "stages");
-  __shared__ __attribute__((aligned(128))) char buf0[ROWS * 128];
-  __shared__ __attribute__((aligned(128))) char buf1[ROWS * 128];
-  __shared__ __attribute__((aligned(128))) char buf2[STAGES == 3 ? ROWS * 128 : 128];
+  __shared__ __attribute__((aligned(128))) char slots[STAGES][ROWS * 128];
   __shared__ SoftStats sh[WV][MT];
   const uint32_t count = w.count ? *w.count : a.nrows, mtiles = (count + MT - 1) / MT;
   // Workgroups go to the 8 XCDs in turn: an XCD takes every eighth of the head's tiles, and all
@@ -178,20 +180,24 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
     return w.count ? w.row_of[at] : at;
   };
 
-  // this lane's rows of the loads, at its chunk
-  const Elem* from[LOADS];
-  uint32_t chunk[LOADS];
+  // A load takes 8 rows of hidden states or of the head; this lane's row of load i, at its chunk.
+  const char* const hidden0 = (const char*)a.hidden;
+  const char* const weight0 = (const char*)a.weight + (int64_t)vt * NT * a.weight_stride * sizeof(Elem);
+  static_assert(MT % (8 * WAVES) == 0, "a wave's load i is of the same kind for all waves");
+  auto of_hidden = [](uint32_t i) { return i < MT / 8 / WAVES; };
+  static_assert(WAVES % 2 == 0, "a lane's chunk is the same for all of its loads");
+  const uint32_t chunk = (lane & 7) ^ swizzle(wave * 8 + (lane >> 3));
+  using Offset = std::conditional_t<DIRECT, uint32_t, uint64_t>;  // bytes; the launch looks after the 32 bits
+  Offset from[LOADS];
 #pragma unroll
   for (uint32_t i = 0; i < LOADS; ++i) {
     const uint32_t r = (wave + i * WAVES) * 8 + (lane >> 3);
-    chunk[i] = (lane & 7) ^ swizzle(r);
-    if ((wave + i * WAVES) * 8 < MT) {
-      from[i] = (const Elem*)a.hidden + (int64_t)row_of(mt * MT + r) * a.hidden_stride;
+    if (of_hidden(i)) {
+      from[i] = (Offset)((uint64_t)row_of(mt * MT + r) * a.hidden_stride * sizeof(Elem)) + chunk * 16;
     } else {
-      const uint32_t v = vt * NT + r - MT;
-      from[i] = (const Elem*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
+      const uint32_t v = r - MT;
+      from[i] = (Offset)((uint64_t)(vt * NT + v < a.vocab ? v : a.vocab - 1 - vt * NT) * a.weight_stride * sizeof(Elem)) + chunk * 16;
     }
-    from[i] += chunk[i] * E;
   }
   f32x4 acc[TF][VF];
 #pragma unroll
@@ -199,80 +205,104 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
 #pragma unroll
     for (int j = 0; j < VF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // one tile of rows: nothing reads the head again, and its lines need not stay (6.5 TB/s for 5.9)
-  constexpr bool ONCE = STAGES == 3;
-  u32x4 held[LOADS];  // !DIRECT: a slab on its way
-  const uint32_t slabs = (a.width + K - 1) / K;
-  auto fetch = [&](uint32_t k, char* buf) {
-    const bool tail = (k + 1) * K > a.width;
+  // Products of the slab in `here`; `between` runs after each of the first VF groups of TF products. Operands
+  // are read two groups ahead.
+  const uint32_t lane_row = (lane & 15) * 128;
+  auto products = [&](const char* here, auto between) {
+    const char* bt = here + wt * 16 * TF * 128 + lane_row;
+    const char* bv = here + (MT + wv * 16 * VF) * 128 + lane_row;
+    const uint32_t at[2] = {((lane >> 4) ^ swizzle(lane & 15)) * 16, ((4 + (lane >> 4)) ^ swizzle(lane & 15)) * 16};
+    V xt[2][TF], xv[2 * VF];
+    auto read_v = [&](int g) { xv[g] = *(const V*)(bv + g % VF * 2048 + at[g / VF]); };
 #pragma unroll
-    for (uint32_t i = 0; i < LOADS; ++i) {
-      const Elem* p = from[i] + (uint64_t)k * K;
-      const uint32_t at = k * K + chunk[i] * E;
-      if constexpr (DIRECT) {
-        if (tail && at >= a.width) p = (const Elem*)zeros16;
-        to_lds<ONCE>(p, buf + (wave + i * WAVES) * 1024);
+    for (int i = 0; i < TF; ++i) xt[0][i] = *(const V*)(bt + i * 2048 + at[0]);
+    read_v(0);
+    read_v(1);
+#pragma unroll
+    for (int g = 0; g < 2 * VF; ++g) {
+      if (g + 2 < 2 * VF) read_v(g + 2);
+#pragma unroll
+      for (int i = 0; i < TF; ++i)
+        if (g == (VF > TF ? VF - TF + i : VF - 1)) xt[1][i] = *(const V*)(bt + i * 2048 + at[1]);
+#pragma unroll
+      for (int i = 0; i < TF; ++i) acc[i][g % VF] = Frag<T>::mma(xv[g], xt[g / VF][i], acc[i][g % VF]);
+      if (g < VF) between(g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const uint32_t slabs = (a.width + K - 1) / K;
+  if constexpr (DIRECT) {
+    // one tile of rows: nothing reads the head again, and its lines need not stay (6.5 TB/s for 5.9)
+    constexpr bool ONCE = STAGES == 3;
+    const uint32_t full = a.width / K;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&slots[0][wave * 1024]);
+    auto load = [&](uint32_t i, uint32_t k, uint32_t lds) {
+      if (of_hidden(i)) to_lds<false>(hidden0 + (uint64_t)k * 128, from[i], lds + i * WAVES * 1024);
+      else to_lds<ONCE>(weight0 + (uint64_t)k * 128, from[i], lds + i * WAVES * 1024);
+    };
+    // a slab of which the last columns, or all, lie past the width
+    auto load_end = [&](uint32_t k, uint32_t lds) {
+#pragma unroll
+      for (uint32_t i = 0; i < LOADS; ++i) {
+        const char* p = (of_hidden(i) ? hidden0 : weight0) + from[i] + (uint64_t)k * 128;
+        if (k * K + chunk * E >= a.width) p = (const char*)zeros16;
+        to_lds(p, lds + i * WAVES * 1024);
+      }
+    };
+    auto next_slot = [](uint32_t s) { return s + 1 == STAGES ? 0 : s + 1; };
+#pragma unroll
+    for (uint32_t k = 0; k < STAGES - 1; ++k) {
+      if (k < full) {
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) load(i, k, lds0 + k * ROWS * 128);
       } else {
+        load_end(k, lds0 + k * ROWS * 128);
+      }
+    }
+    uint32_t slot = 0, fill = STAGES - 1, k = 0;
+    for (; k + STAGES - 1 < full; ++k) {
+      arrive<(STAGES - 2) * LOADS>();  // slab k is there, and the products of slab k - 1, whose place the next one takes, are done
+      const uint32_t lds = lds0 + fill * ROWS * 128;
+      products(slots[slot], [&](int g) {
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i)
+          if (i * VF / LOADS == (uint32_t)g) load(i, k + STAGES - 1, lds);
+      });
+      slot = next_slot(slot);
+      fill = next_slot(fill);
+    }
+    for (; k < slabs; ++k) {
+      arrive<(STAGES - 2) * LOADS>();
+      // with three stages, slabs past the last one are loaded too (zeros), so that the wait is one number
+      if (STAGES == 3 || k + 1 < slabs) load_end(k + STAGES - 1, lds0 + fill * ROWS * 128);
+      products(slots[slot], [](int) {});
+      slot = next_slot(slot);
+      fill = next_slot(fill);
+    }
+    if (STAGES == 3) arrive<0>();  // a workgroup must not end, and give its LDS away, with loads to it on their way
+  } else {
+    u32x4 held[LOADS];  // a slab on its way
+    auto fetch = [&](uint32_t k) {
+      const bool tail = (k + 1) * K > a.width;
+#pragma unroll
+      for (uint32_t i = 0; i < LOADS; ++i) {
+        const Elem* p = (const Elem*)((of_hidden(i) ? hidden0 : weight0) + from[i] + (uint64_t)k * 128);
+        const uint32_t at = k * K + chunk * E;
         const V x = tail ? load16<T>(p, 0, at < a.width ? a.width - at : 0) : (V)*(const typename Frag<T>::Loose*)p;
         held[i] = __builtin_bit_cast(u32x4, x);
       }
-    }
-  };
-  auto put = [&](char* buf) {
-    if constexpr (!DIRECT)
-#pragma unroll
-      for (uint32_t i = 0; i < LOADS; ++i) *(u32x4*)(buf + (wave + i * WAVES) * 1024 + lane * 16) = held[i];
-  };
-  auto products = [&](const char* buf) {
-    const char* bt = buf + (wt * 16 * TF + (lane & 15)) * 128;
-    const char* bv = buf + (MT + wv * 16 * VF + (lane & 15)) * 128;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const uint32_t at = ((kk * 4 + (lane >> 4)) ^ swizzle(lane & 15)) * 16;
-      V xt[TF], xv[VF];
-#pragma unroll
-      for (int i = 0; i < TF; ++i) xt[i] = *(const V*)(bt + i * 2048 + at);
-#pragma unroll
-      for (int j = 0; j < VF; ++j) xv[j] = *(const V*)(bv + j * 2048 + at);
-#pragma unroll
-      for (int j = 0; j < VF; ++j)
-#pragma unroll
-        for (int i = 0; i < TF; ++i) acc[i][j] = Frag<T>::mma(xv[j], xt[i], acc[i][j]);
-    }
-  };
-  if constexpr (STAGES == 3) {
-    // Two slabs past the last one are loaded too (zeros), so that the wait is one number.
-    fetch(0, buf0);
-    fetch(1, buf1);
-    // slab k is there, and the products of slab k - 1, whose place slab k + 2 takes, are done
-    auto step = [&](uint32_t k, const char* here, char* next) {
-      arrive<LOADS>();
-      fetch(k + 2, next);
-      products(here);
     };
-    for (uint32_t k = 0;;) {
-      step(k, buf0, buf2);
-      if (++k >= slabs) break;
-      step(k, buf1, buf0);
-      if (++k >= slabs) break;
-      step(k, buf2, buf1);
-      if (++k >= slabs) break;
-    }
-    arrive<0>();  // a workgroup must not end, and give its LDS away, with loads to it on their way
-  } else {
-    fetch(0, buf0);
-    put(buf0);
-    auto step = [&](uint32_t k, const char* here, char* next) {
-      // slab k is there; the products of slab k - 1 are done
-      if (DIRECT) arrive<0>();
-      else __syncthreads();
-      if (k + 1 < slabs) fetch(k + 1, next);
-      products(here);
-      if (k + 1 < slabs) put(next);
+    auto put = [&](char* there) {
+#pragma unroll
+      for (uint32_t i = 0; i < LOADS; ++i) *(u32x4*)(there + (wave + i * WAVES) * 1024 + lane * 16) = held[i];
     };
-    for (uint32_t k = 0; k < slabs; k += 2) {
-      step(k, buf0, buf1);
-      if (k + 1 < slabs) step(k + 1, buf1, buf0);
+    fetch(0);
+    put(slots[0]);
+    for (uint32_t k = 0; k < slabs; ++k) {
+      __syncthreads();  // slab k is there; the products of slab k - 1 are done
+      if (k + 1 < slabs) fetch(k + 1);
+      products(slots[k & 1], [](int) {});
+      if (k + 1 < slabs) put(slots[~k & 1]);
     }
   }
 #pragma unroll
@@ -345,9 +375,10 @@ void tile(const HeadRows& a, const Work& w, uint32_t tiles, bool direct, hipStre
 }
 template <class T>
 void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, hipStream_t st) {
-  // whole 16-byte chunks, which can go to LDS without a stop in registers
+  // whole 16-byte chunks, at offsets of 32 bits, can go to LDS without a stop in registers
   const uint64_t es = sizeof(typename T::Elem);
-  const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0;
+  const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0 &&
+                      (uint64_t)a.hidden_stride * es * a.nrows < (1ull << 32) && (uint64_t)a.weight_stride * es * p.head_tile < (1ull << 32);
   if (p.row_tile == 32) return tile<T, 2, 2, 1, 4, 3>(a, w, tiles, direct, st);
   if (a.nrows <= 64) return tile<T, 4, 2, 1, 4, 3>(a, w, tiles, direct, st);
   if constexpr (sizeof(typename T::Elem) == 4) return tile<T, 2, 4, 2, 2, 2>(a, w, tiles, direct, st);
