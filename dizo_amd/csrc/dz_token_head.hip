@@ -9,30 +9,40 @@
 namespace dz {
 namespace {
 
-// 16 bytes of a row's width per lane: lane l holds row l & 15, bytes
-// 16 (l >> 4) .. + 15 of a 64-byte slab. The products of one slab: 16 head
-// rows by 16 tokens; lane l then holds token l & 15, head rows 4 (l >> 4) .. + 3.
+// Products of M = 16 or 32 head rows by M tokens. A lane holds 16 bytes of a row's width: row l % M of
+// the M, chunk l / M of the 64 / M that one step takes. The results: lane l holds token l % M, head rows
+// 4 (l / M) .. + 3 of every 256 / M.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <int M>
+using Acc = std::conditional_t<M == 16, f32x4, f32x16>;
+
 template <class T>
 struct Frag;
 template <>
 struct Frag<TypeF16> {
-  using V = TypeF16::V;
   typedef TypeF16::V Loose __attribute__((aligned(2)));  // at any element
+  using V = TypeF16::V;
   __device__ static f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  __device__ static f32x16 mma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<TypeBF16> {
+  typedef TypeBF16::V Loose __attribute__((aligned(2)));
   using V = TypeBF16::V;
-  typedef TypeBF16::V Loose __attribute__((aligned(2)));  // at any element
   __device__ static f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  __device__ static f32x16 mma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<TypeF32> {
+  typedef TypeF32::V Loose __attribute__((aligned(4)));
   using V = TypeF32::V;
-  typedef TypeF32::V Loose __attribute__((aligned(4)));  // at any element
-  // the slab's 16 columns in the order (0, 4, 8, 12), (1, 5, ...), the same on both sides
+  // the chunks' columns in the order (0, 4, ...), (1, 5, ...), the same on both sides
   __device__ static f32x4 mma(V a, V b, f32x4 c) {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+  __device__ static f32x16 mma(V a, V b, f32x16 c) {
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
     return c;
   }
 };
@@ -89,36 +99,38 @@ __device__ __forceinline__ typename T::V load16(const typename T::Elem* row, uin
   return v;
 }
 
-// A token's logits over a lane's head rows (4 of each of VF slabs of 16) to their statistics: over the
-// four lanes that hold the token's. v0: the first head row of the wave. Leaves the token's own logit.
-template <int VF>
-__device__ __forceinline__ SoftStats lane_stats(f32x4 (&acc)[VF], uint32_t v0, uint32_t vocab, int64_t tok, bool live, float* token_logit) {
-  const uint32_t lane = threadIdx.x & 63, first = v0 + 4 * (lane >> 4);
-  if (v0 + 16 * VF > vocab) {  // head rows past the last one take no part
+// A token's logits over a lane's head rows (those of VF products) to their statistics over the 64 / M
+// lanes that hold the token's. v0: the first head row of the wave. Leaves the token's own logit.
+template <int M, int VF>
+__device__ __forceinline__ SoftStats lane_stats(Acc<M> (&acc)[VF], uint32_t v0, uint32_t vocab, int64_t tok, bool live, float* token_logit) {
+  const uint32_t lane = threadIdx.x & 63, first = v0 + 4 * (lane / M);
+  auto row = [](int i, int j) { return (uint32_t)(i * M + j / 4 * (256 / M) + j % 4); };
+  constexpr int N = M * M / 64;
+  if (v0 + M * VF > vocab) {  // head rows past the last one take no part
 #pragma unroll
     for (int i = 0; i < VF; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (first + 16 * i + j >= vocab) acc[i][j] = -INFINITY;
+      for (int j = 0; j < N; ++j)
+        if (first + row(i, j) >= vocab) acc[i][j] = -INFINITY;
   }
   const uint64_t rel = (uint64_t)(tok - (int64_t)first);
-  if (__any(live && rel < 16 * VF)) {
+  if (__any(live && rel < M * VF)) {
 #pragma unroll
     for (int i = 0; i < VF; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (rel == (uint64_t)(16 * i + j) && live && first + 16 * i + j < vocab) *token_logit = acc[i][j];
+      for (int j = 0; j < N; ++j)
+        if (rel == (uint64_t)row(i, j) && live && first + row(i, j) < vocab) *token_logit = acc[i][j];
   }
   SoftStats st = SoftStats::of(-INFINITY);
 #pragma unroll
   for (int i = 0; i < VF; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) st.m = fmaxf(st.m, acc[i][j]);
+    for (int j = 0; j < N; ++j) st.m = fmaxf(st.m, acc[i][j]);
 #pragma unroll
   for (int i = 0; i < VF; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) st.add(acc[i][j], kLog2e);
-  for (int off = 16; off <= 32; off *= 2) {
+    for (int j = 0; j < N; ++j) st.add(acc[i][j], kLog2e);
+  for (int off = M; off <= 32; off *= 2) {
     SoftStats o;
     o.m = __shfl_xor(st.m, off, 64);
     o.s = __shfl_xor(st.s, off, 64);
@@ -159,14 +171,14 @@ __device__ __forceinline__ void arrive() {
   asm volatile("" ::: "memory");
 }
 
-template <class T, int TF, int VF, int WT, int WV, int STAGES, bool DIRECT>
-__global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
+template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE, bool DIRECT>
+__global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
   using Elem = typename T::Elem;
   using V = typename T::V;
   constexpr uint32_t E = T::kPer16, K = 8 * E, WAVES = WT * WV;
-  constexpr uint32_t MT = 16 * TF * WT, NT = 16 * VF * WV, ROWS = MT + NT, LOADS = ROWS / 8 / WAVES;
+  constexpr uint32_t MT = M * TF * WT, NT = M * VF * WV, ROWS = MT + NT, LOADS = ROWS / 8 / WAVES;
   static_assert(ROWS % (8 * WAVES) == 0, "loads");
-  static_assert(STAGES == 2 || (STAGES == 3 && DIRECT), "stages");
+  static_assert(STAGES >= 2 && (STAGES == 2 || DIRECT), "stages");
   __shared__ __attribute__((aligned(128))) char slots[STAGES][ROWS * 128];
   __shared__ SoftStats sh[WV][MT];
   const uint32_t count = w.count ? *w.count : a.nrows, mtiles = (count + MT - 1) / MT;
@@ -199,41 +211,42 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
       from[i] = (Offset)((uint64_t)(vt * NT + v < a.vocab ? v : a.vocab - 1 - vt * NT) * a.weight_stride * sizeof(Elem)) + chunk * 16;
     }
   }
-  f32x4 acc[TF][VF];
+  Acc<M> acc[TF][VF];
 #pragma unroll
   for (int i = 0; i < TF; ++i)
 #pragma unroll
-    for (int j = 0; j < VF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < VF; ++j) acc[i][j] = Acc<M>(0.f);
 
-  // Products of the slab in `here`; `between` runs after each of the first VF groups of TF products. Operands
-  // are read two groups ahead.
-  const uint32_t lane_row = (lane & 15) * 128;
+  // Products of the slab in `here`, in groups of TF; `between` runs after each of the first half of the
+  // groups. A group's operands are read while the two before it run.
+  constexpr int PARTS = 8 * M / 64, GROUPS = PARTS * VF;
+  uint32_t at[PARTS];  // this lane's chunks
+#pragma unroll
+  for (int n = 0; n < PARTS; ++n) at[n] = (lane % M) * 128 + ((n * (64 / M) + lane / M) ^ swizzle(lane % M)) * 16;
   auto products = [&](const char* here, auto between) {
-    const char* bt = here + wt * 16 * TF * 128 + lane_row;
-    const char* bv = here + (MT + wv * 16 * VF) * 128 + lane_row;
-    const uint32_t at[2] = {((lane >> 4) ^ swizzle(lane & 15)) * 16, ((4 + (lane >> 4)) ^ swizzle(lane & 15)) * 16};
-    V xt[2][TF], xv[2 * VF];
-    auto read_v = [&](int g) { xv[g] = *(const V*)(bv + g % VF * 2048 + at[g / VF]); };
+    const char* bt = here + wt * M * TF * 128;
+    const char* bv = here + (MT + wv * M * VF) * 128;
+    V xt[PARTS][TF], xv[GROUPS];
+    auto read_v = [&](int g) { xv[g] = *(const V*)(bv + g % VF * M * 128 + at[g / VF]); };
+    auto read_t = [&](int n, int i) { xt[n][i] = *(const V*)(bt + i * M * 128 + at[n]); };
 #pragma unroll
-    for (int i = 0; i < TF; ++i) xt[0][i] = *(const V*)(bt + i * 2048 + at[0]);
+    for (int i = 0; i < TF; ++i) read_t(0, i);
     read_v(0);
-    read_v(1);
+    if (GROUPS > 1) read_v(1);
 #pragma unroll
-    for (int g = 0; g < 2 * VF; ++g) {
-      if (g + 2 < 2 * VF) read_v(g + 2);
+    for (int g = 0; g < GROUPS; ++g) {
+      if (g + 2 < GROUPS) read_v(g + 2);
 #pragma unroll
       for (int i = 0; i < TF; ++i)
-        if (g == (VF > TF ? VF - TF + i : VF - 1)) xt[1][i] = *(const V*)(bt + i * 2048 + at[1]);
+        if (g / VF + 1 < PARTS && g % VF == (VF - 1 - TF + i > 0 ? VF - 1 - TF + i : 0)) read_t(g / VF + 1, i);
 #pragma unroll
       for (int i = 0; i < TF; ++i) acc[i][g % VF] = Frag<T>::mma(xv[g], xt[g / VF][i], acc[i][g % VF]);
-      if (g < VF) between(g);
+      if (g < GROUPS / 2) between(g);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   const uint32_t slabs = (a.width + K - 1) / K;
   if constexpr (DIRECT) {
-    // one tile of rows: nothing reads the head again, and its lines need not stay (6.5 TB/s for 5.9)
-    constexpr bool ONCE = STAGES == 3;
     const uint32_t full = a.width / K;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&slots[0][wave * 1024]);
     auto load = [&](uint32_t i, uint32_t k, uint32_t lds) {
@@ -266,7 +279,7 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
       products(slots[slot], [&](int g) {
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i)
-          if (i * VF / LOADS == (uint32_t)g) load(i, k + STAGES - 1, lds);
+          if (i * (GROUPS / 2) / LOADS == (uint32_t)g) load(i, k + STAGES - 1, lds);
       });
       slot = next_slot(slot);
       fill = next_slot(fill);
@@ -274,12 +287,12 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
     for (; k < slabs; ++k) {
       arrive<(STAGES - 2) * LOADS>();
       // with three stages, slabs past the last one are loaded too (zeros), so that the wait is one number
-      if (STAGES == 3 || k + 1 < slabs) load_end(k + STAGES - 1, lds0 + fill * ROWS * 128);
+      if (STAGES > 2 || k + 1 < slabs) load_end(k + STAGES - 1, lds0 + fill * ROWS * 128);
       products(slots[slot], [](int) {});
       slot = next_slot(slot);
       fill = next_slot(fill);
     }
-    if (STAGES == 3) arrive<0>();  // a workgroup must not end, and give its LDS away, with loads to it on their way
+    if (STAGES > 2) arrive<0>();  // a workgroup must not end, and give its LDS away, with loads to it on their way
   } else {
     u32x4 held[LOADS];  // a slab on its way
     auto fetch = [&](uint32_t k) {
@@ -307,11 +320,11 @@ __global__ __launch_bounds__(64 * WT * WV) void head_tile_kernel(HeadRows a, Wor
   }
 #pragma unroll
   for (int i = 0; i < TF; ++i) {
-    const uint32_t r = wt * 16 * TF + 16 * i + (lane & 15), at = mt * MT + r;
+    const uint32_t r = (wt * TF + i) * M + lane % M, at = mt * MT + r;
     const bool live = at < count;
     const int64_t tok = a.tokens[row_of(at)];
-    const SoftStats st = lane_stats(acc[i], vt * NT + wv * 16 * VF, a.vocab, tok, live, w.token_logit + at);
-    if (lane < 16) sh[wv][r] = st;
+    const SoftStats st = lane_stats<M>(acc[i], vt * NT + wv * M * VF, a.vocab, tok, live, w.token_logit + at);
+    if (lane < M) sh[wv][r] = st;
   }
   __syncthreads();
   for (uint32_t r = threadIdx.x; r < MT; r += 64 * WAVES) {
@@ -367,11 +380,11 @@ Plan plan_of(int dtype, uint32_t nrows) {
   return Plan{nrows <= 128 ? 128u : 256u, 256};
 }
 
-template <class T, int TF, int VF, int WT, int WV, int STAGES>
+template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE>
 void tile(const HeadRows& a, const Work& w, uint32_t tiles, bool direct, hipStream_t st) {
-  const uint32_t grid = (tiles + 7) / 8 * 8 * ((a.nrows + 16 * TF * WT - 1) / (16 * TF * WT));
-  if (direct) head_tile_kernel<T, TF, VF, WT, WV, STAGES, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
-  else head_tile_kernel<T, TF, VF, WT, WV, 2, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
+  const uint32_t grid = (tiles + 7) / 8 * 8 * ((a.nrows + M * TF * WT - 1) / (M * TF * WT));
+  if (direct) head_tile_kernel<T, M, TF, VF, WT, WV, STAGES, ONCE, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
+  else head_tile_kernel<T, M, TF, VF, WT, WV, 2, false, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
 }
 template <class T>
 void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, hipStream_t st) {
@@ -379,11 +392,11 @@ void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, h
   const uint64_t es = sizeof(typename T::Elem);
   const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0 &&
                       (uint64_t)a.hidden_stride * es * a.nrows < (1ull << 32) && (uint64_t)a.weight_stride * es * p.head_tile < (1ull << 32);
-  if (p.row_tile == 32) return tile<T, 2, 2, 1, 4, 3>(a, w, tiles, direct, st);
-  if (a.nrows <= 64) return tile<T, 4, 2, 1, 4, 3>(a, w, tiles, direct, st);
-  if constexpr (sizeof(typename T::Elem) == 4) return tile<T, 2, 4, 2, 2, 2>(a, w, tiles, direct, st);
-  else if (p.row_tile == 128) return tile<T, 4, 8, 2, 2, 3>(a, w, tiles, direct, st);
-  else return tile<T, 4, 8, 4, 2, 2>(a, w, tiles, direct, st);
+  if (p.row_tile == 32) return tile<T, 16, 2, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
+  if (a.nrows <= 64) return tile<T, 16, 4, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
+  if constexpr (sizeof(typename T::Elem) == 4) return tile<T, 16, 2, 4, 2, 2, 2, false>(a, w, tiles, direct, st);
+  else if (p.row_tile == 128) return tile<T, 32, 2, 4, 2, 2, 3, true>(a, w, tiles, direct, st);
+  else return tile<T, 16, 4, 8, 4, 2, 2, false>(a, w, tiles, direct, st);
 }
 
 }  // namespace
