@@ -99,45 +99,67 @@ __device__ __forceinline__ typename T::V load16(const typename T::Elem* row, uin
   return v;
 }
 
-// A token's logits over a lane's head rows (those of VF products) to their statistics over the 64 / M
-// lanes that hold the token's. v0: the first head row of the wave. Leaves the token's own logit.
-template <int M, int VF>
-__device__ __forceinline__ SoftStats lane_stats(Acc<M> (&acc)[VF], uint32_t v0, uint32_t vocab, int64_t tok, bool live, float* token_logit) {
+// f over the 64 / M lanes that hold the same token.
+template <int M, class F>
+__device__ __forceinline__ float over_lanes(float x, F f) {
+  if (M == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
+// TF x M tokens' logits over a lane's head rows (those of VF products) to their statistics over the
+// lanes that hold the same token. v0: the first head row of the wave. Leaves the logits of `tok`
+// (2^32 - 1: none).
+template <int M, int TF, int VF>
+__device__ __forceinline__ void lane_stats(Acc<M> (&acc)[TF][VF], uint32_t v0, uint32_t vocab, const uint32_t (&tok)[TF],
+                                           float* const (&token_logit)[TF], SoftStats (&st)[TF]) {
   const uint32_t lane = threadIdx.x & 63, first = v0 + 4 * (lane / M);
   auto row = [](int i, int j) { return (uint32_t)(i * M + j / 4 * (256 / M) + j % 4); };
   constexpr int N = M * M / 64;
   if (v0 + M * VF > vocab) {  // head rows past the last one take no part
 #pragma unroll
+    for (int n = 0; n < TF; ++n)
+#pragma unroll
+      for (int i = 0; i < VF; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (first + row(i, j) >= vocab) acc[n][i][j] = -INFINITY;
+  }
+#pragma unroll
+  for (int n = 0; n < TF; ++n) {
+    const uint32_t rel = tok[n] - first;
+    if (__any(rel < M * VF)) {
+      float x = 0.f;
+      bool mine = false;
+#pragma unroll
+      for (int i = 0; i < VF; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (rel == row(i, j)) {
+            x = acc[n][i][j];
+            mine = true;
+          }
+      if (mine) *token_logit[n] = x;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < TF; ++n) {
+    float m = -INFINITY;
+#pragma unroll
     for (int i = 0; i < VF; ++i)
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (first + row(i, j) >= vocab) acc[i][j] = -INFINITY;
+      for (int j = 0; j < N; ++j) m = fmaxf(m, acc[n][i][j]);
+    st[n] = SoftStats::of(over_lanes<M>(m, [](float a, float b) { return fmaxf(a, b); }));
   }
-  const uint64_t rel = (uint64_t)(tok - (int64_t)first);
-  if (__any(live && rel < M * VF)) {
 #pragma unroll
-    for (int i = 0; i < VF; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (rel == (uint64_t)row(i, j) && live && first + row(i, j) < vocab) *token_logit = acc[i][j];
+  for (int n = 0; n < TF; ++n) {
+    st[n].template add<true, VF * N>([&](int i) { return acc[n][i / N][i % N]; }, kLog2e);
+    st[n].s = over_lanes<M>(st[n].s, [](float a, float b) { return a + b; });
+    st[n].t = over_lanes<M>(st[n].t, [](float a, float b) { return a + b; });
   }
-  SoftStats st = SoftStats::of(-INFINITY);
-#pragma unroll
-  for (int i = 0; i < VF; ++i)
-#pragma unroll
-    for (int j = 0; j < N; ++j) st.m = fmaxf(st.m, acc[i][j]);
-#pragma unroll
-  for (int i = 0; i < VF; ++i)
-#pragma unroll
-    for (int j = 0; j < N; ++j) st.add(acc[i][j], kLog2e);
-  for (int off = M; off <= 32; off *= 2) {
-    SoftStats o;
-    o.m = __shfl_xor(st.m, off, 64);
-    o.s = __shfl_xor(st.s, off, 64);
-    o.t = __shfl_xor(st.t, off, 64);
-    st.join(o, kLog2e);
-  }
-  return st;
 }
 
 // A workgroup of WT x WV waves takes 16 TF WT live rows by 16 VF WV head rows, in slabs of 128
@@ -171,8 +193,16 @@ __device__ __forceinline__ void arrive() {
   asm volatile("" ::: "memory");
 }
 
+// Every wave of the workgroup is here, and what it wrote to LDS is; loads on their way stay there.
+__device__ __forceinline__ void arrive_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE, bool DIRECT>
-__global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
+__global__ __launch_bounds__(64 * WT * WV, M == 32 ? 1 : 2) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
   using Elem = typename T::Elem;
   using V = typename T::V;
   constexpr uint32_t E = T::kPer16, K = 8 * E, WAVES = WT * WV;
@@ -183,9 +213,13 @@ __global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, 
   __shared__ SoftStats sh[WV][MT];
   const uint32_t count = w.count ? *w.count : a.nrows, mtiles = (count + MT - 1) / MT;
   // Workgroups go to the 8 XCDs in turn: an XCD takes every eighth of the head's tiles, and all
-  // live rows of one after another, so that its L2 holds the tile's slabs for them.
-  const uint32_t vt = blockIdx.x / 8 / (mtiles ? mtiles : 1) * 8 + blockIdx.x % 8, mt = mtiles ? blockIdx.x / 8 % mtiles : 0;
-  if (vt >= tiles || !mtiles) return;
+  // live rows of one after another, so that its L2 holds the tile's slabs for them. A workgroup takes
+  // every gridDim / 8-th of its XCD's list.
+  const uint32_t xcd = blockIdx.x % 8, stride = gridDim.x / 8;
+  auto head_tile = [&](uint32_t n) { return n / mtiles * 8 + xcd; };
+  auto there = [&](uint32_t n) { return head_tile(n) < tiles; };
+  uint32_t tile = blockIdx.x / 8;
+  if (!mtiles || !there(tile)) return;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = wave % WT, wv = wave / WT;
   auto row_of = [&](uint32_t at) {
     if (at >= count) at = count - 1;
@@ -193,30 +227,36 @@ __global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, 
   };
 
   // A load takes 8 rows of hidden states or of the head; this lane's row of load i, at its chunk.
-  const char* const hidden0 = (const char*)a.hidden;
-  const char* const weight0 = (const char*)a.weight + (int64_t)vt * NT * a.weight_stride * sizeof(Elem);
+  constexpr uint32_t HLOADS = MT / 8 / WAVES;
   static_assert(MT % (8 * WAVES) == 0, "a wave's load i is of the same kind for all waves");
-  auto of_hidden = [](uint32_t i) { return i < MT / 8 / WAVES; };
   static_assert(WAVES % 2 == 0, "a lane's chunk is the same for all of its loads");
-  const uint32_t chunk = (lane & 7) ^ swizzle(wave * 8 + (lane >> 3));
+  const uint32_t chunk = (lane & 7) ^ swizzle(wave * 8 + (lane >> 3)), lane_row = wave * 8 + (lane >> 3);
   using Offset = std::conditional_t<DIRECT, uint32_t, uint64_t>;  // bytes; the launch looks after the 32 bits
+  const char* const hidden0 = (const char*)a.hidden;
+  const char* weight0;  // of the tile that is being loaded
   Offset from[LOADS];
+  uint32_t rows[HLOADS];
+  auto take_rows = [&](uint32_t n) {  // the rows of a tile, ahead of its loads
 #pragma unroll
-  for (uint32_t i = 0; i < LOADS; ++i) {
-    const uint32_t r = (wave + i * WAVES) * 8 + (lane >> 3);
-    if (of_hidden(i)) {
-      from[i] = (Offset)((uint64_t)row_of(mt * MT + r) * a.hidden_stride * sizeof(Elem)) + chunk * 16;
-    } else {
-      const uint32_t v = r - MT;
-      from[i] = (Offset)((uint64_t)(vt * NT + v < a.vocab ? v : a.vocab - 1 - vt * NT) * a.weight_stride * sizeof(Elem)) + chunk * 16;
+    for (uint32_t i = 0; i < HLOADS; ++i) rows[i] = row_of(n % mtiles * MT + i * WAVES * 8 + lane_row);
+  };
+  auto take_tile = [&](uint32_t n) {
+    const uint32_t v0 = head_tile(n) * NT;
+    weight0 = (const char*)a.weight + (int64_t)v0 * a.weight_stride * sizeof(Elem);
+#pragma unroll
+    for (uint32_t i = 0; i < LOADS; ++i) {
+      const uint32_t v = (i - HLOADS) * WAVES * 8 + lane_row;
+      const uint64_t at = i < HLOADS ? (uint64_t)rows[i < HLOADS ? i : 0] * a.hidden_stride : (uint64_t)(v0 + v < a.vocab ? v : a.vocab - 1 - v0) * a.weight_stride;
+      from[i] = (Offset)(at * sizeof(Elem)) + chunk * 16;
     }
-  }
+  };
   Acc<M> acc[TF][VF];
+  auto clear = [&]() {
 #pragma unroll
-  for (int i = 0; i < TF; ++i)
+    for (int i = 0; i < TF; ++i)
 #pragma unroll
-    for (int j = 0; j < VF; ++j) acc[i][j] = Acc<M>(0.f);
-
+      for (int j = 0; j < VF; ++j) acc[i][j] = Acc<M>(0.f);
+  };
   // Products of the slab in `here`, in groups of TF; `between` runs after each of the first half of the
   // groups. A group's operands are read while the two before it run.
   constexpr int PARTS = 8 * M / 64, GROUPS = PARTS * VF;
@@ -245,52 +285,96 @@ __global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, 
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // The tokens of a tile's rows, loaded when its products begin.
+  uint32_t tok[TF];
+  auto take_tokens = [&](uint32_t n) {
+#pragma unroll
+    for (int i = 0; i < TF; ++i) {
+      const uint32_t at = n % mtiles * MT + (wt * TF + i) * M + lane % M;
+      const int64_t t = at < count ? a.tokens[row_of(at)] : -1;
+      tok[i] = t >= 0 && t < (int64_t)a.vocab ? (uint32_t)t : ~0u;
+    }
+  };
+  // The statistics of the tile whose logits are there.
+  auto finish = [&](uint32_t n) {
+    const uint32_t vt = head_tile(n), mt = n % mtiles;
+    float* token_logit[TF];
+    SoftStats st[TF];
+#pragma unroll
+    for (int i = 0; i < TF; ++i) token_logit[i] = w.token_logit + mt * MT + (wt * TF + i) * M + lane % M;
+    lane_stats<M>(acc, vt * NT + wv * M * VF, a.vocab, tok, token_logit, st);
+    if (lane < M)
+#pragma unroll
+      for (int i = 0; i < TF; ++i) sh[wv][(wt * TF + i) * M + lane] = st[i];
+    arrive_lds();
+    for (uint32_t r = threadIdx.x; r < MT; r += 64 * WAVES) {
+      const uint32_t at = mt * MT + r;
+      if (at >= count) break;
+      SoftStats st = sh[0][r];
+      for (int i = 1; i < WV; ++i) st.join(sh[i][r], kLog2e);
+      w.partial[(uint64_t)at * tiles + vt] = float4{st.m, st.s, st.t, 0.f};
+    }
+  };
+
   const uint32_t slabs = (a.width + K - 1) / K;
   if constexpr (DIRECT) {
+    // The slabs of all tiles follow each other without a stop: the first ones of a tile are on their way
+    // while the last products of the tile before it run, and its statistics.
     const uint32_t full = a.width / K;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&slots[0][wave * 1024]);
-    auto load = [&](uint32_t i, uint32_t k, uint32_t lds) {
-      if (of_hidden(i)) to_lds<false>(hidden0 + (uint64_t)k * 128, from[i], lds + i * WAVES * 1024);
-      else to_lds<ONCE>(weight0 + (uint64_t)k * 128, from[i], lds + i * WAVES * 1024);
+    auto next_slot = [](uint32_t s) { return s + 1 == STAGES ? 0 : s + 1; };
+    uint32_t load_tile = tile, load_k = 0, fill = 0;  // the next slab to load, and its place
+    bool loading = true;
+    auto load = [&](uint32_t i, uint32_t lds) {
+      if (i < HLOADS) to_lds<false>(hidden0 + (uint64_t)load_k * 128, from[i], lds + i * WAVES * 1024);
+      else to_lds<ONCE>(weight0 + (uint64_t)load_k * 128, from[i], lds + i * WAVES * 1024);
     };
     // a slab of which the last columns, or all, lie past the width
-    auto load_end = [&](uint32_t k, uint32_t lds) {
+    auto load_end = [&](uint32_t lds) {
 #pragma unroll
       for (uint32_t i = 0; i < LOADS; ++i) {
-        const char* p = (of_hidden(i) ? hidden0 : weight0) + from[i] + (uint64_t)k * 128;
-        if (k * K + chunk * E >= a.width) p = (const char*)zeros16;
+        const char* p = (i < HLOADS ? hidden0 : weight0) + from[i] + (uint64_t)load_k * 128;
+        if (!loading || load_k * K + chunk * E >= a.width) p = (const char*)zeros16;
         to_lds(p, lds + i * WAVES * 1024);
       }
     };
-    auto next_slot = [](uint32_t s) { return s + 1 == STAGES ? 0 : s + 1; };
-#pragma unroll
-    for (uint32_t k = 0; k < STAGES - 1; ++k) {
-      if (k < full) {
-#pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) load(i, k, lds0 + k * ROWS * 128);
-      } else {
-        load_end(k, lds0 + k * ROWS * 128);
+    auto loaded = [&]() {
+      fill = next_slot(fill);
+      if (++load_k < slabs || !loading) return;
+      load_k = 0;
+      load_tile += stride;
+      loading = there(load_tile);
+      if (loading) {
+        take_tile(load_tile);
+        take_rows(load_tile + stride);
       }
+    };
+    take_rows(tile);
+    take_tile(tile);
+    take_rows(tile + stride);
+    for (uint32_t k = 0; k < STAGES - 1; ++k) {
+      load_end(lds0 + fill * ROWS * 128);
+      loaded();
     }
-    uint32_t slot = 0, fill = STAGES - 1, k = 0;
-    for (; k + STAGES - 1 < full; ++k) {
-      arrive<(STAGES - 2) * LOADS>();  // slab k is there, and the products of slab k - 1, whose place the next one takes, are done
-      const uint32_t lds = lds0 + fill * ROWS * 128;
-      products(slots[slot], [&](int g) {
+    uint32_t slot = 0;
+    for (; there(tile); tile += stride) {
+      clear();
+      take_tokens(tile);
+      for (uint32_t k = 0; k < slabs; ++k) {
+        arrive<(STAGES - 2) * LOADS>();  // slab k is there, and the products of slab k - 1, whose place the next one takes, are done
+        const uint32_t lds = lds0 + fill * ROWS * 128;
+        const bool whole = loading && load_k < full;
+        // with more than two stages, slabs past the last one are loaded too (zeros), so that the wait is one number
+        if (!whole && (STAGES > 2 || loading)) load_end(lds);
+        products(slots[slot], [&](int g) {
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i)
-          if (i * (GROUPS / 2) / LOADS == (uint32_t)g) load(i, k + STAGES - 1, lds);
-      });
-      slot = next_slot(slot);
-      fill = next_slot(fill);
-    }
-    for (; k < slabs; ++k) {
-      arrive<(STAGES - 2) * LOADS>();
-      // with three stages, slabs past the last one are loaded too (zeros), so that the wait is one number
-      if (STAGES > 2 || k + 1 < slabs) load_end(k + STAGES - 1, lds0 + fill * ROWS * 128);
-      products(slots[slot], [](int) {});
-      slot = next_slot(slot);
-      fill = next_slot(fill);
+          for (uint32_t i = 0; i < LOADS; ++i)
+            if (i * (GROUPS / 2) / LOADS == (uint32_t)g && whole) load(i, lds);
+        });
+        loaded();
+        slot = next_slot(slot);
+      }
+      finish(tile);
     }
     if (STAGES > 2) arrive<0>();  // a workgroup must not end, and give its LDS away, with loads to it on their way
   } else {
@@ -299,7 +383,7 @@ __global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, 
       const bool tail = (k + 1) * K > a.width;
 #pragma unroll
       for (uint32_t i = 0; i < LOADS; ++i) {
-        const Elem* p = (const Elem*)((of_hidden(i) ? hidden0 : weight0) + from[i] + (uint64_t)k * 128);
+        const Elem* p = (const Elem*)((i < HLOADS ? hidden0 : weight0) + from[i] + (uint64_t)k * 128);
         const uint32_t at = k * K + chunk * E;
         const V x = tail ? load16<T>(p, 0, at < a.width ? a.width - at : 0) : (V)*(const typename Frag<T>::Loose*)p;
         held[i] = __builtin_bit_cast(u32x4, x);
@@ -309,30 +393,21 @@ __global__ __launch_bounds__(64 * WT * WV, 2) void head_tile_kernel(HeadRows a, 
 #pragma unroll
       for (uint32_t i = 0; i < LOADS; ++i) *(u32x4*)(there + (wave + i * WAVES) * 1024 + lane * 16) = held[i];
     };
-    fetch(0);
-    put(slots[0]);
-    for (uint32_t k = 0; k < slabs; ++k) {
-      __syncthreads();  // slab k is there; the products of slab k - 1 are done
-      if (k + 1 < slabs) fetch(k + 1);
-      products(slots[k & 1], [](int) {});
-      if (k + 1 < slabs) put(slots[~k & 1]);
+    for (; there(tile); tile += stride) {
+      clear();
+      take_tokens(tile);
+      take_rows(tile);
+      take_tile(tile);
+      fetch(0);
+      put(slots[0]);
+      for (uint32_t k = 0; k < slabs; ++k) {
+        __syncthreads();  // slab k is there; the products of slab k - 1 are done
+        if (k + 1 < slabs) fetch(k + 1);
+        products(slots[k & 1], [](int) {});
+        if (k + 1 < slabs) put(slots[~k & 1]);
+      }
+      finish(tile);
     }
-  }
-#pragma unroll
-  for (int i = 0; i < TF; ++i) {
-    const uint32_t r = (wt * TF + i) * M + lane % M, at = mt * MT + r;
-    const bool live = at < count;
-    const int64_t tok = a.tokens[row_of(at)];
-    const SoftStats st = lane_stats<M>(acc[i], vt * NT + wv * M * VF, a.vocab, tok, live, w.token_logit + at);
-    if (lane < M) sh[wv][r] = st;
-  }
-  __syncthreads();
-  for (uint32_t r = threadIdx.x; r < MT; r += 64 * WAVES) {
-    const uint32_t at = mt * MT + r;
-    if (at >= count) break;
-    SoftStats st = sh[0][r];
-    for (int i = 1; i < WV; ++i) st.join(sh[i][r], kLog2e);
-    w.partial[(uint64_t)at * tiles + vt] = float4{st.m, st.s, st.t, 0.f};
   }
 }
 
@@ -364,7 +439,7 @@ __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint3
   if (lane == 0) {
     const bool valid = st.valid(), inside = tok >= 0 && tok < (int64_t)a.vocab;
     const float log2s = log2_hw(st.s);
-    a.logprobs[r] = valid && inside ? st.lnq(w.token_logit[at], 1.f) : NAN;
+    a.logprobs[r] = valid && inside ? st.lnq(w.token_logit[at], kLog2e, 1.f) : NAN;
     a.entropy[r] = valid ? kLn2 * (log2s - st.t / st.s) : NAN;
   }
 }
@@ -382,7 +457,10 @@ Plan plan_of(int dtype, uint32_t nrows) {
 
 template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE>
 void tile(const HeadRows& a, const Work& w, uint32_t tiles, bool direct, hipStream_t st) {
-  const uint32_t grid = (tiles + 7) / 8 * 8 * ((a.nrows + M * TF * WT - 1) / (M * TF * WT));
+  const uint32_t all = (tiles + 7) / 8 * 8 * ((a.nrows + M * TF * WT - 1) / (M * TF * WT));
+  constexpr uint32_t kLds = STAGES * (M * TF * WT + M * VF * WV) * 128 + WV * M * TF * WT * sizeof(SoftStats);
+  constexpr uint32_t resident = 256 * (160 * 1024 / kLds < 8 / (WT * WV) ? 160 * 1024 / kLds : 8 / (WT * WV));  // two waves a SIMD
+  const uint32_t grid = all < resident ? all : resident;
   if (direct) head_tile_kernel<T, M, TF, VF, WT, WV, STAGES, ONCE, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
   else head_tile_kernel<T, M, TF, VF, WT, WV, 2, false, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
 }

@@ -49,8 +49,8 @@ struct Add {
   __device__ float operator()(float a, float b) const { return a + b; }
 };
 
-template <int THREADS, bool ENTROPY>
-__device__ __forceinline__ SoftStats block_stats(SoftStats st, float c, SoftStats* waves) {
+template <int THREADS, bool ENTROPY, bool FAR>
+__device__ __forceinline__ Stats<FAR> block_stats(Stats<FAR> st, float c, Stats<FAR>* waves) {
   constexpr uint32_t W = THREADS / 64;
   const uint32_t lane = threadIdx.x & 63;
   st.rebase(reduce64(st.m, Max()), c);
@@ -59,7 +59,7 @@ __device__ __forceinline__ SoftStats block_stats(SoftStats st, float c, SoftStat
   if (lane == 0) waves[threadIdx.x >> 6] = st;
   __syncthreads();
   st = waves[lane < W ? lane : 0];
-  if (lane >= W) st = SoftStats::of(-INFINITY);
+  if (lane >= W) st = Stats<FAR>::of(-INFINITY);
   st.rebase(reduce16(st.m, Max()), c);  // W <= 16: lanes 0 .. 15 hold them all
   st.s = reduce16(st.s, Add());
   if (ENTROPY) st.t = reduce16(st.t, Add());
@@ -142,19 +142,16 @@ struct Held {
       for (int k = 0; k < T::kPer16; ++k) m = fmaxf(m, element<T>(raw[i], k));
     return m;
   }
-  template <bool ENTROPY>
-  __device__ __forceinline__ void add_to(SoftStats& st, float c) const {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < T::kPer16; ++k) st.add<ENTROPY>(element<T>(raw[i], k), c);
+  template <bool ENTROPY, bool FAR>
+  __device__ __forceinline__ void add_to(Stats<FAR>& st, float c) const {
+    st.template add<ENTROPY, NV * T::kPer16>([&](int i) { return element<T>(raw[i / T::kPer16], i % T::kPer16); }, c);
   }
 };
 
 // A row's softmax statistics. Leaves the row in `h` where it fits.
-template <class T, int THREADS, int NV, bool ENTROPY>
-__device__ __forceinline__ SoftStats row_stats(const Span<T>& s, Held<T, THREADS, NV>& h, float c, SoftStats* waves) {
-  SoftStats st = SoftStats::of(-INFINITY);
+template <class T, int THREADS, int NV, bool ENTROPY, bool FAR>
+__device__ __forceinline__ Stats<FAR> row_stats(const Span<T>& s, Held<T, THREADS, NV>& h, float c, Stats<FAR>* waves) {
+  auto st = Stats<FAR>::of(-INFINITY);
   for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
     h.load(s, j0);
     st.rebase(fmaxf(st.m, h.largest()), c);
@@ -334,7 +331,7 @@ __device__ __forceinline__ void alternatives(const Span<T>& s, Held<T, THREADS, 
 template <class T, int THREADS, int NV, bool TOP, bool GRAD>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
   using Elem = typename T::Elem;
-  __shared__ SoftStats waves[THREADS / 64];
+  __shared__ Stats<GRAD> waves[THREADS / 64];
   const uint32_t r = blockIdx.x, b = r / a.length, l = r % a.length, tid = threadIdx.x;
   const Elem* x = (const Elem*)a.logits + b * a.logits_s.batch + l * a.logits_s.row;
   Elem* g = GRAD ? (Elem*)a.grad + b * a.grad_s.batch + l * a.grad_s.row : nullptr;
@@ -355,12 +352,12 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
   const float xt = inside ? (float)x[tok] : 0.f;
   const Span<T> s(x, a.vocab);
   Held<T, THREADS, NV> h;
-  const SoftStats st = row_stats<T, THREADS, NV, true>(s, h, kLog2e, waves);
+  const Stats<GRAD> st = row_stats<T, THREADS, NV, true>(s, h, kLog2e, waves);
   const bool valid = st.valid();
   const float log2s = log2_hw(st.s);
   const float entropy = valid ? kLn2 * (log2s - st.t / st.s) : NAN;
   if (tid == 0) {
-    a.logprobs[r] = valid && inside ? st.lnq(xt, 1.f) : NAN;
+    a.logprobs[r] = valid && inside ? st.lnq(xt, kLog2e, 1.f) : NAN;
     a.entropy[r] = entropy;
   }
   if constexpr (TOP) {
@@ -375,7 +372,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
       return;
     }
     alternatives<T, THREADS, NV>(s, h, (uint32_t)a.top, sh, [&](uint32_t rank, uint64_t key) {
-      lp[rank] = st.lnq(key_value(key), 1.f);
+      lp[rank] = st.lnq(key_value(key), kLog2e, 1.f);
       at[rank] = (int64_t)(uint32_t)~(uint32_t)key;
     });
   }
@@ -406,7 +403,7 @@ struct TeacherShared {
 template <class T, int THREADS, int NV, bool GRAD>
 __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
   using Elem = typename T::Elem;
-  __shared__ SoftStats waves[THREADS / 64];
+  __shared__ Stats<GRAD> waves[THREADS / 64];
   __shared__ TeacherShared sh;
   const uint32_t r = blockIdx.x, b = r / a.length, l = r % a.length, tid = threadIdx.x, lane = tid & 63, k = (uint32_t)a.k;
   const Elem* x = (const Elem*)a.logits + b * a.logits_s.batch + l * a.logits_s.row;
@@ -449,14 +446,14 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
   }
   const Span<T> s(x, a.vocab);
   Held<T, THREADS, NV> h;
-  const SoftStats st = row_stats<T, THREADS, NV, false>(s, h, c, waves);
+  const Stats<GRAD> st = row_stats<T, THREADS, NV, false>(s, h, c, waves);
   const float log2s = log2_hw(st.s);
   if (tid < 64) {
     float loss = 0.f, total = 0.f;
     for (uint32_t j = lane; j < k; j += 64) {
       const float lnw = (sh.w[j] - tm) - lse;
       const float w = sh.idx[j] >= 0 ? exp2_hw(lnw * kLog2e) : 0.f;
-      if (w > 0.f) loss += w * (lnw - st.lnq((float)x[sh.idx[j]], inv));
+      if (w > 0.f) loss += w * (lnw - st.lnq((float)x[sh.idx[j]], c, inv));
       sh.w[j] = w;
       total += w;
     }

@@ -36,41 +36,74 @@ struct TypeBF16 {
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
 
-// Statistics of logits x: their maximum m, s = sum 2^y and t = sum 2^y y with
-// y = (x - m) c (c = log2 e / temperature). Then log softmax(x) = (x - m) / temperature -
-// ln 2 log2 s and the entropy is ln 2 (log2 s - t / s): both of its terms are of one sign.
-struct SoftStats {
+// Statistics of logits x: their maximum m, s = sum 2^y and t = sum 2^y y with y = x c - K,
+// c = log2 e / temperature. K is m c rounded to fp32: what its rounding leaves shifts every y alike,
+// so that log softmax(x) = ln 2 (y - log2 s) and the entropy ln 2 (log2 s - t / s), of which both terms
+// are of one sign, do not see it, and y is one fused multiply-add. Where m c leaves the range of
+// fp32 (logits at the type's limits), and where no logit is above -inf, y = (x - m) c instead; FAR
+// takes that everywhere: y is 0 for the largest logit, and so are the gradients of a row that
+// is certain.
+template <bool FAR>
+struct Stats {
   float m, s, t;
 
-  __device__ static SoftStats of(float m) { return SoftStats{m, 0.f, 0.f}; }
+  __device__ static Stats of(float m) { return Stats{m, 0.f, 0.f}; }
 
-  // y of one logit; no logits above -inf: y of any is taken against 0, so that 2^y is 0
-  __device__ float y_of(float x, float c) const { return (x - (m == -INFINITY ? 0.f : m)) * c; }
+  __device__ static bool in_range(float k) { return !FAR && fabsf(k) < 1e37f; }
+  __device__ bool plain(float c) const { return in_range(m * c); }
+  __device__ float y_plain(float x, float c) const { return __builtin_fmaf(x, c, -(m * c)); }
+  // no logits above -inf: y of any is taken against 0, so that 2^y is 0
+  __device__ float y_far(float x, float c) const { return (x - (m == -INFINITY ? 0.f : m)) * c; }
+  __device__ float y_of(float x, float c) const { return plain(c) ? y_plain(x, c) : y_far(x, c); }
 
-  // log softmax of one logit, with `inv` the inverse of the temperature. Not from y:
-  // a logit near the type's lowest value has a y past the range of fp32.
-  __device__ float lnq(float x, float inv) const { return __builtin_fmaf(-kLn2, log2_hw(s), (x - m) * inv); }
-
-  // 2^y y is 0 where y is -inf; a NaN logit leaves a NaN in s
-  template <bool ENTROPY = true>
-  __device__ void add(float x, float c) {
+  // log softmax of one logit, with `inv` the inverse of the temperature. A logit near the
+  // type's lowest value has a y past the range of fp32.
+  __device__ float lnq(float x, float c, float inv) const {
     const float y = y_of(x, c);
-    const float e = exp2_hw(y);
-    s += e;
-    if (ENTROPY) t = __builtin_fmaf(e, fmaxf(y, -1e30f), t);
+    return y == -INFINITY ? __builtin_fmaf(-kLn2, log2_hw(s), (x - m) * inv) : kLn2 * (y - log2_hw(s));
+  }
+
+  // Adds x(0) .. x(N - 1). 2^y y is 0 where y is -inf: such a y makes t a NaN, and t is then taken
+  // again with care. (A NaN logit leaves a NaN in s.)
+  template <bool ENTROPY, int N, class F>
+  __device__ __forceinline__ void add(F x, float c) {
+    const float t0 = t;
+    if (plain(c)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = y_plain(x(i), c);
+        const float e = exp2_hw(y);
+        s += e;
+        if (ENTROPY) t = __builtin_fmaf(e, y, t);
+      }
+      if (!ENTROPY || t == t) return;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s += exp2_hw(y_far(x(i), c));
+    }
+    if (ENTROPY) {
+      t = t0;
+      asm("" : "+v"(c));  // or the compiler keeps all of the first pass's values for this one
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = y_of(x(i), c);
+        t = __builtin_fmaf(exp2_hw(y), fmaxf(y, -1e30f), t);
+      }
+    }
   }
 
   // The same statistics against another maximum, m2 >= m.
   __device__ void rebase(float m2, float c) {
     if (s != 0.f) {  // a NaN passes
-      const float d = (m - m2) * c;
+      const float k = m * c, k2 = m2 * c;
+      const float d = in_range(k) && in_range(k2) ? k - k2 : (m - m2) * c;
       const float f = exp2_hw(d);
       t = f * __builtin_fmaf(fmaxf(d, -1e30f), s, t);
       s *= f;
     }
     m = m2;
   }
-  __device__ void join(SoftStats o, float c) {
+  __device__ void join(Stats o, float c) {
     const float m2 = fmaxf(m, o.m);
     rebase(m2, c);
     o.rebase(m2, c);
@@ -80,5 +113,6 @@ struct SoftStats {
   // A distribution: at least one finite logit, and no NaN or +inf.
   __device__ bool valid() const { return s == s && fabsf(m) != INFINITY; }
 };
+using SoftStats = Stats<false>;
 
 }  // namespace dz
