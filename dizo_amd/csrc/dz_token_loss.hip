@@ -3,15 +3,15 @@
 // largest logits, and their gradients.
 //
 // One workgroup takes one row. What bounds these kernels is reading the row
-// once (and writing its gradient once), so a row that fits is held in the
-// workgroup's registers as it was read, in 16-byte vectors: the statistics, the
-// alternatives and the gradient are all taken from there. A longer row goes by
-// in chunks of as much, and is read again for the later passes. A thread's
-// vectors lie THREADS apart, so that a wave's loads cover consecutive bytes.
+// once (and writing its gradient once). Where only sums are asked for, the row
+// streams by (stream_stats). The alternatives and the gradient need the row a second
+// time: a row that fits is held in the workgroup's registers as it was read, in
+// 16-byte vectors; a longer one goes by in chunks of as much, and is read again. A
+// thread's vectors lie THREADS apart, so that a wave's loads cover consecutive bytes.
 //
-// Rows start where they start (an odd vocabulary, a view): vectors are taken at
-// the 16-byte boundaries of memory, and the row's first and last one, where they
-// are not whole, element by element, so that nothing outside the row is read.
+// Rows start where they start (an odd vocabulary, a view), and so do their vectors:
+// loads and stores of 16 bytes at the element's alignment. The last vector, where it is
+// not whole, is the row's last 16 bytes, and what it repeats is taken out.
 #include "dz_token_loss.h"
 #include "dz_token_math.h"
 
@@ -70,37 +70,19 @@ __device__ __forceinline__ Stats<FAR> block_stats(Stats<FAR> st, float c, Stats<
 }
 
 // --------------------------------------------------------------- the row --
-// The 16-byte vectors that v elements at p lie in.
 template <class T>
-struct Span {
-  using Elem = typename T::Elem;
-  static constexpr uint32_t E = T::kPer16;
-  uint64_t base;      // of vector 0
-  uint32_t lead;      // elements of vector 0 before the row
-  uint32_t v;
-  uint32_t nvec;      // vectors
-  uint32_t end_full;  // vector end_full is the last one where it is not whole
-
-  __device__ Span(const void* p, uint32_t n) {
-    const uint64_t a = (uint64_t)p;
-    base = a & ~(uint64_t)15;
-    lead = (uint32_t)(a & 15) / sizeof(Elem);
-    v = n;
-    end_full = (v + lead) / E;
-    nvec = (v + lead + E - 1) / E;
-  }
-  __device__ bool whole(uint32_t j) const { return j >= (lead ? 1u : 0u) && j < end_full; }
-  __device__ uint32_t first(uint32_t j) const { return j * E - lead; }  // index of a vector's element 0 (wraps below 0)
-  __device__ const Elem* row() const { return (const Elem*)base + lead; }
-
-  __device__ u32x4 edge(uint32_t j) const {
-    typename T::V x;
-    for (uint32_t k = 0; k < E; ++k) {
-      const uint32_t i = first(j) + k;
-      x[k] = i < v ? row()[i] : (Elem)-INFINITY;
-    }
-    return __builtin_bit_cast(u32x4, x);
-  }
+struct Loose16;
+template <>
+struct Loose16<TypeF32> {
+  typedef f32x4 type __attribute__((aligned(4)));
+};
+template <>
+struct Loose16<TypeF16> {
+  typedef f16x8 type __attribute__((aligned(2)));
+};
+template <>
+struct Loose16<TypeBF16> {
+  typedef bf16x8 type __attribute__((aligned(2)));
 };
 
 template <class T>
@@ -113,63 +95,124 @@ template <class T>
 __device__ __forceinline__ float element(const u32x4& raw, int k) {
   return (float)__builtin_bit_cast(typename T::V, raw)[k];
 }
+// Makes the compiler read `raw` anew, instead of keeping what an earlier pass made of it.
+__device__ __forceinline__ void afresh(u32x4& raw) { asm("" : "+v"(raw)); }
+
+// v elements at p as 16-byte vectors.
+template <class T>
+struct Row {
+  using Elem = typename T::Elem;
+  using Loose = typename Loose16<T>::type;
+  static constexpr uint32_t E = T::kPer16;
+  const Elem* p;
+  uint32_t v, nvec;
+
+  __device__ Row(const Elem* p_, uint32_t v_) : p(p_), v(v_), nvec((v_ + E - 1) / E) {}
+
+  // the element that vector j starts with: the last vector ends with the row
+  __device__ __forceinline__ uint32_t first(uint32_t j) const { return (j + 1) * E <= v ? j * E : v >= E ? v - E : 0; }
+
+  // Vector j, of a wave whose vectors end before j_end (the same for the whole wave).
+  __device__ __forceinline__ u32x4 load(uint32_t j, uint32_t j_end) const {
+    if (j_end * E <= v) return __builtin_bit_cast(u32x4, (typename T::V)*(const Loose*)(p + j * E));
+    typename T::V x = __builtin_bit_cast(typename T::V, none16<T>());
+    if (v >= E) {
+      const uint32_t at = first(j);
+      x = *(const Loose*)(p + at);
+#pragma unroll
+      for (uint32_t k = 0; k < E; ++k)
+        if (at + k < j * E) x[k] = (Elem)-INFINITY;  // the vector before has it, or there is no vector j
+    } else if (j == 0) {
+      for (uint32_t k = 0; k < E; ++k)
+        if (k < v) x[k] = p[k];
+    }
+    return __builtin_bit_cast(u32x4, x);
+  }
+
+  // Writes vector j of `out`, a row of the same length.
+  __device__ __forceinline__ void store(Elem* out, uint32_t j, const typename T::V& x) const {
+    if ((j + 1) * E <= v) {
+      *(Loose*)(out + j * E) = x;
+    } else {
+      const uint32_t at = first(j);
+#pragma unroll
+      for (uint32_t k = 0; k < E; ++k)
+        if (at + k >= j * E && at + k < v) out[at + k] = x[k];
+    }
+  }
+};
 
 // THREADS x NV vectors of a row from vector j0 on, in registers.
 template <class T, int THREADS, int NV>
 struct Held {
+  static constexpr int E = T::kPer16, STEP = NV < 4 ? NV : 4;  // vectors that are added at a time
+  static_assert(NV % STEP == 0, "steps");
   u32x4 raw[NV];
 
   __device__ __forceinline__ static uint32_t index(uint32_t j0, int i) { return j0 + i * THREADS + threadIdx.x; }
 
-  __device__ __forceinline__ void load(const Span<T>& s, uint32_t j0) {
-    const uint32_t tail = s.end_full < s.nvec ? s.end_full : ~0u;
-    u32x4 last = none16<T>();
-    if (tail != ~0u && tail % THREADS == threadIdx.x) last = s.edge(tail);  // j0 is a multiple of THREADS
+  __device__ __forceinline__ void load(const Row<T>& s, uint32_t j0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t j = index(j0, i);
       raw[i] = none16<T>();
-      if (s.whole(j)) raw[i] = *(const u32x4*)(s.base + (uint64_t)j * 16);
-      if (j == tail) raw[i] = last;
+      if (j0 + i * THREADS < s.nvec) raw[i] = s.load(index(j0, i), j0 + (i + 1) * THREADS);
     }
-    if (s.lead && tail != 0 && index(j0, 0) == 0) raw[0] = s.edge(0);
   }
-  __device__ __forceinline__ float largest() const {
-    float m = -INFINITY;
+  __device__ __forceinline__ float largest(int i) const {
+    float m = element<T>(raw[i], 0);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < T::kPer16; ++k) m = fmaxf(m, element<T>(raw[i], k));
+    for (int k = 1; k < E; ++k) m = fmaxf(m, element<T>(raw[i], k));
     return m;
   }
+  // The statistics with these vectors added.
   template <bool ENTROPY, bool FAR>
-  __device__ __forceinline__ void add_to(Stats<FAR>& st, float c) const {
-    st.template add<ENTROPY, NV * T::kPer16>([&](int i) { return element<T>(raw[i / T::kPer16], i % T::kPer16); }, c);
+  __device__ __forceinline__ void add_to(const Row<T>& s, uint32_t j0, Stats<FAR>& st, float c) {
+    float m = st.m;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      m = fmaxf(m, largest(i));
+      afresh(raw[i]);
+    }
+    st.rebase(m, c);
+#pragma unroll
+    for (int i = 0; i < NV; i += STEP)
+      if (j0 + i * THREADS < s.nvec) {
+        st.template add<ENTROPY, STEP * E>([&](int n) { return element<T>(raw[i + n / E], n % E); }, c);
+#pragma unroll
+        for (int n = 0; n < STEP; ++n) afresh(raw[i + n]);
+      }
   }
 };
 
-// A row's softmax statistics. Leaves the row in `h` where it fits.
+// A row's softmax statistics, for the whole workgroup. Leaves the row in `h` where it fits.
 template <class T, int THREADS, int NV, bool ENTROPY, bool FAR>
-__device__ __forceinline__ Stats<FAR> row_stats(const Span<T>& s, Held<T, THREADS, NV>& h, float c, Stats<FAR>* waves) {
+__device__ __forceinline__ Stats<FAR> row_stats(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<FAR>* waves) {
   auto st = Stats<FAR>::of(-INFINITY);
   for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
     h.load(s, j0);
-    st.rebase(fmaxf(st.m, h.largest()), c);
-    h.template add_to<ENTROPY>(st, c);
+    h.template add_to<ENTROPY>(s, j0, st, c);
   }
   return block_stats<THREADS, ENTROPY>(st, c, waves);
 }
 
-// Writes f(logit, index) for the whole row. Vector by vector where the output
-// lies at the input's place within 16 bytes, else element by element.
-template <class T, int THREADS, int NV, class F>
-__device__ __forceinline__ void write_row(const Span<T>& s, Held<T, THREADS, NV>& h, typename T::Elem* out, F f) {
-  const Span<T> o(out, s.v);
-  if (o.lead != s.lead) {
-    const typename T::Elem* x = s.row();
-    for (uint32_t i = threadIdx.x; i < s.v; i += THREADS) out[i] = (typename T::Elem)f((float)x[i], i);
-    return;
+// The same where the row is not needed again: the next NV vectors are on their way while these are added.
+template <class T, int THREADS, int NV, bool ENTROPY>
+__device__ __forceinline__ SoftStats stream_stats(const Row<T>& s, float c, SoftStats* waves) {
+  Held<T, THREADS, NV> a, b;
+  auto st = SoftStats::of(-INFINITY);
+  a.load(s, 0);
+  for (uint32_t j0 = 0; j0 < s.nvec; j0 += 2 * THREADS * NV) {
+    b.load(s, j0 + THREADS * NV);
+    a.template add_to<ENTROPY>(s, j0, st, c);
+    a.load(s, j0 + 2 * THREADS * NV);
+    b.template add_to<ENTROPY>(s, j0 + THREADS * NV, st, c);
   }
+  return block_stats<THREADS, ENTROPY>(st, c, waves);
+}
+
+// Writes f(logit) for the whole row.
+template <class T, int THREADS, int NV, class F>
+__device__ __forceinline__ void write_row(const Row<T>& s, Held<T, THREADS, NV>& h, typename T::Elem* out, F f) {
   for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
     if (s.nvec > THREADS * NV) h.load(s, j0);
 #pragma unroll
@@ -178,14 +221,8 @@ __device__ __forceinline__ void write_row(const Span<T>& s, Held<T, THREADS, NV>
       if (j < s.nvec) {
         typename T::V g;
 #pragma unroll
-        for (int k = 0; k < T::kPer16; ++k) g[k] = (typename T::Elem)f(element<T>(h.raw[i], k), s.first(j) + k);
-        if (s.whole(j)) {
-          *(u32x4*)(o.base + (uint64_t)j * 16) = __builtin_bit_cast(u32x4, g);
-        } else {
-#pragma unroll
-          for (int k = 0; k < T::kPer16; ++k)
-            if (s.first(j) + k < s.v) out[s.first(j) + k] = g[k];
-        }
+        for (int k = 0; k < T::kPer16; ++k) g[k] = (typename T::Elem)f(element<T>(h.raw[i], k));
+        s.store(out, j, g);
       }
     }
   }
@@ -193,29 +230,21 @@ __device__ __forceinline__ void write_row(const Span<T>& s, Held<T, THREADS, NV>
 
 template <class T, int THREADS>
 __device__ __forceinline__ void write_zeros(typename T::Elem* out, uint32_t v) {
-  const Span<T> o(out, v);
-  for (uint32_t j = threadIdx.x; j < o.nvec; j += THREADS) {
-    if (o.whole(j)) {
-      *(u32x4*)(o.base + (uint64_t)j * 16) = u32x4{0, 0, 0, 0};
-    } else {
-      for (uint32_t k = 0; k < T::kPer16; ++k)
-        if (o.first(j) + k < v) out[o.first(j) + k] = (typename T::Elem)0.f;
-    }
-  }
+  const Row<T> s(out, v);
+  const typename T::V zeros = __builtin_bit_cast(typename T::V, u32x4{0, 0, 0, 0});
+  for (uint32_t j = threadIdx.x; j < s.nvec; j += THREADS) s.store(out, j, zeros);
 }
 
 // ----------------------------------------------------------- alternatives --
-// Orders (logit, index): larger logits first, equal ones by index. Keys of
-// different indexes differ; 0 is below every key. -0 and +0 are equal.
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t i) {
+// Orders logits: the larger one has the larger key; -0 and +0 are equal. 0 is below every key.
+__device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
-  const uint32_t o = u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-  return ((uint64_t)o << 32) | (uint32_t)~i;
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint64_t k) {
-  const uint32_t o = (uint32_t)(k >> 32);
-  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
-}
+__device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
+// Orders (logit, index): equal logits by index, the lower one first. Keys of different indexes differ.
+__device__ __forceinline__ uint64_t order_key(float x, uint32_t i) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~i; }
+__device__ __forceinline__ float key_value(uint64_t k) { return value_of((uint32_t)(k >> 32)); }
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 struct TopShared {
@@ -227,9 +256,10 @@ struct TopShared {
   uint32_t count;
 };
 
-// How many of keys[0, n) are above `mine` (two a load: the same address for the whole wave).
+// How many of keys[0, n) are above `mine`.
 __device__ __forceinline__ uint32_t above(const uint64_t* keys, uint32_t n, uint64_t mine) {
   uint32_t r = 0;
+#pragma unroll 8
   for (uint32_t i = 0; i < n; ++i) r += keys[i] > mine;
   return r;
 }
@@ -238,70 +268,83 @@ __device__ __forceinline__ uint32_t above(const uint64_t* keys, uint32_t n, uint
 //
 // The maxima of 256 groups of threads give a bound: at least `top` logits are not
 // below the top-th largest of them, and about -256 ln(1 - top / 256) are. Those are
-// collected, and each finds its place by counting the ones above it. Keys hold the
-// index, so that ties (a constant row) do not swell the collection; where an adverse
-// order does (large logits in few groups), the largest below the last one is taken
-// `top` times.
+// collected, and each finds its place by counting the ones above it. Where ties, or an
+// order that puts large logits in few groups, leave more than the collection holds, the
+// groups' maxima are taken again with their indexes (of a constant row the lowest indexes
+// stay); and where that is not enough, the largest below the last one is taken `top` times.
 template <class T, int THREADS, int NV, class F>
-__device__ __forceinline__ void alternatives(const Span<T>& s, Held<T, THREADS, NV>& h, uint32_t top, TopShared& sh, F emit) {
+__device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, NV>& h, uint32_t top, TopShared& sh, F emit) {
+  constexpr int E = T::kPer16;
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const bool again = s.nvec > THREADS * NV;
-  // f(key) for the logits that this thread holds
-  auto each = [&](auto f) {
+  // f(i, j) for each vector j of this thread, held at i
+  auto vectors = [&](auto f) {
     for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
       if (again) h.load(s, j0);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < T::kPer16; ++k) {
-          const uint32_t at = s.first(h.index(j0, i)) + k;
-          f(element<T>(h.raw[i], k), at);
-        }
+        if (j0 + i * THREADS < s.nvec) f(i, h.index(j0, i));
     }
   };
-  float m = -INFINITY;
-  uint32_t at = ~0u;
-  each([&](float x, uint32_t i) {
-    if (i < s.v && (x > m || at == ~0u)) {
-      m = x;
-      at = i;
+  // f(logit, index), from memory, where speed is not asked for
+  auto logits = [&](auto f) {
+    for (uint32_t i = tid; i < s.v; i += THREADS) f((float)s.p[i], i);
+  };
+  // The top-th largest of the groups' keys goes to sh.bound (0: fewer groups than that have logits).
+  auto bound_of = [&](uint64_t best) {
+    if (THREADS > 256) best = max64(best, __shfl_xor((unsigned long long)best, 32, 64));
+    if (THREADS > 512) best = max64(best, __shfl_xor((unsigned long long)best, 16, 64));
+    constexpr uint32_t kGroupsOfWave = THREADS == 256 ? 64 : THREADS == 512 ? 32 : 16;
+    __syncthreads();
+    const uint32_t mine = (tid >> 6) * kGroupsOfWave + lane;
+    if (lane < kGroupsOfWave) sh.group[mine] = best;
+    if (tid < kGroups) sh.rank[tid] = 0;
+    if (tid == 0) {
+      sh.bound = 0;
+      sh.count = 0;
     }
-  });
-  uint64_t best = at == ~0u ? 0 : order_key(m, at);
-  if (THREADS > 256) best = max64(best, __shfl_xor((unsigned long long)best, 32, 64));
-  if (THREADS > 512) best = max64(best, __shfl_xor((unsigned long long)best, 16, 64));
-  constexpr uint32_t kGroupsOfWave = THREADS == 256 ? 64 : THREADS == 512 ? 32 : 16;
-  if (lane < kGroupsOfWave) sh.group[(tid >> 6) * kGroupsOfWave + lane] = best;
-  if (tid < kGroups) sh.rank[tid] = 0;
-  if (tid == 0) {
-    sh.bound = 0;
-    sh.count = 0;
-  }
-  __syncthreads();
-  {
+    __syncthreads();
     constexpr uint32_t kParts = THREADS / kGroups, kPart = kGroups / kParts;
     const uint32_t g = tid % kGroups, part = tid / kGroups;
     const uint32_t r = above(sh.group + part * kPart, kPart, sh.group[g]);
     if (kParts > 1) atomicAdd(&sh.rank[g], r);  // whole numbers: any order
     else sh.rank[g] = r;
-  }
-  __syncthreads();
-  if (tid < kGroups && sh.rank[tid] == top - 1 && sh.group[tid]) sh.bound = sh.group[tid];
-  __syncthreads();
-  const uint64_t bound = sh.bound;
-  const float floor = bound ? key_value(bound) : -INFINITY;
-  if (m >= floor)
-    each([&](float x, uint32_t i) {
-      if (x >= floor && i < s.v) {
-        const uint64_t key = order_key(x, i);
-        if (key >= bound) {
-          const uint32_t n = atomicAdd(&sh.count, 1u);
-          if (n < kCandidates) sh.candidate[n] = key;
-        }
+    __syncthreads();
+    if (tid < kGroups && sh.rank[tid] == top - 1 && sh.group[tid]) sh.bound = sh.group[tid];
+    __syncthreads();
+    return sh.bound;
+  };
+  auto collect = [&](uint64_t key) {
+    const uint32_t n = atomicAdd(&sh.count, 1u);
+    if (n < kCandidates) sh.candidate[n] = key;
+  };
+  float m = -INFINITY;
+  vectors([&](int i, uint32_t) { m = fmaxf(m, h.largest(i)); });
+  // groups of equal maxima are told apart by their number; the bound is the value alone
+  const float floor = key_value(bound_of(((uint64_t)order_of(m) << 32) | (0xffffu - tid)));
+  vectors([&](int i, uint32_t j) {
+    if (h.largest(i) >= floor) {
+      const uint32_t at = s.first(j);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float x = element<T>(h.raw[i], k);
+        if (x >= floor && at + k >= j * E && at + k < s.v) collect(order_key(x, at + k));
       }
-    });
+    }
+  });
   __syncthreads();
-  const uint32_t count = sh.count;
+  uint32_t count = sh.count;
+  if (count > kCandidates) {
+    uint64_t best = 0;
+    logits([&](float x, uint32_t i) { best = max64(best, order_key(x, i)); });
+    const uint64_t bound = bound_of(best);
+    logits([&](float x, uint32_t i) {
+      const uint64_t key = order_key(x, i);
+      if (key >= bound) collect(key);
+    });
+    __syncthreads();
+    count = sh.count;
+  }
   if (count <= kCandidates) {
     for (uint32_t n = tid; n < count; n += THREADS) {
       const uint64_t key = sh.candidate[n];
@@ -313,9 +356,9 @@ __device__ __forceinline__ void alternatives(const Span<T>& s, Held<T, THREADS, 
   uint64_t prev = ~0ull;
   for (uint32_t r = 0; r < top; ++r) {
     uint64_t next = 0;
-    each([&](float x, uint32_t i) {
+    logits([&](float x, uint32_t i) {
       const uint64_t key = order_key(x, i);
-      if (i < s.v && key < prev && key > next) next = key;
+      if (key < prev && key > next) next = key;
     });
     for (int off = 32; off >= 1; off >>= 1) next = max64(next, __shfl_xor((unsigned long long)next, off, 64));
     __syncthreads();
@@ -328,6 +371,13 @@ __device__ __forceinline__ void alternatives(const Span<T>& s, Held<T, THREADS, 
 }
 
 // ---------------------------------------------------------------- kernels --
+// The statistics of a row that is only read (KEEP false), or is held for a second look.
+template <class T, int THREADS, int NV, bool ENTROPY, bool KEEP, bool FAR>
+__device__ __forceinline__ Stats<FAR> stats_of(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<FAR>* waves) {
+  if constexpr (KEEP) return row_stats<T, THREADS, NV, ENTROPY>(s, h, c, waves);
+  else return stream_stats<T, THREADS, NV, ENTROPY>(s, c, waves);
+}
+
 template <class T, int THREADS, int NV, bool TOP, bool GRAD>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
   using Elem = typename T::Elem;
@@ -350,9 +400,9 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
   }
   const bool inside = tok >= 0 && tok < (int64_t)a.vocab;
   const float xt = inside ? (float)x[tok] : 0.f;
-  const Span<T> s(x, a.vocab);
+  const Row<T> s(x, a.vocab);
   Held<T, THREADS, NV> h;
-  const Stats<GRAD> st = row_stats<T, THREADS, NV, true>(s, h, kLog2e, waves);
+  const Stats<GRAD> st = stats_of<T, THREADS, NV, true, TOP || GRAD>(s, h, kLog2e, waves);
   const bool valid = st.valid();
   const float log2s = log2_hw(st.s);
   const float entropy = valid ? kLn2 * (log2s - st.t / st.s) : NAN;
@@ -382,24 +432,26 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
     if (!(valid && inside)) w = NAN;
     // d = w ([i = tok] - q) - u q (ln q + entropy), z = log2 q
     const float wu = __builtin_fmaf(u, entropy, w), ul = u * kLn2;
-    write_row<T, THREADS, NV>(s, h, g, [&](float xi, uint32_t i) {
-      const float z = st.y_of(xi, kLog2e) - log2s;
-      const float d = -exp2_hw(z) * __builtin_fmaf(ul, fmaxf(z, -1e30f), wu);
-      return i == (uint32_t)tok ? d + w : d;
-    });
+    const auto d = [&](float xi) {
+      const float z = st.y_far(xi, kLog2e) - log2s;
+      return -exp2_hw(z) * __builtin_fmaf(ul, fmaxf(z, -1e30f), wu);
+    };
+    write_row<T, THREADS, NV>(s, h, g, d);
+    __syncthreads();  // the row's stores are done before the token's is written again
+    if (tid == 0 && inside) g[tok] = (Elem)(d(xt) + w);
   }
 }
 
 struct TeacherShared {
   float w[kMaxTeacher];
+  float x[kMaxTeacher];  // the student's logits of the entries
   int32_t idx[kMaxTeacher];
   float total;
   int32_t bad;
 };
 
-// The teacher's softmax over its entries, by one wave: weights and tokens (-1: no
-// entry) in LDS. Returns the row's loss but for the student's log sum:
-// sum w (ln w - x / T) and the weights' sum.
+// One wave makes the teacher's softmax over its entries, in LDS, before the row's statistics, and sums
+// the loss after them.
 template <class T, int THREADS, int NV, bool GRAD>
 __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
   using Elem = typename T::Elem;
@@ -428,6 +480,7 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
       const float t = values[j] * tinv;
       bad |= i != -1 && (!in || !(t < INFINITY));
       sh.idx[j] = in ? (int32_t)i : -1;
+      sh.x[j] = in ? (float)x[i] : 0.f;
       sh.w[j] = in ? t : -INFINITY;
       if (in) tm = fmaxf(tm, t);
     }
@@ -444,16 +497,16 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
     }
     bad = __any(bad);
   }
-  const Span<T> s(x, a.vocab);
+  const Row<T> s(x, a.vocab);
   Held<T, THREADS, NV> h;
-  const Stats<GRAD> st = row_stats<T, THREADS, NV, false>(s, h, c, waves);
+  const Stats<GRAD> st = stats_of<T, THREADS, NV, false, GRAD>(s, h, c, waves);
   const float log2s = log2_hw(st.s);
   if (tid < 64) {
     float loss = 0.f, total = 0.f;
     for (uint32_t j = lane; j < k; j += 64) {
       const float lnw = (sh.w[j] - tm) - lse;
       const float w = sh.idx[j] >= 0 ? exp2_hw(lnw * kLog2e) : 0.f;
-      if (w > 0.f) loss += w * (lnw - st.lnq((float)x[sh.idx[j]], c, inv));
+      if (w > 0.f) loss += w * (lnw - st.lnq(sh.x[j], c, inv));
       sh.w[j] = w;
       total += w;
     }
@@ -471,7 +524,7 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
     const float total = sh.total;
     const float up = sh.bad ? NAN : a.temperature * a.weights[b * a.weights_s.batch + l * a.weights_s.row];
     const float up_total = up * total;
-    auto soft = [&](float xi, uint32_t) { return up_total * exp2_hw(st.y_of(xi, c) - log2s); };
+    auto soft = [&](float xi) { return up_total * exp2_hw(st.y_far(xi, c) - log2s); };
     write_row<T, THREADS, NV>(s, h, g, soft);
     __syncthreads();  // the row's stores are done before its entries are written again
     for (uint32_t j = tid; j < k; j += THREADS) {
@@ -484,7 +537,7 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
           if (n < j) first = false;
           w += sh.w[n];
         }
-      if (first) g[i] = (Elem)(up * (total * exp2_hw(st.y_of((float)x[i], c) - log2s) - w));
+      if (first) g[i] = (Elem)(up * (total * exp2_hw(st.y_far(sh.x[j], c) - log2s) - w));
     }
   }
 }
@@ -492,7 +545,7 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
 // A workgroup's size and the vectors that each thread holds, by the row's length.
 template <class T, class F>
 hipError_t by_length(uint32_t vocab, F launch) {
-  const uint32_t nvec = (vocab + 2 * (T::kPer16 - 1)) / T::kPer16;  // the most that a row of this length spans
+  const uint32_t nvec = (vocab + T::kPer16 - 1) / T::kPer16;
   if (nvec <= 256 * 4) launch(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
   else if (nvec <= 512 * 8) launch(std::integral_constant<int, 512>(), std::integral_constant<int, 8>());
   else if (nvec <= 1024 * 8) launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 8>());
@@ -500,22 +553,39 @@ hipError_t by_length(uint32_t vocab, F launch) {
   return hipGetLastError();
 }
 
+// The same where the row streams by: 256 threads, of which 8 workgroups share a compute unit; 1,024
+// where there are fewer rows than compute units, and each has one to itself.
+template <class F>
+hipError_t by_rows(uint32_t nrows, uint32_t vocab, F launch) {
+  if (nrows <= 256 && vocab > 8192) launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+  else launch(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+  return hipGetLastError();
+}
+
 template <class T>
 hipError_t launch_logprobs(const VocabRows& a, hipStream_t st) {
+  if (!a.grad && !a.top)
+    return by_rows(a.nrows, a.vocab, [&](auto threads, auto nv) {
+      constexpr int N = decltype(threads)::value, V = decltype(nv)::value;
+      token_logprobs_kernel<T, N, V, false, false><<<a.nrows, N, 0, st>>>(a);
+    });
   return by_length<T>(a.vocab, [&](auto threads, auto nv) {
     constexpr int N = decltype(threads)::value, V = decltype(nv)::value;
     if (a.grad) token_logprobs_kernel<T, N, V, false, true><<<a.nrows, N, 0, st>>>(a);
-    else if (a.top) token_logprobs_kernel<T, N, V, true, false><<<a.nrows, N, 0, st>>>(a);
-    else token_logprobs_kernel<T, N, V, false, false><<<a.nrows, N, 0, st>>>(a);
+    else token_logprobs_kernel<T, N, V, true, false><<<a.nrows, N, 0, st>>>(a);
   });
 }
 
 template <class T>
 hipError_t launch_distill(const VocabRows& a, hipStream_t st) {
+  if (!a.grad)
+    return by_rows(a.nrows, a.vocab, [&](auto threads, auto nv) {
+      constexpr int N = decltype(threads)::value, V = decltype(nv)::value;
+      topk_distill_kernel<T, N, V, false><<<a.nrows, N, 0, st>>>(a);
+    });
   return by_length<T>(a.vocab, [&](auto threads, auto nv) {
     constexpr int N = decltype(threads)::value, V = decltype(nv)::value;
-    if (a.grad) topk_distill_kernel<T, N, V, true><<<a.nrows, N, 0, st>>>(a);
-    else topk_distill_kernel<T, N, V, false><<<a.nrows, N, 0, st>>>(a);
+    topk_distill_kernel<T, N, V, true><<<a.nrows, N, 0, st>>>(a);
   });
 }
 
