@@ -10,8 +10,8 @@
 // thread's vectors lie THREADS apart, so that a wave's loads cover consecutive bytes.
 //
 // Rows start where they start (an odd vocabulary, a view), and so do their vectors:
-// loads and stores of 16 bytes at the element's alignment. The last vector, where it is
-// not whole, is the row's last 16 bytes, and what it repeats is taken out.
+// loads and stores of 16 bytes at the element's alignment. The elements after the last
+// whole vector are one each to the workgroup's first threads.
 #include "dz_token_loss.h"
 #include "dz_token_math.h"
 
@@ -93,70 +93,50 @@ __device__ __forceinline__ u32x4 none16() {  // no logits: -inf
 }
 template <class T>
 __device__ __forceinline__ float element(const u32x4& raw, int k) {
+  // bf16 by its bits: of a maximum of extended values the compiler makes an extended maximum of
+  // bf16 values, which it then rounds after every step
+  if (std::is_same<T, TypeBF16>::value) return __uint_as_float(k & 1 ? raw[k / 2] & 0xffff0000u : raw[k / 2] << 16);
   return (float)__builtin_bit_cast(typename T::V, raw)[k];
 }
 // Makes the compiler read `raw` anew, instead of keeping what an earlier pass made of it.
 __device__ __forceinline__ void afresh(u32x4& raw) { asm("" : "+v"(raw)); }
 
-// v elements at p as 16-byte vectors.
+// v elements at p: `full` vectors of 16 bytes, and `rem` elements.
 template <class T>
 struct Row {
   using Elem = typename T::Elem;
   using Loose = typename Loose16<T>::type;
   static constexpr uint32_t E = T::kPer16;
   const Elem* p;
-  uint32_t v, nvec;
+  uint32_t v, full, rem;
 
-  __device__ Row(const Elem* p_, uint32_t v_) : p(p_), v(v_), nvec((v_ + E - 1) / E) {}
+  __device__ Row(const Elem* p_, uint32_t v_) : p(p_), v(v_), full(v_ / E), rem(v_ % E) {}
 
-  // the element that vector j starts with: the last vector ends with the row
-  __device__ __forceinline__ uint32_t first(uint32_t j) const { return (j + 1) * E <= v ? j * E : v >= E ? v - E : 0; }
-
-  // Vector j, of a wave whose vectors end before j_end (the same for the whole wave).
-  __device__ __forceinline__ u32x4 load(uint32_t j, uint32_t j_end) const {
-    if (j_end * E <= v) return __builtin_bit_cast(u32x4, (typename T::V)*(const Loose*)(p + j * E));
-    typename T::V x = __builtin_bit_cast(typename T::V, none16<T>());
-    if (v >= E) {
-      const uint32_t at = first(j);
-      x = *(const Loose*)(p + at);
-#pragma unroll
-      for (uint32_t k = 0; k < E; ++k)
-        if (at + k < j * E) x[k] = (Elem)-INFINITY;  // the vector before has it, or there is no vector j
-    } else if (j == 0) {
-      for (uint32_t k = 0; k < E; ++k)
-        if (k < v) x[k] = p[k];
-    }
-    return __builtin_bit_cast(u32x4, x);
-  }
-
-  // Writes vector j of `out`, a row of the same length.
-  __device__ __forceinline__ void store(Elem* out, uint32_t j, const typename T::V& x) const {
-    if ((j + 1) * E <= v) {
-      *(Loose*)(out + j * E) = x;
-    } else {
-      const uint32_t at = first(j);
-#pragma unroll
-      for (uint32_t k = 0; k < E; ++k)
-        if (at + k >= j * E && at + k < v) out[at + k] = x[k];
-    }
-  }
+  // vector j0 + this thread's number: a base that is the same for the workgroup, and an offset
+  __device__ __forceinline__ static auto at(const Elem* p, uint32_t j0) { return (const Loose*)(p + (uint64_t)j0 * E) + threadIdx.x; }
+  __device__ __forceinline__ u32x4 load(uint32_t j0) const { return __builtin_bit_cast(u32x4, (typename T::V)__builtin_nontemporal_load(at(p, j0))); }
+  // this thread's element after the last whole vector, and its index
+  __device__ __forceinline__ bool has_extra() const { return threadIdx.x < rem; }
+  __device__ __forceinline__ uint32_t extra_at() const { return full * E + threadIdx.x; }
+  __device__ __forceinline__ float extra() const { return has_extra() ? (float)p[extra_at()] : -INFINITY; }
 };
 
-// THREADS x NV vectors of a row from vector j0 on, in registers.
+// THREADS x NV vectors of a row from vector j0 on, in registers; -inf where there are none.
 template <class T, int THREADS, int NV>
 struct Held {
-  static constexpr int E = T::kPer16, STEP = NV < 4 ? NV : 4;  // vectors that are added at a time
-  static_assert(NV % STEP == 0, "steps");
+  static constexpr int E = T::kPer16;
   u32x4 raw[NV];
-
-  __device__ __forceinline__ static uint32_t index(uint32_t j0, int i) { return j0 + i * THREADS + threadIdx.x; }
 
   __device__ __forceinline__ void load(const Row<T>& s, uint32_t j0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       raw[i] = none16<T>();
-      if (j0 + i * THREADS < s.nvec) raw[i] = s.load(index(j0, i), j0 + (i + 1) * THREADS);
+      if (j0 + i * THREADS + threadIdx.x < s.full) raw[i] = s.load(j0 + i * THREADS);
     }
+  }
+  __device__ __forceinline__ void load_whole(const Row<T>& s, uint32_t j0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = s.load(j0 + i * THREADS);
   }
   __device__ __forceinline__ float largest(int i) const {
     float m = element<T>(raw[i], 0);
@@ -165,8 +145,8 @@ struct Held {
     return m;
   }
   // The statistics with these vectors added.
-  template <bool ENTROPY, bool FAR>
-  __device__ __forceinline__ void add_to(const Row<T>& s, uint32_t j0, Stats<FAR>& st, float c) {
+  template <bool ENTROPY>
+  __device__ __forceinline__ void add_to(Stats<true>& st, float c) {
     float m = st.m;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -175,64 +155,94 @@ struct Held {
     }
     st.rebase(m, c);
 #pragma unroll
-    for (int i = 0; i < NV; i += STEP)
-      if (j0 + i * THREADS < s.nvec) {
-        st.template add<ENTROPY, STEP * E>([&](int n) { return element<T>(raw[i + n / E], n % E); }, c);
-#pragma unroll
-        for (int n = 0; n < STEP; ++n) afresh(raw[i + n]);
-      }
+    for (int i = 0; i < NV; ++i) {
+      st.template add_far<ENTROPY, E>([&](int n) { return element<T>(raw[i], n); }, c);
+      afresh(raw[i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 };
 
-// A row's softmax statistics, for the whole workgroup. Leaves the row in `h` where it fits.
-template <class T, int THREADS, int NV, bool ENTROPY, bool FAR>
-__device__ __forceinline__ Stats<FAR> row_stats(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<FAR>* waves) {
-  auto st = Stats<FAR>::of(-INFINITY);
-  for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
+// A row's softmax statistics, for the whole workgroup, and the largest logit that this thread holds. Leaves
+// the row in `h` where it fits.
+template <class T, int THREADS, int NV, bool ENTROPY>
+__device__ __forceinline__ Stats<true> row_stats(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<true>* waves, float& own_max) {
+  const float extra = s.extra();
+  auto st = Stats<true>::of(extra);
+  st.template add_far<ENTROPY, 1>([&](int) { return extra; }, c);
+  for (uint32_t j0 = 0; j0 < s.full; j0 += THREADS * NV) {
     h.load(s, j0);
-    h.template add_to<ENTROPY>(s, j0, st, c);
+    h.template add_to<ENTROPY>(st, c);
   }
+  own_max = st.m;
   return block_stats<THREADS, ENTROPY>(st, c, waves);
 }
 
-// The same where the row is not needed again: the next NV vectors are on their way while these are added.
+// The same where the row is not needed again: NV vectors a thread at a time, the next ones on their way while
+// these are added, and the last ones from the start on. The statistics' m need not be
+// the maximum: 2^y up to 2^8 do no harm, and moving it takes as long as several logits.
 template <class T, int THREADS, int NV, bool ENTROPY>
 __device__ __forceinline__ SoftStats stream_stats(const Row<T>& s, float c, SoftStats* waves) {
-  Held<T, THREADS, NV> a, b;
-  auto st = SoftStats::of(-INFINITY);
-  a.load(s, 0);
-  for (uint32_t j0 = 0; j0 < s.nvec; j0 += 2 * THREADS * NV) {
-    b.load(s, j0 + THREADS * NV);
-    a.template add_to<ENTROPY>(s, j0, st, c);
-    a.load(s, j0 + 2 * THREADS * NV);
-    b.template add_to<ENTROPY>(s, j0 + THREADS * NV, st, c);
+  constexpr uint32_t STEP = THREADS * NV;
+  Held<T, THREADS, NV> a, b, last;
+  const uint32_t whole = s.full / STEP;  // steps
+  last.load(s, whole * STEP);
+  const float extra = s.extra();
+  auto st = SoftStats::of(extra);
+  auto add = [&](Held<T, THREADS, NV>& h) {
+    float m = h.largest(0);
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, h.largest(i));
+    if (__any(!((m - st.m) * c <= 8.f))) st.rebase(fmaxf(st.m, m), c);
+    st.template add<ENTROPY, NV * T::kPer16>([&](int n) { return element<T>(h.raw[n / T::kPer16], n % T::kPer16); }, c);
+  };
+  st.template add<ENTROPY, 1>([&](int) { return extra; }, c);
+  if (whole) {
+    uint32_t n = 0;
+    a.load_whole(s, 0);
+    for (; n + 2 < whole; n += 2) {
+      b.load_whole(s, (n + 1) * STEP);
+      add(a);
+      a.load_whole(s, (n + 2) * STEP);
+      add(b);
+    }
+    if (n + 1 < whole) {
+      b.load_whole(s, (n + 1) * STEP);
+      add(a);
+      add(b);
+    } else {
+      add(a);
+    }
   }
+  if (whole * STEP < s.full) add(last);
   return block_stats<THREADS, ENTROPY>(st, c, waves);
 }
 
 // Writes f(logit) for the whole row.
 template <class T, int THREADS, int NV, class F>
 __device__ __forceinline__ void write_row(const Row<T>& s, Held<T, THREADS, NV>& h, typename T::Elem* out, F f) {
-  for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
-    if (s.nvec > THREADS * NV) h.load(s, j0);
+  using Elem = typename T::Elem;
+  using Loose = typename Row<T>::Loose;
+  for (uint32_t j0 = 0; j0 < s.full; j0 += THREADS * NV) {
+    if (s.full > THREADS * NV) h.load(s, j0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t j = h.index(j0, i);
-      if (j < s.nvec) {
-        typename T::V g;
+      typename T::V g;
 #pragma unroll
-        for (int k = 0; k < T::kPer16; ++k) g[k] = (typename T::Elem)f(element<T>(h.raw[i], k));
-        s.store(out, j, g);
-      }
+      for (int k = 0; k < T::kPer16; ++k) g[k] = (Elem)f(element<T>(h.raw[i], k));
+      if (j0 + i * THREADS + threadIdx.x < s.full) *(Loose*)Row<T>::at(out, j0 + i * THREADS) = g;
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+  if (s.has_extra()) out[s.extra_at()] = (Elem)f(s.extra());
 }
 
 template <class T, int THREADS>
 __device__ __forceinline__ void write_zeros(typename T::Elem* out, uint32_t v) {
   const Row<T> s(out, v);
   const typename T::V zeros = __builtin_bit_cast(typename T::V, u32x4{0, 0, 0, 0});
-  for (uint32_t j = threadIdx.x; j < s.nvec; j += THREADS) s.store(out, j, zeros);
+  for (uint32_t j0 = 0; j0 + threadIdx.x < s.full; j0 += THREADS) *(typename Row<T>::Loose*)Row<T>::at(out, j0) = zeros;
+  if (s.has_extra()) out[s.extra_at()] = (typename T::Elem)0.f;
 }
 
 // ----------------------------------------------------------- alternatives --
@@ -273,19 +283,9 @@ __device__ __forceinline__ uint32_t above(const uint64_t* keys, uint32_t n, uint
 // groups' maxima are taken again with their indexes (of a constant row the lowest indexes
 // stay); and where that is not enough, the largest below the last one is taken `top` times.
 template <class T, int THREADS, int NV, class F>
-__device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, NV>& h, uint32_t top, TopShared& sh, F emit) {
+__device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, NV>& h, uint32_t top, float own_max, TopShared& sh, F emit) {
   constexpr int E = T::kPer16;
   const uint32_t tid = threadIdx.x, lane = tid & 63;
-  const bool again = s.nvec > THREADS * NV;
-  // f(i, j) for each vector j of this thread, held at i
-  auto vectors = [&](auto f) {
-    for (uint32_t j0 = 0; j0 < s.nvec; j0 += THREADS * NV) {
-      if (again) h.load(s, j0);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (j0 + i * THREADS < s.nvec) f(i, h.index(j0, i));
-    }
-  };
   // f(logit, index), from memory, where speed is not asked for
   auto logits = [&](auto f) {
     for (uint32_t i = tid; i < s.v; i += THREADS) f((float)s.p[i], i);
@@ -318,20 +318,23 @@ __device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, N
     const uint32_t n = atomicAdd(&sh.count, 1u);
     if (n < kCandidates) sh.candidate[n] = key;
   };
-  float m = -INFINITY;
-  vectors([&](int i, uint32_t) { m = fmaxf(m, h.largest(i)); });
   // groups of equal maxima are told apart by their number; the bound is the value alone
-  const float floor = key_value(bound_of(((uint64_t)order_of(m) << 32) | (0xffffu - tid)));
-  vectors([&](int i, uint32_t j) {
-    if (h.largest(i) >= floor) {
-      const uint32_t at = s.first(j);
+  const float floor = key_value(bound_of(((uint64_t)order_of(own_max) << 32) | (0xffffu - tid)));
+  for (uint32_t j0 = 0; j0 < s.full; j0 += THREADS * NV) {
+    if (s.full > THREADS * NV) h.load(s, j0);
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        const float x = element<T>(h.raw[i], k);
-        if (x >= floor && at + k >= j * E && at + k < s.v) collect(order_key(x, at + k));
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t j = j0 + i * THREADS + tid;
+      if (h.largest(i) >= floor && j < s.full) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          const float x = element<T>(h.raw[i], k);
+          if (x >= floor) collect(order_key(x, j * E + k));
+        }
       }
     }
-  });
+  }
+  if (s.has_extra() && s.extra() >= floor) collect(order_key(s.extra(), s.extra_at()));
   __syncthreads();
   uint32_t count = sh.count;
   if (count > kCandidates) {
@@ -372,16 +375,16 @@ __device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, N
 
 // ---------------------------------------------------------------- kernels --
 // The statistics of a row that is only read (KEEP false), or is held for a second look.
-template <class T, int THREADS, int NV, bool ENTROPY, bool KEEP, bool FAR>
-__device__ __forceinline__ Stats<FAR> stats_of(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<FAR>* waves) {
-  if constexpr (KEEP) return row_stats<T, THREADS, NV, ENTROPY>(s, h, c, waves);
+template <class T, int THREADS, int NV, bool ENTROPY, bool KEEP>
+__device__ __forceinline__ Stats<KEEP> stats_of(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<KEEP>* waves, float& own_max) {
+  if constexpr (KEEP) return row_stats<T, THREADS, NV, ENTROPY>(s, h, c, waves, own_max);
   else return stream_stats<T, THREADS, NV, ENTROPY>(s, c, waves);
 }
 
 template <class T, int THREADS, int NV, bool TOP, bool GRAD>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
   using Elem = typename T::Elem;
-  __shared__ Stats<GRAD> waves[THREADS / 64];
+  __shared__ Stats<TOP || GRAD> waves[THREADS / 64];
   const uint32_t r = blockIdx.x, b = r / a.length, l = r % a.length, tid = threadIdx.x;
   const Elem* x = (const Elem*)a.logits + b * a.logits_s.batch + l * a.logits_s.row;
   Elem* g = GRAD ? (Elem*)a.grad + b * a.grad_s.batch + l * a.grad_s.row : nullptr;
@@ -402,7 +405,8 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
   const float xt = inside ? (float)x[tok] : 0.f;
   const Row<T> s(x, a.vocab);
   Held<T, THREADS, NV> h;
-  const Stats<GRAD> st = stats_of<T, THREADS, NV, true, TOP || GRAD>(s, h, kLog2e, waves);
+  float own_max = -INFINITY;
+  const Stats<TOP || GRAD> st = stats_of<T, THREADS, NV, true, TOP || GRAD>(s, h, kLog2e, waves, own_max);
   const bool valid = st.valid();
   const float log2s = log2_hw(st.s);
   const float entropy = valid ? kLn2 * (log2s - st.t / st.s) : NAN;
@@ -421,7 +425,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
       }
       return;
     }
-    alternatives<T, THREADS, NV>(s, h, (uint32_t)a.top, sh, [&](uint32_t rank, uint64_t key) {
+    alternatives<T, THREADS, NV>(s, h, (uint32_t)a.top, own_max, sh, [&](uint32_t rank, uint64_t key) {
       lp[rank] = st.lnq(key_value(key), kLog2e, 1.f);
       at[rank] = (int64_t)(uint32_t)~(uint32_t)key;
     });
@@ -432,8 +436,9 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(VocabRows a) {
     if (!(valid && inside)) w = NAN;
     // d = w ([i = tok] - q) - u q (ln q + entropy), z = log2 q
     const float wu = __builtin_fmaf(u, entropy, w), ul = u * kLn2;
+    const float m0 = st.m == -INFINITY ? 0.f : st.m;
     const auto d = [&](float xi) {
-      const float z = st.y_far(xi, kLog2e) - log2s;
+      const float z = __builtin_fmaf(xi - m0, kLog2e, -log2s);
       return -exp2_hw(z) * __builtin_fmaf(ul, fmaxf(z, -1e30f), wu);
     };
     write_row<T, THREADS, NV>(s, h, g, d);
@@ -499,7 +504,8 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
   }
   const Row<T> s(x, a.vocab);
   Held<T, THREADS, NV> h;
-  const Stats<GRAD> st = stats_of<T, THREADS, NV, false, GRAD>(s, h, c, waves);
+  float own_max = -INFINITY;
+  const Stats<GRAD> st = stats_of<T, THREADS, NV, false, GRAD>(s, h, c, waves, own_max);
   const float log2s = log2_hw(st.s);
   if (tid < 64) {
     float loss = 0.f, total = 0.f;
@@ -524,7 +530,8 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
     const float total = sh.total;
     const float up = sh.bad ? NAN : a.temperature * a.weights[b * a.weights_s.batch + l * a.weights_s.row];
     const float up_total = up * total;
-    auto soft = [&](float xi) { return up_total * exp2_hw(st.y_far(xi, c) - log2s); };
+    const float m0 = st.m == -INFINITY ? 0.f : st.m;
+    const auto soft = [&](float xi) { return up_total * exp2_hw(__builtin_fmaf(xi - m0, c, -log2s)); };
     write_row<T, THREADS, NV>(s, h, g, soft);
     __syncthreads();  // the row's stores are done before its entries are written again
     for (uint32_t j = tid; j < k; j += THREADS) {
@@ -537,18 +544,21 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
           if (n < j) first = false;
           w += sh.w[n];
         }
-      if (first) g[i] = (Elem)(up * (total * exp2_hw(st.y_far(sh.x[j], c) - log2s) - w));
+      if (first) g[i] = (Elem)(up * (total * exp2_hw(__builtin_fmaf(sh.x[j] - m0, c, -log2s)) - w));
     }
   }
 }
 
-// A workgroup's size and the vectors that each thread holds, by the row's length.
+// A workgroup's size and the vectors that each thread holds, by the row's length: steps of a factor of 2 to 1.25, and
+// workgroups of which two or three share a compute unit, so that one's loads overlap another's sums.
 template <class T, class F>
 hipError_t by_length(uint32_t vocab, F launch) {
-  const uint32_t nvec = (vocab + T::kPer16 - 1) / T::kPer16;
-  if (nvec <= 256 * 4) launch(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+  const uint32_t nvec = vocab / T::kPer16;
+  if (nvec <= 256 * 8) launch(std::integral_constant<int, 256>(), std::integral_constant<int, 8>());
   else if (nvec <= 512 * 8) launch(std::integral_constant<int, 512>(), std::integral_constant<int, 8>());
+  else if (nvec <= 512 * 13) launch(std::integral_constant<int, 512>(), std::integral_constant<int, 13>());
   else if (nvec <= 1024 * 8) launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 8>());
+  else if (nvec <= 1024 * 13) launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 13>());
   else launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
   return hipGetLastError();
 }
@@ -557,8 +567,8 @@ hipError_t by_length(uint32_t vocab, F launch) {
 // where there are fewer rows than compute units, and each has one to itself.
 template <class F>
 hipError_t by_rows(uint32_t nrows, uint32_t vocab, F launch) {
-  if (nrows <= 256 && vocab > 8192) launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
-  else launch(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+  if (nrows <= 256 && vocab > 8192) launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+  else launch(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
   return hipGetLastError();
 }
 

@@ -63,33 +63,38 @@ struct Stats {
     return y == -INFINITY ? __builtin_fmaf(-kLn2, log2_hw(s), (x - m) * inv) : kLn2 * (y - log2_hw(s));
   }
 
-  // Adds x(0) .. x(N - 1). 2^y y is 0 where y is -inf: such a y makes t a NaN, and t is then taken
-  // again with care. (A NaN logit leaves a NaN in s.)
+  // Adds x(0) .. x(N - 1). 2^y y is 0 where y is -inf, which has to be said to a product. (A NaN logit
+  // leaves a NaN in s.)
+  template <bool ENTROPY, int N, class F>
+  __device__ __forceinline__ void add_far(F x, float c) {
+    const float m0 = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float y = (x(i) - m0) * c;
+      if (!FAR) y = in_range(m * c) ? y_plain(x(i), c) : y;
+      const float e = exp2_hw(y);
+      s += e;
+      if (ENTROPY) t = __builtin_fmaf(e, fmaxf(y, -1e30f), t);
+    }
+  }
+  // The same with one operation for y, and none for its limit unless it is met.
   template <bool ENTROPY, int N, class F>
   __device__ __forceinline__ void add(F x, float c) {
-    const float t0 = t;
-    if (plain(c)) {
+    const float k = m * c, s0 = s, t0 = t;
+    if (__all(in_range(k))) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float y = y_plain(x(i), c);
+        const float y = __builtin_fmaf(x(i), c, -k);
         const float e = exp2_hw(y);
         s += e;
         if (ENTROPY) t = __builtin_fmaf(e, y, t);
       }
-      if (!ENTROPY || t == t) return;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) s += exp2_hw(y_far(x(i), c));
-    }
-    if (ENTROPY) {
+      if (!ENTROPY || !__any(t != t)) return;
+      s = s0;
       t = t0;
-      asm("" : "+v"(c));  // or the compiler keeps all of the first pass's values for this one
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float y = y_of(x(i), c);
-        t = __builtin_fmaf(exp2_hw(y), fmaxf(y, -1e30f), t);
-      }
     }
+    asm("" : "+v"(c));  // or the compiler keeps all of the first pass's values for this one
+    add_far<ENTROPY, N>(x, c);
   }
 
   // The same statistics against another maximum, m2 >= m.
