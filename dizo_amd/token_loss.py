@@ -28,7 +28,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from ._lib import DzError
-from .table import _on, _ptr, dtype_code, stream_handle
+from .table import _ptr, dtype_code, stream_handle
 
 IGNORE_INDEX = -100  # the masked label of shift_option_labels
 MAX_TOP = 128
@@ -73,31 +73,30 @@ _INT = (torch.int64, torch.int32)
 _F32 = (torch.float32,)
 
 
-def _two(lead) -> Tuple[int, int]:
-    """Leading dimensions as (batch, length)."""
-    n = len(lead)
+def _rows(t: Optional[torch.Tensor], n: int, inner: int):
+    """A tensor of n leading dimensions as (address, batch stride, row stride), and what keeps it alive.
+    More than two are made one: a view where the strides allow it, else a copy."""
+    if t is None:
+        return None, 0, 0, None
+    if n > 2:
+        t = t.reshape(-1, *t.shape[n:]) if inner else t.reshape(-1)
+    s = t.stride()
     if n == 2:
-        return lead[0], lead[1]
-    if n == 1:
-        return 1, lead[0]
-    total = 1
-    for d in lead:
-        total *= d
-    return 1, total
+        return t.data_ptr(), s[0], s[1], t
+    return t.data_ptr(), 0, s[0] if n else 0, t
 
 
-def _strides(t: torch.Tensor, n: int) -> Tuple[int, int]:
-    """(batch, row) strides of a tensor of n leading dimensions, n <= 2."""
-    if n == 2:
-        return t.stride(0), t.stride(1)
-    return (0, t.stride(0)) if n == 1 else (0, 0)
+def _batch_length(lead) -> Tuple[int, int]:
+    return (lead[0], lead[1]) if len(lead) == 2 else (1, lead.numel())
 
 
-def _flat(t: Optional[torch.Tensor], n: int, inner: int):
-    """More than two leading dimensions as one (a view where the strides allow it, else a copy)."""
-    if t is None or n <= 2:
-        return t
-    return t.reshape(-1, *t.shape[n:]) if inner else t.reshape(-1)
+def _call(device, name: str, *args) -> None:
+    """The entry point on the device's current stream."""
+    if device.index == torch._C._cuda_getDevice():
+        L.call(name, *args, stream_handle())
+    else:
+        with torch.cuda.device(device):
+            L.call(name, *args, stream_handle())
 
 
 def _grad_like(logits: torch.Tensor) -> torch.Tensor:
@@ -106,26 +105,23 @@ def _grad_like(logits: torch.Tensor) -> torch.Tensor:
 
 def _score(logits, tokens, top, ignore_index, weights, entropy_weights, grad):
     """One launch over checked operands. grad: a tensor to write, or None."""
-    lead = logits.shape[:-1]
-    n, (batch, length) = len(lead), _two(lead)
-    dev = logits.device
-    lp = torch.empty(lead, dtype=torch.float32, device=dev)
-    ent = torch.empty(lead, dtype=torch.float32, device=dev)
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    n = len(lead)
+    batch, length = _batch_length(lead)
+    lp = logits.new_empty(lead, dtype=torch.float32)
+    ent = logits.new_empty(lead, dtype=torch.float32)
     tlp = ttok = None
     if top:
-        tlp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
-        ttok = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+        tlp = logits.new_empty((*lead, top), dtype=torch.float32)
+        ttok = logits.new_empty((*lead, top), dtype=torch.int64)
     if batch * length:
-        x, t = _flat(logits, n, 1), _flat(tokens, n, 0)
-        w, u, g = _flat(weights, n, 0), _flat(entropy_weights, n, 0), _flat(grad, n, 1)
-        m = min(n, 2) if n <= 2 else 1
-        zero = (0, 0)
-        with _on(dev):
-            L.call("dz_token_logprobs", x.data_ptr(), dtype_code(x.dtype), batch, length, x.shape[-1],
-                   *_strides(x, m), t.data_ptr(), *_strides(t, m), ignore_index, top, lp.data_ptr(), ent.data_ptr(),
-                   _ptr(tlp), _ptr(ttok), _ptr(w), *(zero if w is None else _strides(w, m)), _ptr(u),
-                   *(zero if u is None else _strides(u, m)), _ptr(g), *(zero if g is None else _strides(g, m)),
-                   stream_handle())
+        x, x_b, x_l, _x = _rows(logits, n, 1)
+        t, t_b, t_l, _t = _rows(tokens, n, 0)
+        w, w_b, w_l, _w = _rows(weights, n, 0)
+        u, u_b, u_l, _u = _rows(entropy_weights, n, 0)
+        g, g_b, g_l, _g = _rows(grad, n, 1)
+        _call(logits.device, "dz_token_logprobs", x, dtype_code(logits.dtype), batch, length, vocab, x_b, x_l, t, t_b, t_l,
+              ignore_index, top, lp.data_ptr(), ent.data_ptr(), _ptr(tlp), _ptr(ttok), w, w_b, w_l, u, u_b, u_l, g, g_b, g_l)
     return lp, ent, tlp, ttok
 
 
@@ -193,17 +189,16 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, weights: Opt
 
 def _distill(logits, values, tokens, temperature, normalize, weights, grad):
     lead = logits.shape[:-1]
-    n, (batch, length) = len(lead), _two(lead)
-    loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    n = len(lead)
+    batch, length = _batch_length(lead)
+    loss = logits.new_empty(lead, dtype=torch.float32)
     if batch * length:
-        x, w, g = _flat(logits, n, 1), _flat(weights, n, 0), _flat(grad, n, 1)
-        m = min(n, 2) if n <= 2 else 1
-        zero = (0, 0)
-        with _on(logits.device):
-            L.call("dz_topk_distill", x.data_ptr(), dtype_code(x.dtype), batch, length, x.shape[-1], *_strides(x, m),
-                   values.data_ptr(), tokens.data_ptr(), values.shape[-1], temperature, int(normalize),
-                   loss.data_ptr(), _ptr(w), *(zero if w is None else _strides(w, m)), _ptr(g),
-                   *(zero if g is None else _strides(g, m)), stream_handle())
+        x, x_b, x_l, _x = _rows(logits, n, 1)
+        w, w_b, w_l, _w = _rows(weights, n, 0)
+        g, g_b, g_l, _g = _rows(grad, n, 1)
+        _call(logits.device, "dz_topk_distill", x, dtype_code(logits.dtype), batch, length, logits.shape[-1], x_b, x_l,
+              values.data_ptr(), tokens.data_ptr(), values.shape[-1], temperature, int(normalize), loss.data_ptr(), w, w_b, w_l,
+              g, g_b, g_l)
     return loss
 
 
@@ -293,15 +288,13 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: to
     if h.stride(1) != 1 and width > 1:
         h = h.contiguous()
     t = tokens.reshape(-1).long().contiguous()
-    lp = torch.empty(lead, dtype=torch.float32, device=hidden.device)
-    ent = torch.empty(lead, dtype=torch.float32, device=hidden.device)
+    lp = hidden.new_empty(lead, dtype=torch.float32)
+    ent = hidden.new_empty(lead, dtype=torch.float32)
     rows = h.shape[0]
     if rows:
         need = C.c_int64()
         L.call("dz_linear_token_logprobs_workspace", code, rows, width, vocab, C.byref(need))
         work = torch.empty(need.value, dtype=torch.uint8, device=hidden.device)
-        with _on(hidden.device):
-            L.call("dz_linear_token_logprobs", h.data_ptr(), weight.data_ptr(), code, rows, width, vocab, h.stride(0),
-                   weight.stride(0), t.data_ptr(), ignore_index, lp.data_ptr(), ent.data_ptr(), work.data_ptr(),
-                   need.value, stream_handle())
+        _call(hidden.device, "dz_linear_token_logprobs", h.data_ptr(), weight.data_ptr(), code, rows, width, vocab, h.stride(0),
+              weight.stride(0), t.data_ptr(), ignore_index, lp.data_ptr(), ent.data_ptr(), work.data_ptr(), need.value)
     return TokenLogprobs(lp, ent, None, None)
