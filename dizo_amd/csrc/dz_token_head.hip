@@ -186,9 +186,9 @@ __device__ __forceinline__ void to_lds(const void* p, uint32_t lds) {
 // All but the last N of this wave's loads are done, and every wave of the workgroup is here.
 template <int N>
 __device__ __forceinline__ void arrive() {
-  static_assert(N < 16, "a count of four bits");
+  static_assert(N < 64, "a count of six bits");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0F70 | N);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -421,13 +421,18 @@ __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint3
   }
   const uint32_t at = w.count ? w.live_of[r] : r;
   SoftStats st = SoftStats::of(-INFINITY);
-  for (uint32_t i = lane; i < tiles; i += 64) {
-    const float4 p = w.partial[(uint64_t)at * tiles + i];
-    SoftStats o;
-    o.m = p.x;
-    o.s = p.y;
-    o.t = p.z;
-    st.join(o, kLog2e);
+  for (uint32_t i = lane; i < tiles; i += 256) {  // four loads at a time
+    float4 p[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) p[j] = i + 64 * j < tiles ? w.partial[(uint64_t)at * tiles + i + 64 * j] : float4{-INFINITY, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      SoftStats o;
+      o.m = p[j].x;
+      o.s = p[j].y;
+      o.t = p[j].z;
+      st.join(o, kLog2e);
+    }
   }
   for (int off = 32; off >= 1; off >>= 1) {
     SoftStats o;
@@ -450,8 +455,9 @@ struct Plan {
   uint32_t row_tile, head_tile;
 };
 Plan plan_of(int dtype, uint32_t nrows) {
-  if (nrows <= 32) return Plan{32, 128};
-  if (nrows <= 64 || dtype == DZ_F32) return Plan{64, 128};
+  if (nrows <= 32) return Plan{32, 256};
+  if (nrows <= 64) return Plan{64, 256};
+  if (dtype == DZ_F32) return Plan{64, 128};
   return Plan{nrows <= 128 ? 128u : 256u, 256};
 }
 
@@ -470,8 +476,8 @@ void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, h
   const uint64_t es = sizeof(typename T::Elem);
   const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0 &&
                       (uint64_t)a.hidden_stride * es * a.nrows < (1ull << 32) && (uint64_t)a.weight_stride * es * p.head_tile < (1ull << 32);
-  if (p.row_tile == 32) return tile<T, 16, 2, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
-  if (a.nrows <= 64) return tile<T, 16, 4, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
+  if (p.row_tile == 32) return tile<T, 32, 1, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
+  if (a.nrows <= 64) return tile<T, 32, 2, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
   if constexpr (sizeof(typename T::Elem) == 4) return tile<T, 16, 2, 4, 2, 2, 2, false>(a, w, tiles, direct, st);
   else if (p.row_tile == 128) return tile<T, 32, 2, 4, 2, 2, 3, true>(a, w, tiles, direct, st);
   else return tile<T, 16, 4, 8, 4, 2, 2, false>(a, w, tiles, direct, st);
