@@ -449,16 +449,21 @@ __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint3
   }
 }
 
-// A workgroup's rows and head rows, by the number of rows: up to 64 rows the head's bytes bound the
-// kernel, from there on the products.
+// A workgroup's rows and head rows. Up to 64 rows the head's bytes bound the kernel, from there on the
+// products: large tiles then (256 x 256 read and write half of what 128 x 128 do). Where such tiles
+// would leave half of the 256 compute units without one, smaller ones that more of them share, and that keep more
+// slabs on their way, since the width is then walked through at the pace of a load (2,048 rows by
+// 1,000 tokens, 5,120 wide, fp16: 111 us in 32 large tiles, 49 in 256 small ones; at 128 large ones they
+// meet: 2,048 by 4,000, 1,024 wide 40 and 35 us, 700 by 16,000 in 189 tiles 38 and 42).
 struct Plan {
   uint32_t row_tile, head_tile;
 };
-Plan plan_of(int dtype, uint32_t nrows) {
-  if (nrows <= 32) return Plan{32, 256};
-  if (nrows <= 64) return Plan{64, 256};
-  if (dtype == DZ_F32) return Plan{64, 128};
-  return Plan{nrows <= 128 ? 128u : 256u, 256};
+Plan plan_of(int dtype, uint32_t nrows, uint32_t vocab) {
+  const uint32_t row_tile = nrows <= 32 ? 32 : nrows <= 64 ? 64 : nrows <= 128 ? 128 : 256;
+  const bool few_tiles = (uint64_t)head_tiles(vocab, 256) * ((nrows + row_tile - 1) / row_tile) <= 128;
+  if (nrows <= 64) return Plan{row_tile, few_tiles ? 64u : 256u};
+  if (dtype == DZ_F32 || few_tiles) return Plan{64, 128};
+  return Plan{row_tile, 256};
 }
 
 template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE>
@@ -476,22 +481,30 @@ void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, h
   const uint64_t es = sizeof(typename T::Elem);
   const bool direct = ((uint64_t)a.hidden | (uint64_t)a.weight | (uint64_t)a.hidden_stride * es | (uint64_t)a.weight_stride * es | a.width * es) % 16 == 0 &&
                       (uint64_t)a.hidden_stride * es * a.nrows < (1ull << 32) && (uint64_t)a.weight_stride * es * p.head_tile < (1ull << 32);
-  if (p.row_tile == 32) return tile<T, 32, 1, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
-  if (a.nrows <= 64) return tile<T, 32, 2, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
-  if constexpr (sizeof(typename T::Elem) == 4) return tile<T, 16, 2, 4, 2, 2, 2, false>(a, w, tiles, direct, st);
-  else if (p.row_tile == 128) return tile<T, 32, 2, 4, 2, 2, 3, true>(a, w, tiles, direct, st);
-  else return tile<T, 16, 4, 8, 4, 2, 2, false>(a, w, tiles, direct, st);
+  if (a.nrows <= 32) {
+    if (p.head_tile == 64) return tile<T, 16, 2, 1, 1, 4, 6, true>(a, w, tiles, direct, st);
+    return tile<T, 32, 1, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
+  }
+  if (a.nrows <= 64) {
+    if (p.head_tile == 64) return tile<T, 16, 4, 1, 1, 4, 5, true>(a, w, tiles, direct, st);
+    return tile<T, 32, 2, 2, 1, 4, 3, true>(a, w, tiles, direct, st);
+  }
+  if (p.head_tile == 128) return tile<T, 16, 2, 4, 2, 2, 3, false>(a, w, tiles, direct, st);
+  if constexpr (sizeof(typename T::Elem) == 2) {
+    if (p.row_tile == 128) return tile<T, 32, 2, 4, 2, 2, 3, true>(a, w, tiles, direct, st);
+    return tile<T, 16, 4, 8, 4, 2, 2, false>(a, w, tiles, direct, st);
+  }
 }
 
 }  // namespace
 
 int64_t head_workspace(int dtype, uint32_t nrows, uint32_t width, uint32_t vocab) {
   (void)width;
-  return (int64_t)(256 + 3 * align256((uint64_t)nrows * 4) + (uint64_t)nrows * head_tiles(vocab, plan_of(dtype, nrows).head_tile) * sizeof(float4));
+  return (int64_t)(256 + 3 * align256((uint64_t)nrows * 4) + (uint64_t)nrows * head_tiles(vocab, plan_of(dtype, nrows, vocab).head_tile) * sizeof(float4));
 }
 
 hipError_t launch_head(int dtype, const HeadRows& a, void* workspace, hipStream_t st) {
-  const Plan p = plan_of(dtype, a.nrows);
+  const Plan p = plan_of(dtype, a.nrows, a.vocab);
   Work w = work_of(workspace, a.nrows);
   const uint32_t tiles = head_tiles(a.vocab, p.head_tile);
   if (a.nrows <= 64) {  // one tile: all of them
