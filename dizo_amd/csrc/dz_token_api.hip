@@ -57,6 +57,17 @@ int32_t check_distinct(int64_t batch, int64_t length, int64_t bs, int64_t ls, in
   return DZ_OK;
 }
 
+// A gradient may be written over its logits, row over row; otherwise the two share nothing.
+int32_t check_apart(const void* logits, const void* grad, int64_t es, int64_t batch, int64_t length, int64_t vocab, int64_t logits_bs,
+                    int64_t logits_ls, int64_t grad_bs, int64_t grad_ls) {
+  if (logits == grad && (batch == 1 || logits_bs == grad_bs) && (length == 1 || logits_ls == grad_ls)) return DZ_OK;
+  const uint64_t x = (uint64_t)(uintptr_t)logits, g = (uint64_t)(uintptr_t)grad;
+  const uint64_t x_end = x + (uint64_t)(((batch - 1) * logits_bs + (length - 1) * logits_ls + vocab) * es);
+  const uint64_t g_end = g + (uint64_t)(((batch - 1) * grad_bs + (length - 1) * grad_ls + vocab) * es);
+  if (x < g_end && g < x_end) return api_fail(DZ_ERR_INVALID, "grad and logits overlap");
+  return DZ_OK;
+}
+
 int64_t size_of(int32_t dtype) { return dtype == DZ_DTYPE_F32 ? 4 : 2; }
 
 int32_t launched(hipError_t e, const char* what) {
@@ -98,6 +109,7 @@ int32_t dz_token_logprobs(const void* logits, int32_t dtype, int64_t batch, int6
     if (!weights && !entropy_weights) return api_fail(DZ_ERR_INVALID, "a gradient needs weights or entropy_weights");
     DZ_TRY(check_strided(grad, es, batch, length, grad_bs, grad_ls, vocab, "grad"));
     DZ_TRY(check_distinct(batch, length, grad_bs, grad_ls, vocab, "grad"));
+    DZ_TRY(check_apart(logits, grad, es, batch, length, vocab, logits_bs, logits_ls, grad_bs, grad_ls));
     if (weights) DZ_TRY(check_strided(weights, 4, batch, length, weights_bs, weights_ls, 1, "weights"));
     if (entropy_weights)
       DZ_TRY(check_strided(entropy_weights, 4, batch, length, entropy_weights_bs, entropy_weights_ls, 1, "entropy_weights"));
@@ -145,6 +157,7 @@ int32_t dz_topk_distill(const void* logits, int32_t dtype, int64_t batch, int64_
   if (grad) {
     DZ_TRY(check_strided(grad, es, batch, length, grad_bs, grad_ls, vocab, "grad"));
     DZ_TRY(check_distinct(batch, length, grad_bs, grad_ls, vocab, "grad"));
+    DZ_TRY(check_apart(logits, grad, es, batch, length, vocab, logits_bs, logits_ls, grad_bs, grad_ls));
     DZ_TRY(check_strided(weights, 4, batch, length, weights_bs, weights_ls, 1, "weights"));
   }
   dz::VocabRows a{};

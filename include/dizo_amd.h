@@ -240,7 +240,8 @@ int32_t dz_group_dot(dz_table* t, const uint64_t* other_ptrs, double* d_dot, flo
  * token outside the vocabulary gives NaN.
  * With grad (top = 0 then): grad_r = the gradient of
  * weights_r logprobs_r + entropy_weights_r entropy_r with respect to logits_r
- * (either weights may be NULL: zeros), in `dtype`. */
+ * (either weights may be NULL: zeros), in `dtype`; grad may be the logits
+ * themselves, with their strides, and else shares nothing with them. */
 int32_t dz_token_logprobs(const void* logits, int32_t dtype, int64_t batch, int64_t length, int64_t vocab,
                           int64_t logits_bs, int64_t logits_ls, const int64_t* tokens, int64_t tokens_bs,
                           int64_t tokens_ls, int64_t ignore_index, int32_t top, float* logprobs, float* entropy,
@@ -256,7 +257,8 @@ int32_t dz_token_logprobs(const void* logits, int32_t dtype, int64_t batch, int6
  * the rest of the teacher's mass is left out). Entries of weight 0 add nothing.
  * A row without entries is not read: 0. A token outside the vocabulary, or a
  * teacher value of NaN or +inf, gives NaN. With grad: grad_r = weights_r times the
- * gradient of loss[r] with respect to logits_r, in `dtype`. */
+ * gradient of loss[r] with respect to logits_r, in `dtype`; it may be written over
+ * the logits, as above. */
 int32_t dz_topk_distill(const void* logits, int32_t dtype, int64_t batch, int64_t length, int64_t vocab,
                         int64_t logits_bs, int64_t logits_ls, const float* teacher_values,
                         const int64_t* teacher_tokens, int32_t k, float temperature, int32_t normalize, float* loss,

@@ -623,3 +623,104 @@ def test_refusals():
     with pytest.raises(DzError, match="are needed"):
         L.call("dz_linear_token_logprobs", x.data_ptr(), x.data_ptr(), L.DZ_DTYPE_F16, 4, 16, 4, 16, 16, t.data_ptr(), -100, w.data_ptr(), w.data_ptr(),
                x.data_ptr(), n, stream_handle())
+
+
+# ------------------------------------------------- lengths of every variant --
+HELD = [8 * 2048, 8 * 2048 + 8, 8 * 4096 + 3, 8 * 512 * 13, 8 * 512 * 13 + 9, 8 * 8192 + 1, 8 * 1024 * 13 + 5, 8 * 16384, 8 * 16384 + 7, 8 * 32768 + 4099]
+
+
+@pytest.mark.parametrize("v", HELD)
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_rows_at_the_borders_of_what_a_workgroup_holds(dtype, v):
+    """Lengths at and past the sizes between which the kernels change, in 16-bit types and in fp32; more rows than one
+    workgroup a compute unit, and fewer."""
+    if dtype == torch.float32:
+        v = v // 2 + v % 2
+    x, t = rows(3, v, dtype, v), torch.tensor([v - 1, -100, v // 2]).cuda()
+    x[2, : v // 3] = -math.inf
+    check_score(x, t, top=50)
+    check_score(x, t)
+    w, u = torch.tensor([0.7, 1.0, -1.2]).cuda(), torch.tensor([0.1, 1.0, 0.3]).cuda()
+    _, g = T.token_logprobs_grad(x, t, w, u)
+    want, tol = score_grad_tol(f64(x), t.cpu().numpy(), f64(w), f64(u), dtype)
+    close(f64(g), want, tol, "gradient")
+    val, at = teacher(x.clamp(min=-30), 7, v, ragged=False)
+    check_distill(x.clamp(min=-30), val, at, 1.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("n", [255, 256, 257, 700])
+def test_many_and_few_rows_agree(dtype, n):
+    """The rule on the number of rows changes the kernel, not the results beyond rounding: rows of 9,000 tokens, twice over."""
+    x, t = rows(n, 9001, dtype, 3), some_tokens(n, 9001, 4)
+    check_score(x, t)
+    few, many = T.token_logprobs(x[:5], t[:5]), T.token_logprobs(x, t)
+    tol = lp_tol(f64(few.logprobs), 9001)
+    close(f64(many.logprobs[:5]), f64(few.logprobs), 2 * tol)
+
+
+def test_a_rising_maximum_moves_the_statistics():
+    """Logits that rise along the row by far more than the 8 binary orders that the running maximum may lag behind."""
+    v = 40000
+    ramp = torch.arange(v).float()
+    x = torch.stack([ramp / 64, ramp / 4096, -ramp / 64, torch.where(ramp < v - 3, -500.0, ramp - v), ramp.remainder(4096) / 8 - 100]).cuda()
+    t = torch.tensor([v - 1, v - 2, 0, v - 2, 4095]).cuda()
+    for dtype in TYPES:
+        check_score(x.to(dtype), t)
+        check_score(x.to(dtype), t, top=64)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_a_gradient_may_be_written_over_its_logits(dtype):
+    for v in (7, 1001, 40000, 150001):
+        x, t = rows(4, v, dtype, v), some_tokens(4, v, 1)
+        val, at = teacher(x, 3, 2, ragged=False)
+        w = torch.linspace(0.5, 1.5, 4).cuda()
+        _, want = T.token_logprobs_grad(x, t, w, w)
+        _, want2 = T.topk_distill_grad(x, val, at, w)
+        out, y = torch.empty(8, device="cuda"), x.clone()
+        L.call("dz_token_logprobs", y.data_ptr(), dtype_code(dtype), 1, 4, v, 0, v, t.data_ptr(), 0, 1, -100, 0, out.data_ptr(), out[4:].data_ptr(),
+               None, None, w.data_ptr(), 0, 1, w.data_ptr(), 0, 1, y.data_ptr(), 0, v, stream_handle())
+        assert torch.equal(y, want)
+        y = x.clone()
+        L.call("dz_topk_distill", y.data_ptr(), dtype_code(dtype), 1, 4, v, 0, v, val.data_ptr(), at.data_ptr(), 3, 1.0, 1, out.data_ptr(),
+               w.data_ptr(), 0, 1, y.data_ptr(), 0, v, stream_handle())
+        assert torch.equal(y, want2)
+        big = torch.empty(5 * v, dtype=dtype, device="cuda")
+        with pytest.raises(DzError, match="overlap"):
+            L.call("dz_topk_distill", big.data_ptr(), dtype_code(dtype), 1, 4, v, 0, v, val.data_ptr(), at.data_ptr(), 3, 1.0, 1, out.data_ptr(),
+                   w.data_ptr(), 0, 1, big[v:].data_ptr(), 0, v, stream_handle())
+
+
+@pytest.mark.parametrize("n, d, v", [(1, 64, 33000), (31, 72, 32800), (33, 136, 33001), (64, 64, 33000), (65, 64, 33000), (128, 200, 32800), (129, 64, 33000),
+                                     (300, 136, 17000), (520, 8, 12000), (257, 1000, 16500)])
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_token_logprobs_in_large_tiles(dtype, odd, n, d, v):
+    """Enough tiles for every compute unit, and more than one for some; widths that do and do not fill 16 bytes."""
+    h, w = head(n, d + odd, v, dtype, n + d + v)
+    t = some_tokens(n, v, 3)
+    t[-1] = v - 1
+    check_head(h, w, t)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_bad_head_rows_count_where_they_are(dtype):
+    """A head row of NaN makes every row a NaN; one that gives -inf takes no part; +inf makes a NaN."""
+    for n, d, v in ((20, 96, 200), (90, 64, 33000)):
+        h, w = head(n, d, v, dtype, 6)
+        h = h.abs() + 0.5
+        t = some_tokens(n, v, 2)
+        w[7] = -math.inf
+        out = T.linear_token_logprobs(h, w, t)
+        x = h.double().cpu() @ w.double().cpu().nan_to_num(neginf=0.0).T
+        x[:, 7] = -math.inf
+        lp, ent, _, _ = O.token_logprobs(x.numpy(), t.cpu().numpy())
+        off = 2 * 16 * E * math.sqrt(d) * float((h.double().square() @ w.double().nan_to_num(neginf=0.0).square().T).max().sqrt())
+        close(f64(out.logprobs), lp, lp_tol(lp, v) + off, "logprobs")
+        close(f64(out.entropy), ent, ent_tol(v) + off * (1 + math.log(v)), "entropy")
+        for bad in (math.nan, math.inf):
+            w[9, 3] = bad
+            out = T.linear_token_logprobs(h, w, t)
+            live = t != -100
+            assert out.logprobs[live].isnan().all() and out.entropy[live].isnan().all() and (out.logprobs[~live] == 0).all()
