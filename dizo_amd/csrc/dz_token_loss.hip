@@ -126,6 +126,7 @@ template <class T, int THREADS, int NV>
 struct Held {
   static constexpr int E = T::kPer16;
   u32x4 raw[NV];
+  float peak[NV];  // the largest logits of the vectors, after add_to
 
   __device__ __forceinline__ void load(const Row<T>& s, uint32_t j0) {
 #pragma unroll
@@ -150,7 +151,8 @@ struct Held {
     float m = st.m;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      m = fmaxf(m, largest(i));
+      peak[i] = largest(i);
+      m = fmaxf(m, peak[i]);
       afresh(raw[i]);
     }
     st.rebase(m, c);
@@ -266,11 +268,10 @@ __device__ __forceinline__ float key_value(uint64_t k) { return value_of((uint32
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 struct TopShared {
-  uint64_t group[kGroups];
-  uint32_t rank[kGroups];
+  uint32_t group[kGroups];
   uint64_t candidate[kCandidates];
   uint64_t wave[16];
-  uint64_t bound;
+  float floor;
   uint32_t count;
 };
 
@@ -286,54 +287,57 @@ __device__ __forceinline__ uint32_t above(const uint64_t* keys, uint32_t n, uint
 //
 // The maxima of 256 groups of threads give a bound: at least `top` logits are not
 // below the top-th largest of them, and about -256 ln(1 - top / 256) are. Those are
-// collected, and each finds its place by counting the ones above it. Where ties, or an
-// order that puts large logits in few groups, leave more than the collection holds, the
-// groups' maxima are taken again with their indexes (of a constant row the lowest indexes
-// stay); and where that is not enough, the largest below the last one is taken `top` times.
+// collected, and each finds its place by counting the ones above it. Where that leaves more
+// than the collection holds, because many are equal to the bound (a constant row, or a mask
+// that leaves fewer than `top`), those above it are collected, and then equal ones in the row's order;
+// and where an adverse order puts large logits in few groups, the largest below the last one is
+// taken `top` times.
 template <class T, int THREADS, int NV, class F>
 __device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, NV>& h, uint32_t top, float own_max, TopShared& sh, F emit) {
   constexpr int E = T::kPer16;
   const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const bool again = s.full > THREADS * NV;
   // f(logit, index), from memory, where speed is not asked for
   auto logits = [&](auto f) {
     for (uint32_t i = tid; i < s.v; i += THREADS) f((float)s.p[i], i);
-  };
-  // The top-th largest of the groups' keys goes to sh.bound (0: fewer groups than that have logits).
-  auto bound_of = [&](uint64_t best) {
-    if (THREADS > 256) best = max64(best, __shfl_xor((unsigned long long)best, 32, 64));
-    if (THREADS > 512) best = max64(best, __shfl_xor((unsigned long long)best, 16, 64));
-    constexpr uint32_t kGroupsOfWave = THREADS == 256 ? 64 : THREADS == 512 ? 32 : 16;
-    __syncthreads();
-    const uint32_t mine = (tid >> 6) * kGroupsOfWave + lane;
-    if (lane < kGroupsOfWave) sh.group[mine] = best;
-    if (tid < kGroups) sh.rank[tid] = 0;
-    if (tid == 0) {
-      sh.bound = 0;
-      sh.count = 0;
-    }
-    __syncthreads();
-    constexpr uint32_t kParts = THREADS / kGroups, kPart = kGroups / kParts;
-    const uint32_t g = tid % kGroups, part = tid / kGroups;
-    const uint32_t r = above(sh.group + part * kPart, kPart, sh.group[g]);
-    if (kParts > 1) atomicAdd(&sh.rank[g], r);  // whole numbers: any order
-    else sh.rank[g] = r;
-    __syncthreads();
-    if (tid < kGroups && sh.rank[tid] == top - 1 && sh.group[tid]) sh.bound = sh.group[tid];
-    __syncthreads();
-    return sh.bound;
   };
   auto collect = [&](uint64_t key) {
     const uint32_t n = atomicAdd(&sh.count, 1u);
     if (n < kCandidates) sh.candidate[n] = key;
   };
-  // groups of equal maxima are told apart by their number; the bound is the value alone
-  const float floor = key_value(bound_of(((uint64_t)order_of(own_max) << 32) | (0xffffu - tid)));
+  uint32_t best = order_of(own_max);
+  if (THREADS > 256) best = max(best, (uint32_t)__shfl_xor((int)best, 32, 64));
+  if (THREADS > 512) best = max(best, (uint32_t)__shfl_xor((int)best, 16, 64));
+  constexpr uint32_t kGroupsOfWave = THREADS == 256 ? 64 : THREADS == 512 ? 32 : 16;
+  if (lane < kGroupsOfWave) sh.group[(tid >> 6) * kGroupsOfWave + lane] = best;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  if (tid < 64) {
+    // the top-th largest, bit by bit: the largest number that `top` groups are not below. The bits that a
+    // 16-bit type does not have are 0 of positive values, and 1 in the order of negative ones.
+    constexpr int kLowest = std::is_same<T, TypeBF16>::value ? 16 : std::is_same<T, TypeF16>::value ? 13 : 0;
+    uint32_t k[kGroups / 64], bound = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups / 64; ++i) k[i] = sh.group[64 * i + lane];
+#pragma unroll
+    for (int bit = 31; bit >= kLowest; --bit) {
+      const uint32_t next = bound | (1u << bit);
+      uint32_t n = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < kGroups / 64; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= next));
+      if (n >= top) bound = next;
+    }
+    if (!(bound >> 31)) bound |= (1u << kLowest) - 1;
+    if (lane == 0) sh.floor = value_of(bound);
+  }
+  __syncthreads();
+  const float floor = sh.floor;
   for (uint32_t j0 = 0; j0 < s.full; j0 += THREADS * NV) {
-    if (s.full > THREADS * NV) h.load(s, j0);
+    if (again) h.load(s, j0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t j = j0 + i * THREADS + tid;
-      if (h.largest(i) >= floor && j < s.full) {
+      if ((again ? h.largest(i) : h.peak[i]) >= floor && j < s.full) {
 #pragma unroll
         for (int k = 0; k < E; ++k) {
           const float x = element<T>(h.raw[i], k);
@@ -346,15 +350,20 @@ __device__ __forceinline__ void alternatives(const Row<T>& s, Held<T, THREADS, N
   __syncthreads();
   uint32_t count = sh.count;
   if (count > kCandidates) {
-    uint64_t best = 0;
-    logits([&](float x, uint32_t i) { best = max64(best, order_key(x, i)); });
-    const uint64_t bound = bound_of(best);
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
     logits([&](float x, uint32_t i) {
-      const uint64_t key = order_key(x, i);
-      if (key >= bound) collect(key);
+      if (x > floor) collect(order_key(x, i));
     });
     __syncthreads();
     count = sh.count;
+    for (uint32_t i0 = 0; count < top && i0 < s.v; i0 += THREADS) {  // the lowest indexes among equals
+      __syncthreads();
+      if (i0 + tid < s.v && (float)s.p[i0 + tid] == floor) collect(order_key(floor, i0 + tid));
+      __syncthreads();
+      count = sh.count;
+    }
   }
   if (count <= kCandidates) {
     for (uint32_t n = tid; n < count; n += THREADS) {
