@@ -201,8 +201,42 @@ __device__ __forceinline__ void arrive_lds() {
   asm volatile("" ::: "memory");
 }
 
+// The row that is the at-th of the live ones, and its token (2^32 - 1: none that is asked for).
+__device__ __forceinline__ uint32_t row_of(const Work& w, uint32_t at, uint32_t count) {
+  if (at >= count) at = count - 1;
+  return w.count ? w.row_of[at] : at;
+}
+__device__ __forceinline__ uint32_t token_of(const HeadRows& a, const Work& w, uint32_t at, uint32_t count) {
+  const int64_t t = at < count ? a.tokens[row_of(w, at, count)] : -1;
+  return t >= 0 && t < (int64_t)a.vocab ? (uint32_t)t : ~0u;
+}
+
+// The statistics of a tile whose logits are there, from all waves of the workgroup.
+template <int M, int TF, int VF, int WT, int WV>
+__device__ __forceinline__ void finish_tile(const HeadRows& a, const Work& w, Acc<M> (&acc)[TF][VF], const uint32_t (&tok)[TF],
+                                            SoftStats (&sh)[WV][M * TF * WT], uint32_t vt, uint32_t mt, uint32_t count, uint32_t tiles) {
+  constexpr uint32_t MT = M * TF * WT, NT = M * VF * WV;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = wave % WT, wv = wave / WT;
+  float* token_logit[TF];
+  SoftStats st[TF];
+#pragma unroll
+  for (int i = 0; i < TF; ++i) token_logit[i] = w.token_logit + mt * MT + (wt * TF + i) * M + lane % M;
+  lane_stats<M>(acc, vt * NT + wv * M * VF, a.vocab, tok, token_logit, st);
+  if (lane < M)
+#pragma unroll
+    for (int i = 0; i < TF; ++i) sh[wv][(wt * TF + i) * M + lane] = st[i];
+  arrive_lds();
+  for (uint32_t r = threadIdx.x; r < MT; r += 64 * WT * WV) {
+    const uint32_t at = mt * MT + r;
+    if (at >= count) break;
+    SoftStats s = sh[0][r];
+    for (int i = 1; i < WV; ++i) s.join(sh[i][r], kLog2e);
+    w.partial[(uint64_t)at * tiles + vt] = float4{s.m, s.s, s.t, 0.f};
+  }
+}
+
 template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE, bool DIRECT>
-__global__ __launch_bounds__(64 * WT * WV, M == 32 ? 1 : 2) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
+__global__ __launch_bounds__(64 * WT * WV, M == 32 || STAGES == 5 ? 1 : 2) void head_tile_kernel(HeadRows a, Work w, uint32_t tiles) {
   using Elem = typename T::Elem;
   using V = typename T::V;
   constexpr uint32_t E = T::kPer16, K = 8 * E, WAVES = WT * WV;
@@ -221,11 +255,6 @@ __global__ __launch_bounds__(64 * WT * WV, M == 32 ? 1 : 2) void head_tile_kerne
   uint32_t tile = blockIdx.x / 8;
   if (!mtiles || !there(tile)) return;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = wave % WT, wv = wave / WT;
-  auto row_of = [&](uint32_t at) {
-    if (at >= count) at = count - 1;
-    return w.count ? w.row_of[at] : at;
-  };
-
   // A load takes 8 rows of hidden states or of the head; this lane's row of load i, at its chunk.
   constexpr uint32_t HLOADS = MT / 8 / WAVES;
   static_assert(MT % (8 * WAVES) == 0, "a wave's load i is of the same kind for all waves");
@@ -238,7 +267,7 @@ __global__ __launch_bounds__(64 * WT * WV, M == 32 ? 1 : 2) void head_tile_kerne
   uint32_t rows[HLOADS];
   auto take_rows = [&](uint32_t n) {  // the rows of a tile, ahead of its loads
 #pragma unroll
-    for (uint32_t i = 0; i < HLOADS; ++i) rows[i] = row_of(n % mtiles * MT + i * WAVES * 8 + lane_row);
+    for (uint32_t i = 0; i < HLOADS; ++i) rows[i] = row_of(w, n % mtiles * MT + i * WAVES * 8 + lane_row, count);
   };
   auto take_tile = [&](uint32_t n) {
     const uint32_t v0 = head_tile(n) * NT;
@@ -285,36 +314,12 @@ __global__ __launch_bounds__(64 * WT * WV, M == 32 ? 1 : 2) void head_tile_kerne
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // The tokens of a tile's rows, loaded when its products begin.
-  uint32_t tok[TF];
+  uint32_t tok[TF];  // of the tile's rows, loaded when its products begin
   auto take_tokens = [&](uint32_t n) {
 #pragma unroll
-    for (int i = 0; i < TF; ++i) {
-      const uint32_t at = n % mtiles * MT + (wt * TF + i) * M + lane % M;
-      const int64_t t = at < count ? a.tokens[row_of(at)] : -1;
-      tok[i] = t >= 0 && t < (int64_t)a.vocab ? (uint32_t)t : ~0u;
-    }
+    for (int i = 0; i < TF; ++i) tok[i] = token_of(a, w, n % mtiles * MT + (wt * TF + i) * M + lane % M, count);
   };
-  // The statistics of the tile whose logits are there.
-  auto finish = [&](uint32_t n) {
-    const uint32_t vt = head_tile(n), mt = n % mtiles;
-    float* token_logit[TF];
-    SoftStats st[TF];
-#pragma unroll
-    for (int i = 0; i < TF; ++i) token_logit[i] = w.token_logit + mt * MT + (wt * TF + i) * M + lane % M;
-    lane_stats<M>(acc, vt * NT + wv * M * VF, a.vocab, tok, token_logit, st);
-    if (lane < M)
-#pragma unroll
-      for (int i = 0; i < TF; ++i) sh[wv][(wt * TF + i) * M + lane] = st[i];
-    arrive_lds();
-    for (uint32_t r = threadIdx.x; r < MT; r += 64 * WAVES) {
-      const uint32_t at = mt * MT + r;
-      if (at >= count) break;
-      SoftStats st = sh[0][r];
-      for (int i = 1; i < WV; ++i) st.join(sh[i][r], kLog2e);
-      w.partial[(uint64_t)at * tiles + vt] = float4{st.m, st.s, st.t, 0.f};
-    }
-  };
+  auto finish = [&](uint32_t n) { finish_tile<M, TF, VF, WT, WV>(a, w, acc, tok, sh, head_tile(n), n % mtiles, count, tiles); };
 
   const uint32_t slabs = (a.width + K - 1) / K;
   if constexpr (DIRECT) {
@@ -411,6 +416,191 @@ __global__ __launch_bounds__(64 * WT * WV, M == 32 ? 1 : 2) void head_tile_kerne
   }
 }
 
+// Many rows of fp32. The fp32 matrix instructions multiply at 1/16 of the rate of bf16's, so each
+// number is taken as a sum of three bf16 numbers, hi + mid + lo, each the rounding of what the ones
+// before leave (27 bits together), and a product as the six of their nine products that are not
+// below 2^-25 of it: what is left out (two of at most 2^-26, one of 2^-34) is less than a rounding of an fp32 sum, which every
+// product of the fp32 instructions has too. Against a kernel with fp32 instructions, by 50,272 tokens, 768
+// wide: 2,048 rows 869 us for 1,230 (184 TFLOP/s of products of fp32 numbers), 300 rows, of whose 384 in tiles 84
+// are not there, 209 for 243. Taking apart is as much work for the vector units as the products
+// are for the matrix units; 128 rows a tile share it (64: 1,066 us).
+//
+// An infinity among the operands (or a number that rounds to one) has no such sum: its parts make a
+// NaN. A row of hidden states with one has no distribution whatever the head is; the logits of a head row with one are
+// taken again by themselves.
+//
+// A workgroup of 2 x 4 waves takes 128 live rows by 256 head rows, in slabs of 32 columns, which come
+// through registers: one slab is on its way, one is being taken apart into LDS, and one multiplies. A part's 16-byte chunk c
+// of row r lies at r * 64 + (c ^ split_swizzle(r)) * 16.
+__device__ __forceinline__ uint32_t split_swizzle(uint32_t r) {
+  const uint32_t q = r >> 2 & 3;  // 0, 2, 3, 1: rows 0 to 3 and 12 to 15 of one chunk are read with rows 4 to 11 of the next
+  return ((q ^ q >> 1) & 1) << 1 | q >> 1;
+}
+constexpr int kSplitTF = 4, kSplitVF = 4, kSplitWT = 2, kSplitWV = 4;
+constexpr uint32_t kSplitMT = 16 * kSplitTF * kSplitWT, kSplitNT = 16 * kSplitVF * kSplitWV;
+
+__device__ __forceinline__ void take_apart(const float (&x)[8], bf16x8 (&part)[3]) {
+  float r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = x[j];
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[p][j] = (__bf16)r[j];
+    const u32x4 bits = __builtin_bit_cast(u32x4, part[p]);
+    if (p < 2)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] -= __uint_as_float(j & 1 ? bits[j / 2] & 0xffff0000u : bits[j / 2] << 16);
+  }
+}
+
+__global__ __launch_bounds__(512, 2) void head_split_kernel(HeadRows a, Work w, uint32_t tiles) {
+  constexpr int TF = kSplitTF, VF = kSplitVF, WT = kSplitWT, WV = kSplitWV;
+  constexpr uint32_t MT = kSplitMT, NT = kSplitNT, ROWS = MT + NT, UNITS = ROWS * 4, PER = (UNITS + 511) / 512;
+  __shared__ __attribute__((aligned(256))) char slots[2][3][ROWS * 64];
+  __shared__ SoftStats sh[WV][MT];
+  __shared__ uint32_t bad[MT];  // rows with a number that is not finite
+  const uint32_t count = *w.count, mtiles = (count + MT - 1) / MT;
+  // tiles in the order of head_tile_kernel
+  const uint32_t vt = mtiles ? blockIdx.x / 8 / mtiles * 8 + blockIdx.x % 8 : tiles, mt = mtiles ? blockIdx.x / 8 % mtiles : 0;
+  if (vt >= tiles) return;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wv = wave / WT;
+  if (tid < MT) bad[tid] = 0;
+
+  // this thread's units of 8 columns: unit u is chunk u % 4 of row u / 4
+  const float* from[PER];
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) {
+    const uint32_t r = (i * 512 + tid) / 4 < ROWS ? (i * 512 + tid) / 4 : ROWS - 1;
+    const uint32_t v = vt * NT + r - MT;
+    from[i] = r < MT ? (const float*)a.hidden + (int64_t)row_of(w, mt * MT + r, count) * a.hidden_stride
+                     : (const float*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
+    from[i] += tid % 4 * 8;
+  }
+  uint32_t tok[TF];
+#pragma unroll
+  for (int i = 0; i < TF; ++i) tok[i] = token_of(a, w, mt * MT + (wt * TF + i) * 16 + lane % 16, count);
+  Acc<16> acc[TF][VF];
+#pragma unroll
+  for (int i = 0; i < TF; ++i)
+#pragma unroll
+    for (int j = 0; j < VF; ++j) acc[i][j] = Acc<16>(0.f);
+
+  struct Slab {
+    f32x4 x[PER][2];
+  };
+  Slab even, odd;
+  auto fetch_whole = [&](Slab& s, uint32_t k) {
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i)
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n) s.x[i][n] = *(const Frag<TypeF32>::Loose*)(from[i] + (uint64_t)k * 32 + 4 * n);
+  };
+  auto fetch = [&](Slab& s, uint32_t k) {  // any slab
+    if ((k + 1) * 32 <= a.width) return fetch_whole(s, k);
+    const uint32_t at = k * 32 + tid % 4 * 8;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i)
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n) s.x[i][n] = load16<TypeF32>(from[i] + (uint64_t)k * 32 + 4 * n, 0, at + 4 * n < a.width ? a.width - at - 4 * n : 0);
+  };
+  auto put = [&](const Slab& s, char (&there)[3][ROWS * 64], int i) {
+    if (i * 512 + wave * 64 >= UNITS) return;
+    const uint32_t r = (i * 512 + tid) / 4, to = r * 64 + ((tid & 3) ^ split_swizzle(r)) * 16;
+    float x[8];
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = s.x[i][j / 4][j % 4];
+      if (i * 512 + wave * 64 < MT * 4) finite &= fabsf(x[j]) < INFINITY;
+    }
+    if (!finite) bad[r] = 1;
+    bf16x8 part[3];
+    take_apart(x, part);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *(bf16x8*)(there[p] + to) = part[p];
+  };
+  const uint32_t at = (lane % 16) * 64 + ((lane / 16) ^ split_swizzle(lane % 16)) * 16;
+  auto products = [&](const char (&here)[3][ROWS * 64], auto between) {
+    bf16x8 t[3][TF], v[2][3];
+    auto read_v = [&](int j) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) v[j & 1][p] = *(const bf16x8*)(here[p] + (MT + (wv * VF + j) * 16) * 64 + at);
+    };
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int i = 0; i < TF; ++i) t[p][i] = *(const bf16x8*)(here[p] + (wt * TF + i) * 16 * 64 + at);
+    read_v(0);
+#pragma unroll
+    for (int j = 0; j < VF; ++j) {
+      if (j + 1 < VF) read_v(j + 1);
+      constexpr int kPart[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};  // the small ones first
+#pragma unroll
+      for (int n = 0; n < 6; ++n)
+#pragma unroll
+        for (int i = 0; i < TF; ++i) acc[i][j] = Frag<TypeBF16>::mma(v[j & 1][kPart[n][0]], t[kPart[n][1]][i], acc[i][j]);
+      between(j);
+    }
+  };
+  const uint32_t slabs = (a.width + 31) / 32;
+  __syncthreads();  // `bad` is cleared
+  fetch(even, 0);
+  if (slabs > 1) fetch(odd, 1);
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) put(even, slots[0], i);
+  // Slab k multiplies; slab k + 1, which `next` holds, is taken apart; slab k + 2 is asked for. The
+  // steps whose slab k + 2 is a whole one have no branch at their loads, at which the compiler would wait.
+  auto step = [&](uint32_t k, Slab& next, Slab& after, auto whole) {
+    arrive_lds();
+    if (whole) fetch_whole(after, k + 2);
+    else if (k + 2 < slabs) fetch(after, k + 2);
+    const bool more = whole || k + 1 < slabs;
+    products(slots[k & 1], [&](int j) {
+      if (more && j < (int)PER) put(next, slots[~k & 1], j);
+    });
+  };
+  uint32_t k = 0;
+  for (; k + 3 < a.width / 32; k += 2) {
+    step(k, odd, even, std::true_type());
+    step(k + 1, even, odd, std::true_type());
+  }
+  for (; k < slabs; k += 2) {
+    step(k, odd, even, std::false_type());
+    if (k + 1 < slabs) step(k + 1, even, odd, std::false_type());
+  }
+
+  // logits that infinities have spoilt
+  bool spoilt = false;
+#pragma unroll
+  for (int i = 0; i < TF; ++i)
+#pragma unroll
+    for (int j = 0; j < VF; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) spoilt |= acc[i][j][e] != acc[i][j][e];
+  if (__any(spoilt)) {
+#pragma unroll 1
+    for (int n = 0; n < TF * VF * 4; ++n) {
+      const int ni = n / (VF * 4), nj = n / 4 % VF, ne = n % 4;
+      float x = 0.f;
+#pragma unroll
+      for (int m = 0; m < TF * VF * 4; ++m)
+        if (m == n) x = acc[m / (VF * 4)][m / 4 % VF][m % 4];
+      const uint32_t r = (wt * TF + ni) * 16 + lane % 16, v = vt * NT + (wv * VF + nj) * 16 + 4 * (lane / 16) + ne;
+      if (x != x && !bad[r] && v < a.vocab) {
+        const float* h = (const float*)a.hidden + (int64_t)row_of(w, mt * MT + r, count) * a.hidden_stride;
+        const float* e = (const float*)a.weight + (int64_t)v * a.weight_stride;
+        x = 0.f;
+        for (uint32_t c = 0; c < a.width; ++c) x = __builtin_fmaf(h[c], e[c], x);
+      }
+#pragma unroll
+      for (int m = 0; m < TF * VF * 4; ++m)
+        if (m == n) acc[m / (VF * 4)][m / 4 % VF][m % 4] = x;
+    }
+  }
+  finish_tile<16, TF, VF, WT, WV>(a, w, acc, tok, sh, vt, mt, count, tiles);
+}
+
 // One wave joins a row's statistics over the head's tiles.
 __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint32_t tiles) {
   const uint32_t r = blockIdx.x, lane = threadIdx.x;
@@ -462,7 +652,8 @@ Plan plan_of(int dtype, uint32_t nrows, uint32_t vocab) {
   const uint32_t row_tile = nrows <= 32 ? 32 : nrows <= 64 ? 64 : nrows <= 128 ? 128 : 256;
   const bool few_tiles = (uint64_t)head_tiles(vocab, 256) * ((nrows + row_tile - 1) / row_tile) <= 128;
   if (nrows <= 64) return Plan{row_tile, few_tiles ? 64u : 256u};
-  if (dtype == DZ_F32 || few_tiles) return Plan{64, 128};
+  if (few_tiles) return Plan{64, 128};
+  if (dtype == DZ_F32) return Plan{kSplitMT, kSplitNT};
   return Plan{row_tile, 256};
 }
 
@@ -493,6 +684,8 @@ void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, h
   if constexpr (sizeof(typename T::Elem) == 2) {
     if (p.row_tile == 128) return tile<T, 32, 2, 4, 2, 2, 3, true>(a, w, tiles, direct, st);
     return tile<T, 16, 4, 8, 4, 2, 2, false>(a, w, tiles, direct, st);
+  } else {
+    head_split_kernel<<<(tiles + 7) / 8 * 8 * ((a.nrows + kSplitMT - 1) / kSplitMT), 512, 0, st>>>(a, w, tiles);
   }
 }
 
