@@ -437,6 +437,7 @@ __device__ __forceinline__ uint32_t split_swizzle(uint32_t r) {
   return ((q ^ q >> 1) & 1) << 1 | q >> 1;
 }
 constexpr int kSplitTF = 4, kSplitVF = 4, kSplitWT = 2, kSplitWV = 4;
+constexpr uint32_t kSplitGrid = 256;  // one workgroup a compute unit
 constexpr uint32_t kSplitMT = 16 * kSplitTF * kSplitWT, kSplitNT = 16 * kSplitVF * kSplitWV;
 
 __device__ __forceinline__ void take_apart(const float (&x)[8], bf16x8 (&part)[3]) {
@@ -462,143 +463,147 @@ __global__ __launch_bounds__(512, 2) void head_split_kernel(HeadRows a, Work w, 
   __shared__ uint32_t bad[MT];  // rows with a number that is not finite
   const uint32_t count = *w.count, mtiles = (count + MT - 1) / MT;
   // tiles in the order of head_tile_kernel
-  const uint32_t vt = mtiles ? blockIdx.x / 8 / mtiles * 8 + blockIdx.x % 8 : tiles, mt = mtiles ? blockIdx.x / 8 % mtiles : 0;
-  if (vt >= tiles) return;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wv = wave / WT;
-  if (tid < MT) bad[tid] = 0;
+  uint32_t n = blockIdx.x / 8, vt, mt;
+  if (!mtiles) return;
+  for (; (vt = n / mtiles * 8 + blockIdx.x % 8) < tiles; n += gridDim.x / 8) {
+    mt = n % mtiles;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wv = wave / WT;
+    if (tid < MT) bad[tid] = 0;
 
-  // this thread's units of 8 columns: unit u is chunk u % 4 of row u / 4
-  const float* from[PER];
+    // this thread's units of 8 columns: unit u is chunk u % 4 of row u / 4
+    const float* from[PER];
 #pragma unroll
-  for (uint32_t i = 0; i < PER; ++i) {
-    const uint32_t r = (i * 512 + tid) / 4 < ROWS ? (i * 512 + tid) / 4 : ROWS - 1;
-    const uint32_t v = vt * NT + r - MT;
-    from[i] = r < MT ? (const float*)a.hidden + (int64_t)row_of(w, mt * MT + r, count) * a.hidden_stride
-                     : (const float*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
-    from[i] += tid % 4 * 8;
-  }
-  uint32_t tok[TF];
-#pragma unroll
-  for (int i = 0; i < TF; ++i) tok[i] = token_of(a, w, mt * MT + (wt * TF + i) * 16 + lane % 16, count);
-  Acc<16> acc[TF][VF];
-#pragma unroll
-  for (int i = 0; i < TF; ++i)
-#pragma unroll
-    for (int j = 0; j < VF; ++j) acc[i][j] = Acc<16>(0.f);
-
-  struct Slab {
-    f32x4 x[PER][2];
-  };
-  Slab even, odd;
-  auto fetch_whole = [&](Slab& s, uint32_t k) {
-#pragma unroll
-    for (uint32_t i = 0; i < PER; ++i)
-#pragma unroll
-      for (uint32_t n = 0; n < 2; ++n) s.x[i][n] = *(const Frag<TypeF32>::Loose*)(from[i] + (uint64_t)k * 32 + 4 * n);
-  };
-  auto fetch = [&](Slab& s, uint32_t k) {  // any slab
-    if ((k + 1) * 32 <= a.width) return fetch_whole(s, k);
-    const uint32_t at = k * 32 + tid % 4 * 8;
-#pragma unroll
-    for (uint32_t i = 0; i < PER; ++i)
-#pragma unroll
-      for (uint32_t n = 0; n < 2; ++n) s.x[i][n] = load16<TypeF32>(from[i] + (uint64_t)k * 32 + 4 * n, 0, at + 4 * n < a.width ? a.width - at - 4 * n : 0);
-  };
-  auto put = [&](const Slab& s, char (&there)[3][ROWS * 64], int i) {
-    if (i * 512 + wave * 64 >= UNITS) return;
-    const uint32_t r = (i * 512 + tid) / 4, to = r * 64 + ((tid & 3) ^ split_swizzle(r)) * 16;
-    float x[8];
-    bool finite = true;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = s.x[i][j / 4][j % 4];
-      if (i * 512 + wave * 64 < MT * 4) finite &= fabsf(x[j]) < INFINITY;
+    for (uint32_t i = 0; i < PER; ++i) {
+      const uint32_t r = (i * 512 + tid) / 4 < ROWS ? (i * 512 + tid) / 4 : ROWS - 1;
+      const uint32_t v = vt * NT + r - MT;
+      from[i] = r < MT ? (const float*)a.hidden + (int64_t)row_of(w, mt * MT + r, count) * a.hidden_stride
+                       : (const float*)a.weight + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
+      from[i] += tid % 4 * 8;
     }
-    if (!finite) bad[r] = 1;
-    bf16x8 part[3];
-    take_apart(x, part);
+    uint32_t tok[TF];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *(bf16x8*)(there[p] + to) = part[p];
-  };
-  const uint32_t at = (lane % 16) * 64 + ((lane / 16) ^ split_swizzle(lane % 16)) * 16;
-  auto products = [&](const char (&here)[3][ROWS * 64], auto between) {
-    bf16x8 t[3][TF], v[2][3];
-    auto read_v = [&](int j) {
+    for (int i = 0; i < TF; ++i) tok[i] = token_of(a, w, mt * MT + (wt * TF + i) * 16 + lane % 16, count);
+    Acc<16> acc[TF][VF];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) v[j & 1][p] = *(const bf16x8*)(here[p] + (MT + (wv * VF + j) * 16) * 64 + at);
+    for (int i = 0; i < TF; ++i)
+#pragma unroll
+      for (int j = 0; j < VF; ++j) acc[i][j] = Acc<16>(0.f);
+
+    struct Slab {
+      f32x4 x[PER][2];
     };
+    Slab even, odd;
+    auto fetch_whole = [&](Slab& s, uint32_t k) {
 #pragma unroll
-    for (int p = 0; p < 3; ++p)
+      for (uint32_t i = 0; i < PER; ++i)
 #pragma unroll
-      for (int i = 0; i < TF; ++i) t[p][i] = *(const bf16x8*)(here[p] + (wt * TF + i) * 16 * 64 + at);
-    read_v(0);
+        for (uint32_t n = 0; n < 2; ++n) s.x[i][n] = *(const Frag<TypeF32>::Loose*)(from[i] + (uint64_t)k * 32 + 4 * n);
+    };
+    auto fetch = [&](Slab& s, uint32_t k) {  // any slab
+      if ((k + 1) * 32 <= a.width) return fetch_whole(s, k);
+      const uint32_t at = k * 32 + tid % 4 * 8;
 #pragma unroll
-    for (int j = 0; j < VF; ++j) {
-      if (j + 1 < VF) read_v(j + 1);
-      constexpr int kPart[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};  // the small ones first
+      for (uint32_t i = 0; i < PER; ++i)
 #pragma unroll
-      for (int n = 0; n < 6; ++n)
+        for (uint32_t n = 0; n < 2; ++n) s.x[i][n] = load16<TypeF32>(from[i] + (uint64_t)k * 32 + 4 * n, 0, at + 4 * n < a.width ? a.width - at - 4 * n : 0);
+    };
+    auto put = [&](const Slab& s, char (&there)[3][ROWS * 64], int i) {
+      if (i * 512 + wave * 64 >= UNITS) return;
+      const uint32_t r = (i * 512 + tid) / 4, to = r * 64 + ((tid & 3) ^ split_swizzle(r)) * 16;
+      float x[8];
+      bool finite = true;
 #pragma unroll
-        for (int i = 0; i < TF; ++i) acc[i][j] = Frag<TypeBF16>::mma(v[j & 1][kPart[n][0]], t[kPart[n][1]][i], acc[i][j]);
-      between(j);
-    }
-  };
-  const uint32_t slabs = (a.width + 31) / 32;
-  __syncthreads();  // `bad` is cleared
-  fetch(even, 0);
-  if (slabs > 1) fetch(odd, 1);
-#pragma unroll
-  for (uint32_t i = 0; i < PER; ++i) put(even, slots[0], i);
-  // Slab k multiplies; slab k + 1, which `next` holds, is taken apart; slab k + 2 is asked for. The
-  // steps whose slab k + 2 is a whole one have no branch at their loads, at which the compiler would wait.
-  auto step = [&](uint32_t k, Slab& next, Slab& after, auto whole) {
-    arrive_lds();
-    if (whole) fetch_whole(after, k + 2);
-    else if (k + 2 < slabs) fetch(after, k + 2);
-    const bool more = whole || k + 1 < slabs;
-    products(slots[k & 1], [&](int j) {
-      if (more && j < (int)PER) put(next, slots[~k & 1], j);
-    });
-  };
-  uint32_t k = 0;
-  for (; k + 3 < a.width / 32; k += 2) {
-    step(k, odd, even, std::true_type());
-    step(k + 1, even, odd, std::true_type());
-  }
-  for (; k < slabs; k += 2) {
-    step(k, odd, even, std::false_type());
-    if (k + 1 < slabs) step(k + 1, even, odd, std::false_type());
-  }
-
-  // logits that infinities have spoilt
-  bool spoilt = false;
-#pragma unroll
-  for (int i = 0; i < TF; ++i)
-#pragma unroll
-    for (int j = 0; j < VF; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) spoilt |= acc[i][j][e] != acc[i][j][e];
-  if (__any(spoilt)) {
-#pragma unroll 1
-    for (int n = 0; n < TF * VF * 4; ++n) {
-      const int ni = n / (VF * 4), nj = n / 4 % VF, ne = n % 4;
-      float x = 0.f;
-#pragma unroll
-      for (int m = 0; m < TF * VF * 4; ++m)
-        if (m == n) x = acc[m / (VF * 4)][m / 4 % VF][m % 4];
-      const uint32_t r = (wt * TF + ni) * 16 + lane % 16, v = vt * NT + (wv * VF + nj) * 16 + 4 * (lane / 16) + ne;
-      if (x != x && !bad[r] && v < a.vocab) {
-        const float* h = (const float*)a.hidden + (int64_t)row_of(w, mt * MT + r, count) * a.hidden_stride;
-        const float* e = (const float*)a.weight + (int64_t)v * a.weight_stride;
-        x = 0.f;
-        for (uint32_t c = 0; c < a.width; ++c) x = __builtin_fmaf(h[c], e[c], x);
+      for (int j = 0; j < 8; ++j) {
+        x[j] = s.x[i][j / 4][j % 4];
+        if (i * 512 + wave * 64 < MT * 4) finite &= fabsf(x[j]) < INFINITY;
       }
+      if (!finite) bad[r] = 1;
+      bf16x8 part[3];
+      take_apart(x, part);
 #pragma unroll
-      for (int m = 0; m < TF * VF * 4; ++m)
-        if (m == n) acc[m / (VF * 4)][m / 4 % VF][m % 4] = x;
+      for (int p = 0; p < 3; ++p) *(bf16x8*)(there[p] + to) = part[p];
+    };
+    const uint32_t at = (lane % 16) * 64 + ((lane / 16) ^ split_swizzle(lane % 16)) * 16;
+    auto products = [&](const char (&here)[3][ROWS * 64], auto between) {
+      bf16x8 t[3][TF], v[2][3];
+      auto read_v = [&](int j) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p) v[j & 1][p] = *(const bf16x8*)(here[p] + (MT + (wv * VF + j) * 16) * 64 + at);
+      };
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+#pragma unroll
+        for (int i = 0; i < TF; ++i) t[p][i] = *(const bf16x8*)(here[p] + (wt * TF + i) * 16 * 64 + at);
+      read_v(0);
+#pragma unroll
+      for (int j = 0; j < VF; ++j) {
+        if (j + 1 < VF) read_v(j + 1);
+        constexpr int kPart[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};  // the small ones first
+#pragma unroll
+        for (int n = 0; n < 6; ++n)
+#pragma unroll
+          for (int i = 0; i < TF; ++i) acc[i][j] = Frag<TypeBF16>::mma(v[j & 1][kPart[n][0]], t[kPart[n][1]][i], acc[i][j]);
+        between(j);
+      }
+    };
+    const uint32_t slabs = (a.width + 31) / 32;
+    __syncthreads();  // `bad` is cleared
+    fetch(even, 0);
+    if (slabs > 1) fetch(odd, 1);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) put(even, slots[0], i);
+    // Slab k multiplies; slab k + 1, which `next` holds, is taken apart; slab k + 2 is asked for. The
+    // steps whose slab k + 2 is a whole one have no branch at their loads, at which the compiler would wait.
+    auto step = [&](uint32_t k, Slab& next, Slab& after, auto whole) {
+      arrive_lds();
+      if (whole) fetch_whole(after, k + 2);
+      else if (k + 2 < slabs) fetch(after, k + 2);
+      const bool more = whole || k + 1 < slabs;
+      products(slots[k & 1], [&](int j) {
+        if (more && j < (int)PER) put(next, slots[~k & 1], j);
+      });
+    };
+    uint32_t k = 0;
+    for (; k + 3 < a.width / 32; k += 2) {
+      step(k, odd, even, std::true_type());
+      step(k + 1, even, odd, std::true_type());
     }
+    for (; k < slabs; k += 2) {
+      step(k, odd, even, std::false_type());
+      if (k + 1 < slabs) step(k + 1, even, odd, std::false_type());
+    }
+
+    // logits that infinities have spoilt
+    bool spoilt = false;
+#pragma unroll
+    for (int i = 0; i < TF; ++i)
+#pragma unroll
+      for (int j = 0; j < VF; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) spoilt |= acc[i][j][e] != acc[i][j][e];
+    if (__any(spoilt)) {
+#pragma unroll 1
+      for (int n = 0; n < TF * VF * 4; ++n) {
+        const int ni = n / (VF * 4), nj = n / 4 % VF, ne = n % 4;
+        float x = 0.f;
+#pragma unroll
+        for (int m = 0; m < TF * VF * 4; ++m)
+          if (m == n) x = acc[m / (VF * 4)][m / 4 % VF][m % 4];
+        const uint32_t r = (wt * TF + ni) * 16 + lane % 16, v = vt * NT + (wv * VF + nj) * 16 + 4 * (lane / 16) + ne;
+        if (x != x && !bad[r] && v < a.vocab) {
+          const float* h = (const float*)a.hidden + (int64_t)row_of(w, mt * MT + r, count) * a.hidden_stride;
+          const float* e = (const float*)a.weight + (int64_t)v * a.weight_stride;
+          x = 0.f;
+          for (uint32_t c = 0; c < a.width; ++c) x = __builtin_fmaf(h[c], e[c], x);
+        }
+#pragma unroll
+        for (int m = 0; m < TF * VF * 4; ++m)
+          if (m == n) acc[m / (VF * 4)][m / 4 % VF][m % 4] = x;
+      }
+    }
+    finish_tile<16, TF, VF, WT, WV>(a, w, acc, tok, sh, vt, mt, count, tiles);
+    __syncthreads();
   }
-  finish_tile<16, TF, VF, WT, WV>(a, w, acc, tok, sh, vt, mt, count, tiles);
 }
 
 // One wave joins a row's statistics over the head's tiles.
@@ -659,10 +664,10 @@ Plan plan_of(int dtype, uint32_t nrows, uint32_t vocab) {
 
 template <class T, int M, int TF, int VF, int WT, int WV, int STAGES, bool ONCE>
 void tile(const HeadRows& a, const Work& w, uint32_t tiles, bool direct, hipStream_t st) {
-  const uint32_t all = (tiles + 7) / 8 * 8 * ((a.nrows + M * TF * WT - 1) / (M * TF * WT));
+  const uint64_t all = (uint64_t)((tiles + 7) / 8 * 8) * ((a.nrows + M * TF * WT - 1) / (M * TF * WT));
   constexpr uint32_t kLds = STAGES * (M * TF * WT + M * VF * WV) * 128 + WV * M * TF * WT * sizeof(SoftStats);
   constexpr uint32_t resident = 256 * (160 * 1024 / kLds < 8 / (WT * WV) ? 160 * 1024 / kLds : 8 / (WT * WV));  // two waves a SIMD
-  const uint32_t grid = all < resident ? all : resident;
+  const uint32_t grid = all < resident ? (uint32_t)all : resident;
   if (direct) head_tile_kernel<T, M, TF, VF, WT, WV, STAGES, ONCE, true><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
   else head_tile_kernel<T, M, TF, VF, WT, WV, 2, false, false><<<grid, 64 * WT * WV, 0, st>>>(a, w, tiles);
 }
@@ -685,7 +690,8 @@ void products(const HeadRows& a, const Work& w, const Plan& p, uint32_t tiles, h
     if (p.row_tile == 128) return tile<T, 32, 2, 4, 2, 2, 3, true>(a, w, tiles, direct, st);
     return tile<T, 16, 4, 8, 4, 2, 2, false>(a, w, tiles, direct, st);
   } else {
-    head_split_kernel<<<(tiles + 7) / 8 * 8 * ((a.nrows + kSplitMT - 1) / kSplitMT), 512, 0, st>>>(a, w, tiles);
+    const uint64_t all = (uint64_t)((tiles + 7) / 8 * 8) * ((a.nrows + kSplitMT - 1) / kSplitMT);
+    head_split_kernel<<<all < kSplitGrid ? (uint32_t)all : kSplitGrid, 512, 0, st>>>(a, w, tiles);
   }
 }
 

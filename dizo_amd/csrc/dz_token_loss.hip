@@ -113,7 +113,10 @@ struct Row {
   __device__ Row(const Elem* p_, uint32_t v_) : p(p_), v(v_), full(v_ / E), rem(v_ % E) {}
 
   // vector j0 + this thread's number: a base that is the same for the workgroup, and an offset
-  __device__ __forceinline__ static auto at(const Elem* p, uint32_t j0) { return (const Loose*)(p + (uint64_t)j0 * E) + threadIdx.x; }
+  __device__ __forceinline__ static auto at(const Elem* p, uint32_t j0) {
+    const uint32_t offset = threadIdx.x * 16;  // of 32 bits: the base stays in scalar registers
+    return (const Loose*)((const char*)(p + (uint64_t)j0 * E) + offset);
+  }
   __device__ __forceinline__ u32x4 load(uint32_t j0) const { return __builtin_bit_cast(u32x4, (typename T::V)__builtin_nontemporal_load(at(p, j0))); }
   // this thread's element after the last whole vector, and its index
   __device__ __forceinline__ bool has_extra() const { return threadIdx.x < rem; }
@@ -167,13 +170,14 @@ struct Held {
 // the row in `h` where it fits.
 template <class T, int THREADS, int NV, bool ENTROPY>
 __device__ __forceinline__ Stats<true> row_stats(const Row<T>& s, Held<T, THREADS, NV>& h, float c, Stats<true>* waves, float& own_max) {
-  const float extra = s.extra();
-  auto st = Stats<true>::of(extra);
-  st.template add_far<ENTROPY, 1>([&](int) { return extra; }, c);
+  auto st = Stats<true>::of(-INFINITY);
   for (uint32_t j0 = 0; j0 < s.full; j0 += THREADS * NV) {
     h.load(s, j0);
     h.template add_to<ENTROPY>(st, c);
   }
+  const float extra = s.extra();
+  st.rebase(fmaxf(st.m, extra), c);
+  st.template add_far<ENTROPY, 1>([&](int) { return extra; }, c);
   own_max = st.m;
   return block_stats<THREADS, ENTROPY>(st, c, waves);
 }
@@ -187,8 +191,7 @@ __device__ __forceinline__ SoftStats stream_stats(const Row<T>& s, float c, Soft
   Held<T, THREADS, NV> a, b, last;
   const uint32_t whole = s.full / STEP;  // steps
   last.load(s, whole * STEP);
-  const float extra = s.extra();
-  auto st = SoftStats::of(extra);
+  auto st = SoftStats::of(-INFINITY);
   auto add = [&](Held<T, THREADS, NV>& h) {
     constexpr int N = NV * T::kPer16;
     float x[N];
@@ -204,7 +207,6 @@ __device__ __forceinline__ SoftStats stream_stats(const Row<T>& s, float c, Soft
     if (__any(!((m - st.m) * c <= 8.f))) st.rebase(fmaxf(st.m, m), c);
     st.template add<ENTROPY, N>([&](int n) { return x[n]; }, c);
   };
-  st.template add<ENTROPY, 1>([&](int) { return extra; }, c);
   if (whole) {
     uint32_t n = 0;
     a.load_whole(s, 0);
@@ -223,6 +225,9 @@ __device__ __forceinline__ SoftStats stream_stats(const Row<T>& s, float c, Soft
     }
   }
   if (whole * STEP < s.full) add(last);
+  const float extra = s.extra();
+  st.rebase(fmaxf(st.m, extra), c);
+  st.template add<ENTROPY, 1>([&](int) { return extra; }, c);
   return block_stats<THREADS, ENTROPY>(st, c, waves);
 }
 
