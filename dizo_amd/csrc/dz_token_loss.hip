@@ -471,7 +471,7 @@ __global__ __launch_bounds__(THREADS, TOP && THREADS == 512 ? 6 : 1) void token_
 struct TeacherShared {
   float w[kMaxTeacher];
   float x[kMaxTeacher];  // the student's logits of the entries
-  int32_t idx[kMaxTeacher];
+  __attribute__((aligned(16))) int32_t idx[kMaxTeacher + 4];  // -1: no entry; fours are read
   float total;
   int32_t bad;
 };
@@ -510,13 +510,14 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
       sh.w[j] = in ? t : -INFINITY;
       if (in) tm = fmaxf(tm, t);
     }
+    if (lane < 4) sh.idx[k + lane] = -1;
     tm = reduce64(tm, Max());
     if (a.normalize) {
       float ts = 0.f;
       for (uint32_t j = lane; j < k; j += 64)
         if (sh.idx[j] >= 0) ts += exp2_hw((sh.w[j] - tm) * kLog2e);
       ts = reduce64(ts, Add());
-      lse = __builtin_fmaf(kLn2, log2_hw(ts), 0.f);
+      lse = kLn2 * log2_hw(ts);
       bad |= tm == -INFINITY;
     } else {
       tm = 0.f;
@@ -559,12 +560,17 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
       const int32_t i = sh.idx[j];
       if (i < 0) continue;
       bool first = true;  // that names this token
-      float w = 0.f;
-      for (uint32_t n = 0; n < k; ++n)
-        if (sh.idx[n] == i) {
-          if (n < j) first = false;
-          w += sh.w[n];
-        }
+      float w = sh.w[j];
+#pragma unroll 4
+      for (uint32_t n = 0; n < k; n += 4) {
+        const i32x4 four = *(const i32x4*)(sh.idx + n);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+          if (four[e] == i && n + e != j) {
+            if (n + e < j) first = false;
+            w += sh.w[n + e];
+          }
+      }
       if (first) g[i] = (Elem)(up * (total * exp2_hw(__builtin_fmaf(sh.x[j] - m0, c, -log2s)) - w));
     }
   }
