@@ -42,6 +42,7 @@ struct VocabRows {
   RowStrides weights_s;
   void* grad;
   RowStrides grad_s;
+  bool past_caches;  // of the gradient's stores
 };
 
 constexpr int kMaxTop = 128;      // alternatives of a row
