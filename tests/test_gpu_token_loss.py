@@ -724,3 +724,18 @@ def test_bad_head_rows_count_where_they_are(dtype):
             out = T.linear_token_logprobs(h, w, t)
             live = t != -100
             assert out.logprobs[live].isnan().all() and out.entropy[live].isnan().all() and (out.logprobs[~live] == 0).all()
+
+
+def test_head_and_hidden_rows_gigabytes_apart():
+    """Offsets between 2^31 and 2^32 bytes inside a tile: 64 head rows, and then 60 hidden states, 33,000,000 elements apart."""
+    far = 33_000_000
+    buf = torch.empty(63 * far + 64, dtype=torch.bfloat16, device="cuda")
+    h, w0 = head(60, 64, 64, torch.bfloat16, 4)
+    t = some_tokens(60, 64, 5)
+    w = buf.as_strided((64, 64), (far, 1))
+    w.copy_(w0)
+    want = check_head(h, w, t)
+    assert torch.equal(want.logprobs, T.linear_token_logprobs(h, w0, t).logprobs)
+    x = buf.as_strided((60, 64), (far, 1))
+    x.copy_(h)
+    assert torch.equal(T.linear_token_logprobs(x, w0, t).logprobs, want.logprobs)
