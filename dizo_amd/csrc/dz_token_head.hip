@@ -162,7 +162,7 @@ __device__ __forceinline__ void lane_stats(Acc<M> (&acc)[TF][VF], uint32_t v0, u
   }
 }
 
-// A workgroup of WT x WV waves takes 16 TF WT live rows by 16 VF WV head rows, in slabs of 128
+// A workgroup of WT x WV waves takes M TF WT live rows by M VF WV head rows, in slabs of 128
 // bytes a row through LDS, STAGES of them: the next ones are on their way while this one's
 // products run.
 // What bounds it: up to 64 rows reading the head (64 rows by 50,272 tokens, 5,120 wide, fp16: 95 us, 5.4
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(512, 2) void head_split_kernel(HeadRows a, Work w, 
   __shared__ __attribute__((aligned(256))) char slots[2][3][ROWS * 64];
   __shared__ SoftStats sh[WV][MT];
   __shared__ uint32_t bad[MT];  // rows with a number that is not finite
-  const uint32_t count = *w.count, mtiles = (count + MT - 1) / MT;
+  const uint32_t count = w.count ? *w.count : a.nrows, mtiles = (count + MT - 1) / MT;
   // tiles in the order of head_tile_kernel
   uint32_t n = blockIdx.x / 8, vt, mt;
   if (!mtiles) return;
@@ -709,7 +709,7 @@ hipError_t launch_head(int dtype, const HeadRows& a, void* workspace, hipStream_
   const Plan p = plan_of(dtype, a.nrows, a.vocab);
   Work w = work_of(workspace, a.nrows);
   const uint32_t tiles = head_tiles(a.vocab, p.head_tile);
-  if (a.nrows <= 64) {  // one tile: all of them
+  if (a.nrows <= p.row_tile) {  // one tile, whichever rows are asked for: all of them
     w.count = nullptr;
   } else {
     live_rows_kernel<<<1, 1024, 0, st>>>(a, w);

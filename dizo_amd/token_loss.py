@@ -267,7 +267,7 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: to
                           ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
     """token_logprobs of the logits hidden @ weight.T, which are not stored (and not rounded: products
     and sums are fp32). hidden (..., width) and weight (vocab, width) of one dtype; the width has to be
-    contiguous. Ignored rows give 0 (from 65 rows on they are not multiplied). Where autograd records (hidden or weight require a
+    contiguous. Ignored rows give 0 (of many rows, they are not multiplied). Where autograd records (hidden or weight require a
     gradient), the logits are made by F.linear and scored by token_logprobs instead."""
     what = "linear_token_logprobs"
     if not hidden.is_cuda:
