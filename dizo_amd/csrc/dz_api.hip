@@ -29,9 +29,14 @@ int32_t fail(int32_t code, const std::string& msg) {
   return code;
 }
 
-int32_t hip_fail(hipError_t e, const char* what) {
-  return fail(DZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+// The error's text. The runtime's record of it is cleared: it is reported here, and would otherwise be
+// taken by the next launch of this thread, the caller's own included, for its own.
+std::string hip_text(hipError_t e) {
+  (void)hipGetLastError();
+  return hipGetErrorString(e);
 }
+
+int32_t hip_fail(hipError_t e, const char* what) { return fail(DZ_ERR_HIP, std::string(what) + ": " + hip_text(e)); }
 
 int elem_size(int32_t dtype) { return dtype == DZ_DTYPE_F32 ? 4 : 2; }
 
@@ -175,7 +180,7 @@ int32_t check_range(uint64_t p, uint64_t bytes, const char* what, int32_t i) {
   hipError_t e = hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)(uintptr_t)p);
   if (e != hipSuccess) {
     return fail(DZ_ERR_RANGE, std::string(what) + " of tensor " + std::to_string(i) +
-                                  " is not device memory: " + hipGetErrorString(e));
+                                  " is not device memory: " + hip_text(e));
   }
   const uint64_t b = (uint64_t)(uintptr_t)base;
   if (p < b || p + bytes > b + (uint64_t)size) {
@@ -190,12 +195,13 @@ int32_t check_range(uint64_t p, uint64_t bytes, const char* what, int32_t i) {
 namespace dz {
 
 int32_t api_fail(int32_t code, const std::string& msg) { return fail(code, msg); }
+int32_t api_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
 
 int32_t api_check_range(const void* p, uint64_t bytes, const char* what) {
   hipDeviceptr_t base = nullptr;
   size_t size = 0;
   const hipError_t e = hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)(uintptr_t)p);
-  if (e != hipSuccess) return fail(DZ_ERR_RANGE, std::string(what) + " is not device memory: " + hipGetErrorString(e));
+  if (e != hipSuccess) return fail(DZ_ERR_RANGE, std::string(what) + " is not device memory: " + hip_text(e));
   const uint64_t b = (uint64_t)(uintptr_t)base, q = (uint64_t)(uintptr_t)p;
   if (q < b || bytes > (uint64_t)size || q - b > (uint64_t)size - bytes)
     return fail(DZ_ERR_RANGE, std::string(what) + " range exceeds its allocation");

@@ -70,9 +70,7 @@ int32_t check_apart(const void* logits, const void* grad, int64_t es, int64_t ba
 
 int64_t size_of(int32_t dtype) { return dtype == DZ_DTYPE_F32 ? 4 : 2; }
 
-int32_t launched(hipError_t e, const char* what) {
-  return e == hipSuccess ? DZ_OK : api_fail(DZ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
-}
+int32_t launched(hipError_t e, const char* what) { return e == hipSuccess ? DZ_OK : dz::api_hip_fail(e, what); }
 
 }  // namespace
 
