@@ -15,6 +15,8 @@ dimension has to be contiguous; rows may be strided (``logits[:, :-1]`` is read 
 fp32: a row's sums are kept in fp32, and rounding them to a 16-bit type would leave a log probability
 of -10 with a step of 1/16 (bf16).
 
+Derivatives are reverse-mode, and first order; an operand with a forward-mode tangent is refused.
+
 Work goes to the current stream of the logits' device; tensors made on another stream are the
 caller's to order, as with torch's own operators.
 """
@@ -24,6 +26,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn.functional as F
 
 from . import _lib as L
@@ -67,6 +70,15 @@ def _check_rows(what: str, name: str, t: torch.Tensor, lead, device, dtypes) -> 
         _fail(what, f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
     if t.shape != lead:
         _fail(what, f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+
+
+def _no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Derivatives are reverse-mode only: results of a dual tensor would lack its tangent without a word.
+    (Dual tensors exist only inside a dual level; calls outside of one cost a comparison.)"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail(what, "forward-mode derivatives are not supported (an operand carries a tangent)")
 
 
 _INT = (torch.int64, torch.int32)
@@ -140,6 +152,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_lp, d_ent, _tlp, _ttok):
         logits, tokens = ctx.saved_tensors
+        _no_tangents("token_logprobs' backward", d_lp, d_ent)
         if d_lp is None and d_ent is None:
             return None, None, None, None
         grad = _grad_like(logits)
@@ -147,8 +160,9 @@ class _TokenLogprobs(torch.autograd.Function):
         return grad, None, None, None
 
 
-def _score_checked(what, logits, tokens, top, ignore_index):
+def _score_checked(what, logits, tokens, top, weights=None, entropy_weights=None):
     _check_logits(what, logits)
+    _no_tangents(what, logits, weights, entropy_weights)
     _check_rows(what, "tokens", tokens, logits.shape[:-1], logits.device, _INT)
     if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
         _fail(what, f"top must be 0 to {min(MAX_TOP, logits.shape[-1])}, got {top}")
@@ -163,7 +177,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     Rows whose token is ignore_index are not read: 0, 0, -inf and -1. Another token outside the
     vocabulary gives NaN, and so does a row without a distribution (NaN, +inf, or nothing above -inf).
     Gradients flow to the logits through logprobs and entropy; the alternatives are a report."""
-    tokens = _score_checked("token_logprobs", logits, tokens, top, ignore_index)
+    tokens = _score_checked("token_logprobs", logits, tokens, top)
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top, ignore_index))
     return TokenLogprobs(*_score(logits, tokens, top, ignore_index, None, None, None))
@@ -175,7 +189,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, weights: Opt
     """token_logprobs, and the gradient of sum(weights logprobs) + sum(entropy_weights entropy) with
     respect to the logits, in their dtype. Weights are fp32, shaped like tokens; None stands for zeros."""
     what = "token_logprobs_grad"
-    tokens = _score_checked(what, logits, tokens, 0, ignore_index)
+    tokens = _score_checked(what, logits, tokens, 0, weights, entropy_weights)
     if weights is None and entropy_weights is None:
         _fail(what, "weights or entropy_weights are needed")
     for name, w in (("weights", weights), ("entropy_weights", entropy_weights)):
@@ -213,13 +227,15 @@ class _TopkDistill(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss):
         logits, values, tokens = ctx.saved_tensors
+        _no_tangents("topk_distill's backward", d_loss)
         grad = _grad_like(logits)
         _distill(logits, values, tokens, *ctx.how, d_loss, grad)
         return grad, None, None, None, None
 
 
-def _distill_checked(what, logits, values, tokens, temperature):
+def _distill_checked(what, logits, values, tokens, temperature, weights=None):
     _check_logits(what, logits)
+    _no_tangents(what, logits, values, weights)
     lead, k = logits.shape[:-1], values.shape[-1] if values.dim() else 0
     if not 1 <= k <= MAX_TEACHER:
         _fail(what, f"a teacher has 1 to {MAX_TEACHER} entries a row, got {k}")
@@ -255,7 +271,7 @@ def topk_distill_grad(logits: torch.Tensor, values: torch.Tensor, tokens: torch.
     """topk_distill, and the gradient of sum(weights loss) with respect to the logits, in their dtype.
     weights: fp32, one per row."""
     what = "topk_distill_grad"
-    values, tokens = _distill_checked(what, logits, values, tokens, temperature)
+    values, tokens = _distill_checked(what, logits, values, tokens, temperature, weights)
     _check_rows(what, "weights", weights, logits.shape[:-1], logits.device, _F32)
     with torch.no_grad():
         grad = _grad_like(logits)
@@ -272,6 +288,7 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: to
     what = "linear_token_logprobs"
     if not hidden.is_cuda:
         _fail(what, f"hidden must live on a GPU, got {hidden.device}")
+    _no_tangents(what, hidden, weight)
     code = dtype_code(hidden.dtype)
     if weight.device != hidden.device or weight.dtype != hidden.dtype:
         _fail(what, f"weight is {weight.dtype} on {weight.device}, hidden {hidden.dtype} on {hidden.device}")
