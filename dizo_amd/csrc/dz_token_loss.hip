@@ -471,7 +471,7 @@ __global__ __launch_bounds__(THREADS, TOP && THREADS == 512 ? 6 : 1) void token_
     const float m0 = st.m == -INFINITY ? 0.f : st.m;
     const auto d = [&](float xi) {
       const float z = __builtin_fmaf(xi - m0, kLog2e, -log2s);
-      return -exp2_hw(z) * __builtin_fmaf(ul, fmaxf(z, -1e30f), wu);
+      return -exp2_hw(z) * __builtin_fmaf(ul, fmaxf(z, kLowestY), wu);
     };
     write_row<T, THREADS, NV>(s, h, g, a.past_caches, d);
     __syncthreads();  // the row's stores are done before the token's is written again

@@ -37,6 +37,10 @@ struct TypeBF16 {
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
 
+// 2^y is 0 from y = -150 on; a product with y takes no less than this for it, so that it is 0 there too
+// (-inf would make it a NaN, and a large bound one that overflows with a factor beside it).
+constexpr float kLowestY = -256.f;
+
 // Statistics of logits x: their maximum m, s = sum 2^y and t = sum 2^y y with y = x c - K,
 // c = log2 e / temperature. K is m c rounded to fp32: what its rounding leaves shifts every y alike,
 // so that log softmax(x) = ln 2 (y - log2 s) and the entropy ln 2 (log2 s - t / s), of which both terms
@@ -64,8 +68,7 @@ struct Stats {
     return y == -INFINITY ? __builtin_fmaf(-kLn2, log2_hw(s), (x - m) * inv) : kLn2 * (y - log2_hw(s));
   }
 
-  // Adds x(0) .. x(N - 1). 2^y y is 0 where y is -inf, which has to be said to a product. (A NaN logit
-  // leaves a NaN in s.)
+  // Adds x(0) .. x(N - 1). (A NaN logit leaves a NaN in s.)
   template <bool ENTROPY, int N, class F>
   __device__ __forceinline__ void add_far(F x, float c) {
     const float m0 = m == -INFINITY ? 0.f : m;
@@ -75,7 +78,7 @@ struct Stats {
       if (!FAR) y = in_range(m * c) ? y_plain(x(i), c) : y;
       const float e = exp2_hw(y);
       s += e;
-      if (ENTROPY) t = __builtin_fmaf(e, fmaxf(y, -1e30f), t);
+      if (ENTROPY) t = __builtin_fmaf(e, fmaxf(y, kLowestY), t);
     }
   }
   // The same with one operation for y, and none for its limit unless it is met.
@@ -104,7 +107,7 @@ struct Stats {
       const float k = m * c, k2 = m2 * c;
       const float d = in_range(k) && in_range(k2) ? k - k2 : (m - m2) * c;
       const float f = exp2_hw(d);
-      t = f * __builtin_fmaf(fmaxf(d, -1e30f), s, t);
+      t = f * __builtin_fmaf(fmaxf(d, kLowestY), s, t);
       s *= f;
     }
     m = m2;
