@@ -507,14 +507,14 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
     return;
   }
   const float inv = 1.f / a.temperature, c = kLog2e * inv;
-  const float tinv = a.normalize ? inv : 1.f;
+  const float tinv = a.normalize ? inv : 1.f;  // of differences: a value at fp32's limits may leave it divided by T
   float tm = -INFINITY, lse = 0.f;
   bool bad = false;
   if (tid < 64) {
     for (uint32_t j = lane; j < k; j += 64) {
       const int64_t i = tokens[j];
       const bool in = i >= 0 && i < (int64_t)a.vocab;
-      const float t = values[j] * tinv;
+      const float t = values[j];
       bad |= i != -1 && (!in || !(t < INFINITY));
       sh.idx[j] = in ? (int32_t)i : -1;
       sh.x[j] = in ? (float)x[i] : 0.f;
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
     if (a.normalize) {
       float ts = 0.f;
       for (uint32_t j = lane; j < k; j += 64)
-        if (sh.idx[j] >= 0) ts += exp2_hw((sh.w[j] - tm) * kLog2e);
+        if (sh.idx[j] >= 0) ts += exp2_hw((sh.w[j] - tm) * tinv * kLog2e);
       ts = reduce64(ts, Add());
       lse = kLn2 * log2_hw(ts);
       bad |= tm == -INFINITY;
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
   if (tid < 64) {
     float loss = 0.f, total = 0.f;
     for (uint32_t j = lane; j < k; j += 64) {
-      const float lnw = (sh.w[j] - tm) - lse;
+      const float lnw = (sh.w[j] - tm) * tinv - lse;
       const float w = sh.idx[j] >= 0 ? exp2_hw(lnw * kLog2e) : 0.f;
       if (w > 0.f) loss += w * (lnw - st.lnq(sh.x[j], c, inv));
       sh.w[j] = w;

@@ -1,10 +1,12 @@
 """dizo_amd.token_loss on the GPU at the ends of what its operands can hold."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from dizo_amd import token_loss as T
+from oracle import vocab as O
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +32,46 @@ def test_large_entropy_weights_beside_masked_columns(v, exponent):
     _, g = T.token_logprobs_grad(x, t, None, u * 2.0**exponent)
     assert torch.equal(g, one * 2.0**exponent)
     assert not g[:, v // 3:].any() and not g.isnan().any()
+
+
+@pytest.mark.parametrize("tau", [0.25, 0.5, 0.7, 1.0, 3.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_teacher_values_at_the_limits_of_fp32(dtype, tau):
+    """Entries masked by the type's lowest value, and its largest: a row of equal ones is uniform at every temperature,
+    and the lowest have weight 0 beside others.
+
+    Differences to the largest value are 0, exact or past every exponent here, so that a weight is off by
+    (2 k + 10) e; the loss T^2 sum w (ln w - ln q) by T^2 e (v / 256 + 60 + 2 k + 4 max |x| / T) (1 + sum w (|ln w| + |ln q|)),
+    a gradient by T e (v / 256 + 100 + 2 k + 4 max |x| / T) (q + w)."""
+    v, k = 500, 6
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = rows(7, v, torch.float32, 3)
+    at = torch.stack([torch.randperm(v, generator=torch.Generator().manual_seed(i))[:k] for i in range(7)]).cuda()
+    val = torch.zeros(7, k, dtype=dtype, device="cuda")
+    val[0] = low
+    val[1] = high
+    val[2, 1:] = low
+    val[3] = low
+    val[3, 2] = high
+    val[4] = low
+    val[4, 3:] = -math.inf
+    val[5, ::2] = high
+    val[6] = low
+    at[6, 1:] = -1
+    w = torch.linspace(0.5, 1.5, 7, device="cuda")
+    loss, grad = T.topk_distill_grad(x, val, at, w, temperature=tau)
+    x64, val64, at64, w64 = (t.double().cpu().numpy() for t in (x, val, at, w))
+    at64 = at64.astype(np.int64)
+    want, want_grad = O.topk_distill(x64, val64, at64, tau, True, w64)
+    assert np.isfinite(want).all()
+    logq = O.log_softmax(x64 / tau)
+    e, steps = 2.0**-24, v / 256 + 60 + 2 * k + 4 * np.abs(x64).max() / tau
+    for r in range(7):
+        tw, tl = O.teacher_weights(val64[r], at64[r], v, tau, True)
+        there = tw > 0
+        size = (tw[there] * (np.abs(tl[there]) + np.abs(logq[r][at64[r][there]]))).sum()
+        assert abs(float(loss[r]) - want[r]) <= tau * tau * e * steps * (1 + size), r
+        term = np.exp(logq[r])
+        np.add.at(term, at64[r][there], tw[there])
+        assert (np.abs(grad[r].double().cpu().numpy() - want_grad[r]) <= tau * w64[r] * e * (steps + 40) * term + 2.0**-126).all(), r
+    assert torch.equal(T.topk_distill(x, val, at, temperature=tau).isnan(), torch.zeros(7, dtype=torch.bool, device="cuda"))
