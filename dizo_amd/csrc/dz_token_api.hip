@@ -144,8 +144,10 @@ int32_t dz_topk_distill(const void* logits, int32_t dtype, int64_t batch, int64_
   if (k < 1 || k > dz::kMaxTeacher)
     return api_fail(DZ_ERR_INVALID, "teacher entries out of range: " + std::to_string(k) + " (1 to " +
                                         std::to_string(dz::kMaxTeacher) + ")");
-  if (!(temperature > 0.f) || !isfinite(temperature) || !isfinite(1.f / temperature))
-    return api_fail(DZ_ERR_INVALID, "temperature must be positive and finite");
+  // the loss has the square as a factor: one that is 0 or infinite leaves nothing of it, and the inverse
+  // times log2 e is finite then
+  if (!(temperature > 0.f) || !isnormal(temperature * temperature))
+    return api_fail(DZ_ERR_INVALID, "temperature must be positive and finite, and so its square (2^-63 to 2^64)");
   if (batch * length == 0) return DZ_OK;
   const int64_t es = size_of(dtype), n = batch * length;
   DZ_TRY(check_strided(logits, es, batch, length, logits_bs, logits_ls, vocab, "logits"));

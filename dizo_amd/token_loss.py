@@ -241,8 +241,8 @@ def _distill_checked(what, logits, values, tokens, temperature, weights=None):
         _fail(what, f"a teacher has 1 to {MAX_TEACHER} entries a row, got {k}")
     _check_rows(what, "values", values, (*lead, k), logits.device, (torch.float32, torch.float16, torch.bfloat16))
     _check_rows(what, "tokens", tokens, (*lead, k), logits.device, _INT)
-    if not (0.0 < temperature < float("inf")):
-        _fail(what, f"temperature must be positive and finite, got {temperature}")
+    if not (2.0**-63 <= temperature < 2.0**64):
+        _fail(what, f"temperature must be positive and finite, and so its square (2^-63 to 2^64), got {temperature}")
     if values.requires_grad and torch.is_grad_enabled():
         _fail(what, "the teacher's values take no gradient (detach them)")
     return values.detach().float().contiguous(), tokens.long().contiguous()
@@ -254,6 +254,7 @@ def topk_distill(logits: torch.Tensor, values: torch.Tensor, tokens: torch.Tenso
 
         T^2 sum_j w_j (log w_j - log softmax(logits / T)[tokens_j])
 
+    (T from 2^-63 up to 2^64, so that its square is one of fp32.)
     values, tokens: (..., k), the teacher's entries: logits, or log probabilities (both give the same
     with normalize=True, where w = softmax(values / T) over the row's entries; with normalize=False
     w = exp(values), log probabilities at temperature T, and the rest of the teacher's mass is left

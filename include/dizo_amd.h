@@ -255,6 +255,7 @@ int32_t dz_token_logprobs(const void* logits, int32_t dtype, int64_t batch, int6
  * = softmax(teacher_values[r] / T) over the row's entries (normalize != 0) or w
  * = exp(teacher_values[r]) (normalize = 0: log probabilities at temperature T;
  * the rest of the teacher's mass is left out). Entries of weight 0 add nothing.
+ * T's square has to be a normal fp32 number (T from 2^-63 up to 2^64).
  * A row without entries is not read: 0. A token outside the vocabulary, or a
  * teacher value of NaN or +inf, gives NaN. With grad: grad_r = weights_r times the
  * gradient of loss[r] with respect to logits_r, in `dtype`; it may be written over
