@@ -176,7 +176,8 @@ __device__ u32x4 zeros16[1];  // what the columns past the width are read from
 // 16 bytes a lane to LDS, 1,024 consecutive bytes from address `lds` on (the same for the whole wave), from
 // base + offset or from p. In assembly, so that the compiler, which cannot tell the slabs' places apart
 // from one round of the loop to the next, does not wait for every load before it reads LDS; arrive() waits.
-// (M0 is not named as overwritten, since it cannot be: nothing else here uses it.)
+// (M0 cannot be reserved by a statement. Nothing else here uses it: tests/test_head_asm.py looks for it in
+// the generated code.)
 template <bool ONCE>
 __device__ __forceinline__ void to_lds(const void* base, uint32_t offset, uint32_t lds) {
   if (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
