@@ -422,8 +422,9 @@ __global__ __launch_bounds__(64 * WT * WV, M == 32 || STAGES == 5 ? 1 : 2) void 
 
 // Many rows of fp32. The fp32 matrix instructions multiply at 1/16 of the rate of bf16's, so each
 // number is taken as a sum of three bf16 numbers, hi + mid + lo, each the rounding of what the ones
-// before leave (27 bits together), and a product as the six of their nine products that are not
-// below 2^-25 of it: what is left out (two of at most 2^-26, one of 2^-34) is less than a rounding of an fp32 sum, which every
+// before leave: |mid| <= 2^-8 and |lo| <= 2^-17 of the number (bf16 has 8 bits, a rounding leaves half of the last one), and nothing is
+// left of its 24 bits (of numbers below 2^-110 the last ones are below bf16's smallest number: 2^-120 keeps 14). A product is taken as the six of their nine products that can be above 2^-25 of it. What is left out, mid lo of
+// both (2^-25 each, and close to it for 1 + 2^-8 - 2^-17) and lo lo (2^-34), is together not more than a rounding of an fp32 sum, 2^-24, which every
 // product of the fp32 instructions has too. Against a kernel with fp32 instructions, by 50,272 tokens, 768
 // wide: 2,048 rows 869 us for 1,230 (184 TFLOP/s of products of fp32 numbers), 300 rows, of whose 384 in tiles 84
 // are not there, 209 for 243. Taking apart is as much work for the vector units as the products

@@ -269,7 +269,7 @@ int32_t dz_topk_distill(const void* logits, int32_t dtype, int64_t batch, int64_
 /* dz_token_logprobs' logprobs and entropy of the logits hidden weight^T, which
  * are not stored: hidden (rows, width) and weight (vocab, width) of `dtype`,
  * rows hidden_stride and weight_stride elements apart, products and sums in
- * fp32 (fp32 operands of many rows as three bf16 parts each, to 27 bits). Ignored
+ * fp32 (fp32 operands of many rows as three bf16 parts each, a product to 2^-24). Ignored
  * rows give 0, 0. `workspace` is device memory (16-byte
  * aligned) of at least the bytes that the first call reports; calls that overlap in
  * time need one each. */
