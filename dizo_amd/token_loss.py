@@ -5,7 +5,7 @@
 ``topk_distill``          the distance to a teacher of which the largest logits were kept
                           (``token_logprobs(..., top=k)`` records them), differentiable in the logits
 ``linear_token_logprobs`` log probabilities and entropies straight from the last hidden states and
-                          the language-model head: the logits are never stored
+                          the language-model head, under no_grad: the logits are not stored
 ``token_logprobs_grad``, ``topk_distill_grad``   value and gradient in one call, for callers that
                           know the rows' weights beforehand (the logits are then read once)
 
@@ -284,8 +284,12 @@ def linear_token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: to
                           ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
     """token_logprobs of the logits hidden @ weight.T, which are not stored (and not rounded: products
     and sums are fp32). hidden (..., width) and weight (vocab, width) of one dtype; the width has to be
-    contiguous. Ignored rows give 0 (of many rows, they are not multiplied). Where autograd records (hidden or weight require a
-    gradient), the logits are made by F.linear and scored by token_logprobs instead."""
+    contiguous. Ignored rows give 0 (of many rows, they are not multiplied).
+
+    A parameter requires a gradient: score under torch.no_grad(). Where autograd records (grad mode is
+    on, and hidden or weight require a gradient) the logits are F.linear's, stored and rounded to the
+    operands' dtype, and token_logprobs takes them from there: a logit of 8 is off by up to 2^-5 in
+    bf16, and log probabilities differ by as much from those of the kernel."""
     what = "linear_token_logprobs"
     if not hidden.is_cuda:
         _fail(what, f"hidden must live on a GPU, got {hidden.device}")
