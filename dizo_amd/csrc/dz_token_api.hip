@@ -57,7 +57,7 @@ int32_t check_distinct(int64_t batch, int64_t length, int64_t bs, int64_t ls, in
   return DZ_OK;
 }
 
-// A gradient may be written over its logits, row over row; otherwise the two share nothing.
+// A gradient may be written over its logits, row over row; otherwise the ranges from first to last element lie apart.
 int32_t check_apart(const void* logits, const void* grad, int64_t es, int64_t batch, int64_t length, int64_t vocab, int64_t logits_bs,
                     int64_t logits_ls, int64_t grad_bs, int64_t grad_ls) {
   if (logits == grad && (batch == 1 || logits_bs == grad_bs) && (length == 1 || logits_ls == grad_ls)) return DZ_OK;

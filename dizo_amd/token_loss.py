@@ -187,7 +187,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, weights: Opt
                         entropy_weights: Optional[torch.Tensor] = None, *,
                         ignore_index: int = IGNORE_INDEX) -> Tuple[TokenLogprobs, torch.Tensor]:
     """token_logprobs, and the gradient of sum(weights logprobs) + sum(entropy_weights entropy) with
-    respect to the logits, in their dtype. Weights are fp32, shaped like tokens; None stands for zeros."""
+    respect to the logits, in their dtype. Weights are fp32, shaped like tokens; None stands for zeros.
+    Nothing is recorded by autograd."""
     what = "token_logprobs_grad"
     tokens = _score_checked(what, logits, tokens, 0, weights, entropy_weights)
     if weights is None and entropy_weights is None:
@@ -270,7 +271,7 @@ def topk_distill(logits: torch.Tensor, values: torch.Tensor, tokens: torch.Tenso
 def topk_distill_grad(logits: torch.Tensor, values: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor, *,
                       temperature: float = 1.0, normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """topk_distill, and the gradient of sum(weights loss) with respect to the logits, in their dtype.
-    weights: fp32, one per row."""
+    weights: fp32, one per row. Nothing is recorded by autograd."""
     what = "topk_distill_grad"
     values, tokens = _distill_checked(what, logits, values, tokens, temperature, weights)
     _check_rows(what, "weights", weights, logits.shape[:-1], logits.device, _F32)

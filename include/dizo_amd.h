@@ -241,7 +241,8 @@ int32_t dz_group_dot(dz_table* t, const uint64_t* other_ptrs, double* d_dot, flo
  * With grad (top = 0 then): grad_r = the gradient of
  * weights_r logprobs_r + entropy_weights_r entropy_r with respect to logits_r
  * (either weights may be NULL: zeros), in `dtype`; grad may be the logits
- * themselves, with their strides, and else shares nothing with them. */
+ * themselves, with their strides, and else lies before or after all of them
+ * (rows interleaved with the logits' are refused). */
 int32_t dz_token_logprobs(const void* logits, int32_t dtype, int64_t batch, int64_t length, int64_t vocab,
                           int64_t logits_bs, int64_t logits_ls, const int64_t* tokens, int64_t tokens_bs,
                           int64_t tokens_ls, int64_t ignore_index, int32_t top, float* logprobs, float* entropy,
