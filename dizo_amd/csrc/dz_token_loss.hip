@@ -541,19 +541,26 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
   const Stats<GRAD> st = stats_of<T, THREADS, NV, false, GRAD>(s, h, c, waves, own_max);
   const float log2s = log2_hw(st.s);
   if (tid < 64) {
-    float loss = 0.f, total = 0.f;
+    float loss = 0.f, far = 0.f, total = 0.f;
     for (uint32_t j = lane; j < k; j += 64) {
       const float lnw = (sh.w[j] - tm) * tinv - lse;
       const float w = sh.idx[j] >= 0 ? exp2_hw(lnw * kLog2e) : 0.f;
-      if (w > 0.f) loss += w * (lnw - st.lnq(sh.x[j], c, inv));
+      if (w > 0.f) {
+        const float lnq = st.lnq(sh.x[j], c, inv);
+        // a logit of the type's lowest value, which a temperature below 1 takes past fp32's range: beside it
+        // nothing else counts, and its distance is taken undivided
+        if (lnq == -INFINITY) far += w * (st.m - sh.x[j]);
+        else loss += w * (lnw - lnq);
+      }
       sh.w[j] = w;
       total += w;
     }
     loss = reduce64(loss, Add());
+    far = reduce64(far, Add());
     total = reduce64(total, Add());
     bad |= !st.valid();
     if (lane == 0) {
-      a.loss[r] = bad ? NAN : a.temperature * a.temperature * loss;
+      a.loss[r] = bad ? NAN : a.temperature * a.temperature * loss + a.temperature * far;
       sh.total = total;
       sh.bad = bad;
     }

@@ -75,3 +75,37 @@ def test_teacher_values_at_the_limits_of_fp32(dtype, tau):
         np.add.at(term, at64[r][there], tw[there])
         assert (np.abs(grad[r].double().cpu().numpy() - want_grad[r]) <= tau * w64[r] * e * (steps + 40) * term + 2.0**-126).all(), r
     assert torch.equal(T.topk_distill(x, val, at, temperature=tau).isnan(), torch.zeros(7, dtype=torch.bool, device="cuda"))
+
+
+@pytest.mark.parametrize("tau", [0.3, 0.5, 0.9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_masked_student_logits_that_a_temperature_takes_past_fp32(dtype, tau):
+    """A student's logits at the type's lowest value, of which a teacher's entries name some: their log probabilities
+    divided by a temperature below 1 are no numbers of fp32, the distance is. Within T^2 e (v / 256 + 60 + k + 4 max |t| / T)
+    (1 + sum w (|ln w| + |ln q|)); a masked logit of -inf stays an infinite distance."""
+    v, k = 700, 5
+    x = rows(6, v, dtype, 5)
+    g = torch.Generator().manual_seed(6)
+    at = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(6)]).cuda()
+    val = (torch.randn(6, k, generator=g) * 4).cuda()
+    low = torch.finfo(dtype).min
+    x[0, at[0, 2]] = low
+    x[1, at[1]] = low
+    x[2, : v // 2] = low
+    val[3, 4] = -40 * tau  # little weight, and a large distance for it
+    x[3, at[3, 4]] = low
+    x[4, at[4, 1]] = -math.inf
+    x[5, at[5, 0]], x[5, at[5, 1]] = low, -math.inf
+    x64, val64, at64 = x.double().cpu().numpy(), val.double().cpu().numpy(), at.cpu().numpy()
+    want, _ = O.topk_distill(x64, val64, at64, tau)
+    assert np.isfinite(want[:4]).all() and (want[:2] > 1e20).all() and np.isinf(want[4:]).all()
+    logq = O.log_softmax(x64 / tau)
+    w = torch.ones(6, device="cuda")
+    for got in (T.topk_distill(x, val, at, temperature=tau), T.topk_distill_grad(x, val, at, w, temperature=tau)[0]):
+        got = got.double().cpu().numpy()
+        for r in range(4):
+            tw, tl = O.teacher_weights(val64[r], at64[r], v, tau, True)
+            size = (tw * (np.abs(tl) + np.abs(logq[r][at64[r]]))).sum()
+            steps = v / 256 + 60 + k + 4 * np.abs(val64[r]).max() / tau
+            assert abs(got[r] - want[r]) <= tau * tau * 2.0**-24 * steps * (1 + size), (r, got[r], want[r])
+        assert np.isposinf(got[4:]).all()
