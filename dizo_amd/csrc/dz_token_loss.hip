@@ -547,9 +547,9 @@ __global__ __launch_bounds__(THREADS) void topk_distill_kernel(VocabRows a) {
       const float w = sh.idx[j] >= 0 ? exp2_hw(lnw * kLog2e) : 0.f;
       if (w > 0.f) {
         const float lnq = st.lnq(sh.x[j], c, inv);
-        // a logit of the type's lowest value, which a temperature below 1 takes past fp32's range: beside it
-        // nothing else counts, and its distance is taken undivided
-        if (lnq == -INFINITY) far += w * (st.m - sh.x[j]);
+        // a logit of the type's lowest value, which a temperature below 1, or a largest one at the other end, takes
+        // past fp32's range: beside it nothing else counts, and its distance is taken undivided, weight by weight
+        if (lnq == -INFINITY) far += w * st.m - w * sh.x[j];
         else loss += w * (lnw - lnq);
       }
       sh.w[j] = w;

@@ -109,3 +109,20 @@ def test_masked_student_logits_that_a_temperature_takes_past_fp32(dtype, tau):
             steps = v / 256 + 60 + k + 4 * np.abs(val64[r]).max() / tau
             assert abs(got[r] - want[r]) <= tau * tau * 2.0**-24 * steps * (1 + size), (r, got[r], want[r])
         assert np.isposinf(got[4:]).all()
+
+
+@pytest.mark.parametrize("tau", [0.5, 1.0, 1.7])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_student_logits_at_both_ends_of_their_type(dtype, tau):
+    """The largest logit at the type's largest value and a named one at its lowest, whose difference is no number of fp32:
+    the distance is one where the weight is small. Its size is w (max - min) T, off by the weight's (2 k + 10 + 4 max |t| / T) e."""
+    v, k = 300, 4
+    x = rows(2, v, dtype, 5)
+    at = torch.tensor([[1, 2, 3, 4], [5, 6, 7, 8]], device="cuda")
+    val = torch.tensor([[0.0, 0.0, 0.0, -20 * tau], [3.0, -9 * tau, 1.0, -30 * tau]], device="cuda")
+    x[0, 1:4], x[0, 4] = torch.finfo(dtype).max, torch.finfo(dtype).min
+    x[1, 5:8], x[1, 8] = torch.finfo(dtype).max, torch.finfo(dtype).min
+    want, _ = O.topk_distill(x.double().cpu().numpy(), val.double().cpu().numpy(), at.cpu().numpy(), tau)
+    for got in (T.topk_distill(x, val, at, temperature=tau), T.topk_distill_grad(x, val, at, torch.ones(2, device="cuda"), temperature=tau)[0]):
+        tol = want * 2.0**-24 * (2 * k + 10 + 4 * val.abs().amax(-1).double().cpu().numpy() / tau + 10)
+        assert (np.abs(got.double().cpu().numpy() - want) <= tol).all(), (got.tolist(), want.tolist())
