@@ -426,8 +426,8 @@ __global__ __launch_bounds__(64 * WT * WV, M == 32 || STAGES == 5 ? 1 : 2) void 
 // left of its 24 bits (of numbers below 2^-110 the last ones are below bf16's smallest number: 2^-120 keeps 14). A product is taken as the six of their nine products that can be above 2^-25 of it. What is left out, mid lo of
 // both (2^-25 each, and close to it for 1 + 2^-8 - 2^-17) and lo lo (2^-34), is together not more than a rounding of an fp32 sum, 2^-24, which every
 // product of the fp32 instructions has too. Against a kernel with fp32 instructions, by 50,272 tokens, 768
-// wide: 2,048 rows 869 us for 1,230 (184 TFLOP/s of products of fp32 numbers), 300 rows, of whose 384 in tiles 84
-// are not there, 209 for 243. Taking apart is as much work for the vector units as the products
+// wide: 2,048 rows 869 us for 1,230 (184 TFLOP/s of products of fp32 numbers, of 231 that six bf16 products at a library's rate
+// would be), 300 rows, of whose 384 in tiles 84 are not there, 209 for 243. Taking apart is as much work for the vector units as the products
 // are for the matrix units; 128 rows a tile share it (64: 1,066 us).
 //
 // An infinity among the operands (or a number that rounds to one) has no such sum: its parts make a
@@ -654,7 +654,9 @@ __global__ __launch_bounds__(64) void head_join_kernel(HeadRows a, Work w, uint3
 // would leave half of the 256 compute units without one, smaller ones that more of them share, and that keep more
 // slabs on their way, since the width is then walked through at the pace of a load (2,048 rows by
 // 1,000 tokens, 5,120 wide, fp16: 111 us in 32 large tiles, 49 in 256 small ones; at 128 large ones they
-// meet: 2,048 by 4,000, 1,024 wide 40 and 35 us, 700 by 16,000 in 189 tiles 38 and 42).
+// meet: 2,048 by 4,000, 1,024 wide 40 and 35 us, 700 by 16,000 in 189 tiles 38 and 42). Rounds of tiles are
+// not weighed: 50,272 tokens make 197 of 256 head rows, which leaves 59 compute units without one for one tile of
+// rows (256 rows of 5,120 fp16: 158 us), and 2.31 tiles each take three rounds (300 fp32 rows of 768: 187 us).
 struct Plan {
   uint32_t row_tile, head_tile;
 };
