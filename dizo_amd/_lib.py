@@ -38,6 +38,7 @@ _i64 = C.c_int64
 _i32 = C.c_int32
 _u32 = C.c_uint32
 _f32 = C.c_float
+_f64 = C.c_double
 
 # name -> (restype, argtypes); mirrors include/dizo_amd.h.
 SIGNATURES = {
@@ -69,6 +70,12 @@ SIGNATURES = {
                                _p, _i64, _i64, _p]),
     "dz_linear_token_logprobs_workspace": (_i32, [_i32, _i64, _i64, _i64, C.POINTER(_i64)]),
     "dz_linear_token_logprobs": (_i32, [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p]),
+    # the structs come as their packed bytes
+    "dz_shared_prefix_attention_workspace": (_i32, [C.c_char_p, C.POINTER(_i64)]),
+    "dz_shared_prefix_attention": (_i32, [C.c_char_p, _p, _i64, _p]),
+    "dz_cache_write": (_i32, [C.c_char_p, C.c_char_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p]),
+    "dz_cache_read": (_i32, [C.c_char_p, C.c_char_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
+    "dz_sample_tokens": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _f64, _i32, _f64, _f64, _p, _p, _p, _p, _p, _p]),
 }
 
 _lock = threading.Lock()

@@ -1,6 +1,7 @@
 // Log probabilities and entropies straight from hidden states and the
 // language-model head: the products are reduced to softmax statistics where
 // they are made, and the logits are never stored.
+#include "dz_lds.h"
 #include "dz_token_loss.h"
 #include "dz_token_math.h"
 
@@ -172,20 +173,6 @@ __device__ __forceinline__ void lane_stats(Acc<M> (&acc)[TF][VF], uint32_t v0, u
 // A slab's 16-byte chunk c of row r lies at r * 128 + (c ^ swizzle(r)) * 16.
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r >> 1) & 7; }
 __device__ u32x4 zeros16[1];  // what the columns past the width are read from
-
-// 16 bytes a lane to LDS, 1,024 consecutive bytes from address `lds` on (the same for the whole wave), from
-// base + offset or from p. In assembly, so that the compiler, which cannot tell the slabs' places apart
-// from one round of the loop to the next, does not wait for every load before it reads LDS; arrive() waits.
-// (M0 cannot be reserved by a statement. Nothing else here uses it: tests/test_head_asm.py looks for it in
-// the generated code.)
-template <bool ONCE>
-__device__ __forceinline__ void to_lds(const void* base, uint32_t offset, uint32_t lds) {
-  if (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
-  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
-}
-__device__ __forceinline__ void to_lds(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
-}
 
 // All but the last N of this wave's loads are done, and every wave of the workgroup is here.
 template <int N>

@@ -280,6 +280,91 @@ int32_t dz_linear_token_logprobs(const void* hidden, const void* weight, int32_t
                                  int64_t ignore_index, float* logprobs, float* entropy, void* workspace,
                                  int64_t workspace_bytes, void* stream);
 
+/* ---- candidates and answers that share a prompt --------------------------- */
+/* Keys and values of a call below, by strides in elements (bytes of an 8-bit
+ * store): group, sequence, head, slot; the width is contiguous. Addresses and
+ * strides are multiples of 16 bytes (8 of an 8-bit store), slots less than 2^24
+ * elements apart. 8-bit stores hold e4m3 codes (OCP: largest 448, no
+ * infinities) and for each slot of a head an e8m0 scale s, 2^(s - 127). */
+typedef struct dz_keys_values {
+  const void* k;
+  const void* v;
+  int64_t k_strides[4];
+  int64_t v_strides[4];
+  const uint8_t* k_scales; /* NULL: not an 8-bit store */
+  const uint8_t* v_scales;
+  int64_t k_scale_strides[4];
+  int64_t v_scale_strides[4];
+} dz_keys_values;
+
+/* Attention of groups x sequences sequences of `length` queries. Token t of
+ * sequence n of group g sees the first prefix_lengths[g] (0 to prefix_slots)
+ * slots of its group's prefix and the first positions[g, n] + t + 1 (0 to slots)
+ * of its own keys:
+ *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q k_j)
+ * and 0 where it sees nothing. heads is a multiple of kv_heads; query heads
+ * heads / kv_heads h .. + heads / kv_heads - 1 read key head h. width is a
+ * multiple of 8 up to 128. Lengths and positions outside their ranges are taken
+ * as the nearest in it. Slots that no query of a sequence sees are not looked
+ * at, whatever they hold; a query's weights of slots that it does not see itself
+ * are 0, which leaves NaN of an infinite or NaN value there. Products and sums
+ * are fp32; weights are rounded to `dtype` before they multiply values (bf16:
+ * 2^-8 of each at most, as their sum is taken before). Both stores are of
+ * `dtype`, or both 8-bit. `out` may not overlap an input. Replaces, for
+ * candidates that share a prompt, the attention of the forwards in
+ * trainer.py:1524-1542, which repeats it for each. */
+typedef struct dz_attention {
+  const void* q;
+  void* out;
+  int64_t q_strides[4]; /* group, sequence, head, token */
+  int64_t out_strides[4];
+  dz_keys_values own;    /* slots of each sequence; slots = 0: none */
+  dz_keys_values prefix; /* slots of each group (its sequence strides are not used); prefix_slots = 0: none */
+  const int32_t* positions;      /* (groups, sequences), dense; NULL: slots - length */
+  const int32_t* prefix_lengths; /* (groups), dense; NULL: prefix_slots */
+  int64_t groups, sequences, heads, kv_heads, length, width, slots, prefix_slots;
+  int32_t dtype;
+  float scale; /* positive and finite */
+} dz_attention;
+
+/* `workspace` is device memory (16-byte aligned) of at least the bytes that the
+ * first call reports (0 for many shapes); calls that overlap in time need one
+ * each. Calls allocate nothing and may be captured. */
+int32_t dz_shared_prefix_attention_workspace(const dz_attention* a, int64_t* bytes);
+int32_t dz_shared_prefix_attention(const dz_attention* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Puts `length` tokens' keys and values of `dtype` (kv->k and kv->v with their
+ * strides: batch, unused, head, token) into an 8-bit store (batch, unused, head,
+ * slot) from slot positions[b] on (NULL: `position` for all). Tokens that fall outside
+ * of the store's slots are left out. A row (one token's head) is kept as code
+ * 2^e, with e the least (from -100) that leaves nothing above 448 and codes rounded to
+ * nearest even. fp16 numbers above 61440 are kept as that. A row with an infinity or
+ * NaN becomes NaN. dz_cache_read gives code 2^e in `dtype`, of slots
+ * position .. position + length - 1. */
+int32_t dz_cache_write(const dz_keys_values* kv, const dz_keys_values* cache, int32_t dtype, int64_t batch, int64_t heads,
+                       int64_t length, int64_t width, int64_t slots, const int32_t* positions, int64_t position,
+                       void* stream);
+int32_t dz_cache_read(const dz_keys_values* cache, const dz_keys_values* kv, int32_t dtype, int64_t batch, int64_t heads,
+                      int64_t length, int64_t width, int64_t slots, int64_t position, void* stream);
+
+/* tokens[r] = one token of row r (rows of `vocab`, at most 2^20, contiguous
+ * elements, logits_stride apart), drawn by uniform[r] (0 to 1) from softmax(logits_r /
+ * temperature) restricted to its top_k largest (0: no limit; equal logits by
+ * token), of these to the fewest, largest first, that hold top_p of their
+ * probability (1 or more: all), and of these to those of at least min_p times the
+ * largest one's: the first token up to which the sum of what is left exceeds uniform[r]
+ * of the whole. Weights are kept as whole numbers of 2^-46 of the largest (2^-42 for
+ * the longest rows), so that results do not depend on an order. Temperature 0
+ * takes the largest logit. Temperatures are 0, or from 2^-63 up to 2^64. Each
+ * parameter may be given per row (a pointer that is not NULL). Rows with a
+ * NaN, or nothing above -inf, or whose parameters are NaN or out of range, give -1;
+ * logits of +inf share the whole. Replaces the sampling of
+ * model.generate in trainer.py:1544-1568. */
+int32_t dz_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t logits_stride,
+                         const float* uniform, double temperature, int32_t top_k, double top_p, double min_p,
+                         const float* temperatures, const int32_t* top_ks, const float* top_ps, const float* min_ps,
+                         int64_t* tokens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
