@@ -19,64 +19,90 @@ constexpr int kLeastPower = -100;
 // fp16 values above 61,440 would round to 65,536, which fp16 does not have.
 constexpr float kLargestHalf = 61440.f;
 
-constexpr int kRowLanes = 16;  // of 8 elements: a width of up to 128
+constexpr int kThreads = 256;
 
-template <class T, bool READ>
-__global__ __launch_bounds__(256) void cache_kernel(CacheRows a) {
+// LANES lanes a row, 8 elements each; a thread takes EACH rows, whose loads are all on their way before the first is used.
+// Keys in the grid's first plane, values in its second. Rows go along the store, a head's slots next to each other: its
+// lines and scales are whole then, and the other side's rows are 16 to 512 consecutive bytes in either order.
+template <class T, bool READ, int LANES, int EACH>
+__global__ __launch_bounds__(kThreads) void cache_kernel(CacheRows a) {
   using Elem = typename T::Elem;
   typedef Elem Eight __attribute__((ext_vector_type(8)));
-  // Rows in the order of a projection's output, heads next to each other; keys, then values.
-  const uint64_t rows = (uint64_t)a.batch * a.length * a.heads;
-  const uint64_t at = (uint64_t)blockIdx.x * (256 / kRowLanes) + threadIdx.x / kRowLanes;
-  const uint32_t col = threadIdx.x % kRowLanes * 8;
-  if (at >= 2 * rows) return;
-  const int which = at >= rows;
-  const uint64_t i = at - which * rows;
-  const uint32_t h = (uint32_t)(i % a.heads), t = (uint32_t)(i / a.heads % a.length), b = (uint32_t)(i / a.heads / a.length);
-  const int64_t slot = (int64_t)(a.positions ? a.positions[b] : a.position) + t;
-  if (slot < 0 || slot >= a.slots) return;
-  const int64_t(&xs)[3] = a.x_s[which], (&cs)[3] = a.code_s[which], (&ss)[3] = a.scale_s[which];
-  Elem* x = (Elem*)a.x[which] + (int64_t)b * xs[0] + (int64_t)h * xs[1] + (int64_t)t * xs[2] + col;
-  uint8_t* code = (uint8_t*)a.code[which] + (int64_t)b * cs[0] + (int64_t)h * cs[1] + slot * cs[2] + col;
-  uint8_t* scale = (uint8_t*)a.scale[which] + (int64_t)b * ss[0] + (int64_t)h * ss[1] + slot * ss[2];
+  constexpr uint32_t ROWS = kThreads / LANES;
+  const uint32_t rows = (uint32_t)a.batch * a.length * a.heads, which = blockIdx.y;
+  const uint32_t col = threadIdx.x % LANES * 8;
+  const int64_t* const xs = a.x_s[which];
+  const int64_t* const cs = a.code_s[which];
+  const int64_t* const ss = a.scale_s[which];
   const bool there = col < (uint32_t)a.width;
-  if constexpr (READ) {
-    if (!there) return;
-    const float f = __uint_as_float((uint32_t)*scale << 23);
-    const u32x2 c = *(const u32x2*)code;
-    Eight v;
+  bool live[EACH];
+  Elem* x[EACH];
+  uint8_t *code[EACH], *scale[EACH];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[j], f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[j], f, true);
-      v[4 * j] = (Elem)lo[0];
-      v[4 * j + 1] = (Elem)lo[1];
-      v[4 * j + 2] = (Elem)hi[0];
-      v[4 * j + 3] = (Elem)hi[1];
+  for (int r = 0; r < EACH; ++r) {
+    const uint32_t i = (blockIdx.x * EACH + r) * ROWS + threadIdx.x / LANES;
+    const uint32_t bh = i / a.length, t = i - bh * a.length, b = bh / a.heads, h = bh - b * a.heads;
+    live[r] = i < rows;
+    int64_t slot = 0;
+    if (live[r]) {
+      slot = (int64_t)(a.positions ? a.positions[b] : a.position) + t;
+      live[r] = slot >= 0 && slot < a.slots;
     }
-    *(Eight*)x = v;
+    x[r] = (Elem*)a.x[which] + (int64_t)b * xs[0] + (int64_t)h * xs[1] + (int64_t)t * xs[2] + col;
+    code[r] = (uint8_t*)a.code[which] + (int64_t)b * cs[0] + (int64_t)h * cs[1] + slot * cs[2] + col;
+    scale[r] = (uint8_t*)a.scale[which] + (int64_t)b * ss[0] + (int64_t)h * ss[1] + slot * ss[2];
+  }
+  if constexpr (READ) {
+    u32x2 c[EACH];
+    uint8_t e[EACH];
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+      if (live[r] && there) {
+        c[r] = *(const u32x2*)code[r];
+        e[r] = *scale[r];
+      }
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+      if (live[r] && there) {
+        const float f = __uint_as_float((uint32_t)e[r] << 23);
+        Eight v;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[r][j], f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[r][j], f, true);
+          v[4 * j] = (Elem)lo[0];
+          v[4 * j + 1] = (Elem)lo[1];
+          v[4 * j + 2] = (Elem)hi[0];
+          v[4 * j + 3] = (Elem)hi[1];
+        }
+        __builtin_nontemporal_store(v, (Eight*)x[r]);
+      }
   } else {
-    float v[8];
-    uint32_t most = 0;  // bits of the largest magnitude: NaN above infinity above numbers
-    if (there) {
-      const Eight e = *(const Eight*)x;
+    Eight in[EACH];
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      in[r] = Eight(Elem(0.f));
+      if (live[r] && there) in[r] = *(const Eight*)x[r];
+    }
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      float v[8];
+      uint32_t most = 0;  // bits of the largest magnitude: NaN above infinity above numbers
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = (float)e[j];
+        v[j] = (float)in[r][j];
         const uint32_t m = __float_as_uint(v[j]) & 0x7fffffffu;
         most = m > most ? m : most;
       }
-    }
 #pragma unroll
-    for (int d = 1; d < kRowLanes; d *= 2) {
-      const uint32_t o = __shfl_xor(most, d);
-      most = o > most ? o : most;
-    }
-    const bool finite = most < 0x7f800000u;
-    constexpr bool kHalf = sizeof(Elem) == 2 && T::kPer16 == 8 && __is_same(T, TypeF16);
-    if (kHalf && finite && most > __float_as_uint(kLargestHalf)) most = __float_as_uint(kLargestHalf);
-    int e = (int)(most >> 23) - 135 + ((most & 0x7fffffu) > 0x600000u);
-    e = most == 0 || !finite ? 0 : e < kLeastPower ? kLeastPower : e;
-    if (there) {
+      for (int d = 1; d < LANES; d *= 2) {
+        const uint32_t o = __shfl_xor(most, d);
+        most = o > most ? o : most;
+      }
+      const bool finite = most < 0x7f800000u;
+      constexpr bool kHalf = __is_same(T, TypeF16);
+      if (kHalf && finite && most > __float_as_uint(kLargestHalf)) most = __float_as_uint(kLargestHalf);
+      int e = (int)(most >> 23) - 135 + ((most & 0x7fffffu) > 0x600000u);
+      e = most == 0 || !finite ? 0 : e < kLeastPower ? kLeastPower : e;
       const float f = __uint_as_float((uint32_t)(127 - e) << 23);
       u32x2 c;
 #pragma unroll
@@ -91,18 +117,25 @@ __global__ __launch_bounds__(256) void cache_kernel(CacheRows a) {
         c[j] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
       }
       if (!finite) c = u32x2(0x7f7f7f7fu);
-      *(u32x2*)code = c;
-      if (col == 0) *scale = (uint8_t)(e + 127);
+      if (live[r] && there) {
+        *(u32x2*)code[r] = c;
+        if (col == 0) *scale[r] = (uint8_t)(e + 127);
+      }
     }
   }
 }
 
+template <class T, bool READ, int LANES>
+void launch_lanes(const CacheRows& a, hipStream_t st) {
+  const uint32_t rows = (uint32_t)a.batch * a.length * a.heads, each = kThreads / LANES;
+  // four rows a thread where that leaves two workgroups a compute unit
+  if (rows >= 4 * each * 256) cache_kernel<T, READ, LANES, 4><<<dim3((rows + 4 * each - 1) / (4 * each), 2), kThreads, 0, st>>>(a);
+  else cache_kernel<T, READ, LANES, 1><<<dim3((rows + each - 1) / each, 2), kThreads, 0, st>>>(a);
+}
 template <class T>
 void launch_typed(const CacheRows& a, bool read, hipStream_t st) {
-  const uint64_t rows = 2 * (uint64_t)a.batch * a.length * a.heads;
-  const uint32_t grid = (uint32_t)((rows + 256 / kRowLanes - 1) / (256 / kRowLanes));
-  if (read) cache_kernel<T, true><<<grid, 256, 0, st>>>(a);
-  else cache_kernel<T, false><<<grid, 256, 0, st>>>(a);
+  if (a.width <= 64) read ? launch_lanes<T, true, 8>(a, st) : launch_lanes<T, false, 8>(a, st);
+  else read ? launch_lanes<T, true, 16>(a, st) : launch_lanes<T, false, 16>(a, st);
 }
 
 }  // namespace

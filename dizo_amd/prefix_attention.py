@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import NamedTuple, Optional, Union
 
 import torch
 
@@ -59,71 +59,56 @@ _STORE = "2Q8q2Q8q"
 _ATTENTION = struct.Struct("2Q8q" + 2 * _STORE + "2Q8qif")
 _KEYS_VALUES = struct.Struct(_STORE)
 _NOTHING = (0,) * 20
+_NO_SCALES = (0,) * 10
 
 
-def _fits(t: torch.Tensor, align: int) -> bool:
-    """Whether the kernels read t where it is: width contiguous, rows at multiples of `align` bytes, slots near enough."""
-    s = t.stride()
+def _rows(t: torch.Tensor):
+    """(t, its strides but for the width's) where the kernels can read t: the width contiguous, rows at multiples of 16 bytes
+    (codes: 8), slots near enough; otherwise those of a copy."""
+    *s, last = t.stride()
     es = t.element_size()
-    if s[-1] != 1 or t.data_ptr() % align or s[-2] >= MAX_SLOT_STRIDE:
-        return False
-    for x in s[:-1]:
-        if x * es % align:
-            return False
-    return True
+    low = t.data_ptr()
+    for x in s:
+        low |= x * es
+    if last != 1 or low & (7 if es == 1 else 15) or s[-1] >= MAX_SLOT_STRIDE:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = t.stride()[:-1]
+    return t, s
 
 
-def _placed(t: torch.Tensor, align: int) -> torch.Tensor:
-    return t if _fits(t, align) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _check_operands(what: str, device, *tensors: Optional[torch.Tensor]) -> None:
+def _check_operands(what: str, index: int, tensors) -> None:
+    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None:
-            if t.device != device:
-                _fail(what, f"tensors on {device} and {t.device}")
-            if t.requires_grad and torch.is_grad_enabled():
-                _fail(what, "nothing is recorded by autograd: call it under torch.no_grad(), or detach the operands")
+        if t.get_device() != index:
+            _fail(what, f"tensors on cuda:{index} and {t.device}")
+        if grad and t.requires_grad:
+            _fail(what, "nothing is recorded by autograd: call it under torch.no_grad(), or detach the operands")
     _no_tangents(what, *tensors)
 
 
-def _check_store(what: str, name: str, kv, lead: Tuple[int, ...], width: int, dtype, device) -> bool:
-    """Checks a KV or QuantizedKV whose leading dimensions (and heads) are `lead`; whether it is an 8-bit one."""
-    bytes_ = isinstance(kv, QuantizedKV) or (not isinstance(kv, KV) and len(kv) == 4)
+def _check_store(what: str, name: str, kv, shape, dtype, index: int) -> bool:
+    """Checks a KV or QuantizedKV of a shape (its slots are not looked at); whether it is an 8-bit one."""
+    bytes_ = len(kv) == 4
+    _check_operands(what, index, kv)
     k, v = kv[0], kv[1]
-    _check_operands(what, device, *kv)
-    if k.shape != v.shape or k.dim() != len(lead) + 2 or tuple(k.shape[:-2]) != lead or k.shape[-1] != width:
-        _fail(what, f"{name} keys and values must be {(*lead, 'slots', width)}, got {tuple(k.shape)} and {tuple(v.shape)}")
+    got = k.shape
+    if v.shape != got or len(got) != len(shape) or got[:-2] != shape[:-2] or got[-1] != shape[-1]:
+        _fail(what, f"{name} keys and values must be {(*shape[:-2], 'slots', shape[-1])}, got {tuple(got)} and {tuple(v.shape)}")
     want = CODES if bytes_ else dtype
     if k.dtype != want or v.dtype != want:
         _fail(what, f"{name} keys and values must be {want}, got {k.dtype} and {v.dtype}")
     if bytes_:
         for s in kv[2:]:
-            if s.shape != k.shape[:-1] or s.dtype != SCALES:
-                _fail(what, f"{name} scales must be {SCALES} {tuple(k.shape[:-1])}, got {s.dtype} {tuple(s.shape)}")
+            if s.shape != got[:-1] or s.dtype != SCALES:
+                _fail(what, f"{name} scales must be {SCALES} {tuple(got[:-1])}, got {s.dtype} {tuple(s.shape)}")
     return bytes_
 
 
-def _place_store(kv, bytes_: bool):
-    """The store's tensors where the kernels can read them (a copy of those that they cannot)."""
-    if not bytes_:
-        return _placed(kv[0], 16), _placed(kv[1], 16)
-    return _placed(kv[0], 8), _placed(kv[1], 8), kv[2], kv[3]
-
-
-def _packed(kv, four) -> tuple:
-    """The store's fields in dz_keys_values' order; `four` makes four strides of a tensor's (without the width's)."""
-    k, v = four(kv[0].stride()[:-1]), four(kv[1].stride()[:-1])
-    if len(kv) == 2:
-        return (kv[0].data_ptr(), kv[1].data_ptr(), *k, *v, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    return (kv[0].data_ptr(), kv[1].data_ptr(), *k, *v, kv[2].data_ptr(), kv[3].data_ptr(), *four(kv[2].stride()), *four(kv[3].stride()))
-
-
-def _check_int32(what: str, name: str, t: Optional[torch.Tensor], shape, device):
+def _check_int32(what: str, name: str, t: Optional[torch.Tensor], shape, index: int):
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != tuple(shape):
-        _fail(what, f"{name} must be torch.int32 {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype != torch.int32 or t.get_device() != index or t.shape != shape:
+        _fail(what, f"{name} must be torch.int32 {tuple(shape)} on cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -146,79 +131,104 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
     what = "shared_prefix_attention"
     if not q.is_cuda:
         _fail(what, f"q must live on a GPU, got {q.device}")
-    device = q.device
-    code = dtype_code(q.dtype)
+    index, dtype = q.get_device(), q.dtype
+    code = dtype_code(dtype)
     if q.dim() != 5:
         _fail(what, f"q must be (groups, sequences, heads, length, width), got {tuple(q.shape)}")
     groups, sequences, heads, length, width = q.shape
-    _check_operands(what, device, q, out)
-    if own is None and prefix is None:
+    _check_operands(what, index, (q,) if out is None else (q, out))
+    some = own if own is not None else prefix
+    if some is None:
         _fail(what, "neither own keys nor a prefix")
-    kv_heads = (own if own is not None else prefix)[0].shape[-3] if (own if own is not None else prefix)[0].dim() > 2 else 0
+    kv_heads = some[0].shape[-3] if some[0].dim() > 2 else 0
     if kv_heads < 1 or heads % kv_heads:
         _fail(what, f"heads ({heads}) is not a multiple of the stores' ({kv_heads})")
     slots = prefix_slots = 0
-    own_bytes = prefix_bytes = None
     if own is not None:
-        own_bytes = _check_store(what, "own", own, (groups, sequences, kv_heads), width, q.dtype, device)
-        slots = own[0].shape[-2]
+        own_bytes = _check_store(what, "own", own, (groups, sequences, kv_heads, 0, width), dtype, index)
+        slots = own[0].shape[3]
     if prefix is not None:
-        prefix_bytes = _check_store(what, "prefix", prefix, (groups, kv_heads), width, q.dtype, device)
-        prefix_slots = prefix[0].shape[-2]
-    if own_bytes is not None and prefix_bytes is not None and own_bytes != prefix_bytes:
-        _fail(what, "one of own and prefix is an 8-bit store and the other is not")
-    positions = _check_int32(what, "positions", positions, (groups, sequences), device)
-    prefix_lengths = _check_int32(what, "prefix_lengths", prefix_lengths, (groups,), device)
+        prefix_bytes = _check_store(what, "prefix", prefix, (groups, kv_heads, 0, width), dtype, index)
+        prefix_slots = prefix[0].shape[2]
+        if own is not None and own_bytes != prefix_bytes:
+            _fail(what, "one of own and prefix is an 8-bit store and the other is not")
+    positions = _check_int32(what, "positions", positions, (groups, sequences), index)
+    prefix_lengths = _check_int32(what, "prefix_lengths", prefix_lengths, (groups,), index)
     if out is None:
         out = torch.empty_like(q)
-        if not _fits(out, 16):
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        _fail(what, f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-    elif out.stride(-1) != 1 and width > 1:
+        if out.stride(-1) != 1 or width * out.element_size() % 16:
+            out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype:
+        _fail(what, f"out must be {dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+    elif out.stride(-1) != 1:
         _fail(what, "the width of out must be contiguous")
     if not q.numel():
         return out
     if not slots and not prefix_slots:
         return out.zero_()
-    q = _placed(q, 16)
+    q, qs = _rows(q)
     own_f = prefix_f = _NOTHING
     if slots:
-        own = _place_store(own, own_bytes)
-        own_f = _packed(own, tuple)
+        k, ks = _rows(own[0])
+        v, vs = _rows(own[1])
+        own_f = (k.data_ptr(), v.data_ptr(), *ks, *vs, *_NO_SCALES) if not own_bytes else \
+            (k.data_ptr(), v.data_ptr(), *ks, *vs, own[2].data_ptr(), own[3].data_ptr(), *own[2].stride(), *own[3].stride())
     if prefix_slots:
-        prefix = _place_store(prefix, prefix_bytes)
-        prefix_f = _packed(prefix, lambda s: (s[0], 0, s[1], s[2]))
-    args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), *q.stride()[:4], *out.stride()[:4], *own_f, *prefix_f,
+        pk, (a, b, c) = _rows(prefix[0])
+        pv, (d, e, f) = _rows(prefix[1])
+        prefix_f = (pk.data_ptr(), pv.data_ptr(), a, 0, b, c, d, 0, e, f, *_NO_SCALES)
+        if prefix_bytes:
+            a, b, c = prefix[2].stride()
+            d, e, f = prefix[3].stride()
+            prefix_f = (*prefix_f[:10], prefix[2].data_ptr(), prefix[3].data_ptr(), a, 0, b, c, d, 0, e, f)
+    args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), *qs, *out.stride()[:4], *own_f, *prefix_f,
                            0 if positions is None else positions.data_ptr(), 0 if prefix_lengths is None else prefix_lengths.data_ptr(),
                            groups, sequences, heads, kv_heads, length, width, slots, prefix_slots, code,
                            width ** -0.5 if scale is None else scale)
     need = C.c_int64()
     L.call("dz_shared_prefix_attention_workspace", args, C.byref(need))
-    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    _call(device, "dz_shared_prefix_attention", args, work.data_ptr() if need.value else None, need.value)
+    need = need.value
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _call(q.device, "dz_shared_prefix_attention", args, work.data_ptr(), need)
+    else:
+        _call(q.device, "dz_shared_prefix_attention", args, None, 0)
     return out
 
 
-def _cache_operands(what: str, cache):
+def _one_lead(what: str, t: torch.Tensor, n: int):
+    """t's strides of (batch, unused, ...) with its first n dimensions taken as one."""
+    s = t.stride()
+    if n == 1:
+        return s[0], 0, s[1], s[2]
+    if n == 0:
+        return 0, 0, s[0], s[1]
+    shape = t.shape
+    for i in range(n - 1):
+        if shape[i] != 1 and s[i] != s[i + 1] * shape[i + 1]:
+            _fail(what, "the cache's leading dimensions must be one by their strides")
+    return s[n - 1], 0, s[n], s[n + 1]
+
+
+def _cache_fields(what: str, cache):
+    """(batch, dimensions before the heads, the fields of dz_keys_values)"""
     if not isinstance(cache, QuantizedKV):
         _fail(what, f"the cache must be a QuantizedKV, got {type(cache).__name__}")
-    k = cache.k
+    k, v, k_scale, v_scale = cache
     if not k.is_cuda:
         _fail(what, f"the cache must live on a GPU, got {k.device}")
-    if k.dim() < 3:
-        _fail(what, f"the cache must be (..., heads, slots, width), got {tuple(k.shape)}")
-    _check_store(what, "cache", cache, tuple(k.shape[:-2]), k.shape[-1], None, k.device)
-    for t in cache[:2]:
-        if not _fits(t, 8):
-            _fail(what, "the cache's rows must be contiguous and start at multiples of 8 bytes")
+    shape = k.shape
+    n = len(shape) - 3
+    if n < 0:
+        _fail(what, f"the cache must be (..., heads, slots, width), got {tuple(shape)}")
+    _check_store(what, "cache", cache, shape, None, k.get_device())
+    if k.stride(-1) != 1 or v.stride(-1) != 1:
+        _fail(what, "the width of the cache must be contiguous")
     batch = 1
-    for n in k.shape[:-3]:
-        batch *= n
-    try:  # one leading dimension: a view, since the cache is written
-        return batch, [t.view(batch, *t.shape[k.dim() - 3:]) for t in cache]
-    except RuntimeError:
-        _fail(what, "the cache's leading dimensions must be one by their strides")
+    for x in shape[:n]:
+        batch *= x
+    return batch, n, (k.data_ptr(), v.data_ptr(), *_one_lead(what, k, n), *_one_lead(what, v, n), k_scale.data_ptr(), v_scale.data_ptr(),
+                      *_one_lead(what, k_scale, n), *_one_lead(what, v_scale, n))
 
 
 def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, positions: Union[int, torch.Tensor]) -> None:
@@ -229,42 +239,44 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, positions:
     rounded to the nearest e4m3 number, ties to even. fp16 numbers beyond 61440 are kept as that. A row with an infinity
     or a NaN becomes NaN."""
     what = "cache_write"
-    batch, store = _cache_operands(what, cache)
-    device = cache.k.device
-    heads, slots, width = cache.k.shape[-3:]
-    lead = cache.k.shape[:-3]
-    _check_operands(what, device, k, v)
+    batch, n, fields = _cache_fields(what, cache)
+    shape, got = cache.k.shape, k.shape
+    heads, slots, width = shape[n:]
+    index = cache.k.get_device()
+    _check_operands(what, index, (k, v))
     code = dtype_code(k.dtype)
-    if k.shape != v.shape or v.dtype != k.dtype or k.dim() != cache.k.dim() or k.shape[:-2] != cache.k.shape[:-2] or k.shape[-1] != width:
-        _fail(what, f"k and v must be alike, {(*lead, heads, 'length', width)}, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    length = k.shape[-2]
+    if got != v.shape or v.dtype != k.dtype or len(got) != n + 3 or got[:-2] != shape[:-2] or got[-1] != width:
+        _fail(what, f"k and v must be alike, {(*shape[:-2], 'length', width)}, got {k.dtype} {tuple(got)} and {v.dtype} {tuple(v.shape)}")
+    length = got[-2]
     at, position = None, 0
     if torch.is_tensor(positions):
-        at = _check_int32(what, "positions", positions, lead, device)
+        at = _check_int32(what, "positions", positions, shape[:n], index)
     else:
         position = positions
     if not k.numel():
         return
-    k, v = (_placed(t.reshape(batch, *t.shape[-3:]), 16) for t in (k, v))
-    rows = lambda s: (s[0], 0, s[1], s[2])  # noqa: E731
-    _call(device, "dz_cache_write", _KEYS_VALUES.pack(*_packed((k, v), rows)), _KEYS_VALUES.pack(*_packed(store, rows)), code, batch, heads,
-          length, width, slots, None if at is None else at.data_ptr(), position)
+    if n > 1:
+        k, v = k.flatten(0, n - 1), v.flatten(0, n - 1)
+    elif n == 0:
+        k, v = k.unsqueeze(0), v.unsqueeze(0)
+    k, (a, b, c) = _rows(k)
+    v, (d, e, f) = _rows(v)
+    _call(k.device, "dz_cache_write", _KEYS_VALUES.pack(k.data_ptr(), v.data_ptr(), a, 0, b, c, d, 0, e, f, *_NO_SCALES),
+          _KEYS_VALUES.pack(*fields), code, batch, heads, length, width, slots, None if at is None else at.data_ptr(), position)
 
 
 def cache_read(cache: QuantizedKV, length: int, dtype: torch.dtype, start: int = 0) -> KV:
-    """Slots start .. start + length - 1 of the cache as keys and values of a dtype, laid out (..., length, heads, width) and
-    seen as (..., heads, length, width)."""
+    """Slots start .. start + length - 1 of the cache as keys and values (..., heads, length, width) of a dtype."""
     what = "cache_read"
-    batch, store = _cache_operands(what, cache)
-    device = cache.k.device
-    heads, slots, width = cache.k.shape[-3:]
+    batch, n, fields = _cache_fields(what, cache)
+    shape = cache.k.shape
+    heads, slots, width = shape[n:]
     code = dtype_code(dtype)
     if length < 0 or start < 0 or start + length > slots:
         _fail(what, f"slots {start} to {start + length} of {slots}")
-    kv = [torch.empty(batch, length, heads, width, dtype=dtype, device=device).transpose(1, 2) for _ in range(2)]
-    if batch * length:
-        rows = lambda s: (s[0], 0, s[1], s[2])  # noqa: E731
-        _call(device, "dz_cache_read", _KEYS_VALUES.pack(*_packed(store, rows)), _KEYS_VALUES.pack(*_packed(kv, rows)), code, batch, heads,
-              length, width, slots, start)
-    lead = cache.k.shape[:-3]
-    return KV(*(t if len(lead) == 1 else t.unflatten(0, lead) if lead else t[0] for t in kv))
+    k, v = (torch.empty((*shape[:-2], length, width), dtype=dtype, device=cache.k.device) for _ in range(2))
+    if k.numel():
+        s = (heads * length * width, 0, length * width, width)
+        _call(k.device, "dz_cache_read", _KEYS_VALUES.pack(*fields), _KEYS_VALUES.pack(k.data_ptr(), v.data_ptr(), *s, *s, *_NO_SCALES), code,
+              batch, heads, length, width, slots, start)
+    return KV(k, v)

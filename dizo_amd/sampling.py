@@ -22,7 +22,11 @@ def _parameter(what: str, name: str, value, lead, device, dtype):
     if not torch.is_tensor(value):
         return value, None
     _check_rows(what, name, value, lead, device, (dtype,))
-    return 0, value.reshape(-1).contiguous()
+    return 0, _dense(value)
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: Union[float, torch.Tensor] = 1.0,
@@ -59,12 +63,11 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: U
     for name, x, xs in (("top_p", p, ps), ("min_p", m, ms)):
         if xs is None and not 0.0 <= x <= 1.0:
             _fail(what, f"{name} must be 0 to 1, got {x}")
-    logits = logits.detach()
     tokens = torch.empty(lead, dtype=torch.int64, device=device)
     rows = tokens.numel()
     if rows:
-        x = logits.reshape(-1, vocab)
-        u = uniform.reshape(-1).contiguous()
+        x = logits if logits.dim() == 2 else logits.detach().reshape(-1, vocab)
+        u = _dense(uniform)
         _call(device, "dz_sample_tokens", x.data_ptr(), dtype_code(logits.dtype), rows, vocab, x.stride(0), u.data_ptr(), t, k, p, m,
               *(None if a is None else a.data_ptr() for a in (ts, ks, ps, ms)), tokens.data_ptr())
     return tokens
