@@ -18,15 +18,30 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
 constexpr int kMaxPieces = (int)(kMaxSampleVocab / (kThreads * 4)) * kWaves;  // a wave's part of 1,024 vectors
+constexpr int kMaxHeld = 8;      // slabs in LDS: 128 KB
+constexpr int kList = kThreads;  // logits that are sorted one by one
 
+struct Entry {
+  uint64_t order;  // the logit's key, and its token from the last on: larger first, equal ones by token
+  uint64_t weight;
+};
+__device__ __forceinline__ uint32_t token_of(uint64_t order) { return ~(uint32_t)order; }
+__device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t token) { return (uint64_t)key << 32 | (uint32_t)~token; }
+
+template <int PIECES>
 struct Shared {
-  uint64_t bins[kBins];
-  uint64_t pieces[kMaxPieces];
+  union {  // sums by bins, then what one of them holds
+    uint64_t bins[kBins];
+    Entry list[kList];
+  };
+  uint64_t pieces[PIECES];
+  double powers[64];  // 2^(i / 64)
   uint64_t wave_sum[kWaves];
   float wave_max[kWaves];
   uint32_t wave_flag[kWaves];
   uint64_t found_before;
-  uint32_t found, low, high, token;
+  uint64_t cut;
+  uint32_t found, low, high, listed;
 };
 
 // fp32 numbers as whole ones of the same order. (-0 equals 0.)
@@ -46,22 +61,35 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t x) {  // sums up to and w
   return x;
 }
 
+// Sums up to and with this thread, and of all of them. Every thread has read what the last call left.
+template <class Sh>
+__device__ __forceinline__ uint64_t block_scan(Sh& sh, uint64_t x, uint64_t& all) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  x = wave_scan(x);
+  __syncthreads();
+  if (lane == 63) sh.wave_sum[wave] = x;
+  __syncthreads();
+  all = 0;
+  for (uint32_t i = 0; i < kWaves; ++i) {
+    if (i < wave) x += sh.wave_sum[i];
+    all += sh.wave_sum[i];
+  }
+  return x;
+}
+
 // The first of n places whose sum with all before it reaches `target` (at least 1), and the sum before it: found and
 // found_before. n where none does.
-__device__ __forceinline__ void find(Shared& sh, const uint64_t* values, uint32_t n, uint64_t target) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (n + kThreads - 1) / kThreads;
-  uint64_t mine = 0;
+template <class Sh>
+__device__ __forceinline__ void find(Sh& sh, const uint64_t* values, uint32_t n, uint64_t target) {
+  const uint32_t tid = threadIdx.x, each = (n + kThreads - 1) / kThreads;
+  uint64_t mine = 0, all;
   for (uint32_t i = 0; i < each; ++i)
     if (tid * each + i < n) mine += values[tid * each + i];
-  const uint64_t upto = wave_scan(mine);
-  if (lane == 63) sh.wave_sum[wave] = upto;
-  if (tid == 0) {
+  uint64_t before = block_scan(sh, mine, all) - mine;
+  if (tid == 0 && all < target) {
     sh.found = n;
-    sh.found_before = 0;
+    sh.found_before = all;
   }
-  __syncthreads();
-  uint64_t before = upto - mine;
-  for (uint32_t i = 0; i < wave; ++i) before += sh.wave_sum[i];
   if (before < target && before + mine >= target) {
     for (uint32_t i = 0; i < each; ++i) {
       const uint64_t v = tid * each + i < n ? values[tid * each + i] : 0;
@@ -76,64 +104,127 @@ __device__ __forceinline__ void find(Shared& sh, const uint64_t* values, uint32_
   __syncthreads();
 }
 
-template <class T>
+// A row, 16 bytes a thread and slab: HELD in LDS, or read again for each pass.
+template <class T, bool HELD>
 struct Row {
   typedef typename T::V Loose __attribute__((aligned(sizeof(typename T::Elem))));
+  using Elem = typename T::Elem;
   static constexpr int PER = T::kPer16;
-  const typename T::Elem* x;
+  const Elem* x;
+  typename T::V* held;  // slab after slab
   uint32_t vocab, slabs;
   bool infinite;  // the largest logit is +inf: those are 0, the others -inf
 
-  // f(logits of the thread's vector of a slab, the first one's token); those past the row are -inf
-  template <class F>
-  __device__ __forceinline__ void slab(uint32_t s, F f) const {
+  __device__ __forceinline__ typename T::V load(uint32_t s) const {  // those past the row are -inf
     const uint32_t at = (s * kThreads + threadIdx.x) * PER;
-    float v[PER];
+    typename T::V v;
     if (at + PER <= vocab) {
-      const typename T::V e = *(const Loose*)(x + at);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) v[j] = (float)e[j];
+      v = *(const Loose*)(x + at);
     } else {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) v[j] = at + j < vocab ? (float)x[at + j] : -INFINITY;
+      for (int j = 0; j < PER; ++j) v[j] = at + j < vocab ? x[at + j] : (Elem)-INFINITY;
     }
+    return v;
+  }
+  // f(the logits of the thread's vector of a slab, the first one's token)
+  template <class F>
+  __device__ __forceinline__ void give(const typename T::V& e, uint32_t s, F f) const {
+    float v[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = (float)e[j];
     if (infinite)
 #pragma unroll
       for (int j = 0; j < PER; ++j) v[j] = v[j] == INFINITY ? 0.f : -INFINITY;
-    f(v, at);
+    f(v, (s * kThreads + threadIdx.x) * PER);
+  }
+  template <class F>
+  __device__ __forceinline__ void slab(uint32_t s, F f) const {
+    give(HELD ? held[s * kThreads + threadIdx.x] : load(s), s, f);
+  }
+  // for each slab: f(s, logits, first token)
+  template <class F>
+  __device__ __forceinline__ void slabs_do(F f) const {
+#pragma unroll 1
+    for (uint32_t s = 0; s < slabs; ++s) slab(s, [&](const float(&v)[PER], uint32_t at) { f(s, v, at); });
   }
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    for (uint32_t s = 0; s < slabs; ++s) slab(s, [&](const float(&v)[PER], uint32_t) {
+    slabs_do([&](uint32_t, const float(&v)[PER], uint32_t at) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) f(v[j]);
+      for (int j = 0; j < PER; ++j) f(v[j], at + j);
     });
+  }
+  // The first pass: four slabs' loads at a time.
+  template <class F>
+  __device__ __forceinline__ void first(F f) const {
+    for (uint32_t s0 = 0; s0 < slabs; s0 += 4) {
+      typename T::V e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < slabs) e[i] = load(s0 + i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < slabs) {
+          if (HELD) held[(s0 + i) * kThreads + threadIdx.x] = e[i];
+#pragma unroll
+          for (int j = 0; j < PER; ++j) f((float)e[i][j]);
+        }
+    }
   }
 };
 
-// What is kept: logits above the cut's, and the first `equal` of those that equal it.
-struct Cut {
-  uint32_t key, equal;
-  uint32_t there;  // that equal it
-};
+// Sorts n' = 2^i >= n entries, one a thread, the largest order first.
+template <class Sh>
+__device__ __forceinline__ void sort(Sh& sh, Entry& e, uint32_t n) {
+  const uint32_t tid = threadIdx.x;
+  uint32_t size = 2;
+  while (size < n) size *= 2;
+  for (uint32_t k = 2; k <= size; k *= 2)
+    for (uint32_t j = k / 2; j > 0; j /= 2) {
+      Entry o;
+      if (j >= 64) {
+        __syncthreads();
+        sh.list[tid] = e;
+        __syncthreads();
+        o = sh.list[tid ^ j];
+      } else {
+        o.order = __shfl_xor(e.order, j);
+        o.weight = __shfl_xor(e.weight, j);
+      }
+      const bool first = (tid & j) == 0, down = (tid & k) == 0;  // the larger one goes first
+      if (first == down ? o.order > e.order : o.order < e.order) e = o;
+    }
+}
 
-template <class T>
+// What is kept: logits whose order is the cut's or above it.
+template <class T, bool HELD>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
-  __shared__ Shared sh;
-  constexpr int PER = Row<T>::PER;
+  constexpr int PER = T::kPer16;
+  __shared__ Shared<HELD ? kMaxHeld * kWaves : kMaxPieces> sh;
+  extern __shared__ __attribute__((aligned(16))) char held[];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x;
-  Row<T> row{(const typename T::Elem*)a.logits + (int64_t)r * a.stride, a.vocab, (a.vocab + kThreads * PER - 1) / (kThreads * PER), false};
+  Row<T, HELD> row;
+  row.x = (const typename T::Elem*)a.logits + (int64_t)r * a.stride;
+  row.vocab = a.vocab;
+  row.slabs = (a.vocab + kThreads * PER - 1) / (kThreads * PER);
+  row.infinite = false;
+  row.held = (typename T::V*)held;
   const float u = a.uniform[r];
   const double temperature = a.temperatures ? a.temperatures[r] : a.temperature;
-  const double top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p0 = a.min_ps ? a.min_ps[r] : a.min_p, min_p = min_p0 < 1.0 ? min_p0 : 1.0;  // the largest is always kept
+  const double top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p = a.min_ps ? a.min_ps[r] : a.min_p;
   const int32_t top_k = temperature == 0 ? 1 : a.top_ks ? a.top_ks[r] : a.top_k;
+  const double unit = temperature == 0 ? 1.0 : temperature;
 
-  float m = -INFINITY;
-  bool none = !(u >= 0.f && u <= 1.f) || !(temperature == 0 || (temperature >= 0x1p-63 && temperature < 0x1p64)) || top_p != top_p || min_p0 != min_p0;
-  row.each([&](float x) {
-    m = fmaxf(m, x);
+  if (tid < 64) sh.powers[tid] = exp2(tid / 64.0);
+  for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+  if (tid == 0) sh.listed = 0;
+  bool none = !(u >= 0.f && u <= 1.f) || !(temperature == 0 || (temperature >= 0x1p-63 && temperature < 0x1p64)) || top_p != top_p || min_p != min_p;
+  float mine = -INFINITY;  // the largest of this thread's
+  row.first([&](float x) {
+    mine = fmaxf(mine, x);
     none |= x != x;
   });
+  float m = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
   none = __any(none);
@@ -152,49 +243,93 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   }
   if (m == INFINITY) {
     row.infinite = true;
+    mine = mine == INFINITY ? 0.f : -INFINITY;
     m = 0.f;
   }
 
-  // Weights as whole numbers of 2^-shift.
+  // Weights as whole numbers of 2^-shift. 2^t = 2^(n / 64) 2^r, n / 64 the nearest such number to t: the table, and Taylor's
+  // polynomial of 2^r (|r| <= 2^-7: the next term is under 2^-54).
   const int lg = 32 - __clz((a.vocab - 1) | 1), shift = 62 - lg < 46 ? 62 - lg : 46;
-  const double inverse = 1.4426950408889634074 / (temperature == 0 ? 1.0 : temperature);
-  auto weight = [&](float x) -> uint64_t {
-    const double t = ((double)x - (double)m) * inverse;
-    return t < -(double)(shift + 2) ? 0 : (uint64_t)__builtin_rint(exp2(t + shift));
+  const double inverse = 1.4426950408889634074 / unit, wide_m = m, far = -(double)(shift + 2);
+  auto power_of = [&](float x) { return ((double)x - wide_m) * inverse; };
+  auto weight_at = [&](double t) -> uint64_t {
+    constexpr double kNearest = 0x1.8p46;  // adding it leaves the nearest n / 64, with n in the low bits
+    const double q = t + kNearest, f = t - (q - kNearest);
+    const int32_t n = (int32_t)__double_as_longlong(q);
+    double p = __builtin_fma(f, 0x1.5d87fe78a673p-10, 0x1.3b2ab6fba4e77p-7);
+    p = __builtin_fma(f, p, 0x1.c6b08d704a0bfp-5);
+    p = __builtin_fma(f, p, 0x1.ebfbdff82c58ep-3);
+    p = __builtin_fma(f, p, 0x1.62e42fefa39efp-1) * f;
+    const double w = sh.powers[n & 63], y = __builtin_fma(w, p, w);
+    const double scaled = __longlong_as_double(__double_as_longlong(y) + ((int64_t)((n >> 6) + shift) << 52));
+    const uint64_t whole = (uint64_t)__double_as_longlong(scaled + 0x1p52) & 0xfffffffffffffull;
+    return t < far ? 0 : whole;
   };
+  auto weight = [&](float x) -> uint64_t { return weight_at(power_of(x)); };
+  // min_p as the power that a kept weight's reaches; the largest is always kept
+  const double least_power = min_p > 0 ? fmin(log2(min_p), 0.0) : -INFINITY;
 
   auto clear = [&]() {
     for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
   };
-  // Adds value(x) of the logits of keys low to high to bins by their key, the largest first.
-  auto by_key = [&](uint32_t low, uint32_t high, int s, auto value) {
-    row.each([&](float x) {
-      const uint32_t k = key_of(x);
-      if (k >= low && k <= high && x != -INFINITY) atomicAdd((unsigned long long*)&sh.bins[(high - k) >> s], (unsigned long long)value(x));
-    });
-  };
-  // And to bins by their distance to the largest: 64 a unit of the logits over the temperature, the last one what is further away.
-  const float per_unit = (float)(64.0 / (temperature == 0 ? 1.0 : temperature));
+  auto add_to = [&](uint32_t bin, uint64_t value) { atomicAdd((unsigned long long*)&sh.bins[bin], (unsigned long long)value); };
+  // Bins by the distance to the largest: 64 a unit of the logits over the temperature, the last one what is further away.
+  const float per_unit = (float)(64.0 / unit);
   auto bin_of = [&](float x) {
     const float d = (m - x) * per_unit;
     return d < (float)(kBins - 1) ? (uint32_t)d : (uint32_t)kBins - 1;
   };
-  // The cut at which the values of the logits above the one `above` (keys greater than that), summed from the largest on, reach `target`.
-  auto cut_at = [&](uint64_t target, uint32_t above, auto value) -> Cut {
-    // sh.bins has the sums by distance
+  // Logits (above -inf) that `take` takes, one a thread and sorted; the others are 0 (of no order). How many: more than kList if they
+  // do not fit, and nothing then.
+  Entry e;
+  auto list = [&](auto take) -> uint32_t {
+    __syncthreads();
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    row.each([&](float x, uint32_t token) {
+      if (x != -INFINITY && take(x, token)) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kList) sh.list[at].order = order_of(key_of(x), token);
+      }
+    });
+    __syncthreads();
+    const uint32_t n = sh.listed;
+    e = Entry{0, 0};
+    if (n <= kList) {
+      if (tid < n) {
+        e.order = sh.list[tid].order;
+        e.weight = weight(of_key((uint32_t)(e.order >> 32)));
+      }
+      sort(sh, e, n);
+    }
+    return n;
+  };
+  // The order at which the values of the logits of an order of `least` or above, summed from the largest on, reach `target`; sh.bins
+  // has the sums by distance. 0: they do not.
+  auto cut_at = [&](uint64_t target, uint64_t least, bool counts) -> uint64_t {
+    auto value = [&](float x) -> uint64_t { return counts ? 1 : weight(x); };
     find(sh, sh.bins, kBins, target);
-    uint32_t bin = sh.found;
+    const uint32_t bin = sh.found;
     uint64_t before = sh.found_before;
-    if (bin == kBins) return Cut{above, 0, 0};  // all of them
+    if (bin == kBins) return least;
+    if (list([&](float x, uint32_t token) { return bin_of(x) == bin && order_of(key_of(x), token) >= least; }) <= kList) {
+      uint64_t all;
+      const uint64_t v = !e.order ? 0 : counts ? 1 : e.weight, upto = block_scan(sh, v, all);
+      if (before + upto - v < target && before + upto >= target) sh.cut = e.order;
+      __syncthreads();
+      return sh.cut;
+    }
+    // Too many for that: bins of keys, down to one key, and the first of those that have it by their token.
+    uint32_t low = ~0u, high = 0;
     if (tid == 0) {
       sh.low = ~0u;
       sh.high = 0;
     }
     __syncthreads();
-    uint32_t low = ~0u, high = 0;
-    row.each([&](float x) {
-      const uint32_t k = key_of(x);
-      if (k > above && x != -INFINITY && bin_of(x) == bin) {
+    auto of_bin = [&](float x, uint32_t token) { return x != -INFINITY && bin_of(x) == bin && order_of(key_of(x), token) >= least; };
+    row.each([&](float x, uint32_t token) {
+      if (of_bin(x, token)) {
+        const uint32_t k = key_of(x);
         low = k < low ? k : low;
         high = k > high ? k : high;
       }
@@ -211,154 +346,169 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
       __syncthreads();
       clear();
       __syncthreads();
-      by_key(low, high, s, value);
+      row.each([&](float x, uint32_t token) {
+        const uint32_t k = key_of(x);
+        if (k >= low && k <= high && of_bin(x, token)) add_to((high - k) >> s, value(x));
+      });
       __syncthreads();
       find(sh, sh.bins, kBins, target - before);
       if (sh.found >= kBins) break;  // (the sums are the ones that found the bin)
       before += sh.found_before;
       high = high - (sh.found << s);
-      const uint32_t last = high - low < (1u << s) - 1 ? low : high - ((1u << s) - 1);
-      low = last;
+      low = high - low < (1u << s) - 1 ? low : high - ((1u << s) - 1);
     }
-    // `low` is the cut
+    const uint64_t one = value(of_key(low)), nth = (target - before + one - 1) / one;  // of those equal to the cut
+    auto is_equal = [&](float x, uint32_t token) { return x != -INFINITY && key_of(x) == low && order_of(low, token) >= least; };
     __syncthreads();
-    if (tid == 0) sh.found = 0;
-    __syncthreads();
-    uint32_t n = 0;
-    row.each([&](float x) { n += x != -INFINITY && key_of(x) == low; });
-    if (n) atomicAdd(&sh.found, n);
-    __syncthreads();
-    const uint64_t one = value(of_key(low));
-    const uint64_t equal = (target - before + one - 1) / one;
-    return Cut{low, (uint32_t)(equal < sh.found ? equal : sh.found), sh.found};
-  };
-
-  Cut cut{0, 0, 0};
-  if (top_k > 0 && (uint32_t)top_k < a.vocab) {
-    clear();
-    __syncthreads();
-    row.each([&](float x) {
-      if (x != -INFINITY) atomicAdd((unsigned long long*)&sh.bins[bin_of(x)], 1ull);
+    row.slabs_do([&](uint32_t s, const float(&v)[PER], uint32_t at) {
+      uint64_t n = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) n += is_equal(v[j], at + j);
+      n = wave_scan(n);
+      if (lane == 63) sh.pieces[s * kWaves + wave] = n;
     });
     __syncthreads();
-    cut = cut_at(top_k, 0, [](float) -> uint64_t { return 1; });
+    find(sh, sh.pieces, row.slabs * kWaves, nth);
+    const uint32_t piece = sh.found;
+    if (piece < row.slabs * kWaves && wave == piece % kWaves) {
+      row.slab(piece / kWaves, [&](const float(&v)[PER], uint32_t at) {
+        uint64_t n = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) n += is_equal(v[j], at + j);
+        uint64_t upto = sh.found_before + wave_scan(n) - n;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (is_equal(v[j], at + j) && ++upto == nth) sh.cut = order_of(low, at + j);
+      });
+    }
+    __syncthreads();
+    return sh.cut;
+  };
+  // What top-p keeps of a sum: whole numbers that have to be reached.
+  auto share_of = [&](uint64_t total) -> uint64_t {
+    const double share = __builtin_ceil(top_p * (double)total);
+    return share < 1.0 ? 1 : (uint64_t)share;
+  };
+  // u of a sum, as what has to be reached.
+  auto drawn_of = [&](uint64_t sum) -> uint64_t {
+    const uint64_t target = (uint64_t)__builtin_floor((double)u * (double)sum) + 1;
+    return target < sum ? target : sum;
+  };
+
+  uint64_t cut = 0;
+  if (top_k > 0 && (uint32_t)top_k < a.vocab) {
+    // The bin up to which top_k threads have their largest holds top_k logits, too: nothing further away is among the largest.
+    uint32_t last_bin = kBins;
+    if (top_k <= kThreads) {
+      if (mine != -INFINITY) add_to(bin_of(mine), 1);
+      __syncthreads();
+      find(sh, sh.bins, kBins, top_k);
+      last_bin = sh.found;
+    }
+    const uint32_t n = top_k <= kThreads ? list([&](float x, uint32_t) { return bin_of(x) <= last_bin; }) : kList + 1;
+    if (n <= kList) {
+      // All that matters is in the list, sorted: what is kept is its beginning.
+      uint64_t total, sum;
+      if (tid >= (uint32_t)top_k) e = Entry{0, 0};
+      const uint64_t upto = block_scan(sh, e.weight, total);
+      if (top_p < 1.0 && upto - e.weight >= share_of(total)) e = Entry{0, 0};
+      if (!e.order || power_of(of_key((uint32_t)(e.order >> 32))) < least_power) e = Entry{0, 0};
+      const uint32_t kept = __syncthreads_count(e.order != 0);
+      e.order &= 0xffffffffu;  // by token from here on (the first one has the largest order)
+      sort(sh, e, kept);
+      const uint64_t before = block_scan(sh, e.weight, sum) - e.weight, target = drawn_of(sum);
+      if (before < target && before + e.weight >= target) a.tokens[r] = token_of(e.order);
+      return;
+    }
+    __syncthreads();
+    clear();
+    __syncthreads();
+    row.each([&](float x, uint32_t) {
+      if (x != -INFINITY && bin_of(x) <= last_bin) add_to(bin_of(x), 1);
+    });
+    __syncthreads();
+    cut = cut_at(top_k, 0, true);
+    __syncthreads();
+    clear();
+    __syncthreads();
   }
   if (top_p < 1.0) {
-    __syncthreads();
-    clear();
-    __syncthreads();
-    row.each([&](float x) {
-      if (x != -INFINITY && key_of(x) > cut.key) atomicAdd((unsigned long long*)&sh.bins[bin_of(x)], (unsigned long long)weight(x));
+    uint64_t sum = 0, total;
+    row.each([&](float x, uint32_t token) {
+      if (x != -INFINITY && order_of(key_of(x), token) >= cut) {
+        const uint64_t w = weight(x);
+        sum += w;
+        if (w) add_to(bin_of(x), w);
+      }
     });
-    __syncthreads();
-    uint64_t mine = 0;
-    for (int i = tid; i < kBins; i += kThreads) mine += sh.bins[i];
-    mine = wave_scan(mine);
-    if (lane == 63) sh.wave_sum[wave] = mine;
-    __syncthreads();
-    uint64_t sum = 0;
-    for (int i = 0; i < kWaves; ++i) sum += sh.wave_sum[i];
-    __syncthreads();
-    const uint64_t one = cut.equal ? weight(of_key(cut.key)) : 0, total = sum + cut.equal * one;
-    const double share = __builtin_ceil(top_p * (double)total);
-    const uint64_t target = share < 1.0 ? 1 : (uint64_t)share;
-    if (target <= sum) {
-      const Cut c = cut_at(target, cut.key, [&](float x) { return weight(x); });
-      if (c.key > cut.key) cut = c;
-    } else if (one) {
-      const uint64_t equal = (target - sum + one - 1) / one;
-      if (equal < cut.equal) cut.equal = (uint32_t)equal;
-    }
+    block_scan(sh, sum, total);
+    cut = cut_at(share_of(total), cut, false);
   }
 
-  // Which of the equal ones are kept: up to token `last`.
-  uint32_t last = ~0u;
-  const uint32_t pieces = row.slabs * kWaves;
-  if (cut.equal < cut.there) {
-    __syncthreads();
-    for (uint32_t s = 0; s < row.slabs; ++s) {
-      uint32_t n = 0;
-      row.slab(s, [&](const float(&v)[PER], uint32_t) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) n += v[j] != -INFINITY && key_of(v[j]) == cut.key;
-      });
-      const uint64_t upto = wave_scan(n);
-      if (lane == 63) sh.pieces[s * kWaves + wave] = upto;
-    }
-    __syncthreads();
-    find(sh, sh.pieces, pieces, cut.equal);
-    const uint32_t piece = sh.found;
-    if (wave == piece % kWaves) {
-      row.slab(piece / kWaves, [&](const float(&v)[PER], uint32_t at) {
-        uint32_t n = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) n += v[j] != -INFINITY && key_of(v[j]) == cut.key;
-        uint64_t before = sh.found_before + wave_scan(n) - n;
-        if (before < cut.equal && before + n >= cut.equal)
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (v[j] != -INFINITY && key_of(v[j]) == cut.key && ++before == cut.equal) sh.token = at + j;
-      });
-    }
-    __syncthreads();
-    last = sh.token;
-  }
-
-  auto kept = [&](float x, uint32_t token) -> uint64_t {
-    const uint32_t k = key_of(x);
-    if (x == -INFINITY || k < cut.key || (k == cut.key && token > last)) return 0;
-    const uint64_t w = weight(x);
-    return min_p > 0.0 && exp2(((double)x - (double)m) * inverse) < min_p ? 0 : w;
+  // What is kept of each piece of the row, and the piece and token that u falls on.
+  auto kept = [&](float x, uint32_t token, double& t) {
+    t = power_of(x);
+    return x != -INFINITY && t >= least_power && t >= far && order_of(key_of(x), token) >= cut;
   };
+  const uint32_t pieces = row.slabs * kWaves;
+  uint64_t all = 0, sum;
   __syncthreads();
-  for (uint32_t s = 0; s < row.slabs; ++s) {
+  row.slabs_do([&](uint32_t s, const float(&v)[PER], uint32_t at) {
     uint64_t n = 0;
-    row.slab(s, [&](const float(&v)[PER], uint32_t at) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) n += kept(v[j], at + j);
-    });
-    n = wave_scan(n);
-    if (lane == 63) sh.pieces[s * kWaves + wave] = n;
-  }
-  __syncthreads();
-  uint64_t sum = 0;
-  for (uint32_t i = tid; i < pieces; i += kThreads) sum += sh.pieces[i];
-  sum = wave_scan(sum);
-  if (lane == 63) sh.wave_sum[wave] = sum;
-  __syncthreads();
-  sum = 0;
-  for (int i = 0; i < kWaves; ++i) sum += sh.wave_sum[i];
-  __syncthreads();
-  // the first token up to which the sum exceeds u of the whole: reaches the next whole number
-  uint64_t target = (uint64_t)__builtin_floor((double)u * (double)sum) + 1;
-  if (target > sum) target = sum;
+    for (int j = 0; j < PER; ++j) {
+      double t;
+      if (kept(v[j], at + j, t)) n += weight_at(t);
+    }
+    all += n;
+    if (__any(n != 0)) n = wave_scan(n);
+    if (lane == 63 && s < row.slabs) sh.pieces[s * kWaves + wave] = n;
+  });
+  block_scan(sh, all, sum);
+  const uint64_t target = drawn_of(sum);
   find(sh, sh.pieces, pieces, target);
   const uint32_t piece = sh.found;
-  if (wave == piece % kWaves) {
+  if (piece < pieces && wave == piece % kWaves) {
     row.slab(piece / kWaves, [&](const float(&v)[PER], uint32_t at) {
       uint64_t w[PER], n = 0;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) n += w[j] = kept(v[j], at + j);
+      for (int j = 0; j < PER; ++j) {
+        double t;
+        w[j] = kept(v[j], at + j, t) ? weight_at(t) : 0;
+        n += w[j];
+      }
       uint64_t before = sh.found_before + wave_scan(n) - n;
-      if (before < target && before + n >= target)
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          if (before < target && before + w[j] >= target) a.tokens[r] = at + j;
-          before += w[j];
-        }
+      for (int j = 0; j < PER; ++j) {
+        if (before < target && before + w[j] >= target) a.tokens[r] = at + j;
+        before += w[j];
+      }
     });
   }
+}
+
+template <class T>
+hipError_t launch_typed(const SampleRows& a, hipStream_t st) {
+  const uint32_t slabs = (a.vocab + kThreads * T::kPer16 - 1) / (kThreads * T::kPer16);
+  if (slabs > kMaxHeld) {
+    sample_kernel<T, false><<<a.nrows, kThreads, 0, st>>>(a);
+    return hipGetLastError();
+  }
+  const uint32_t bytes = slabs * kThreads * 16;
+  const hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, kMaxHeld * kThreads * 16);
+  if (e != hipSuccess) return e;
+  sample_kernel<T, true><<<a.nrows, kThreads, bytes, st>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_sample(int dtype, const SampleRows& a, hipStream_t st) {
   switch (dtype) {
-    case 0: sample_kernel<TypeF32><<<a.nrows, kThreads, 0, st>>>(a); break;
-    case 1: sample_kernel<TypeF16><<<a.nrows, kThreads, 0, st>>>(a); break;
-    default: sample_kernel<TypeBF16><<<a.nrows, kThreads, 0, st>>>(a);
+    case 0: return launch_typed<TypeF32>(a, st);
+    case 1: return launch_typed<TypeF16>(a, st);
+    default: return launch_typed<TypeBF16>(a, st);
   }
-  return hipGetLastError();
 }
 
 }  // namespace dz
