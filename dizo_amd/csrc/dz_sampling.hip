@@ -16,25 +16,23 @@
 namespace dz {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
-constexpr int kMaxPieces = (int)(kMaxSampleVocab / (kThreads * 4)) * kWaves;  // a wave's part of 1,024 vectors
-constexpr int kMaxHeld = 8;      // slabs in LDS: 128 KB
-constexpr int kList = kThreads;  // logits that are sorted one by one
+constexpr int kBins = 2048;
+constexpr int kHeldBytes = 128 * 1024;  // of a row in LDS
+constexpr uint32_t kShortRow = 8192;
 
-struct Entry {
-  uint64_t order;  // the logit's key, and its token from the last on: larger first, equal ones by token
-  uint64_t weight;
-};
-__device__ __forceinline__ uint32_t token_of(uint64_t order) { return ~(uint32_t)order; }
+// The order of logits: a logit's key, and its token from the last on. Larger first, equal ones by token.
+__device__ __forceinline__ uint32_t token_of(uint64_t low) { return ~(uint32_t)low; }
 __device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t token) { return (uint64_t)key << 32 | (uint32_t)~token; }
 
-template <int PIECES>
+template <int THREADS, int PIECES>
 struct Shared {
+  static constexpr int kThreads = THREADS, kWaves = THREADS / 64;
+  static constexpr int kList = THREADS;  // logits that are sorted one by one
   union {  // sums by bins, then what one of them holds
     uint64_t bins[kBins];
-    Entry list[kList];
+    uint64_t list[kList];
   };
-  uint64_t pieces[PIECES];
+  uint64_t pieces[PIECES];  // sums of a wave's part of a slab
   double powers[64];  // 2^(i / 64)
   uint64_t wave_sum[kWaves];
   float wave_max[kWaves];
@@ -70,7 +68,7 @@ __device__ __forceinline__ uint64_t block_scan(Sh& sh, uint64_t x, uint64_t& all
   if (lane == 63) sh.wave_sum[wave] = x;
   __syncthreads();
   all = 0;
-  for (uint32_t i = 0; i < kWaves; ++i) {
+  for (uint32_t i = 0; i < Sh::kWaves; ++i) {
     if (i < wave) x += sh.wave_sum[i];
     all += sh.wave_sum[i];
   }
@@ -81,7 +79,7 @@ __device__ __forceinline__ uint64_t block_scan(Sh& sh, uint64_t x, uint64_t& all
 // found_before. n where none does.
 template <class Sh>
 __device__ __forceinline__ void find(Sh& sh, const uint64_t* values, uint32_t n, uint64_t target) {
-  const uint32_t tid = threadIdx.x, each = (n + kThreads - 1) / kThreads;
+  const uint32_t tid = threadIdx.x, each = (n + Sh::kThreads - 1) / Sh::kThreads;
   uint64_t mine = 0, all;
   for (uint32_t i = 0; i < each; ++i)
     if (tid * each + i < n) mine += values[tid * each + i];
@@ -105,7 +103,7 @@ __device__ __forceinline__ void find(Sh& sh, const uint64_t* values, uint32_t n,
 }
 
 // A row, 16 bytes a thread and slab: HELD in LDS, or read again for each pass.
-template <class T, bool HELD>
+template <class T, bool HELD, int kThreads>
 struct Row {
   typedef typename T::V Loose __attribute__((aligned(sizeof(typename T::Elem))));
   using Elem = typename T::Elem;
@@ -173,37 +171,37 @@ struct Row {
   }
 };
 
-// Sorts n' = 2^i >= n entries, one a thread, the largest order first.
+// Sorts 2^i >= n numbers, one a thread, the largest first.
 template <class Sh>
-__device__ __forceinline__ void sort(Sh& sh, Entry& e, uint32_t n) {
+__device__ __forceinline__ void sort(Sh& sh, uint64_t& e, uint32_t n) {
   const uint32_t tid = threadIdx.x;
   uint32_t size = 2;
   while (size < n) size *= 2;
+  if (n <= 64 && tid >= 64) return;  // (no barrier then)
   for (uint32_t k = 2; k <= size; k *= 2)
     for (uint32_t j = k / 2; j > 0; j /= 2) {
-      Entry o;
+      uint64_t o;
       if (j >= 64) {
         __syncthreads();
         sh.list[tid] = e;
         __syncthreads();
         o = sh.list[tid ^ j];
       } else {
-        o.order = __shfl_xor(e.order, j);
-        o.weight = __shfl_xor(e.weight, j);
+        o = __shfl_xor(e, j);
       }
       const bool first = (tid & j) == 0, down = (tid & k) == 0;  // the larger one goes first
-      if (first == down ? o.order > e.order : o.order < e.order) e = o;
+      if (first == down ? o > e : o < e) e = o;
     }
 }
 
 // What is kept: logits whose order is the cut's or above it.
-template <class T, bool HELD>
+template <class T, bool HELD, int kThreads>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
-  constexpr int PER = T::kPer16;
-  __shared__ Shared<HELD ? kMaxHeld * kWaves : kMaxPieces> sh;
+  constexpr int PER = T::kPer16, kWaves = kThreads / 64, kList = kThreads;
+  __shared__ Shared<kThreads, HELD ? kHeldBytes / 1024 : kMaxSampleVocab / PER / 64> sh;
   extern __shared__ __attribute__((aligned(16))) char held[];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x;
-  Row<T, HELD> row;
+  Row<T, HELD, kThreads> row;
   row.x = (const typename T::Elem*)a.logits + (int64_t)r * a.stride;
   row.vocab = a.vocab;
   row.slabs = (a.vocab + kThreads * PER - 1) / (kThreads * PER);
@@ -253,6 +251,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   const double inverse = 1.4426950408889634074 / unit, wide_m = m, far = -(double)(shift + 2);
   auto power_of = [&](float x) { return ((double)x - wide_m) * inverse; };
   auto weight_at = [&](double t) -> uint64_t {
+    t = fmax(t, far);  // 0, once it is a whole number
     constexpr double kNearest = 0x1.8p46;  // adding it leaves the nearest n / 64, with n in the low bits
     const double q = t + kNearest, f = t - (q - kNearest);
     const int32_t n = (int32_t)__double_as_longlong(q);
@@ -262,8 +261,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     p = __builtin_fma(f, p, 0x1.62e42fefa39efp-1) * f;
     const double w = sh.powers[n & 63], y = __builtin_fma(w, p, w);
     const double scaled = __longlong_as_double(__double_as_longlong(y) + ((int64_t)((n >> 6) + shift) << 52));
-    const uint64_t whole = (uint64_t)__double_as_longlong(scaled + 0x1p52) & 0xfffffffffffffull;
-    return t < far ? 0 : whole;
+    return (uint64_t)__double_as_longlong(scaled + 0x1p52) & 0xfffffffffffffull;
   };
   auto weight = [&](float x) -> uint64_t { return weight_at(power_of(x)); };
   // min_p as the power that a kept weight's reaches; the largest is always kept
@@ -281,7 +279,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   };
   // Logits (above -inf) that `take` takes, one a thread and sorted; the others are 0 (of no order). How many: more than kList if they
   // do not fit, and nothing then.
-  Entry e;
+  uint64_t e;
+  auto weight_of = [&](uint64_t order) -> uint64_t { return order ? weight(of_key((uint32_t)(order >> 32))) : 0; };
   auto list = [&](auto take) -> uint32_t {
     __syncthreads();
     if (tid == 0) sh.listed = 0;
@@ -289,17 +288,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     row.each([&](float x, uint32_t token) {
       if (x != -INFINITY && take(x, token)) {
         const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kList) sh.list[at].order = order_of(key_of(x), token);
+        if (at < kList) sh.list[at] = order_of(key_of(x), token);
       }
     });
     __syncthreads();
     const uint32_t n = sh.listed;
-    e = Entry{0, 0};
+    e = 0;
     if (n <= kList) {
-      if (tid < n) {
-        e.order = sh.list[tid].order;
-        e.weight = weight(of_key((uint32_t)(e.order >> 32)));
-      }
+      if (tid < n) e = sh.list[tid];
       sort(sh, e, n);
     }
     return n;
@@ -314,8 +310,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     if (bin == kBins) return least;
     if (list([&](float x, uint32_t token) { return bin_of(x) == bin && order_of(key_of(x), token) >= least; }) <= kList) {
       uint64_t all;
-      const uint64_t v = !e.order ? 0 : counts ? 1 : e.weight, upto = block_scan(sh, v, all);
-      if (before + upto - v < target && before + upto >= target) sh.cut = e.order;
+      const uint64_t v = counts ? e != 0 : weight_of(e), upto = block_scan(sh, v, all);
+      if (before + upto - v < target && before + upto >= target) sh.cut = e;
       __syncthreads();
       return sh.cut;
     }
@@ -409,15 +405,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     if (n <= kList) {
       // All that matters is in the list, sorted: what is kept is its beginning.
       uint64_t total, sum;
-      if (tid >= (uint32_t)top_k) e = Entry{0, 0};
-      const uint64_t upto = block_scan(sh, e.weight, total);
-      if (top_p < 1.0 && upto - e.weight >= share_of(total)) e = Entry{0, 0};
-      if (!e.order || power_of(of_key((uint32_t)(e.order >> 32))) < least_power) e = Entry{0, 0};
-      const uint32_t kept = __syncthreads_count(e.order != 0);
-      e.order &= 0xffffffffu;  // by token from here on (the first one has the largest order)
+      if (tid >= (uint32_t)top_k) e = 0;
+      if (top_p < 1.0) {
+        const uint64_t w = weight_of(e), before = block_scan(sh, w, total) - w;
+        if (before >= share_of(total)) e = 0;
+      }
+      if (e && power_of(of_key((uint32_t)(e >> 32))) < least_power) e = 0;
+      const uint32_t kept = __syncthreads_count(e != 0);
+      e = e << 32 | e >> 32;  // by token from here on
       sort(sh, e, kept);
-      const uint64_t before = block_scan(sh, e.weight, sum) - e.weight, target = drawn_of(sum);
-      if (before < target && before + e.weight >= target) a.tokens[r] = token_of(e.order);
+      const uint64_t w = weight_of(e << 32 | e >> 32), before = block_scan(sh, w, sum) - w, target = drawn_of(sum);
+      if (before < target && before + w >= target) a.tokens[r] = token_of(e >> 32);
       return;
     }
     __syncthreads();
@@ -487,17 +485,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   }
 }
 
+template <class T, int THREADS>
+hipError_t launch_held(const SampleRows& a, hipStream_t st) {
+  const uint32_t slab = THREADS * 16, bytes = (a.vocab * (16 / T::kPer16) + slab - 1) / slab * slab;
+  const hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<T, true, THREADS>, hipFuncAttributeMaxDynamicSharedMemorySize, kHeldBytes);
+  if (e != hipSuccess) return e;
+  sample_kernel<T, true, THREADS><<<a.nrows, THREADS, bytes, st>>>(a);
+  return hipGetLastError();
+}
+// Short rows leave most of 1,024 threads without a vector: 2,000 rows of 1,000 fp16 logits take 16 us, not 66.
 template <class T>
 hipError_t launch_typed(const SampleRows& a, hipStream_t st) {
-  const uint32_t slabs = (a.vocab + kThreads * T::kPer16 - 1) / (kThreads * T::kPer16);
-  if (slabs > kMaxHeld) {
-    sample_kernel<T, false><<<a.nrows, kThreads, 0, st>>>(a);
-    return hipGetLastError();
-  }
-  const uint32_t bytes = slabs * kThreads * 16;
-  const hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, kMaxHeld * kThreads * 16);
-  if (e != hipSuccess) return e;
-  sample_kernel<T, true><<<a.nrows, kThreads, bytes, st>>>(a);
+  if (a.vocab <= kShortRow) return launch_held<T, 256>(a, st);
+  if (a.vocab <= (uint32_t)(kHeldBytes / 16 * T::kPer16)) return launch_held<T, 1024>(a, st);
+  sample_kernel<T, false, 1024><<<a.nrows, 1024, 0, st>>>(a);
   return hipGetLastError();
 }
 
