@@ -35,6 +35,7 @@ struct Op;
 template <>
 struct Op<TypeF16> {
   using Frag = f16x8;
+  __device__ static Frag widen8(u32x2 c, float scale) { return __builtin_bit_cast(Frag, widen(c, scale)); }
   __device__ static f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   __device__ static u32x4 widen(u32x2 c, float scale) {
     return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[0], scale, false)),
@@ -46,6 +47,7 @@ struct Op<TypeF16> {
 template <>
 struct Op<TypeBF16> {
   using Frag = bf16x8;
+  __device__ static Frag widen8(u32x2 c, float scale) { return __builtin_bit_cast(Frag, widen(c, scale)); }
   __device__ static f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   __device__ static u32x4 widen(u32x2 c, float scale) {
     return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, false)),
@@ -57,6 +59,9 @@ struct Op<TypeBF16> {
 template <>
 struct Op<TypeF32> {
   using Frag = f32x8;
+  __device__ static Frag widen8(u32x2 c, float scale) {
+    return __builtin_shufflevector(__builtin_bit_cast(f32x4, widen(c[0], scale)), __builtin_bit_cast(f32x4, widen(c[1], scale)), 0, 1, 2, 3, 4, 5, 6, 7);
+  }
   __device__ static f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
@@ -76,7 +81,8 @@ __device__ __forceinline__ float both_halves(float x, F f) {
 }
 
 // Where a 16-byte chunk c of row r lies in a tile of CH chunks a row: chunk c ^ swizzle(r). Sixteen consecutive rows
-// at one chunk (a read of keys), and four rows at four chunks (a read of values), then lie in different banks.
+// at one chunk (a read of keys), and the rows and chunks of 32 lanes' read of values, then lie in different banks, or in few of
+// the same.
 template <int CH>
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   if (CH == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
@@ -85,59 +91,106 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   if (CH == 24) return r >> 1 & 7;
   return (r & 3) << 2 | (r >> 2 & 3);
 }
+// The same of rows of CH chunks of 16 codes.
+template <int CH>
+__device__ __forceinline__ uint32_t swizzle_codes(uint32_t r) {
+  if (CH == 4) return r >> 2 & 3;
+  if (CH == 5) return 0;
+  if (CH == 6) return r >> 3 & 1;
+  return (r >> 1 & 1) << 1 | (r >> 3 & 1) << 2 | (r >> 2 & 1);
+}
 
-// QS: sixteenths of the width, rounded up to 4, 5, 6 or 8.
-template <class T, int QS, bool BY_KEYS>
-struct Shape {
-  static constexpr int kWide = std::is_same_v<T, TypeF32> ? 2 : 1;  // chunks of 8 elements
-  static constexpr int CH = 2 * QS * kWide;                           // chunks of 16 bytes a row
-  static constexpr int WAVES = BY_KEYS && kWide == 2 ? 2 : 4;
-  static constexpr int KT = BY_KEYS || kWide == 2 ? 32 : 64;  // keys of a tile
-  static constexpr int ROWS = BY_KEYS ? 32 : 32 * WAVES;      // most rows of a workgroup
-  static constexpr int TILE = KT * CH * 16;                    // bytes of a tile's keys, or of its values
-  static constexpr int LOADERS = BY_KEYS ? 1 : WAVES;            // waves that load a tile
-  static constexpr int SLABS = BY_KEYS ? WAVES : 1;
-  static constexpr int PV = (QS + 1) / 2;  // products of 32 columns of values
+// The rows of a tile: whole sequences, or rows of one.
+struct TileRows {
+  uint32_t row0, rows;
+};
+__device__ __forceinline__ TileRows tile_rows_of(const AttendPlan& plan, uint32_t tile, uint32_t seq_rows, uint32_t all_rows) {
+  const uint32_t most = plan.tile_rows;
+  if (most >= seq_rows) {
+    const uint32_t row0 = tile * most;
+    return {row0, all_rows - row0 < most ? all_rows - row0 : most};
+  }
+  const uint32_t per_seq = (seq_rows + most - 1) / most, r = tile % per_seq * most;
+  return {tile / per_seq * seq_rows + r, seq_rows - r < most ? seq_rows - r : most};
+}
+
+// What a tile in LDS is.
+enum Store {
+  kOperands,   // elements, loaded straight to LDS
+  kConverted,  // elements that were codes: loaded to registers and converted once for all waves
+  kCodes,      // codes, loaded straight to LDS and converted by the wave that takes keys for itself; widths of whole chunks
 };
 
-template <class T, int QS, bool BY_KEYS, bool BYTES, int THREADS = 64 * Shape<T, QS, BY_KEYS>::WAVES>
-__global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend a, AttendPlan plan, float* partial, float2* partial_ms) {
-  using S = Shape<T, QS, BY_KEYS>;
+// QS: sixteenths of the width, rounded up to 4, 5, 6 or 8.
+template <class T, int QS, bool BY_KEYS, Store STORE>
+struct Shape {
+  static constexpr bool kWide = std::is_same_v<T, TypeF32>;
+  static constexpr int CH = STORE == kCodes ? QS : kWide ? 4 * QS : 2 * QS;  // chunks of 16 bytes a row
+  static constexpr int STEPS = STORE == kCodes ? (QS + 1) / 2 * 2 : QS;        // products along the width
+  static constexpr int WAVES = BY_KEYS && kWide && STORE != kCodes ? 2 : 4;
+  static constexpr int KT = BY_KEYS || kWide ? 32 : 64;    // keys of a tile
+  static constexpr int ROWS = BY_KEYS ? 32 : 32 * WAVES;  // most rows of a workgroup
+  static constexpr int TILE = KT * CH * 16;                // bytes of a tile's keys, or of its values
+  static constexpr int LOADERS = BY_KEYS ? 1 : WAVES;        // waves that load a tile
+  static constexpr int SLABS = BY_KEYS ? WAVES : 1;
+  static constexpr int PV = (QS + 1) / 2;  // products of 32 columns of values
+  // workgroups that a compute unit's LDS holds
+  static constexpr int RESIDENT = SLABS * 4 * TILE > 72 * 1024 ? 1 : 2;
+};
+
+template <class T, int QS, bool BY_KEYS, Store STORE, int THREADS = 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES,
+          int RESIDENT = Shape<T, QS, BY_KEYS, STORE>::RESIDENT>
+__global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void attend_kernel(Attend a, AttendPlan plan, float* partial, float2* partial_ms) {
+  using S = Shape<T, QS, BY_KEYS, STORE>;
   using Elem = typename T::Elem;
   using Frag = typename Op<T>::Frag;
+  // Weights of codes carry their row's power of two, which may leave the range of fp16: those are bf16 (and codes are bf16 numbers).
+  using TV = std::conditional_t<STORE == kCodes && std::is_same_v<T, TypeF16>, TypeBF16, T>;
+  using FragV = typename Op<TV>::Frag;
   constexpr int CH = S::CH, KT = S::KT, NK = KT / 32;
+  constexpr bool BYTES = STORE != kOperands;
   __shared__ __attribute__((aligned(256))) char lds[S::SLABS][2][2][S::TILE];
   __shared__ uint32_t ends[S::ROWS + 1];  // key tiles up to the end of a sequence's (first: of the prompt's)
+  __shared__ uint32_t lims[S::ROWS];      // keys that are looked at of each sequence
   __shared__ float2 stats[BY_KEYS ? S::WAVES : 1][32];
-  __shared__ uint32_t lims[S::ROWS];  // keys that are looked at of each sequence
+  __shared__ __attribute__((aligned(16))) float powers[STORE == kCodes ? S::WAVES : 1][32];  // of a tile's values
 
   // Workgroups go to the 8 XCDs in turn: each XCD takes consecutive items, whose keys its L2 holds for them.
-  const uint32_t items = (uint32_t)a.groups * a.kv_heads * plan.tiles * plan.splits, per = gridDim.x / 8;
-  const uint32_t item = blockIdx.x % 8 * per + blockIdx.x / 8;
-  if (item >= items) return;
-  const uint32_t split = item % plan.splits, gh = item / plan.splits / plan.tiles;
-  const uint32_t tile = plan.tiles - 1 - item / plan.splits % plan.tiles;  // the longest first
+  const uint32_t xcd = blockIdx.x % 8, order = blockIdx.x / 8, after = order - plan.whole;
+  const bool parted = order >= (uint32_t)plan.whole;
+  const uint32_t at = parted ? plan.whole + after / plan.splits : order, item = xcd * plan.per + at;
+  if (at >= (uint32_t)plan.per || item >= (uint32_t)plan.items) return;
+  const uint32_t split = parted ? after % plan.splits : 0, splits = parted ? plan.splits : 1;
+  const uint32_t gh = item / plan.tiles, tile = plan.tiles - 1 - item % plan.tiles;  // the longest first
   const uint32_t g = gh / a.kv_heads, hk = gh % a.kv_heads;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const uint32_t shared = a.heads / a.kv_heads, seq_rows = (uint32_t)a.length * shared, all_rows = seq_rows * a.sequences;
 
   // The tile's rows, the sequences they belong to, and how far each looks.
   // (A tile covers whole sequences, or lies inside of one: plan.tile_rows is a multiple of a sequence's rows or tiles restart at each.)
-  uint32_t row0, rows;
-  if ((uint32_t)plan.tile_rows >= seq_rows) {
-    row0 = tile * plan.tile_rows;
-    rows = all_rows - row0 < (uint32_t)plan.tile_rows ? all_rows - row0 : plan.tile_rows;
-  } else {
-    const uint32_t per_seq = (seq_rows + plan.tile_rows - 1) / plan.tile_rows, n = tile / per_seq, r = tile % per_seq * plan.tile_rows;
-    row0 = n * seq_rows + r;
-    rows = seq_rows - r < (uint32_t)plan.tile_rows ? seq_rows - r : plan.tile_rows;
-  }
+  const TileRows tr = tile_rows_of(plan, tile, seq_rows, all_rows);
+  const uint32_t row0 = tr.row0, rows = tr.rows;
   const uint32_t n0 = row0 / seq_rows, nseq = (row0 + rows - 1) / seq_rows - n0 + 1;
+  // This lane's query.
+  const uint32_t lane_row = (BY_KEYS ? 0 : wave * 32) + (lane & 31);
+  const bool live = lane_row < rows;
+  const uint32_t row = row0 + (live ? lane_row : 0), n_row = row / seq_rows, t_row = row % seq_rows / shared, h_row = hk * shared + row % shared;
+  const int64_t q_at = (int64_t)g * a.q_s[0] + (int64_t)n_row * a.q_s[1] + (int64_t)h_row * a.q_s[2] + (int64_t)t_row * a.q_s[3];
+  Frag qf[S::STEPS];
+#pragma unroll
+  for (int s = 0; s < S::STEPS; ++s) {
+    // codes are read 16 at a time, for two steps
+    const uint32_t col = STORE == kCodes ? 16 * (2 * (s / 2) + half) + 8 * (s % 2) : 16 * s + 8 * half;
+    qf[s] = Frag(Elem(0.f));
+    if (live && col < (uint32_t)a.width) qf[s] = *(const Frag*)((const Elem*)a.q + q_at + col);
+  }
+
   auto limit_of = [&](uint32_t n, uint32_t t) {  // own keys that token t of sequence n sees
     const int64_t p = a.positions ? a.positions[(uint64_t)g * a.sequences + n] : a.slots - a.length;
     const int64_t l = p + t + 1;
     return (uint32_t)(l < 0 ? 0 : l > a.slots ? a.slots : l);
   };
+  const uint32_t own_limit = live ? limit_of(n_row, t_row) : 0;
   uint32_t prefix_limit = 0;
   if (a.prefix_slots) {
     const int32_t l = a.prefix_lengths ? a.prefix_lengths[g] : a.prefix_slots;
@@ -149,30 +202,16 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
     lims[tid] = limit_of(n, last);
   }
   __syncthreads();
-  if (tid == 0) {
+  if (tid <= nseq) {
     uint32_t e = (prefix_limit + KT - 1) / KT;
-    ends[0] = e;
-    for (uint32_t i = 0; i < nseq; ++i) ends[i + 1] = e += (lims[i] + KT - 1) / KT;
+    for (uint32_t i = 0; i < tid; ++i) e += (lims[i] + KT - 1) / KT;
+    ends[tid] = e;
   }
   __syncthreads();
   const uint32_t key_tiles = __builtin_amdgcn_readfirstlane(ends[nseq]);
 
-  // This lane's query.
-  const uint32_t lane_row = (BY_KEYS ? 0 : wave * 32) + (lane & 31);
-  const bool live = lane_row < rows;
-  const uint32_t row = row0 + (live ? lane_row : 0), n_row = row / seq_rows, t_row = row % seq_rows / shared, h_row = hk * shared + row % shared;
-  const uint32_t own_limit = live ? limit_of(n_row, t_row) : 0;
-  const int64_t q_at = (int64_t)g * a.q_s[0] + (int64_t)n_row * a.q_s[1] + (int64_t)h_row * a.q_s[2] + (int64_t)t_row * a.q_s[3];
-  Frag qf[QS];
-#pragma unroll
-  for (int s = 0; s < QS; ++s) {
-    const uint32_t col = 16 * s + 8 * half;
-    qf[s] = Frag(Elem(0.f));
-    if (live && col < (uint32_t)a.width) qf[s] = *(const Frag*)((const Elem*)a.q + q_at + col);
-  }
-
   // Tiles of keys, in turn: `step` apart.
-  const uint32_t first = BY_KEYS ? split * S::WAVES + wave : split, step = BY_KEYS ? plan.splits * S::WAVES : plan.splits;
+  const uint32_t first = BY_KEYS ? split * S::WAVES + wave : split, step = BY_KEYS ? splits * S::WAVES : splits;
   struct Part {
     uint32_t k0, limit, n;  // the tile's first key, its part's end, and the sequence (2^32 - 1: the prompt)
   };
@@ -186,9 +225,9 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
   char(*slab)[2][S::TILE] = lds[BY_KEYS ? wave : 0];
   const uint32_t loader = BY_KEYS ? 0 : wave;
   // A tile's loads, keys before values, 64 chunks each.
-  constexpr int OF_KEYS = KT * CH / 64, LOADS = 2 * OF_KEYS / S::LOADERS;
-  static_assert(KT * CH % 64 == 0 && 2 * OF_KEYS % S::LOADERS == 0, "loads");
-  struct Store {  // of keys or of values, from the tile's first one on
+  constexpr int OF_KEYS = KT * CH, LOADS = 2 * OF_KEYS / 64 / S::LOADERS;  // OF_KEYS: chunks
+  static_assert(2 * OF_KEYS % (64 * S::LOADERS) == 0 && (STORE == kCodes || OF_KEYS % 64 == 0), "loads");
+  struct Store_ {  // of keys or of values, from the tile's first one on
     const char* at;
     int64_t stride;  // bytes
     const uint8_t* scale;
@@ -199,7 +238,7 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
     const KeyValues& kv = p.n == ~0u ? a.prefix : a.own;
     const int64_t n = p.n == ~0u ? 0 : p.n;
     const int64_t(&s)[4] = values ? kv.v_s : kv.k_s;
-    Store x;
+    Store_ x;
     x.at = (const char*)(values ? kv.v : kv.k) + SIZE * ((int64_t)g * s[0] + n * s[1] + (int64_t)hk * s[2] + (int64_t)p.k0 * s[3]);
     x.stride = SIZE * s[3];
     if (BYTES) {
@@ -212,36 +251,55 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
   // Row and chunk of a lane's i-th load. Keys past the part's end are the last one again: their weights are 0, and what these
   // multiply is finite where the last key's values are. Chunks past the width are the row's first: finite where the row is,
   // and multiplied by 0 (keys) or not stored (values).
-  constexpr int PER_CHUNK = 16 / sizeof(Elem);
+  constexpr int PER_CHUNK = STORE == kCodes ? 16 : 16 / sizeof(Elem);
   auto place = [&](int i, uint32_t last, uint32_t& r, uint32_t& c) {
-    const uint32_t slot = (i * S::LOADERS + loader) % OF_KEYS * 64 + lane, row = slot / CH;
-    c = (slot % CH) ^ swizzle<CH>(row);
+    const uint32_t slot = ((i * S::LOADERS + loader) * 64 + lane) % OF_KEYS, row = slot / CH;
+    c = (slot % CH) ^ (STORE == kCodes ? swizzle_codes<CH>(row) : swizzle<CH>(row));
     if (c * PER_CHUNK >= (uint32_t)a.width) c = 0;
     r = row < last ? row : last;
   };
   auto load_direct = [&](const Part& p, int stage) {
-    const Store ks = store_of(p, false), vs = store_of(p, true);
+    const Store_ ks = store_of(p, false), vs = store_of(p, true);
     const uint32_t to0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&slab[stage][0][0]);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const uint32_t j = i * S::LOADERS + loader;
-      const bool values = j >= OF_KEYS;
       uint32_t r, c;
       place(i, p.limit - 1 - p.k0, r, c);
-      to_lds<false>(values ? vs.at : ks.at, r * (uint32_t)(values ? vs.stride : ks.stride) + c * 16, to0 + j * 1024);
+      if (OF_KEYS % 64 == 0) {
+        const bool values = j * 64 >= OF_KEYS;
+        to_lds<false>(values ? vs.at : ks.at, r * (uint32_t)(values ? vs.stride : ks.stride) + c * 16, to0 + j * 1024);
+      } else {  // (a load of both)
+        const bool values = j * 64 + lane >= OF_KEYS;
+        to_lds((values ? vs.at : ks.at) + (int64_t)r * (values ? vs.stride : ks.stride) + c * 16, to0 + j * 1024);
+      }
     }
   };
+  // Powers of two of a tile's codes, key lane % 32.
+  struct Powers {
+    uint8_t k, v;
+  };
+  auto load_powers = [&](const Part& p) {
+    Powers x{};
+    if constexpr (STORE == kCodes) {
+      const Store_ ks = store_of(p, false), vs = store_of(p, true);
+      const uint32_t last = p.limit - 1 - p.k0, r = (lane & 31) < last ? (lane & 31) : last;
+      x.k = ks.scale[r * ks.scale_stride];
+      x.v = vs.scale[r * vs.scale_stride];
+    }
+    return x;
+  };
   // 8-bit codes go through registers, where each becomes an element times its row's power of two (exactly).
-  using Code = std::conditional_t<PER_CHUNK == 8, u32x2, uint32_t>;
+  using Code = std::conditional_t<sizeof(Elem) == 2, u32x2, uint32_t>;
   struct Staged {
-    Code code[LOADS];
-    uint8_t scale[LOADS];
+    Code code[STORE == kConverted ? LOADS : 1];
+    uint32_t scale[STORE == kConverted ? LOADS : 1];
   };
   auto load_codes = [&](const Part& p, Staged& s) {
-    const Store ks = store_of(p, false), vs = store_of(p, true);
+    const Store_ ks = store_of(p, false), vs = store_of(p, true);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const Store& x = i * S::LOADERS + loader >= OF_KEYS ? vs : ks;
+      const Store_& x = (i * S::LOADERS + loader) * 64 >= OF_KEYS ? vs : ks;
       uint32_t r, c;
       place(i, p.limit - 1 - p.k0, r, c);
       s.code[i] = *(const Code*)(x.at + r * x.stride + c * PER_CHUNK);
@@ -251,7 +309,7 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
   auto put_codes = [&](const Staged& s, int stage) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
-      *(u32x4*)(&slab[stage][0][0] + ((i * S::LOADERS + loader) * 64 + lane) * 16) = Op<T>::widen(s.code[i], __uint_as_float((uint32_t)s.scale[i] << 23));
+      *(u32x4*)(&slab[stage][0][0] + ((i * S::LOADERS + loader) * 64 + lane) * 16) = Op<T>::widen(s.code[i], __uint_as_float(s.scale[i] << 23));
   };
 
   f32x16 o[S::PV];
@@ -260,27 +318,42 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
   float m = -INFINITY, l = 0.f;  // l: of this lane's keys
   const float c = a.scale * kLog2e;
 
-  auto products = [&](const Part& p, int stage) {
+  auto products = [&](const Part& p, int stage, const Powers& pow) {
     const uint32_t limit = p.n == ~0u ? prefix_limit : p.n == n_row ? own_limit : 0;
     if (__all(limit <= p.k0)) return;  // none of the wave's rows
     const char* kt = slab[stage][0];
     const char* vt = slab[stage][1];
     f32x16 s[NK];
+    if constexpr (STORE == kCodes) {
+      if (half == 0) powers[wave][lane] = __uint_as_float((uint32_t)pow.v << 23);
+      const float power = __uint_as_float((uint32_t)pow.k << 23);
+      const uint32_t r = lane & 31;
+      s[0] = f32x16(0.f);
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      s[i] = f32x16(0.f);
-      const uint32_t r = i * 32 + (lane & 31);
+      for (int q = 0; q < S::STEPS / 2; ++q) {
+        uint32_t c = 2 * q + half;
+        if (CH % 2) c = c < CH ? c : CH - 1;  // (multiplied by 0)
+        const u32x4 codes = *(const u32x4*)(kt + r * CH * 16 + (c ^ swizzle_codes<CH>(r)) * 16);
+        s[0] = Op<T>::mma(Op<T>::widen8(u32x2{codes[0], codes[1]}, power), qf[2 * q], s[0]);
+        s[0] = Op<T>::mma(Op<T>::widen8(u32x2{codes[2], codes[3]}, power), qf[2 * q + 1], s[0]);
+      }
+    } else {
 #pragma unroll
-      for (int q = 0; q < QS; ++q) {
-        Frag kf;
-        if constexpr (S::kWide == 1) {
-          kf = *(const Frag*)(kt + r * CH * 16 + ((2 * q + half) ^ swizzle<CH>(r)) * 16);
-        } else {
-          const f32x4 lo = *(const f32x4*)(kt + r * CH * 16 + ((4 * q + 2 * half) ^ swizzle<CH>(r)) * 16);
-          const f32x4 hi = *(const f32x4*)(kt + r * CH * 16 + ((4 * q + 2 * half + 1) ^ swizzle<CH>(r)) * 16);
-          kf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int i = 0; i < NK; ++i) {
+        s[i] = f32x16(0.f);
+        const uint32_t r = i * 32 + (lane & 31);
+#pragma unroll
+        for (int q = 0; q < S::STEPS; ++q) {
+          Frag kf;
+          if constexpr (!S::kWide) {
+            kf = *(const Frag*)(kt + r * CH * 16 + ((2 * q + half) ^ swizzle<CH>(r)) * 16);
+          } else {
+            const f32x4 lo = *(const f32x4*)(kt + r * CH * 16 + ((4 * q + 2 * half) ^ swizzle<CH>(r)) * 16);
+            const f32x4 hi = *(const f32x4*)(kt + r * CH * 16 + ((4 * q + 2 * half + 1) ^ swizzle<CH>(r)) * 16);
+            kf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+          s[i] = Op<T>::mma(kf, qf[q], s[i]);
         }
-        s[i] = Op<T>::mma(kf, qf[q], s[i]);
       }
     }
     if (!__all(limit >= p.k0 + KT)) {
@@ -296,7 +369,8 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
     top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * c;
-    if (__any(top > m)) {
+    // Weights may exceed 1 by 2^8 before their maximum is taken up: sums change their scale a few times, and not with each tile.
+    if (__any(top > m + 8.f)) {
       const float m2 = fmaxf(m, top);
       const float f = m2 == -INFINITY ? 1.f : exp2_hw(m - m2);
       m = m2;
@@ -305,14 +379,20 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
       for (int d = 0; d < S::PV; ++d) o[d] *= f;
     }
     const float mm = m == -INFINITY ? 0.f : m;
-    Frag w[NK][2];
+    FragV w[NK][2];
 #pragma unroll
     for (int i = 0; i < NK; ++i)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float e = exp2_hw(__builtin_fmaf(s[i][j], c, -mm));
-        l += e;
-        w[i][j / 8][j % 8] = (Elem)e;
+      for (int b = 0; b < 4; ++b) {
+        f32x4 power;
+        if (STORE == kCodes) power = *(const f32x4*)&powers[wave][8 * b + 4 * half];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float e = exp2_hw(__builtin_fmaf(s[i][4 * b + r], c, -mm));
+          l += e;
+          if (STORE == kCodes) e *= power[r];
+          w[i][b / 2][b % 2 * 4 + r] = (typename TV::Elem)e;
+        }
       }
 #pragma unroll
     for (int d = 0; d < S::PV; ++d)
@@ -320,8 +400,16 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          Frag vf;
-          if constexpr (S::kWide == 1) {
+          FragV vf;
+          if constexpr (STORE == kCodes) {
+            // eight rows of 16 codes for each 16 lanes, which get a column each
+            const uint32_t of = 2 * d + (lane & 31) / 16, chunk = of < CH ? of : CH - 1, j = (lane & 15) / 2;
+            const uint32_t r = k * 16 + j / 4 * 8 + 4 * half + j % 4;
+            typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+            const i32x2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) i32x2*)(vt + r * CH * 16 + (chunk ^ swizzle_codes<CH>(r)) * 16 + (lane & 1) * 8));
+            vf = Op<TV>::widen8(__builtin_bit_cast(u32x2, codes), 1.f);
+          } else if constexpr (!S::kWide) {
             // four rows of 16 columns for each 16 lanes, which get a column each
             const uint32_t col = 32 * d + (lane & 31) / 16 * 16, group = col / 8 < CH ? col / 8 : CH - 2, chunk = group + (lane & 3) / 2;
             s16x4 part[2];
@@ -330,7 +418,7 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
               const uint32_t r = i * 32 + k * 16 + j * 8 + 4 * half + (lane & 15) / 4;
               part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + r * CH * 16 + (chunk ^ swizzle<CH>(r)) * 16 + (lane & 1) * 8));
             }
-            vf = __builtin_bit_cast(Frag, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            vf = __builtin_bit_cast(FragV, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
           } else {
             const uint32_t col = 32 * d + (lane & 31), chunk = col / 4 < CH ? col / 4 : CH - 1;
 #pragma unroll
@@ -339,7 +427,7 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
               vf[j] = *(const float*)(vt + r * CH * 16 + (chunk ^ swizzle<CH>(r)) * 16 + (lane & 3) * 4);
             }
           }
-          o[d] = Op<T>::mma(vf, w[i][k], o[d]);
+          o[d] = Op<TV>::mma(vf, w[i][k], o[d]);
         }
   };
 
@@ -353,7 +441,8 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
   if (first < key_tiles) {
     Part now = part_of(first);
     Staged st;
-    if constexpr (BYTES) {
+    Powers pow = load_powers(now);
+    if constexpr (STORE == kConverted) {
       load_codes(now, st);
       put_codes(st, 0);
     } else {
@@ -363,17 +452,20 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
     for (uint32_t i = first; i < key_tiles; i += step) {
       const bool more = i + step < key_tiles;
       Part next = now;
+      Powers next_pow = pow;
       if (more) next = part_of(i + step);
       arrive_all();
       if (more) {
-        if constexpr (BYTES) load_codes(next, st);
+        next_pow = load_powers(next);
+        if constexpr (STORE == kConverted) load_codes(next, st);
         else load_direct(next, stage ^ 1);
       }
-      products(now, stage);
-      if constexpr (BYTES)
+      products(now, stage, pow);
+      if constexpr (STORE == kConverted)
         if (more) put_codes(st, stage ^ 1);
       stage ^= 1;
       now = next;
+      pow = next_pow;
     }
   }
   l = both_halves(l, [](float x, float y) { return x + y; });
@@ -393,14 +485,16 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
     m = top;
     l = sum;
     constexpr int PITCH = S::PV * 32 + 4;  // floats of a row
-    float* mine = (float*)lds + wave * 32 * PITCH;
-    static_assert(S::WAVES * 32 * PITCH * 4 <= (int)sizeof(lds), "room");
+    static_assert((S::WAVES - 1) * 32 * PITCH * 4 <= (int)sizeof(lds), "room");
+    float* mine = (float*)lds + (wave - 1) * 32 * PITCH;
 #pragma unroll
-    for (int d = 0; d < S::PV; ++d)
+    for (int d = 0; d < S::PV; ++d) o[d] *= f;
+    if (wave > 0)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        *(f32x4*)(mine + (lane & 31) * PITCH + 32 * d + 8 * b + 4 * half) =
-            f32x4{o[d][4 * b] * f, o[d][4 * b + 1] * f, o[d][4 * b + 2] * f, o[d][4 * b + 3] * f};
+      for (int d = 0; d < S::PV; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *(f32x4*)(mine + (lane & 31) * PITCH + 32 * d + 8 * b + 4 * half) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
     __syncthreads();
     if (wave != 0) return;  // (the sums that are left take one wave)
 #pragma unroll
@@ -408,15 +502,17 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         f32x4 x = f32x4(0.f);
-        for (int i = 0; i < S::WAVES; ++i) x += *(const f32x4*)((float*)lds + (i * 32 + (lane & 31)) * PITCH + 32 * d + 8 * b + 4 * half);
-        for (int r = 0; r < 4; ++r) o[d][4 * b + r] = x[r];
+#pragma unroll
+        for (int i = 0; i < S::WAVES - 1; ++i) x += *(const f32x4*)((float*)lds + (i * 32 + (lane & 31)) * PITCH + 32 * d + 8 * b + 4 * half);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[d][4 * b + r] += x[r];
       }
   }
   if (!live) return;
-  if (plan.splits > 1) {
-    const uint64_t at = ((uint64_t)gh * all_rows + row) * plan.splits + split;
-    if (half == 0) partial_ms[at] = float2{m, l};
-    float* to = partial + at * a.width;
+  if (splits > 1) {
+    const uint64_t to_row = (((uint64_t)xcd * plan.tail + at - plan.whole) * splits + split) * plan.tile_rows + lane_row;
+    if (half == 0) partial_ms[to_row] = float2{m, l};
+    float* to = partial + to_row * a.width;
 #pragma unroll
     for (int d = 0; d < S::PV; ++d)
 #pragma unroll
@@ -439,57 +535,65 @@ __global__ __launch_bounds__(THREADS, BY_KEYS ? 1 : 2) void attend_kernel(Attend
     }
 }
 
-// The splits' sums of each row, joined. 32 lanes a row, four columns a lane.
+// The splits' sums of each row of a tile, joined. 32 lanes a row, four columns a lane.
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(Attend a, AttendPlan plan, const float* partial, const float2* partial_ms) {
   using Elem = typename T::Elem;
   const uint32_t shared = a.heads / a.kv_heads, seq_rows = (uint32_t)a.length * shared, all_rows = seq_rows * a.sequences;
-  const uint64_t at = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32, total = (uint64_t)a.groups * a.kv_heads * all_rows;
-  const uint32_t col = threadIdx.x % 32 * 4;
-  if (at >= total || col >= (uint32_t)a.width) return;
+  const uint32_t each = (plan.tile_rows + 7) / 8, index = blockIdx.x / each, lane_row = blockIdx.x % each * 8 + threadIdx.x / 32;
+  const uint32_t item = index / plan.tail * plan.per + plan.whole + index % plan.tail, col = threadIdx.x % 32 * 4;
+  if (item >= (uint32_t)plan.items) return;
+  const TileRows t = tile_rows_of(plan, plan.tiles - 1 - item % plan.tiles, seq_rows, all_rows);
+  if (lane_row >= t.rows || col >= (uint32_t)a.width) return;
+  const uint64_t from = (uint64_t)index * plan.splits * plan.tile_rows + lane_row;
   float m = -INFINITY;
-  for (int i = 0; i < plan.splits; ++i) m = fmaxf(m, partial_ms[at * plan.splits + i].x);
+  for (int i = 0; i < plan.splits; ++i) m = fmaxf(m, partial_ms[from + (uint64_t)i * plan.tile_rows].x);
   float l = 0.f;
   f32x4 o = f32x4(0.f);
+#pragma unroll 4
   for (int i = 0; i < plan.splits; ++i) {
-    const float2 ms = partial_ms[at * plan.splits + i];
-    if (ms.x == -INFINITY) continue;  // saw no key
-    const float f = exp2_hw(ms.x - m);
+    const uint64_t at = from + (uint64_t)i * plan.tile_rows;
+    const float2 ms = partial_ms[at];
+    const f32x4 x = *(const f32x4*)(partial + at * a.width + col);
+    const float f = ms.x == -INFINITY ? 0.f : exp2_hw(ms.x - m);  // (saw no key)
     l = __builtin_fmaf(ms.y, f, l);
-    o += *(const f32x4*)(partial + (at * plan.splits + i) * a.width + col) * f;
+    o += x * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const uint32_t gh = (uint32_t)(at / all_rows), row = (uint32_t)(at % all_rows), g = gh / a.kv_heads, h = gh % a.kv_heads * shared + row % shared;
+  const uint32_t gh = item / plan.tiles, row = t.row0 + lane_row, g = gh / a.kv_heads, h = gh % a.kv_heads * shared + row % shared;
   typedef Elem Quad __attribute__((ext_vector_type(4)));
   *(Quad*)((Elem*)a.out + (int64_t)g * a.out_s[0] + (int64_t)(row / seq_rows) * a.out_s[1] + (int64_t)h * a.out_s[2] +
            (int64_t)(row % seq_rows / shared) * a.out_s[3] + col) = Quad{(Elem)(o[0] * inv), (Elem)(o[1] * inv), (Elem)(o[2] * inv), (Elem)(o[3] * inv)};
 }
 
-template <class T, int QS, bool BY_KEYS>
-void launch_one(const Attend& a, const AttendPlan& p, uint32_t grid, float* partial, float2* ms, hipStream_t st) {
-  if (a.bytes) attend_kernel<T, QS, BY_KEYS, true><<<grid, 64 * Shape<T, QS, BY_KEYS>::WAVES, 0, st>>>(a, p, partial, ms);
-  else attend_kernel<T, QS, BY_KEYS, false><<<grid, 64 * Shape<T, QS, BY_KEYS>::WAVES, 0, st>>>(a, p, partial, ms);
+template <class T, int QS, bool BY_KEYS, Store STORE>
+void launch_one(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {
+  attend_kernel<T, QS, BY_KEYS, STORE><<<8 * (p.whole + p.tail * p.splits), 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES, 0, st>>>(a, p, partial, ms);
 }
 template <class T, int QS>
-void launch_qs(const Attend& a, const AttendPlan& p, uint32_t grid, float* partial, float2* ms, hipStream_t st) {
-  if (p.by_keys) launch_one<T, QS, true>(a, p, grid, partial, ms, st);
-  else launch_one<T, QS, false>(a, p, grid, partial, ms, st);
+void launch_qs(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {
+  if (p.by_keys) {
+    if (!a.bytes) launch_one<T, QS, true, kOperands>(a, p, partial, ms, st);
+    else if (a.whole_chunks) launch_one<T, QS, true, kCodes>(a, p, partial, ms, st);
+    else launch_one<T, QS, true, kConverted>(a, p, partial, ms, st);
+  } else {
+    if (!a.bytes) launch_one<T, QS, false, kOperands>(a, p, partial, ms, st);
+    else launch_one<T, QS, false, kConverted>(a, p, partial, ms, st);
+  }
 }
 template <class T>
 hipError_t launch_typed(const Attend& a, const AttendPlan& p, void* workspace, hipStream_t st) {
-  const uint64_t rows = (uint64_t)a.groups * a.heads * a.sequences * a.length;
+  const uint64_t rows = 8ull * p.tail * p.splits * p.tile_rows;
   float2* ms = (float2*)workspace;
-  float* partial = (float*)((char*)workspace + (rows * p.splits * 8 + 15) / 16 * 16);
-  const uint64_t items = (uint64_t)a.groups * a.kv_heads * p.tiles * p.splits;
-  const uint32_t grid = (uint32_t)((items + 7) / 8 * 8);
+  float* partial = (float*)((char*)workspace + (rows * 8 + 15) / 16 * 16);
   const int qs = (a.width + 15) / 16;
-  if (qs <= 4) launch_qs<T, 4>(a, p, grid, partial, ms, st);
-  else if (qs == 5) launch_qs<T, 5>(a, p, grid, partial, ms, st);
-  else if (qs == 6) launch_qs<T, 6>(a, p, grid, partial, ms, st);
-  else launch_qs<T, 8>(a, p, grid, partial, ms, st);
+  if (qs <= 4) launch_qs<T, 4>(a, p, partial, ms, st);
+  else if (qs == 5) launch_qs<T, 5>(a, p, partial, ms, st);
+  else if (qs == 6) launch_qs<T, 6>(a, p, partial, ms, st);
+  else launch_qs<T, 8>(a, p, partial, ms, st);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  join_kernel<T><<<(uint32_t)((rows + 7) / 8), 256, 0, st>>>(a, p, partial, ms);
+  if (e != hipSuccess || p.tail == 0) return e;
+  join_kernel<T><<<8 * p.tail * ((p.tile_rows + 7) / 8), 256, 0, st>>>(a, p, partial, ms);
   return hipGetLastError();
 }
 
@@ -508,18 +612,29 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
     p.tile_rows = (int32_t)most;
     p.tiles = (int32_t)((seq_rows + most - 1) / most * a.sequences);
   }
-  // keys that a tile looks at, at most; a split takes 512 of them or more
+  const int64_t items = heads * p.tiles;
+  if (items > (int64_t)1 << 23) {  // (refused)
+    p.items = INT32_MAX;
+    return p;
+  }
+  p.items = (int32_t)items;
+  p.per = (p.items + 7) / 8;
+  // An XCD's 32 compute units run `slots` workgroups at a time. Items beyond a multiple of that would leave most of them idle for as long as
+  // one takes: as many parts of them as fill the slots once. A part has 256 keys or more.
+  const int slots = 32 * (p.by_keys && !a.bytes && a.width * (dtype == 0 ? 1 : 2) > 128 ? 1 : 2);
   const int64_t seqs = p.tile_rows > seq_rows ? p.tile_rows / seq_rows : 1, keys = a.prefix_slots + seqs * a.slots;
-  const int64_t want = (2 * 256 + heads * p.tiles - 1) / (heads * p.tiles), cap = keys / 512;
-  p.splits = (int32_t)(want < cap ? want : cap);
-  if (p.splits < 1) p.splits = 1;
+  const int rest = p.per % slots;
+  const int64_t fit = rest ? slots / rest : 1, cap = keys / 256;
+  p.splits = (int32_t)(fit < cap ? fit : cap);
+  if (p.splits < 2) p.splits = 1;
+  p.tail = p.splits > 1 ? rest : 0;
+  p.whole = p.per - p.tail;
   return p;
 }
 
 int64_t attend_workspace(const Attend& a, const AttendPlan& p) {
-  if (p.splits == 1) return 0;
-  const int64_t rows = (int64_t)a.groups * a.heads * a.sequences * a.length;
-  return (rows * p.splits * 8 + 15) / 16 * 16 + rows * p.splits * a.width * 4;
+  const int64_t rows = (int64_t)8 * p.tail * p.splits * p.tile_rows;
+  return (rows * 8 + 15) / 16 * 16 + rows * a.width * 4;
 }
 
 hipError_t launch_attend(int dtype, const Attend& a, const AttendPlan& p, void* workspace, hipStream_t st) {

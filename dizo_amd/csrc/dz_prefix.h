@@ -28,13 +28,16 @@ struct Attend {
   const int32_t* prefix_lengths;  // (groups); NULL: prefix_slots
   int32_t groups, sequences, heads, kv_heads, length, width, slots, prefix_slots;
   int32_t bytes;  // an 8-bit store
+  int32_t whole_chunks;  // whose rows are whole chunks of 16 codes, at multiples of 16 bytes
   float scale;
 };
 
-// How a call is cut: `tile_rows` rows of a group's key head a workgroup, its keys over `splits` workgroups.
+// How a call is cut. An item is a tile of up to tile_rows rows of one key head. Each of the 8 XCDs takes `per` items one
+// after another: first `whole` of them, a workgroup each, then `tail`, of which `splits` workgroups each take a part of the keys.
 struct AttendPlan {
   bool by_keys;  // a workgroup's waves share its rows and take keys in turn; else they share keys
-  int32_t tile_rows, tiles, splits;
+  int32_t tile_rows, tiles;
+  int32_t items, per, whole, tail, splits;
 };
 AttendPlan attend_plan(int dtype, const Attend& a);
 int64_t attend_workspace(const Attend& a, const AttendPlan& p);

@@ -149,13 +149,18 @@ int32_t plan_of(const dz_attention* x, dz::Attend* a, dz::AttendPlan* plan) {
   a->scale = x->scale;
   if (!rows) {
     *plan = {};
-    plan->splits = 1;
     return DZ_OK;
   }
   *plan = dz::attend_plan(x->dtype, *a);
-  if ((uint64_t)x->groups * x->kv_heads * plan->tiles * plan->splits > (uint64_t)1 << 23)
-    return invalid("too many tiles of queries");  // a launch counts its threads in 32 bits
+  if (plan->items > 1 << 22) return invalid("too many tiles of queries");  // a launch counts its threads in 32 bits
   return DZ_OK;
+}
+
+// Whether an 8-bit store's rows start at multiples of 16 bytes.
+bool in_chunks(const dz_keys_values& kv) {
+  uint64_t low = (uint64_t)(uintptr_t)kv.k | (uint64_t)(uintptr_t)kv.v;
+  for (int i = 0; i < 4; ++i) low |= (uint64_t)kv.k_strides[i] | (uint64_t)kv.v_strides[i];
+  return low % 16 == 0;
 }
 
 int32_t launched(hipError_t e, const char* what) { return e == hipSuccess ? DZ_OK : dz::api_hip_fail(e, what); }
@@ -282,6 +287,7 @@ int32_t dz_shared_prefix_attention(const dz_attention* x, void* workspace, int64
   copy4(a.out_s, x->out_strides);
   a.own = store_of(x->own);
   a.prefix = store_of(x->prefix);
+  a.whole_chunks = a.bytes && x->width % 16 == 0 && (!x->slots || in_chunks(x->own)) && (!x->prefix_slots || in_chunks(x->prefix));
   a.positions = x->positions;
   a.prefix_lengths = x->prefix_lengths;
   return launched(dz::launch_attend(x->dtype, a, plan, workspace, (hipStream_t)stream), "shared_prefix_attention kernel launch");

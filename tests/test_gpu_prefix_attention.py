@@ -14,15 +14,16 @@ DT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 HALF_STEP = {"fp32": 2.0**-24, "fp16": 2.0**-11, "bf16": 2.0**-8}
 
 
-def bound(dtype, out, spread, reach, keys, width):
+def bound(dtype, out, spread, reach, keys, width, bits):
     """How far a result may be from the definition. Roundings: the result's (half a step of it); the weights', each half a step of
-    a 16-bit type, of sum w |v|; the scores', (width + 4) sums and products in fp32 of sum |q k|, which a weight shows as
+    a 16-bit type (bf16 with an 8-bit store, since a weight carries its value's power of two then), of sum w |v|; the scores', (width + 4) sums and products in fp32 of sum |q k|, which a weight shows as
     a relative error and twice that once it is divided by the sum; exp2's few units; keys sums and products of w v in fp32. An
     fp16 result below 2^-14 rounds in steps of 2^-24."""
     half = HALF_STEP[dtype]
+    weights = 0 if dtype == "fp32" else HALF_STEP["bf16"] if bits == 8 else half
     scores = 2 * (width + 8) * 2.0**-24 * reach.unsqueeze(-1) + 2.0**-20
     floor = 2.0**-25 if dtype == "fp16" else 0.0
-    return half * out.abs() + spread * ((0 if dtype == "fp32" else half) + scores + (keys + 64) * 2.0**-24) * (1 + half) + floor
+    return half * out.abs() + spread * (weights + scores + (keys + 64) * 2.0**-24) * (1 + weights) + floor
 
 
 def inputs(seed, dtype, groups, sequences, heads, kv_heads, length, slots, prefix, width, bits=16, std=1.0):
@@ -61,7 +62,7 @@ def check(dtype, q, own, pre, positions=None, prefix_lengths=None, scale=None, g
     out, spread, reach = O.attend(q, values(own), values(pre), positions, prefix_lengths, scale)
     keys = (own[0].shape[-2] if own else 0) + (pre[0].shape[-2] if pre else 0)
     far = (got.cpu().double() - out).abs()
-    most = bound(dtype, out, spread, reach, keys, q.shape[-1])
+    most = bound(dtype, out, spread, reach, keys, q.shape[-1], 8 if len(own or pre) == 4 else 16)
     assert torch.isfinite(got).all()
     assert (far <= most).all(), f"{float((far / most.clamp(min=1e-300)).max())} times the bound"
     return got
