@@ -210,16 +210,45 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   __syncthreads();
   const uint32_t key_tiles = __builtin_amdgcn_readfirstlane(ends[nseq]);
 
+  // Where a part's keys and values are: the prompt, or one sequence's own.
+  struct Source {
+    const char *k, *v;
+    uint32_t k_step, v_step;  // bytes from slot to slot
+    const uint8_t *k_power, *v_power;
+    uint32_t k_power_step, v_power_step;
+  };
+  constexpr int SIZE = BYTES ? 1 : sizeof(Elem);
+  auto source_of = [&](const KeyValues& kv, int64_t n) {
+    Source x{};
+    x.k = (const char*)kv.k + SIZE * ((int64_t)g * kv.k_s[0] + n * kv.k_s[1] + (int64_t)hk * kv.k_s[2]);
+    x.v = (const char*)kv.v + SIZE * ((int64_t)g * kv.v_s[0] + n * kv.v_s[1] + (int64_t)hk * kv.v_s[2]);
+    x.k_step = (uint32_t)(SIZE * kv.k_s[3]);
+    x.v_step = (uint32_t)(SIZE * kv.v_s[3]);
+    if (BYTES) {
+      x.k_power = kv.k_scale + ((int64_t)g * kv.k_scale_s[0] + n * kv.k_scale_s[1] + (int64_t)hk * kv.k_scale_s[2]);
+      x.v_power = kv.v_scale + ((int64_t)g * kv.v_scale_s[0] + n * kv.v_scale_s[1] + (int64_t)hk * kv.v_scale_s[2]);
+      x.k_power_step = (uint32_t)kv.k_scale_s[3];
+      x.v_power_step = (uint32_t)kv.v_scale_s[3];
+    }
+    return x;
+  };
   // Tiles of keys, in turn: `step` apart.
   const uint32_t first = BY_KEYS ? split * S::WAVES + wave : split, step = BY_KEYS ? splits * S::WAVES : splits;
   struct Part {
     uint32_t k0, limit, n;  // the tile's first key, its part's end, and the sequence (2^32 - 1: the prompt)
   };
-  uint32_t at_seq = 0;  // the part that the last tile asked for lies in
+  uint32_t at_seq = 0, part_begin = 0, part_end = __builtin_amdgcn_readfirstlane(ends[0]), part_limit = prefix_limit;
+  Source source = source_of(a.prefix, 0);  // of the tile that part_of was asked for last
   auto part_of = [&](uint32_t i) {
-    while (i >= __builtin_amdgcn_readfirstlane(ends[at_seq])) ++at_seq;
-    if (at_seq == 0) return Part{i * KT, prefix_limit, ~0u};
-    return Part{(i - (uint32_t)__builtin_amdgcn_readfirstlane(ends[at_seq - 1])) * KT, (uint32_t)__builtin_amdgcn_readfirstlane(lims[at_seq - 1]), n0 + at_seq - 1};
+    if (i >= part_end) {
+      do {
+        part_begin = part_end;
+        part_end = __builtin_amdgcn_readfirstlane(ends[++at_seq]);
+      } while (i >= part_end);
+      part_limit = __builtin_amdgcn_readfirstlane(lims[at_seq - 1]);
+      source = source_of(a.own, n0 + at_seq - 1);
+    }
+    return Part{(i - part_begin) * KT, part_limit, at_seq ? n0 + at_seq - 1 : ~0u};
   };
 
   char(*slab)[2][S::TILE] = lds[BY_KEYS ? wave : 0];
@@ -227,27 +256,6 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   // A tile's loads, keys before values, 64 chunks each.
   constexpr int OF_KEYS = KT * CH, LOADS = 2 * OF_KEYS / 64 / S::LOADERS;  // OF_KEYS: chunks
   static_assert(2 * OF_KEYS % (64 * S::LOADERS) == 0 && (STORE == kCodes || OF_KEYS % 64 == 0), "loads");
-  struct Store_ {  // of keys or of values, from the tile's first one on
-    const char* at;
-    int64_t stride;  // bytes
-    const uint8_t* scale;
-    int64_t scale_stride;
-  };
-  constexpr int SIZE = BYTES ? 1 : sizeof(Elem);
-  auto store_of = [&](const Part& p, bool values) {
-    const KeyValues& kv = p.n == ~0u ? a.prefix : a.own;
-    const int64_t n = p.n == ~0u ? 0 : p.n;
-    const int64_t(&s)[4] = values ? kv.v_s : kv.k_s;
-    Store_ x;
-    x.at = (const char*)(values ? kv.v : kv.k) + SIZE * ((int64_t)g * s[0] + n * s[1] + (int64_t)hk * s[2] + (int64_t)p.k0 * s[3]);
-    x.stride = SIZE * s[3];
-    if (BYTES) {
-      const int64_t(&c)[4] = values ? kv.v_scale_s : kv.k_scale_s;
-      x.scale = (values ? kv.v_scale : kv.k_scale) + ((int64_t)g * c[0] + n * c[1] + (int64_t)hk * c[2] + (int64_t)p.k0 * c[3]);
-      x.scale_stride = c[3];
-    }
-    return x;
-  };
   // Row and chunk of a lane's i-th load. Keys past the part's end are the last one again: their weights are 0, and what these
   // multiply is finite where the last key's values are. Chunks past the width are the row's first: finite where the row is,
   // and multiplied by 0 (keys) or not stored (values).
@@ -258,34 +266,36 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     if (c * PER_CHUNK >= (uint32_t)a.width) c = 0;
     r = row < last ? row : last;
   };
+  // A wave's first half of loads is of keys, the others of values, where that comes out even.
+  constexpr bool EVEN = OF_KEYS % (64 * S::LOADERS) == 0;
+  auto of_values = [&](int i) { return EVEN ? i >= LOADS / 2 : (i * S::LOADERS + loader) * 64 + lane >= OF_KEYS; };
   auto load_direct = [&](const Part& p, int stage) {
-    const Store_ ks = store_of(p, false), vs = store_of(p, true);
+    const uint32_t k_step = source.k_step, v_step = source.v_step;
+    const char* const k = source.k + (uint64_t)p.k0 * k_step;
+    const char* const v = source.v + (uint64_t)p.k0 * v_step;
     const uint32_t to0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&slab[stage][0][0]);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const uint32_t j = i * S::LOADERS + loader;
+      const uint32_t to = to0 + (i * S::LOADERS + loader) * 1024;
       uint32_t r, c;
       place(i, p.limit - 1 - p.k0, r, c);
-      if (OF_KEYS % 64 == 0) {
-        const bool values = j * 64 >= OF_KEYS;
-        to_lds<false>(values ? vs.at : ks.at, r * (uint32_t)(values ? vs.stride : ks.stride) + c * 16, to0 + j * 1024);
-      } else {  // (a load of both)
-        const bool values = j * 64 + lane >= OF_KEYS;
-        to_lds((values ? vs.at : ks.at) + (int64_t)r * (values ? vs.stride : ks.stride) + c * 16, to0 + j * 1024);
+      if (EVEN) {
+        to_lds<false>(of_values(i) ? v : k, r * (of_values(i) ? v_step : k_step) + c * 16, to);
+      } else {
+        to_lds((of_values(i) ? v : k) + (uint64_t)r * (of_values(i) ? v_step : k_step) + c * 16, to);
       }
     }
   };
   // Powers of two of a tile's codes, key lane % 32.
   struct Powers {
-    uint8_t k, v;
+    uint32_t k, v;
   };
   auto load_powers = [&](const Part& p) {
     Powers x{};
     if constexpr (STORE == kCodes) {
-      const Store_ ks = store_of(p, false), vs = store_of(p, true);
-      const uint32_t last = p.limit - 1 - p.k0, r = (lane & 31) < last ? (lane & 31) : last;
-      x.k = ks.scale[r * ks.scale_stride];
-      x.v = vs.scale[r * vs.scale_stride];
+      const uint32_t last = p.limit - 1 - p.k0, r = p.k0 + ((lane & 31) < last ? (lane & 31) : last);
+      x.k = source.k_power[(uint64_t)r * source.k_power_step];
+      x.v = source.v_power[(uint64_t)r * source.v_power_step];
     }
     return x;
   };
@@ -293,23 +303,25 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   using Code = std::conditional_t<sizeof(Elem) == 2, u32x2, uint32_t>;
   struct Staged {
     Code code[STORE == kConverted ? LOADS : 1];
-    uint32_t scale[STORE == kConverted ? LOADS : 1];
+    uint32_t power[STORE == kConverted ? LOADS : 1];
   };
   auto load_codes = [&](const Part& p, Staged& s) {
-    const Store_ ks = store_of(p, false), vs = store_of(p, true);
+    const char *const k = source.k, *const v = source.v;
+    const uint8_t *const k_power = source.k_power, *const v_power = source.v_power;
+    const uint32_t k_step = source.k_step, v_step = source.v_step, k_power_step = source.k_power_step, v_power_step = source.v_power_step;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const Store_& x = (i * S::LOADERS + loader) * 64 >= OF_KEYS ? vs : ks;
       uint32_t r, c;
       place(i, p.limit - 1 - p.k0, r, c);
-      s.code[i] = *(const Code*)(x.at + r * x.stride + c * PER_CHUNK);
-      s.scale[i] = x.scale[r * x.scale_stride];
+      const uint64_t key = p.k0 + r;
+      s.code[i] = *(const Code*)((of_values(i) ? v : k) + key * (of_values(i) ? v_step : k_step) + c * PER_CHUNK);
+      s.power[i] = (of_values(i) ? v_power : k_power)[key * (of_values(i) ? v_power_step : k_power_step)];
     }
   };
   auto put_codes = [&](const Staged& s, int stage) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
-      *(u32x4*)(&slab[stage][0][0] + ((i * S::LOADERS + loader) * 64 + lane) * 16) = Op<T>::widen(s.code[i], __uint_as_float(s.scale[i] << 23));
+      *(u32x4*)(&slab[stage][0][0] + ((i * S::LOADERS + loader) * 64 + lane) * 16) = Op<T>::widen(s.code[i], __uint_as_float(s.power[i] << 23));
   };
 
   f32x16 o[S::PV];
@@ -338,23 +350,35 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
         s[0] = Op<T>::mma(Op<T>::widen8(u32x2{codes[2], codes[3]}, power), qf[2 * q + 1], s[0]);
       }
     } else {
+      // All of the tile's keys on their way, then products of two sums in turn: each waits for the one before it.
+      constexpr int SUMS = NK == 1 ? 2 : NK;
+      f32x16 sum[SUMS];
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        s[i] = f32x16(0.f);
-        const uint32_t r = i * 32 + (lane & 31);
+      for (int i = 0; i < SUMS; ++i) sum[i] = f32x16(0.f);
+      Frag kf[S::STEPS][NK];
 #pragma unroll
-        for (int q = 0; q < S::STEPS; ++q) {
-          Frag kf;
+      for (int q = 0; q < S::STEPS; ++q)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          const uint32_t r = i * 32 + (lane & 31);
           if constexpr (!S::kWide) {
-            kf = *(const Frag*)(kt + r * CH * 16 + ((2 * q + half) ^ swizzle<CH>(r)) * 16);
+            kf[q][i] = *(const Frag*)(kt + r * CH * 16 + ((2 * q + half) ^ swizzle<CH>(r)) * 16);
           } else {
             const f32x4 lo = *(const f32x4*)(kt + r * CH * 16 + ((4 * q + 2 * half) ^ swizzle<CH>(r)) * 16);
             const f32x4 hi = *(const f32x4*)(kt + r * CH * 16 + ((4 * q + 2 * half + 1) ^ swizzle<CH>(r)) * 16);
-            kf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            kf[q][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
           }
-          s[i] = Op<T>::mma(kf, qf[q], s[i]);
         }
-      }
+      if (!S::kWide) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < S::STEPS; ++q)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          f32x16& to = sum[NK == 1 ? q % 2 : i];
+          to = Op<T>::mma(kf[q][i], qf[q], to);
+        }
+#pragma unroll
+      for (int i = 0; i < NK; ++i) s[i] = NK == 1 ? sum[0] + sum[1] : sum[i];
     }
     if (!__all(limit >= p.k0 + KT)) {
 #pragma unroll
@@ -395,11 +419,11 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
         }
       }
 #pragma unroll
-    for (int d = 0; d < S::PV; ++d)
+    for (int i = 0; i < NK; ++i)
 #pragma unroll
-      for (int i = 0; i < NK; ++i)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int d = 0; d < S::PV; ++d) {
           FragV vf;
           if constexpr (STORE == kCodes) {
             // eight rows of 16 codes for each 16 lanes, which get a column each

@@ -92,6 +92,8 @@ int32_t check_store(const dz_keys_values& kv, int32_t dtype, bool bytes, const i
   if (bytes) {
     DZ_TRY(check_tensor(kv.k_scales, 1, dims, kv.k_scale_strides, 1, 1, (name + " key scales").c_str(), extents + 2));
     DZ_TRY(check_tensor(kv.v_scales, 1, dims, kv.v_scale_strides, 1, 1, (name + " value scales").c_str(), extents + 3));
+    if (dims[3] > 1 && (kv.k_scale_strides[3] >= kMaxSlotStride || kv.v_scale_strides[3] >= kMaxSlotStride))
+      return invalid(name + " scales: slots are " + std::to_string(kMaxSlotStride) + " bytes or more apart");
   }
   return DZ_OK;
 }
