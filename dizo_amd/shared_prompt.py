@@ -1,0 +1,203 @@
+"""Candidates and answers of a shared prompt through an HF causal language model, on the kernels of prefix_attention and
+sampling.
+
+``shared_prompt_logprobs``  what the option-masked loss reads (trainer.py:1466-1500), with each example's prompt
+                            computed once instead of once for every candidate. ZOArguments.zo_shared_prompt makes the
+                            zeroth-order forwards use it (model.dz_shared_prompt)
+``generate``                answers drawn from prompts, several from each (trainer.py:1544-1568): a prompt is computed
+                            once, its keys and values are kept once for all of its answers, in the model's dtype or in
+                            8 bits, and each answer keeps its own
+
+Both run the model's own layers, OPT's, LLaMA's or others that call the attention HF registers by name, with one of this
+module's in its place: a forward gets one row for each prompt, and the attention is told where things lie by
+the keyword argument dz_shared. Nothing is recorded by autograd.
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+
+from ._lib import DzError
+from .prefix_attention import KV, QuantizedKV, cache_write, shared_prefix_attention
+from .sampling import sample_tokens
+
+ATTN_IMPL = "dizo_shared_prompt"
+_registered = False
+
+
+class _Candidates:
+    """One forward over rows [prompt | candidate 0 | candidate 1 | ...]: prompts of up to `room` tokens, left-aligned,
+    `each` tokens of every candidate."""
+
+    def __init__(self, room: int, candidates: int, each: int, lengths: torch.Tensor):
+        self.room, self.candidates, self.each, self.lengths = room, candidates, each, lengths
+
+    def attend(self, module, q, k, v, scale):
+        p, n, t = self.room, self.candidates, self.each
+        out = q.new_empty(q.shape[0], q.shape[2], q.shape[1], q.shape[3])
+        prompt = KV(k[:, :, :p], v[:, :, :p])
+        shared_prefix_attention(q[:, :, :p].unsqueeze(1), KV(prompt.k.unsqueeze(1), prompt.v.unsqueeze(1)), scale=scale,
+                                out=out[:, :p].unsqueeze(1).transpose(2, 3))
+        if t:
+            q, k, v = (x[:, :, p:].unflatten(2, (n, t)).transpose(1, 2) for x in (q, k, v))
+            shared_prefix_attention(q, KV(k, v), prompt, prefix_lengths=self.lengths, scale=scale,
+                                    out=out[:, p:].unflatten(1, (n, t)).transpose(2, 3))
+        return out
+
+
+class _Answers:
+    """Forwards that draw `answers` answers of up to `room` tokens from each prompt: first the prompts, then one token of
+    every answer at a time."""
+
+    def __init__(self, prompts: int, answers: int, room: int, lengths: torch.Tensor, bits: int):
+        self.prompts, self.answers, self.room, self.lengths, self.bits = prompts, answers, room, lengths, bits
+        self.prefix, self.own = {}, {}
+        self.at = None  # the answers' tokens that were there before this forward's; None: the prompts'
+
+    def attend(self, module, q, k, v, scale):
+        layer = module.layer_idx
+        out = q.new_empty(q.shape[0], q.shape[2], q.shape[1], q.shape[3])
+        if self.at is None:
+            shape = (self.prompts, self.answers, k.shape[1], self.room, k.shape[3])
+            if self.bits == 8:
+                self.prefix[layer] = QuantizedKV.empty(*k.shape, device=k.device)
+                cache_write(self.prefix[layer], k, v, 0)
+                self.own[layer] = QuantizedKV.empty(*shape, device=k.device)
+            else:
+                self.prefix[layer] = KV(k.contiguous(), v.contiguous())
+                self.own[layer] = KV(k.new_empty(shape), v.new_empty(shape))
+            shared_prefix_attention(q.unsqueeze(1), KV(k.unsqueeze(1), v.unsqueeze(1)), scale=scale, out=out.unsqueeze(1).transpose(2, 3))
+            return out
+        q, k, v = (x.unflatten(0, (self.prompts, self.answers)) for x in (q, k, v))
+        own = self.own[layer]
+        if self.bits == 8:
+            cache_write(own, k, v, self.at)
+        else:
+            own.k[:, :, :, self.at:self.at + 1] = k
+            own.v[:, :, :, self.at:self.at + 1] = v
+        own = type(own)(*(x[:, :, :, :self.at + 1] for x in own))
+        shared_prefix_attention(q, own, self.prefix[layer], prefix_lengths=self.lengths, scale=scale,
+                                out=out.unflatten(0, (self.prompts, self.answers)).transpose(2, 3))
+        return out
+
+
+def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, dz_shared=None, **kwargs):
+    if dz_shared is None:
+        raise DzError(f"{ATTN_IMPL} runs inside of shared_prompt's forwards only")
+    scale = query.shape[-1] ** -0.5 if scaling is None else scaling
+    return dz_shared.attend(module, query, key, value, scale), None
+
+
+def _hidden(model, input_ids: torch.Tensor, position_ids: torch.Tensor, layout) -> torch.Tensor:
+    """The last hidden states of a forward whose attention goes by `layout`."""
+    global _registered
+    if not _registered:
+        from transformers import AttentionInterface
+
+        AttentionInterface.register(ATTN_IMPL, _attention)
+        _registered = True
+    config = model.config
+    before = config._attn_implementation
+    config._attn_implementation = ATTN_IMPL
+    try:
+        return model.base_model(input_ids=input_ids, position_ids=position_ids, attention_mask=None, use_cache=False,
+                                dz_shared=layout).last_hidden_state
+    finally:
+        config._attn_implementation = before
+
+
+def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], option_len, candidates: int,
+                           pad_id: Optional[int]) -> torch.Tensor:
+    """The mean log probability of each sequence's last option_len tokens, (sequences,) in the logits' dtype: what
+    trainer.py:1466-1500 selects, for a batch whose examples have `candidates` sequences each, one after another, left-padded
+    (attention_mask 0), that differ in their last option_len tokens only.
+
+    option_len: integers on the host, at least 1. Tokens that equal pad_id are left out, as there. Examples whose
+    sequences do not share their prompt give NaN. (A sequence's last token predicts nothing that is read and is not
+    computed, so that candidates of one token cost nothing beyond the prompt.)"""
+    if torch.is_grad_enabled():
+        raise DzError("shared_prompt_logprobs: nothing is recorded by autograd, call it under torch.no_grad()")
+    sequences, length = input_ids.shape
+    if candidates < 1 or sequences % candidates or len(option_len) != sequences or not 1 <= min(option_len) <= max(option_len) < length:
+        raise DzError(f"shared_prompt_logprobs: {sequences} sequences of {length} tokens, {candidates} candidates each, option_len {list(option_len)[:8]}")
+    device, examples, most = input_ids.device, sequences // candidates, max(option_len)
+    room, each = length - min(option_len), most - 1
+    options = torch.as_tensor(option_len, device=device)
+    pads = torch.zeros_like(options) if attention_mask is None else length - attention_mask.to(torch.int64).sum(1)
+    prompt_len = (length - pads - options).view(examples, candidates)
+    first = prompt_len[:, 0]
+
+    # prompts from their first token on, then what each candidate adds to them
+    place = torch.arange(room, device=device)
+    from_pads = (pads.unsqueeze(1) + place).clamp_(max=length - 1)
+    prompts = input_ids.gather(1, from_pads).view(examples, candidates, room)
+    inside = place < first.view(examples, 1, 1)
+    same = ((prompts == prompts[:, :1]) | ~inside).all(-1) & (prompt_len == prompt_len[:, :1]) & (prompt_len > 0)
+    last = torch.arange(most, device=device)
+    targets = input_ids.gather(1, (length - options.unsqueeze(1) + last).clamp_(max=length - 1))  # (sequences, most)
+    ids = torch.cat([prompts[:, 0], targets[:, :each].reshape(examples, candidates * each)], 1)
+    steps = (first.unsqueeze(1) + last[:each]).repeat(1, candidates)
+    positions = torch.cat([place.expand(examples, room), steps], 1)
+    # (places that hold no token of a sequence repeat one, and nothing that is read sees them)
+    positions = positions.clamp_(max=length - 1)
+
+    hidden = _hidden(model, ids, positions, _Candidates(room, candidates, each, first.to(torch.int32)))
+    width = hidden.shape[-1]
+    ends = hidden.gather(1, (first - 1).clamp(min=0).view(examples, 1, 1).expand(examples, 1, width))
+    rows = torch.cat([ends.unsqueeze(1).expand(examples, candidates, 1, width), hidden[:, room:].view(examples, candidates, each, width)], 2)
+    log_probs = torch.log_softmax(model.get_output_embeddings()(rows), -1)
+    selected = log_probs.gather(-1, targets.view(examples, candidates, most, 1)).view(sequences, most)
+    mask = last < options.unsqueeze(1)
+    if pad_id is not None:
+        mask = mask & (targets != pad_id)
+    return ((selected * mask).sum(-1) / mask.sum(-1)).masked_fill_(~same.view(-1), float("nan"))
+
+
+def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, answers: int = 1, prompt_lengths: Optional[torch.Tensor] = None,
+             uniform: Optional[torch.Tensor] = None, generator: Optional[torch.Generator] = None,
+             temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0, top_p: Union[float, torch.Tensor] = 1.0,
+             min_p: Union[float, torch.Tensor] = 0.0, eos_token_id: Optional[int] = None, kv_bits: int = 16) -> torch.Tensor:
+    """`answers` answers of max_new_tokens tokens, (prompts, answers, max_new_tokens), to each prompt.
+
+    input_ids (prompts, tokens): prompts from their first token on; prompt_lengths (prompts), int32: how many of them are the
+    prompt's (default: all). uniform (prompts, answers, max_new_tokens), fp32: a number from 0 to 1 for each token
+    (default: drawn from `generator`). temperature, top_k, top_p and min_p as sample_tokens takes them, a tensor being
+    (prompts, answers). After eos_token_id an answer repeats it. kv_bits = 8 keeps keys and values in 8 bits
+    (QuantizedKV). The host waits for nothing."""
+    if kv_bits not in (8, 16):
+        raise DzError(f"generate: kv_bits must be 16 (the model's dtype) or 8, got {kv_bits}")
+    if input_ids.dim() != 2 or input_ids.shape[1] < 1 or answers < 1 or max_new_tokens < 1:
+        raise DzError(f"generate: {tuple(input_ids.shape)} prompts, {answers} answers of {max_new_tokens} tokens")
+    prompts, room = input_ids.shape
+    device = input_ids.device
+    if prompt_lengths is None:
+        prompt_lengths = torch.full((prompts,), room, dtype=torch.int32, device=device)
+    elif prompt_lengths.shape != (prompts,) or prompt_lengths.dtype != torch.int32:
+        raise DzError(f"generate: prompt_lengths must be torch.int32 ({prompts},), got {prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
+    if uniform is None:
+        uniform = torch.rand(prompts, answers, max_new_tokens, generator=generator, device=device)
+    elif uniform.shape != (prompts, answers, max_new_tokens):
+        raise DzError(f"generate: uniform must be {(prompts, answers, max_new_tokens)}, got {tuple(uniform.shape)}")
+    lengths = prompt_lengths.clamp(1, room)
+    model.eval()
+    with torch.no_grad():
+        layout = _Answers(prompts, answers, max_new_tokens, lengths, kv_bits)
+        hidden = _hidden(model, input_ids, torch.arange(room, device=device).expand(prompts, room), layout)
+        rows = hidden.gather(1, (lengths.long() - 1).view(prompts, 1, 1).expand(prompts, 1, hidden.shape[-1]))
+        rows = rows.expand(prompts, answers, rows.shape[-1])
+        tokens = torch.empty(prompts, answers, max_new_tokens, dtype=torch.int64, device=device)
+        ended = None
+        for t in range(max_new_tokens):
+            logits = model.get_output_embeddings()(rows)
+            drawn = sample_tokens(logits, uniform[:, :, t], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            if eos_token_id is not None:
+                drawn = drawn if ended is None else torch.where(ended, eos_token_id, drawn)
+                ended = drawn == eos_token_id
+            tokens[:, :, t] = drawn
+            if t + 1 < max_new_tokens:
+                layout.at = t
+                positions = (lengths.long().view(prompts, 1) + t).expand(prompts, answers).reshape(-1, 1)
+                # (a row without a distribution gives -1, which is no token: it goes on from token 0)
+                rows = _hidden(model, drawn.clamp(min=0).view(-1, 1), positions, layout).view(prompts, answers, -1)
+        return tokens

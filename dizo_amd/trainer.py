@@ -92,6 +92,11 @@ class ZOArguments:
     # classification loss reads (HF's logits_to_keep) instead of at every
     # position; the loss agrees with the full-logit one to rounding
     zo_option_head: bool = False
+    # build-specific: compute the prompt that an example's candidates share
+    # once instead of once for each (dizo_amd.shared_prompt): the forwards of
+    # the classification loss get one row per example. The loss agrees to
+    # rounding; batches that have another form run as they do otherwise
+    zo_shared_prompt: bool = False
     # build-specific: run each OPT decoder layer's fc1 + ReLU as one GEMM with
     # a ReLU epilogue, and its k/v/q projections as one GEMM over a [k; v; q]
     # weight buffer, when no autograd graph is recorded (dizo_amd.fused_layers);
@@ -200,6 +205,21 @@ def shift_option_labels(input_ids: torch.Tensor, option_len, pad_id: int,
     return labels
 
 
+def _candidates_loss(selected: torch.Tensor, labels: torch.Tensor, nopt: List[int]) -> torch.Tensor:
+    """trainer.py:1482-1508: cross entropy over each example's candidates, of their mean log probabilities."""
+    loss_fct = CrossEntropyLoss(ignore_index=-100)
+    if any(x != nopt[0] for x in nopt):
+        loss, start, count = 0, 0, 0
+        while start < len(nopt):
+            end = start + nopt[start]
+            loss = loss_fct(selected[start:end].unsqueeze(0), labels[start:end][0].unsqueeze(0)) + loss
+            count += 1
+            start = end
+        return loss / count
+    selected = selected.view(-1, nopt[0])
+    return loss_fct(selected, labels.view(-1, nopt[0])[:, 0])
+
+
 def option_len_loss(model, build_graph: bool, input_ids=None, labels=None, option_len=None, num_options=None,
                     return_dict=None, *, dz_window: Optional[int] = None, **kwargs):
     """The option-masked classification loss of trainer.py:1446-1522 (and of its
@@ -219,10 +239,25 @@ def option_len_loss(model, build_graph: bool, input_ids=None, labels=None, optio
     positions outside it contribute nothing in the reference. The per-row
     arithmetic is the same; the LM-head GEMM has fewer rows, so the logits,
     and with them the loss, can differ from the full-logit ones by rounding.
+    Shared prompt (``model.dz_shared_prompt``, without an autograd graph and with
+    return_dict): where every example has the same number of candidates, each
+    example's prompt is computed once (dizo_amd.shared_prompt); the loss agrees
+    to rounding, and is NaN where an example's candidates have other prompts.
+
     With the option head and return_dict falsy the logits returned are the
     window's. dz_window = 0 asks for the full logits without looking at
     option_len (a captured graph decides the window on the host beforehand).
     """
+    if (getattr(model, "dz_shared_prompt", False) and not build_graph and return_dict and dz_window is None
+            and labels is not None and option_len is not None and num_options is not None and set(kwargs) <= {"attention_mask"}):
+        lens, nopt = host_ints(option_len), host_ints(num_options)
+        if (all(x == nopt[0] for x in nopt) and input_ids.shape[0] % nopt[0] == 0 and len(lens) == input_ids.shape[0]
+                and 0 < min(lens) <= max(lens) < input_ids.shape[1]):
+            from .shared_prompt import shared_prompt_logprobs
+
+            with torch.no_grad():
+                selected = shared_prompt_logprobs(model, input_ids, kwargs.get("attention_mask"), lens, nopt[0], model.config.pad_token_id)
+                return SimpleNamespace(loss=_candidates_loss(selected, labels, nopt))
     kwargs.setdefault("use_cache", False)
     window = dz_window
     if (window is None and labels is not None and option_len is not None and num_options is not None
@@ -254,18 +289,7 @@ def option_len_loss(model, build_graph: bool, input_ids=None, labels=None, optio
         shift_labels.masked_fill_(~mask, 0)
         selected = torch.gather(log_probs, dim=-1, index=shift_labels.unsqueeze(-1)).squeeze(-1)
         selected = (selected * mask).sum(-1) / mask.sum(-1)
-        nopt = host_ints(num_options)
-        if any(x != nopt[0] for x in nopt):
-            loss, start, count = 0, 0, 0
-            while start < len(nopt):
-                end = start + nopt[start]
-                loss = loss_fct(selected[start:end].unsqueeze(0), labels[start:end][0].unsqueeze(0)) + loss
-                count += 1
-                start = end
-            loss = loss / count
-        else:
-            selected = selected.view(-1, nopt[0])
-            loss = loss_fct(selected, labels.view(-1, nopt[0])[:, 0])
+        loss = _candidates_loss(selected, labels, host_ints(num_options))
     else:
         loss = loss_fct(shift_logits.view(-1, model.config.vocab_size), shift_labels.view(-1))
     if not return_dict:
@@ -367,6 +391,7 @@ class ZOTrainerMixin:
         self._pending_update = None   # (seed, eps, g, lr): restore + update of zo_update
         self.kernel_timer = None
         model.dz_option_head = bool(getattr(args, "zo_option_head", False))
+        model.dz_shared_prompt = bool(getattr(args, "zo_shared_prompt", False))
         self.zo_journal = None
         if getattr(args, "zo_journal", False):
             from .checkpoint import ZOJournal
@@ -627,6 +652,8 @@ class ZOTrainer(ZOTrainerMixin):
         self._log_buf: List[tuple] = []
         self._graph = None
         if getattr(args, "zo_graph", False):
+            if getattr(args, "zo_shared_prompt", False):
+                raise DzError("zo_shared_prompt is not part of captured steps (zo_graph)")
             from .graph import GraphedZOStep
 
             self._graph = GraphedZOStep(self)
