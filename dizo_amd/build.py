@@ -14,7 +14,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libdizo_amd.so")
 SOURCES = ["dz_kernels.hip", "dz_api.hip", "dz_token_loss.hip", "dz_token_head.hip", "dz_token_api.hip",
            "dz_attention.hip", "dz_cache.hip", "dz_sampling.hip", "dz_prefix_api.hip"]
-HEADERS = ["dz_common.h", "dz_internal.h", "dz_kernels.h", "dz_lds.h", "dz_prefix.h", "dz_sampling.h", "dz_token_loss.h",
+HEADERS = ["dz_attention.h", "dz_common.h", "dz_internal.h", "dz_kernels.h", "dz_lds.h", "dz_prefix.h", "dz_sampling.h", "dz_token_loss.h",
            "dz_token_math.h"]
 
 # -ffp-contract=off: products must not be contracted into FMAs (bit parity with

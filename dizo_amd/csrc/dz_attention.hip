@@ -8,111 +8,11 @@
 // sequence that the tile touches, in tiles of their own. The prompt is read once for all of the tile's rows; a sequence's own
 // keys are scored against the whole tile and masked for the rows of others, which costs products that the
 // matrix units have to spare: a tile of single tokens waits for its own keys from memory.
-#include "dz_prefix.h"
-
-#include <type_traits>
-
+#include "dz_attention.h"
 #include "dz_lds.h"
-#include "dz_token_math.h"
 
 namespace dz {
 namespace {
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// Products of 32 keys (or columns of values) by 32 queries over 16 of the width (or 16 keys). A lane holds 8
-// elements of row l % 32; the results: lane l holds query l % 32 and rows 8 b + 4 (l / 32) + r (b, r < 4) in
-// element 4 b + r. Which 8 of the 16 a lane holds does not matter as long as both operands agree: scores take 8 (l / 32) + j,
-// and the products with values 8 (j / 4) + 4 (l / 32) + j % 4, which is where the scores lie already.
-template <class T>
-struct Op;
-template <>
-struct Op<TypeF16> {
-  using Frag = f16x8;
-  __device__ static Frag widen8(u32x2 c, float scale) { return __builtin_bit_cast(Frag, widen(c, scale)); }
-  __device__ static f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-  __device__ static u32x4 widen(u32x2 c, float scale) {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[0], scale, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[0], scale, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[1], scale, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[1], scale, true))};
-  }
-};
-template <>
-struct Op<TypeBF16> {
-  using Frag = bf16x8;
-  __device__ static Frag widen8(u32x2 c, float scale) { return __builtin_bit_cast(Frag, widen(c, scale)); }
-  __device__ static f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-  __device__ static u32x4 widen(u32x2 c, float scale) {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, true))};
-  }
-};
-template <>
-struct Op<TypeF32> {
-  using Frag = f32x8;
-  __device__ static Frag widen8(u32x2 c, float scale) {
-    return __builtin_shufflevector(__builtin_bit_cast(f32x4, widen(c[0], scale)), __builtin_bit_cast(f32x4, widen(c[1], scale)), 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-  __device__ static f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
-  __device__ static u32x4 widen(uint32_t c, float scale) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, scale, true);
-    return u32x4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])};
-  }
-};
-
-// f of a lane's value and of the other half wave's, which holds the same query.
-template <class F>
-__device__ __forceinline__ float both_halves(float x, F f) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return f(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-
-// Where a 16-byte chunk c of row r lies in a tile of CH chunks a row: chunk c ^ swizzle(r). Sixteen consecutive rows
-// at one chunk (a read of keys), and the rows and chunks of 32 lanes' read of values, then lie in different banks, or in few of
-// the same.
-template <int CH>
-__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
-  if (CH == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
-  if (CH == 10) return r >> 3 & 1;
-  if (CH == 12 || CH == 20) return r >> 2 & 3;
-  if (CH == 24) return r >> 1 & 7;
-  return (r & 3) << 2 | (r >> 2 & 3);
-}
-// The same of rows of CH chunks of 16 codes.
-template <int CH>
-__device__ __forceinline__ uint32_t swizzle_codes(uint32_t r) {
-  if (CH == 4) return r >> 2 & 3;
-  if (CH == 5) return 0;
-  if (CH == 6) return r >> 3 & 1;
-  return (r >> 1 & 1) << 1 | (r >> 3 & 1) << 2 | (r >> 2 & 1);
-}
-
-// The rows of a tile: whole sequences, or rows of one.
-struct TileRows {
-  uint32_t row0, rows;
-};
-__device__ __forceinline__ TileRows tile_rows_of(const AttendPlan& plan, uint32_t tile, uint32_t seq_rows, uint32_t all_rows) {
-  const uint32_t most = plan.tile_rows;
-  if (most >= seq_rows) {
-    const uint32_t row0 = tile * most;
-    return {row0, all_rows - row0 < most ? all_rows - row0 : most};
-  }
-  const uint32_t per_seq = (seq_rows + most - 1) / most, r = tile % per_seq * most;
-  return {tile / per_seq * seq_rows + r, seq_rows - r < most ? seq_rows - r : most};
-}
 
 // What a tile in LDS is.
 enum Store {
@@ -155,20 +55,15 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   __shared__ float2 stats[BY_KEYS ? S::WAVES : 1][32];
   __shared__ __attribute__((aligned(16))) float powers[STORE == kCodes ? S::WAVES : 1][32];  // of a tile's values
 
-  // Workgroups go to the 8 XCDs in turn: each XCD takes consecutive items, whose keys its L2 holds for them.
-  const uint32_t xcd = blockIdx.x % 8, order = blockIdx.x / 8, after = order - plan.whole;
-  const bool parted = order >= (uint32_t)plan.whole;
-  const uint32_t at = parted ? plan.whole + after / plan.splits : order, item = xcd * plan.per + at;
-  if (at >= (uint32_t)plan.per || item >= (uint32_t)plan.items) return;
-  const uint32_t split = parted ? after % plan.splits : 0, splits = parted ? plan.splits : 1;
-  const uint32_t gh = item / plan.tiles, tile = plan.tiles - 1 - item % plan.tiles;  // the longest first
-  const uint32_t g = gh / a.kv_heads, hk = gh % a.kv_heads;
+  Item item;
+  if (!item_of(a, plan, item)) return;
+  const uint32_t g = item.g, hk = item.hk, split = item.split, splits = item.splits;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const uint32_t shared = a.heads / a.kv_heads, seq_rows = (uint32_t)a.length * shared, all_rows = seq_rows * a.sequences;
 
   // The tile's rows, the sequences they belong to, and how far each looks.
   // (A tile covers whole sequences, or lies inside of one: plan.tile_rows is a multiple of a sequence's rows or tiles restart at each.)
-  const TileRows tr = tile_rows_of(plan, tile, seq_rows, all_rows);
+  const TileRows tr = tile_rows_of(plan, item.tile, seq_rows, all_rows);
   const uint32_t row0 = tr.row0, rows = tr.rows;
   const uint32_t n0 = row0 / seq_rows, nseq = (row0 + rows - 1) / seq_rows - n0 + 1;
   // This lane's query.
@@ -380,6 +275,42 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
 #pragma unroll
       for (int i = 0; i < NK; ++i) s[i] = NK == 1 ? sum[0] + sum[1] : sum[i];
     }
+    // Values of 16 keys, for all columns.
+    constexpr int GROUPS = 2 * NK;
+    using Read = std::conditional_t<STORE == kCodes, u32x2, FragV>;
+    Read values[2][S::PV];
+    auto read_group = [&](int g) {
+#pragma unroll
+      for (int d = 0; d < S::PV; ++d) {
+        Read& to = values[g % 2][d];
+        if constexpr (STORE == kCodes) {
+          // eight rows of 16 codes for each 16 lanes, which get a column each
+          const uint32_t of = 2 * d + (lane & 31) / 16, chunk = of < CH ? of : CH - 1, j = (lane & 15) / 2;
+          const uint32_t r = g * 16 + j / 4 * 8 + 4 * half + j % 4;
+          typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+          to = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)(vt + r * CH * 16 + (chunk ^ swizzle_codes<CH>(r)) * 16 + (lane & 1) * 8)));
+        } else if constexpr (!S::kWide) {
+          // four rows of 16 columns for each 16 lanes, which get a column each
+          const uint32_t col = 32 * d + (lane & 31) / 16 * 16, group = col / 8 < CH ? col / 8 : CH - 2, chunk = group + (lane & 3) / 2;
+          s16x4 part[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t r = g * 16 + j * 8 + 4 * half + (lane & 15) / 4;
+            part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + r * CH * 16 + (chunk ^ swizzle<CH>(r)) * 16 + (lane & 1) * 8));
+          }
+          to = __builtin_bit_cast(FragV, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+          const uint32_t col = 32 * d + (lane & 31), chunk = col / 4 < CH ? col / 4 : CH - 1;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t r = g * 16 + j / 4 * 8 + 4 * half + j % 4;
+            to[j] = *(const float*)(vt + r * CH * 16 + (chunk ^ swizzle<CH>(r)) * 16 + (lane & 3) * 4);
+          }
+        }
+      }
+    };
+    read_group(0);
     if (!__all(limit >= p.k0 + KT)) {
 #pragma unroll
       for (int i = 0; i < NK; ++i)
@@ -403,56 +334,36 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
       for (int d = 0; d < S::PV; ++d) o[d] *= f;
     }
     const float mm = m == -INFINITY ? 0.f : m;
-    FragV w[NK][2];
+    // Weights of 16 keys at a time (those of 8 a lane), each next to the products with the 16 before: their values are read one such
+    // group ahead.
+    FragV w[GROUPS];
+    auto weights = [&](int g) {
 #pragma unroll
-    for (int i = 0; i < NK; ++i)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 2; ++b) {
+        const int of = g % 2 * 2 + b;
         f32x4 power;
-        if (STORE == kCodes) power = *(const f32x4*)&powers[wave][8 * b + 4 * half];
+        if (STORE == kCodes) power = *(const f32x4*)&powers[wave][8 * of + 4 * half];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float e = exp2_hw(__builtin_fmaf(s[i][4 * b + r], c, -mm));
+          float e = exp2_hw(__builtin_fmaf(s[g / 2][4 * of + r], c, -mm));
           l += e;
           if (STORE == kCodes) e *= power[r];
-          w[i][b / 2][b % 2 * 4 + r] = (typename TV::Elem)e;
+          w[g][4 * b + r] = (typename TV::Elem)e;
         }
       }
+    };
+    weights(0);
 #pragma unroll
-    for (int i = 0; i < NK; ++i)
+    for (int g = 0; g < GROUPS; ++g) {
+      if (g + 1 < GROUPS) read_group(g + 1);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int d = 0; d < S::PV; ++d) {
-          FragV vf;
-          if constexpr (STORE == kCodes) {
-            // eight rows of 16 codes for each 16 lanes, which get a column each
-            const uint32_t of = 2 * d + (lane & 31) / 16, chunk = of < CH ? of : CH - 1, j = (lane & 15) / 2;
-            const uint32_t r = k * 16 + j / 4 * 8 + 4 * half + j % 4;
-            typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
-            const i32x2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (__attribute__((address_space(3))) i32x2*)(vt + r * CH * 16 + (chunk ^ swizzle_codes<CH>(r)) * 16 + (lane & 1) * 8));
-            vf = Op<TV>::widen8(__builtin_bit_cast(u32x2, codes), 1.f);
-          } else if constexpr (!S::kWide) {
-            // four rows of 16 columns for each 16 lanes, which get a column each
-            const uint32_t col = 32 * d + (lane & 31) / 16 * 16, group = col / 8 < CH ? col / 8 : CH - 2, chunk = group + (lane & 3) / 2;
-            s16x4 part[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t r = i * 32 + k * 16 + j * 8 + 4 * half + (lane & 15) / 4;
-              part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + r * CH * 16 + (chunk ^ swizzle<CH>(r)) * 16 + (lane & 1) * 8));
-            }
-            vf = __builtin_bit_cast(FragV, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-          } else {
-            const uint32_t col = 32 * d + (lane & 31), chunk = col / 4 < CH ? col / 4 : CH - 1;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t r = i * 32 + k * 16 + j / 4 * 8 + 4 * half + j % 4;
-              vf[j] = *(const float*)(vt + r * CH * 16 + (chunk ^ swizzle<CH>(r)) * 16 + (lane & 3) * 4);
-            }
-          }
-          o[d] = Op<TV>::mma(vf, w[i][k], o[d]);
-        }
+      for (int d = 0; d < S::PV; ++d) {
+        if constexpr (STORE == kCodes) o[d] = Op<TV>::mma(Op<TV>::widen8(values[g % 2][d], 1.f), w[g], o[d]);
+        else o[d] = Op<TV>::mma(values[g % 2][d], w[g], o[d]);
+      }
+      if (g + 1 < GROUPS) weights(g + 1);
+      if (!S::kWide) __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   // Two tiles' room: the next one is on its way while this one's products run.
@@ -534,7 +445,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   }
   if (!live) return;
   if (splits > 1) {
-    const uint64_t to_row = (((uint64_t)xcd * plan.tail + at - plan.whole) * splits + split) * plan.tile_rows + lane_row;
+    const uint64_t to_row = partial_row(plan, item, lane_row);
     if (half == 0) partial_ms[to_row] = float2{m, l};
     float* to = partial + to_row * a.width;
 #pragma unroll
