@@ -27,15 +27,18 @@ struct Shape {
   static constexpr bool kWide = std::is_same_v<T, TypeF32>;
   static constexpr int CH = STORE == kCodes ? QS : kWide ? 4 * QS : 2 * QS;  // chunks of 16 bytes a row
   static constexpr int STEPS = STORE == kCodes ? (QS + 1) / 2 * 2 : QS;        // products along the width
-  static constexpr int WAVES = BY_KEYS && kWide && STORE != kCodes ? 2 : 4;
+  static constexpr int WAVES = 4;
   static constexpr int KT = BY_KEYS || kWide ? 32 : 64;    // keys of a tile
   static constexpr int ROWS = BY_KEYS ? 32 : 32 * WAVES;  // most rows of a workgroup
   static constexpr int TILE = KT * CH * 16;                // bytes of a tile's keys, or of its values
   static constexpr int LOADERS = BY_KEYS ? 1 : WAVES;        // waves that load a tile
   static constexpr int SLABS = BY_KEYS ? WAVES : 1;
   static constexpr int PV = (QS + 1) / 2;  // products of 32 columns of values
+  // Tiles in LDS. Waves that take keys for themselves have one each: the other waves' loads are on their way meanwhile, and
+  // twice as many of them find room.
+  static constexpr int STAGES = BY_KEYS && STORE != kCodes ? 1 : 2;
   // workgroups that a compute unit's LDS holds
-  static constexpr int RESIDENT = SLABS * 4 * TILE > 72 * 1024 ? 1 : 2;
+  static constexpr int RESIDENT = SLABS * STAGES * 2 * TILE > 72 * 1024 ? 1 : 2;
 };
 
 template <class T, int QS, bool BY_KEYS, Store STORE, int THREADS = 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES,
@@ -49,9 +52,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   using FragV = typename Op<TV>::Frag;
   constexpr int CH = S::CH, KT = S::KT, NK = KT / 32;
   constexpr bool BYTES = STORE != kOperands;
-  __shared__ __attribute__((aligned(256))) char lds[S::SLABS][2][2][S::TILE];
-  __shared__ uint32_t ends[S::ROWS + 1];  // key tiles up to the end of a sequence's (first: of the prompt's)
-  __shared__ uint32_t lims[S::ROWS];      // keys that are looked at of each sequence
+  __shared__ __attribute__((aligned(256))) char lds[S::SLABS][S::STAGES][2][S::TILE];
   __shared__ float2 stats[BY_KEYS ? S::WAVES : 1][32];
   __shared__ __attribute__((aligned(16))) float powers[STORE == kCodes ? S::WAVES : 1][32];  // of a tile's values
 
@@ -66,45 +67,12 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   const TileRows tr = tile_rows_of(plan, item.tile, seq_rows, all_rows);
   const uint32_t row0 = tr.row0, rows = tr.rows;
   const uint32_t n0 = row0 / seq_rows, nseq = (row0 + rows - 1) / seq_rows - n0 + 1;
-  // This lane's query.
-  const uint32_t lane_row = (BY_KEYS ? 0 : wave * 32) + (lane & 31);
-  const bool live = lane_row < rows;
-  const uint32_t row = row0 + (live ? lane_row : 0), n_row = row / seq_rows, t_row = row % seq_rows / shared, h_row = hk * shared + row % shared;
-  const int64_t q_at = (int64_t)g * a.q_s[0] + (int64_t)n_row * a.q_s[1] + (int64_t)h_row * a.q_s[2] + (int64_t)t_row * a.q_s[3];
-  Frag qf[S::STEPS];
-#pragma unroll
-  for (int s = 0; s < S::STEPS; ++s) {
-    // codes are read 16 at a time, for two steps
-    const uint32_t col = STORE == kCodes ? 16 * (2 * (s / 2) + half) + 8 * (s % 2) : 16 * s + 8 * half;
-    qf[s] = Frag(Elem(0.f));
-    if (live && col < (uint32_t)a.width) qf[s] = *(const Frag*)((const Elem*)a.q + q_at + col);
-  }
-
-  auto limit_of = [&](uint32_t n, uint32_t t) {  // own keys that token t of sequence n sees
-    const int64_t p = a.positions ? a.positions[(uint64_t)g * a.sequences + n] : a.slots - a.length;
-    const int64_t l = p + t + 1;
-    return (uint32_t)(l < 0 ? 0 : l > a.slots ? a.slots : l);
-  };
-  const uint32_t own_limit = live ? limit_of(n_row, t_row) : 0;
   uint32_t prefix_limit = 0;
   if (a.prefix_slots) {
     const int32_t l = a.prefix_lengths ? a.prefix_lengths[g] : a.prefix_slots;
     prefix_limit = l < 0 ? 0 : l > a.prefix_slots ? a.prefix_slots : l;
   }
   prefix_limit = __builtin_amdgcn_readfirstlane(prefix_limit);
-  if (tid < nseq) {
-    const uint32_t n = n0 + tid, last = n == (row0 + rows - 1) / seq_rows ? (row0 + rows - 1) % seq_rows / shared : a.length - 1;
-    lims[tid] = limit_of(n, last);
-  }
-  __syncthreads();
-  if (tid <= nseq) {
-    uint32_t e = (prefix_limit + KT - 1) / KT;
-    for (uint32_t i = 0; i < tid; ++i) e += (lims[i] + KT - 1) / KT;
-    ends[tid] = e;
-  }
-  __syncthreads();
-  const uint32_t key_tiles = __builtin_amdgcn_readfirstlane(ends[nseq]);
-
   // Where a part's keys and values are: the prompt, or one sequence's own.
   struct Source {
     const char *k, *v;
@@ -113,8 +81,9 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     uint32_t k_power_step, v_power_step;
   };
   constexpr int SIZE = BYTES ? 1 : sizeof(Elem);
-  auto source_of = [&](const KeyValues& kv, int64_t n) {
-    Source x{};
+  Source source{};  // of the tile that was asked for last
+  auto set_source = [&](const KeyValues& kv, int64_t n) {
+    Source& x = source;
     x.k = (const char*)kv.k + SIZE * ((int64_t)g * kv.k_s[0] + n * kv.k_s[1] + (int64_t)hk * kv.k_s[2]);
     x.v = (const char*)kv.v + SIZE * ((int64_t)g * kv.v_s[0] + n * kv.v_s[1] + (int64_t)hk * kv.v_s[2]);
     x.k_step = (uint32_t)(SIZE * kv.k_s[3]);
@@ -125,26 +94,14 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
       x.k_power_step = (uint32_t)kv.k_scale_s[3];
       x.v_power_step = (uint32_t)kv.v_scale_s[3];
     }
-    return x;
   };
   // Tiles of keys, in turn: `step` apart.
   const uint32_t first = BY_KEYS ? split * S::WAVES + wave : split, step = BY_KEYS ? splits * S::WAVES : splits;
   struct Part {
     uint32_t k0, limit, n;  // the tile's first key, its part's end, and the sequence (2^32 - 1: the prompt)
   };
-  uint32_t at_seq = 0, part_begin = 0, part_end = __builtin_amdgcn_readfirstlane(ends[0]), part_limit = prefix_limit;
-  Source source = source_of(a.prefix, 0);  // of the tile that part_of was asked for last
-  auto part_of = [&](uint32_t i) {
-    if (i >= part_end) {
-      do {
-        part_begin = part_end;
-        part_end = __builtin_amdgcn_readfirstlane(ends[++at_seq]);
-      } while (i >= part_end);
-      part_limit = __builtin_amdgcn_readfirstlane(lims[at_seq - 1]);
-      source = source_of(a.own, n0 + at_seq - 1);
-    }
-    return Part{(i - part_begin) * KT, part_limit, at_seq ? n0 + at_seq - 1 : ~0u};
-  };
+  const uint32_t prefix_tiles = (prefix_limit + KT - 1) / KT;
+  set_source(a.prefix, 0);
 
   char(*slab)[2][S::TILE] = lds[BY_KEYS ? wave : 0];
   const uint32_t loader = BY_KEYS ? 0 : wave;
@@ -217,6 +174,55 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
       *(u32x4*)(&slab[stage][0][0] + ((i * S::LOADERS + loader) * 64 + lane) * 16) = Op<T>::widen(s.code[i], __uint_as_float(s.power[i] << 23));
+  };
+
+  // A first tile of the prompt can be sent for before anything else is known.
+  Part now{first * KT, prefix_limit, ~0u};
+  const bool early = first < prefix_tiles;
+  if constexpr (STORE != kConverted)
+    if (early) load_direct(now, 0);
+
+  // This lane's query.
+  const uint32_t lane_row = (BY_KEYS ? 0 : wave * 32) + (lane & 31);
+  const bool live = lane_row < rows;
+  const uint32_t row = row0 + (live ? lane_row : 0), n_row = row / seq_rows, t_row = row % seq_rows / shared, h_row = hk * shared + row % shared;
+  const int64_t q_at = (int64_t)g * a.q_s[0] + (int64_t)n_row * a.q_s[1] + (int64_t)h_row * a.q_s[2] + (int64_t)t_row * a.q_s[3];
+  Frag qf[S::STEPS];
+#pragma unroll
+  for (int s = 0; s < S::STEPS; ++s) {
+    // codes are read 16 at a time, for two steps
+    const uint32_t col = STORE == kCodes ? 16 * (2 * (s / 2) + half) + 8 * (s % 2) : 16 * s + 8 * half;
+    qf[s] = Frag(Elem(0.f));
+    if (live && col < (uint32_t)a.width) qf[s] = *(const Frag*)((const Elem*)a.q + q_at + col);
+  }
+
+  auto limit_of = [&](uint32_t n, uint32_t t) {  // own keys that token t of sequence n sees
+    const int64_t p = a.positions ? a.positions[(uint64_t)g * a.sequences + n] : a.slots - a.length;
+    const int64_t l = p + t + 1;
+    return (uint32_t)(l < 0 ? 0 : l > a.slots ? a.slots : l);
+  };
+  const uint32_t own_limit = live ? limit_of(n_row, t_row) : 0;
+  // Lane i: what is looked at of the tile's i-th sequence, and how many tiles of keys there are up to its end.
+  const uint32_t n1 = n0 + nseq - 1;
+  uint32_t limit_here = 0;
+  if (lane < nseq) limit_here = limit_of(n0 + lane, n0 + lane == n1 ? (row0 + rows - 1) % seq_rows / shared : a.length - 1);
+  uint32_t end_here = (limit_here + KT - 1) / KT + (lane == 0 ? prefix_tiles : 0);
+  for (uint32_t d = 1; d < nseq; d *= 2) {
+    const uint32_t x = __shfl_up(end_here, d);
+    if (lane >= d) end_here += x;
+  }
+  const uint32_t key_tiles = __builtin_amdgcn_readlane(end_here, nseq - 1);
+  uint32_t at_seq = 0, part_begin = 0, part_end = prefix_tiles, part_limit = prefix_limit;
+  auto part_of = [&](uint32_t i) {
+    if (i >= part_end) {
+      do {
+        part_begin = part_end;
+        part_end = __builtin_amdgcn_readlane(end_here, at_seq++);
+      } while (i >= part_end);
+      part_limit = __builtin_amdgcn_readlane(limit_here, at_seq - 1);
+      set_source(a.own, n0 + at_seq - 1);
+    }
+    return Part{(i - part_begin) * KT, part_limit, at_seq ? n0 + at_seq - 1 : ~0u};
   };
 
   f32x16 o[S::PV];
@@ -366,21 +372,21 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     }
   };
 
-  // Two tiles' room: the next one is on its way while this one's products run.
+  // No load or read of LDS is left open, and (tiles of several waves) every wave is here.
   auto arrive_all = [&]() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // no load or read of LDS is left open
+    __builtin_amdgcn_s_waitcnt(0x0070);
     if (!BY_KEYS) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   if (first < key_tiles) {
-    Part now = part_of(first);
+    if (!early || STORE == kConverted) now = part_of(first);
     Staged st;
     Powers pow = load_powers(now);
     if constexpr (STORE == kConverted) {
       load_codes(now, st);
       put_codes(st, 0);
-    } else {
+    } else if (!early) {
       load_direct(now, 0);
     }
     int stage = 0;
@@ -391,14 +397,22 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
       if (more) next = part_of(i + step);
       arrive_all();
       if (more) {
+        // where there is room the next tile is on its way while this one's products run
         next_pow = load_powers(next);
         if constexpr (STORE == kConverted) load_codes(next, st);
-        else load_direct(next, stage ^ 1);
+        else if (S::STAGES == 2) load_direct(next, stage ^ 1);
       }
       products(now, stage, pow);
-      if constexpr (STORE == kConverted)
-        if (more) put_codes(st, stage ^ 1);
-      stage ^= 1;
+      if constexpr (S::STAGES == 1) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // what was read of the tile is here
+        asm volatile("" ::: "memory");
+      }
+      if (more) {
+        if constexpr (STORE == kConverted) put_codes(st, S::STAGES == 1 ? 0 : stage ^ 1);
+        else if (S::STAGES == 1) load_direct(next, 0);
+      }
+      if (S::STAGES == 2) stage ^= 1;
       now = next;
       pow = next_pow;
     }
@@ -556,7 +570,7 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
   p.per = (p.items + 7) / 8;
   // An XCD's 32 compute units run `slots` workgroups at a time. Items beyond a multiple of that would leave most of them idle for as long as
   // one takes: as many parts of them as fill the slots once. A part has 256 keys or more.
-  const int slots = 32 * (p.by_keys && !a.bytes && a.width * (dtype == 0 ? 1 : 2) > 128 ? 1 : 2);
+  const int slots = 32 * (p.by_keys && dtype == 0 && a.width > 64 ? 1 : 2);
   const int64_t seqs = p.tile_rows > seq_rows ? p.tile_rows / seq_rows : 1, keys = a.prefix_slots + seqs * a.slots;
   const int rest = p.per % slots;
   const int64_t fit = rest ? slots / rest : 1, cap = keys / 256;
