@@ -17,6 +17,7 @@ namespace dz {
 namespace {
 
 constexpr int kBins = 2048;
+constexpr int kPowers = 1024;
 constexpr int kHeldBytes = 128 * 1024;  // of a row in LDS
 constexpr uint32_t kShortRow = 8192;
 
@@ -33,7 +34,7 @@ struct Shared {
     uint64_t list[kList];
   };
   uint64_t pieces[PIECES];  // sums of a wave's part of a slab
-  double powers[64];  // 2^(i / 64)
+  double powers[kPowers];  // 2^(i / kPowers)
   uint64_t wave_sum[kWaves];
   float wave_max[kWaves];
   uint32_t wave_flag[kWaves];
@@ -49,14 +50,19 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-__device__ __forceinline__ uint64_t wave_scan(uint64_t x) {  // sums up to and with this lane
-  const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t o = __shfl_up(x, d);
-    if (lane >= (uint32_t)d) x += o;
-  }
+// Sums up to and with this lane: of 24, 24 and 16 bits each, whose sums over 64 lanes fit 32.
+__device__ __forceinline__ uint32_t wave_scan_part(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // the lane before, of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the second 16 lanes, and the third's last to the fourth
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
   return x;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t x) {
+  const uint32_t low = wave_scan_part((uint32_t)x & 0xffffff), middle = wave_scan_part((uint32_t)(x >> 24) & 0xffffff), high = wave_scan_part((uint32_t)(x >> 48));
+  return low + ((uint64_t)middle << 24) + ((uint64_t)high << 48);
 }
 
 // Sums up to and with this thread, and of all of them. Every thread has read what the last call left.
@@ -213,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   const int32_t top_k = temperature == 0 ? 1 : a.top_ks ? a.top_ks[r] : a.top_k;
   const double unit = temperature == 0 ? 1.0 : temperature;
 
-  if (tid < 64) sh.powers[tid] = exp2(tid / 64.0);
+  for (int i = tid; i < kPowers; i += kThreads) sh.powers[i] = exp2(i / (double)kPowers);
   for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
   if (tid == 0) sh.listed = 0;
   bool none = !(u >= 0.f && u <= 1.f) || !(temperature == 0 || (temperature >= 0x1p-63 && temperature < 0x1p64)) || top_p != top_p || min_p != min_p;
@@ -245,27 +251,25 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     m = 0.f;
   }
 
-  // Weights as whole numbers of 2^-shift. 2^t = 2^(n / 64) 2^r, n / 64 the nearest such number to t: the table, and Taylor's
-  // polynomial of 2^r (|r| <= 2^-7: the next term is under 2^-54).
+  // Weights as whole numbers of 2^-shift. A logit's place is its distance to 2^-2 of that, in 1,024ths of a power of two (and 0 below):
+  // place n + f gives 2^(n / 1024 - 2) 2^(f / 1024), by a table, and by Taylor's polynomial (the next term is under 2^-46.6 of
+  // it). Places are exact to 2^-38, which moves a weight by 2^-48 of it.
   const int lg = 32 - __clz((a.vocab - 1) | 1), shift = 62 - lg < 46 ? 62 - lg : 46;
-  const double inverse = 1.4426950408889634074 / unit, wide_m = m, far = -(double)(shift + 2);
-  auto power_of = [&](float x) { return ((double)x - wide_m) * inverse; };
-  auto weight_at = [&](double t) -> uint64_t {
-    t = fmax(t, far);  // 0, once it is a whole number
-    constexpr double kNearest = 0x1.8p46;  // adding it leaves the nearest n / 64, with n in the low bits
-    const double q = t + kNearest, f = t - (q - kNearest);
-    const int32_t n = (int32_t)__double_as_longlong(q);
-    double p = __builtin_fma(f, 0x1.5d87fe78a673p-10, 0x1.3b2ab6fba4e77p-7);
-    p = __builtin_fma(f, p, 0x1.c6b08d704a0bfp-5);
-    p = __builtin_fma(f, p, 0x1.ebfbdff82c58ep-3);
-    p = __builtin_fma(f, p, 0x1.62e42fefa39efp-1) * f;
-    const double w = sh.powers[n & 63], y = __builtin_fma(w, p, w);
-    const double scaled = __longlong_as_double(__double_as_longlong(y) + ((int64_t)((n >> 6) + shift) << 52));
+  const double per = kPowers * 1.4426950408889634074 / unit, wide_m = m, most = kPowers * (double)(shift + 2);
+  auto place_of = [&](float x) { return fmax(__builtin_fma((double)x - wide_m, per, most), 0.0); };
+  auto weight_at = [&](double place) -> uint64_t {
+    constexpr double kLn = 0x1.62e42fefa39efp-11;  // ln 2 / 1024
+    const uint32_t n = (uint32_t)place;
+    const double f = __builtin_amdgcn_fract(place);
+    double p = __builtin_fma(f, kLn * kLn * kLn / 6, kLn * kLn / 2);
+    p = __builtin_fma(f, p, kLn) * f;
+    const double w = sh.powers[n % kPowers], y = __builtin_fma(w, p, w);
+    const double scaled = __longlong_as_double(__double_as_longlong(y) + ((int64_t)((int32_t)(n / kPowers) - 2) << 52));
     return (uint64_t)__double_as_longlong(scaled + 0x1p52) & 0xfffffffffffffull;
   };
-  auto weight = [&](float x) -> uint64_t { return weight_at(power_of(x)); };
-  // min_p as the power that a kept weight's reaches; the largest is always kept
-  const double least_power = min_p > 0 ? fmin(log2(min_p), 0.0) : -INFINITY;
+  auto weight = [&](float x) -> uint64_t { return weight_at(place_of(x)); };
+  // min_p as the place that is reached by what it keeps; the largest is always kept
+  const double least_place = min_p > 0 ? kPowers * (fmin(log2(min_p), 0.0) + (shift + 2)) : 0.0;
 
   auto clear = [&]() {
     for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
@@ -380,6 +384,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     __syncthreads();
     return sh.cut;
   };
+  // An order as a logit and the token after the last one of those that equal it: what is not below it is compared as it stands.
+  struct Border {
+    float x;
+    uint32_t end;
+  };
+  auto border_of = [](uint64_t order) { return order ? Border{of_key((uint32_t)(order >> 32)), token_of(order) + 1} : Border{-INFINITY, 0}; };
+  auto not_below = [](const Border& b, float x, uint32_t token) { return x > b.x || (x == b.x && token < b.end); };
   // What top-p keeps of a sum: whole numbers that have to be reached.
   auto share_of = [&](uint64_t total) -> uint64_t {
     const double share = __builtin_ceil(top_p * (double)total);
@@ -410,7 +421,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
         const uint64_t w = weight_of(e), before = block_scan(sh, w, total) - w;
         if (before >= share_of(total)) e = 0;
       }
-      if (e && power_of(of_key((uint32_t)(e >> 32))) < least_power) e = 0;
+      if (e && place_of(of_key((uint32_t)(e >> 32))) < least_place) e = 0;
       const uint32_t kept = __syncthreads_count(e != 0);
       e = e << 32 | e >> 32;  // by token from here on
       sort(sh, e, kept);
@@ -431,22 +442,28 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     __syncthreads();
   }
   if (top_p < 1.0) {
-    uint64_t sum = 0, total;
-    row.each([&](float x, uint32_t token) {
-      if (x != -INFINITY && order_of(key_of(x), token) >= cut) {
-        const uint64_t w = weight(x);
-        sum += w;
-        if (w) add_to(bin_of(x), w);
-      }
+    const Border border = border_of(cut);
+    row.slabs_do([&](uint32_t, const float(&v)[PER], uint32_t at) {
+      uint64_t w[PER];  // (of all, so that their long chains of operations run next to each other)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) w[j] = weight(v[j]);
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (w[j] && not_below(border, v[j], at + j)) add_to(bin_of(v[j]), w[j]);
     });
+    __syncthreads();
+    uint64_t sum = 0, total;
+    for (int i = tid; i < kBins; i += kThreads) sum += sh.bins[i];
     block_scan(sh, sum, total);
     cut = cut_at(share_of(total), cut, false);
   }
 
   // What is kept of each piece of the row, and the piece and token that u falls on.
-  auto kept = [&](float x, uint32_t token, double& t) {
-    t = power_of(x);
-    return x != -INFINITY && t >= least_power && t >= far && order_of(key_of(x), token) >= cut;
+  const Border border = border_of(cut);
+  auto kept = [&](float x, uint32_t token) -> uint64_t {
+    const double place = place_of(x);
+    const uint64_t w = weight_at(place);
+    return place >= least_place && not_below(border, x, token) ? w : 0;
   };
   const uint32_t pieces = row.slabs * kWaves;
   uint64_t all = 0, sum;
@@ -454,12 +471,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   row.slabs_do([&](uint32_t s, const float(&v)[PER], uint32_t at) {
     uint64_t n = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      double t;
-      if (kept(v[j], at + j, t)) n += weight_at(t);
-    }
+    for (int j = 0; j < PER; ++j) n += kept(v[j], at + j);
     all += n;
-    if (__any(n != 0)) n = wave_scan(n);
+    n = wave_scan(n);
     if (lane == 63 && s < row.slabs) sh.pieces[s * kWaves + wave] = n;
   });
   block_scan(sh, all, sum);
@@ -470,11 +484,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     row.slab(piece / kWaves, [&](const float(&v)[PER], uint32_t at) {
       uint64_t w[PER], n = 0;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        double t;
-        w[j] = kept(v[j], at + j, t) ? weight_at(t) : 0;
-        n += w[j];
-      }
+      for (int j = 0; j < PER; ++j) n += w[j] = kept(v[j], at + j);
       uint64_t before = sh.found_before + wave_scan(n) - n;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
