@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     if (tid == 0) sh.listed = 0;
     __syncthreads();
     row.each([&](float x, uint32_t token) {
-      if (x != -INFINITY && take(x, token)) {
+      if (take(x, token) && x != -INFINITY) {
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < kList) sh.list[at] = order_of(key_of(x), token);
       }
@@ -312,7 +312,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     const uint32_t bin = sh.found;
     uint64_t before = sh.found_before;
     if (bin == kBins) return least;
-    if (list([&](float x, uint32_t token) { return bin_of(x) == bin && order_of(key_of(x), token) >= least; }) <= kList) {
+    // (bin_of in as few operations as it takes: nearly all logits lie elsewhere)
+    const float from = (float)bin, to = bin == kBins - 1 ? NAN : (float)(bin + 1);
+    auto in_bin = [&](float x) {
+      const float d = (m - x) * per_unit;
+      return d >= from && !(d >= to);
+    };
+    if (list([&](float x, uint32_t token) { return in_bin(x) && order_of(key_of(x), token) >= least; }) <= kList) {
       uint64_t all;
       const uint64_t v = counts ? e != 0 : weight_of(e), upto = block_scan(sh, v, all);
       if (before + upto - v < target && before + upto >= target) sh.cut = e;
@@ -326,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
       sh.high = 0;
     }
     __syncthreads();
-    auto of_bin = [&](float x, uint32_t token) { return x != -INFINITY && bin_of(x) == bin && order_of(key_of(x), token) >= least; };
+    auto of_bin = [&](float x, uint32_t token) { return in_bin(x) && x != -INFINITY && order_of(key_of(x), token) >= least; };
     row.each([&](float x, uint32_t token) {
       if (of_bin(x, token)) {
         const uint32_t k = key_of(x);
@@ -444,7 +450,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   if (top_p < 1.0) {
     const Border border = border_of(cut);
     row.slabs_do([&](uint32_t, const float(&v)[PER], uint32_t at) {
-      uint64_t w[PER];  // (of all, so that their long chains of operations run next to each other)
+      uint64_t w[PER];
 #pragma unroll
       for (int j = 0; j < PER; ++j) w[j] = weight(v[j]);
 #pragma unroll
