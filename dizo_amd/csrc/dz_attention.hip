@@ -21,6 +21,126 @@ enum Store {
   kCodes,      // codes, loaded straight to LDS and converted by the wave that takes keys for itself; widths of whole chunks
 };
 
+// The sums of a row by themselves, key by key: a lane takes a key's score, and then a column or two of the values. For rows
+// whose sums came out as NaN: a product with a weight of 0 is NaN where the value is infinite or NaN, so that one such value reaches
+// all rows that its tile was scored against. Here a row meets the keys that it sees and no others.
+template <class T, bool BYTES>
+struct LoneRow {
+  using Elem = typename T::Elem;
+  const Elem* q;
+  float o[2] = {0.f, 0.f}, m = -INFINITY, l = 0.f;
+  uint32_t lane = threadIdx.x & 63;
+
+  __device__ static float value(const void* x, const uint8_t* power, int64_t at, int64_t power_at) {
+    if constexpr (BYTES) return __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)x)[at], 0) * __uint_as_float((uint32_t)power[power_at] << 23);
+    return (float)((const Elem*)x)[at];
+  }
+  // Keys k0 ... k1 - 1, 64 at most; true when the answer is NaN whatever follows.
+  __device__ bool keys(const Attend& a, const KeyValues& kv, uint32_t g, uint32_t n, uint32_t hk, uint32_t k0, uint32_t k1) {
+    auto from = [&](const int64_t* s, uint32_t key) { return (int64_t)g * s[0] + (int64_t)n * s[1] + (int64_t)hk * s[2] + (int64_t)key * s[3]; };
+    float s = -INFINITY;
+    if (k0 + lane < k1) {
+      const int64_t at = from(kv.k_s, k0 + lane), power_at = BYTES ? from(kv.k_scale_s, k0 + lane) : 0;
+      s = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < a.width; ++i) s = __builtin_fmaf((float)q[i], value(kv.k, kv.k_scale, at + i, power_at), s);
+      s *= a.scale * kLog2e;
+    }
+    if (__any(s != s || s == INFINITY)) {
+      o[0] = o[1] = NAN;
+      m = 0.f;
+      l = 1.f;
+      return true;
+    }
+    float top = s;
+    for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+    if (top > m) {
+      const float f = exp2_hw(m - top);
+      m = top;
+      l *= f;
+      o[0] *= f;
+      o[1] *= f;
+    }
+    const float e = s == -INFINITY ? 0.f : exp2_hw(s - m);
+    float sum = e;
+    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+    l += sum;
+#pragma unroll 1
+    for (uint32_t key = k0; key < k1; ++key) {
+      const float w = __shfl(e, key - k0);
+      const int64_t at = from(kv.v_s, key), power_at = BYTES ? from(kv.v_scale_s, key) : 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < (uint32_t)a.width) o[i] = __builtin_fmaf(w, value(kv.v, kv.v_scale, at + lane + 64 * i, power_at), o[i]);
+    }
+    return false;
+  }
+};
+
+// What a kernel is launched with.
+struct Call {
+  Attend a;
+  AttendPlan plan;
+  float* partial;  // sums of rows whose keys several workgroups take, and their maxima and sums of weights
+  float2* partial_ms;
+};
+
+// Own keys that token t of sequence n sees.
+__device__ __forceinline__ uint32_t own_keys(const Attend& a, uint32_t g, uint32_t n, uint32_t t) {
+  const int64_t p = a.positions ? a.positions[(uint64_t)g * a.sequences + n] : a.slots - a.length;
+  const int64_t l = p + t + 1;
+  return (uint32_t)(l < 0 ? 0 : l > a.slots ? a.slots : l);
+}
+// Keys of the group's prompt.
+__device__ __forceinline__ uint32_t prefix_keys(const Attend& a, uint32_t g) {
+  if (!a.prefix_slots) return 0;
+  const int32_t l = a.prefix_lengths ? a.prefix_lengths[g] : a.prefix_slots;
+  return __builtin_amdgcn_readfirstlane(l < 0 ? 0 : l > a.prefix_slots ? a.prefix_slots : l);
+}
+
+// The rows first + (each set bit) of the workgroup's tile by themselves, one after another. Where they are and what they see
+// is found again from the arguments: kept until here, it would take registers from the kernel's loop (8-bit answers: 36 us
+// against 34).
+template <class T, bool BY_KEYS, bool BYTES, uint32_t KT, uint32_t WAVES>
+__device__ __forceinline__ void lone_rows(uint32_t first, uint32_t set) {
+  using Elem = typename T::Elem;
+  auto arguments = (const __attribute__((address_space(4))) Call*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(arguments));
+  const Call& call = *(const Call*)arguments;
+  const Attend& a = call.a;
+  const AttendPlan& plan = call.plan;
+  Item item;
+  if (!item_of(a, plan, item)) return;
+  const uint32_t lane = threadIdx.x & 63, g = item.g, shared = a.heads / a.kv_heads, seq_rows = (uint32_t)a.length * shared;
+  const uint32_t row0 = tile_rows_of(plan, item.tile, seq_rows, seq_rows * a.sequences).row0, n0 = row0 / seq_rows;
+  const uint32_t prefix_limit = prefix_keys(a, g), prefix_tiles = (prefix_limit + KT - 1) / KT;
+  auto mine = [&](uint32_t tile) { return (BY_KEYS ? tile / WAVES : tile) % item.splits == item.split; };
+#pragma unroll 1
+  for (; set; set &= set - 1) {
+    const uint32_t lane_row = first + __builtin_ctz(set), row = row0 + lane_row;
+    const uint32_t n = row / seq_rows, t = row % seq_rows / shared, h = item.hk * shared + row % shared, limit = own_keys(a, g, n, t);
+    LoneRow<T, BYTES> x{(const Elem*)a.q + (int64_t)g * a.q_s[0] + (int64_t)n * a.q_s[1] + (int64_t)h * a.q_s[2] + (int64_t)t * a.q_s[3]};
+    uint32_t begin = prefix_tiles;  // its own tiles' place among the workgroup's
+    for (uint32_t i = n0; i < n; ++i) begin += (own_keys(a, g, i, a.length - 1) + KT - 1) / KT;
+    bool done = false;
+#pragma unroll 1
+    for (uint32_t i = 0; i < prefix_tiles && !done; ++i)
+      if (mine(i)) done = x.keys(a, a.prefix, g, 0, item.hk, i * KT, min((i + 1) * KT, prefix_limit));
+#pragma unroll 1
+    for (uint32_t i = 0; i * KT < limit && !done; ++i)
+      if (mine(begin + i)) done = x.keys(a, a.own, g, n, item.hk, i * KT, min((i + 1) * KT, limit));
+    const uint64_t to_row = item.splits > 1 ? partial_row(plan, item, lane_row) : 0;
+    if (item.splits > 1 && lane == 0) call.partial_ms[to_row] = float2{x.m, x.l};
+    Elem* to = (Elem*)a.out + (int64_t)g * a.out_s[0] + (int64_t)n * a.out_s[1] + (int64_t)h * a.out_s[2] + (int64_t)t * a.out_s[3];
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t col = lane + 64 * i;
+      if (col >= (uint32_t)a.width) continue;
+      if (item.splits > 1) call.partial[to_row * a.width + col] = x.o[i];
+      else to[col] = (Elem)(x.l == 0.f ? 0.f : x.o[i] / x.l);
+    }
+  }
+}
+
 // QS: sixteenths of the width, rounded up to 4, 5, 6 or 8.
 template <class T, int QS, bool BY_KEYS, Store STORE>
 struct Shape {
@@ -43,7 +163,9 @@ struct Shape {
 
 template <class T, int QS, bool BY_KEYS, Store STORE, int THREADS = 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES,
           int RESIDENT = Shape<T, QS, BY_KEYS, STORE>::RESIDENT>
-__global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void attend_kernel(Attend a, AttendPlan plan, float* partial, float2* partial_ms) {
+__global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void attend_kernel(Call call) {
+  const Attend& a = call.a;
+  const AttendPlan& plan = call.plan;
   using S = Shape<T, QS, BY_KEYS, STORE>;
   using Elem = typename T::Elem;
   using Frag = typename Op<T>::Frag;
@@ -67,12 +189,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   const TileRows tr = tile_rows_of(plan, item.tile, seq_rows, all_rows);
   const uint32_t row0 = tr.row0, rows = tr.rows;
   const uint32_t n0 = row0 / seq_rows, nseq = (row0 + rows - 1) / seq_rows - n0 + 1;
-  uint32_t prefix_limit = 0;
-  if (a.prefix_slots) {
-    const int32_t l = a.prefix_lengths ? a.prefix_lengths[g] : a.prefix_slots;
-    prefix_limit = l < 0 ? 0 : l > a.prefix_slots ? a.prefix_slots : l;
-  }
-  prefix_limit = __builtin_amdgcn_readfirstlane(prefix_limit);
+  const uint32_t prefix_limit = prefix_keys(a, g);
   // Where a part's keys and values are: the prompt, or one sequence's own.
   struct Source {
     const char *k, *v;
@@ -196,16 +313,11 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     if (live && col < (uint32_t)a.width) qf[s] = *(const Frag*)((const Elem*)a.q + q_at + col);
   }
 
-  auto limit_of = [&](uint32_t n, uint32_t t) {  // own keys that token t of sequence n sees
-    const int64_t p = a.positions ? a.positions[(uint64_t)g * a.sequences + n] : a.slots - a.length;
-    const int64_t l = p + t + 1;
-    return (uint32_t)(l < 0 ? 0 : l > a.slots ? a.slots : l);
-  };
-  const uint32_t own_limit = live ? limit_of(n_row, t_row) : 0;
+  const uint32_t own_limit = live ? own_keys(a, g, n_row, t_row) : 0;
   // Lane i: what is looked at of the tile's i-th sequence, and how many tiles of keys there are up to its end.
   const uint32_t n1 = n0 + nseq - 1;
   uint32_t limit_here = 0;
-  if (lane < nseq) limit_here = limit_of(n0 + lane, n0 + lane == n1 ? (row0 + rows - 1) % seq_rows / shared : a.length - 1);
+  if (lane < nseq) limit_here = own_keys(a, g, n0 + lane, n0 + lane == n1 ? (row0 + rows - 1) % seq_rows / shared : a.length - 1);
   uint32_t end_here = (limit_here + KT - 1) / KT + (lane == 0 ? prefix_tiles : 0);
   for (uint32_t d = 1; d < nseq; d *= 2) {
     const uint32_t x = __shfl_up(end_here, d);
@@ -457,11 +569,19 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
         for (int r = 0; r < 4; ++r) o[d][4 * b + r] += x[r];
       }
   }
-  if (!live) return;
+  bool nan = false;
+#pragma unroll
+  for (int d = 0; d < S::PV; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) nan |= o[d][j] != o[d][j];  // (columns past the width are finite, or the row's first ones again)
+  const uint64_t nan_lanes = __ballot(live && nan);
+  uint32_t nan_rows = (uint32_t)nan_lanes | (uint32_t)(nan_lanes >> 32);
+  if (nan_rows) lone_rows<T, BY_KEYS, BYTES, KT, S::WAVES>(BY_KEYS ? 0 : wave * 32, nan_rows);
+  if (!live || nan_rows >> (lane & 31) & 1) return;
   if (splits > 1) {
     const uint64_t to_row = partial_row(plan, item, lane_row);
-    if (half == 0) partial_ms[to_row] = float2{m, l};
-    float* to = partial + to_row * a.width;
+    if (half == 0) call.partial_ms[to_row] = float2{m, l};
+    float* to = call.partial + to_row * a.width;
 #pragma unroll
     for (int d = 0; d < S::PV; ++d)
 #pragma unroll
@@ -517,7 +637,7 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, AttendPlan plan, co
 
 template <class T, int QS, bool BY_KEYS, Store STORE>
 void launch_one(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {
-  attend_kernel<T, QS, BY_KEYS, STORE><<<8 * (p.whole + p.tail * p.splits), 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES, 0, st>>>(a, p, partial, ms);
+  attend_kernel<T, QS, BY_KEYS, STORE><<<8 * (p.whole + p.tail * p.splits), 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES, 0, st>>>(Call{a, p, partial, ms});
 }
 template <class T, int QS>
 void launch_qs(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {

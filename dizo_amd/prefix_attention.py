@@ -122,11 +122,12 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
     (default: all). own (groups, sequences, kv_heads, slots, width): a sequence's own, of which query t sees the
     first positions + t + 1; positions (groups, sequences), int32: how many were there before the call's tokens
     (default: slots - length). Either store may be missing. Lengths outside of their range are taken as the nearest in
-    it; a query that sees nothing gives 0. What lies in slots that no query of a sequence sees does not matter.
+    it; a query that sees nothing gives 0. What lies in slots that a query does not see does not matter to it, infinities and
+    NaN included.
 
     Stores are KV, of q's dtype, or both QuantizedKV. heads is a multiple of kv_heads, the width a multiple of 8 up to
     128; scale (default: width ** -0.5) is positive. Products and sums are fp32, and weights are rounded to q's dtype
-    before they multiply values. The result is laid out like q unless `out` is given. Tensors whose rows do not
+    (of an 8-bit store: at least to bf16) before they multiply values. The result is laid out like q unless `out` is given. Tensors whose rows do not
     start at multiples of 16 bytes (codes: 8) are copied first, `out` has to fit."""
     what = "shared_prefix_attention"
     if not q.is_cuda:

@@ -305,12 +305,13 @@ typedef struct dz_keys_values {
  * and 0 where it sees nothing. heads is a multiple of kv_heads; query heads
  * heads / kv_heads h .. + heads / kv_heads - 1 read key head h. width is a
  * multiple of 8 up to 128. Lengths and positions outside their ranges are taken
- * as the nearest in it. Slots that no query of a sequence sees are not looked
- * at, whatever they hold; a query's weights of slots that it does not see itself
- * are 0, which leaves NaN of an infinite or NaN value there. Products and sums
- * are fp32; weights are rounded to `dtype` before they multiply values (bf16:
- * 2^-8 of each at most, as their sum is taken before). Both stores are of
- * `dtype`, or both 8-bit. `out` may not overlap an input. Replaces, for
+ * as the nearest in it. What slots hold that a query does not see, infinities
+ * and NaN too, does not matter to it. Products and sums are fp32; weights are
+ * rounded to `dtype` (of an 8-bit store: at least to bf16) before they multiply
+ * values, 2^-8 of each at most, as their sum is taken before. Both stores are of
+ * `dtype`, or both 8-bit, whose values are taken in `dtype`. `out` may not
+ * overlap an input. Rows whose sums are NaN are taken again by themselves, key
+ * by key: right, and slow where there are many. Replaces, for
  * candidates that share a prompt, the attention of the forwards in
  * trainer.py:1524-1542, which repeats it for each. */
 typedef struct dz_attention {
