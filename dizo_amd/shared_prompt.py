@@ -9,8 +9,10 @@ sampling.
                             8 bits, and each answer keeps its own
 
 Both run the model's own layers, OPT's, LLaMA's or others that call the attention HF registers by name, with one of this
-module's in its place: a forward gets one row for each prompt, and the attention is told where things lie by
-the keyword argument dz_shared. Nothing is recorded by autograd.
+module's in its place (in the model's config, for as long as a forward takes: one call at a time for a model): a forward gets
+one row for each prompt, and the attention is told where things lie by the keyword argument dz_shared. Attention with a
+window, a soft cap or sinks, layers that mix tokens in another way, and heads whose logits are scaled or capped are
+refused. Nothing is recorded by autograd.
 """
 from __future__ import annotations
 
@@ -32,8 +34,9 @@ class _Candidates:
 
     def __init__(self, room: int, candidates: int, each: int, lengths: torch.Tensor):
         self.room, self.candidates, self.each, self.lengths = room, candidates, each, lengths
+        self.keys, self.seen = room + each, set()  # keys that a query sees at most, and the layers that this forward has been through
 
-    def attend(self, module, q, k, v, scale):
+    def attend(self, layer, q, k, v, scale):
         p, n, t = self.room, self.candidates, self.each
         out = q.new_empty(q.shape[0], q.shape[2], q.shape[1], q.shape[3])
         prompt = KV(k[:, :, :p], v[:, :, :p])
@@ -50,13 +53,13 @@ class _Answers:
     """Forwards that draw `answers` answers of up to `room` tokens from each prompt: first the prompts, then one token of
     every answer at a time."""
 
-    def __init__(self, prompts: int, answers: int, room: int, lengths: torch.Tensor, bits: int):
+    def __init__(self, prompts: int, answers: int, input_room: int, room: int, lengths: torch.Tensor, bits: int):
         self.prompts, self.answers, self.room, self.lengths, self.bits = prompts, answers, room, lengths, bits
-        self.prefix, self.own = {}, {}
+        self.keys, self.seen = input_room + room, set()  # as above
+        self.prefix, self.own = {}, {}  # of each layer
         self.at = None  # the answers' tokens that were there before this forward's; None: the prompts'
 
-    def attend(self, module, q, k, v, scale):
-        layer = module.layer_idx
+    def attend(self, layer, q, k, v, scale):
         out = q.new_empty(q.shape[0], q.shape[2], q.shape[1], q.shape[3])
         if self.at is None:
             shape = (self.prompts, self.answers, k.shape[1], self.room, k.shape[3])
@@ -82,11 +85,29 @@ class _Answers:
         return out
 
 
-def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, dz_shared=None, **kwargs):
+def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, dz_shared=None, sliding_window=None,
+               softcap=None, s_aux=None, **kwargs):
     if dz_shared is None:
         raise DzError(f"{ATTN_IMPL} runs inside of shared_prompt's forwards only")
+    if dropout or softcap is not None or s_aux is not None or not getattr(module, "is_causal", True):
+        raise DzError("shared_prompt: attention with dropout, a soft cap or sinks, or that isn't causal")
+    if sliding_window is not None and sliding_window < dz_shared.keys:
+        raise DzError(f"shared_prompt: attention with a window of {sliding_window} of {dz_shared.keys} tokens")
+    layer = getattr(module, "layer_idx", None)
+    if layer is None or layer in dz_shared.seen:
+        raise DzError(f"shared_prompt: {type(module).__name__} without a number of its own (layer_idx)")
+    dz_shared.seen.add(layer)
     scale = query.shape[-1] ** -0.5 if scaling is None else scaling
-    return dz_shared.attend(module, query, key, value, scale), None
+    return dz_shared.attend(layer, query, key, value, scale), None
+
+
+def _check_model(model) -> None:
+    config = model.config
+    if not getattr(model, "_supports_attention_backend", False):
+        raise DzError(f"shared_prompt: {type(model).__name__} does not call an attention that HF registers by name")
+    for name in ("final_logit_softcapping", "logit_scale", "logits_scaling", "output_multiplier_scale"):
+        if getattr(config, name, None) not in (None, 1, 1.0):
+            raise DzError(f"shared_prompt: a model with {name}")
 
 
 def _hidden(model, input_ids: torch.Tensor, position_ids: torch.Tensor, layout) -> torch.Tensor:
@@ -100,11 +121,15 @@ def _hidden(model, input_ids: torch.Tensor, position_ids: torch.Tensor, layout) 
     config = model.config
     before = config._attn_implementation
     config._attn_implementation = ATTN_IMPL
+    layout.seen.clear()
     try:
-        return model.base_model(input_ids=input_ids, position_ids=position_ids, attention_mask=None, use_cache=False,
-                                dz_shared=layout).last_hidden_state
+        hidden = model.base_model(input_ids=input_ids, position_ids=position_ids, attention_mask=None, use_cache=False,
+                                  dz_shared=layout).last_hidden_state
     finally:
         config._attn_implementation = before
+    if len(layout.seen) != config.num_hidden_layers:
+        raise DzError(f"shared_prompt: {len(layout.seen)} of {config.num_hidden_layers} layers called the attention")
+    return hidden
 
 
 def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], option_len, candidates: int,
@@ -121,6 +146,7 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     sequences, length = input_ids.shape
     if candidates < 1 or sequences % candidates or len(option_len) != sequences or not 1 <= min(option_len) <= max(option_len) < length:
         raise DzError(f"shared_prompt_logprobs: {sequences} sequences of {length} tokens, {candidates} candidates each, option_len {list(option_len)[:8]}")
+    _check_model(model)
     device, examples, most = input_ids.device, sequences // candidates, max(option_len)
     room, each = length - min(option_len), most - 1
     options = torch.as_tensor(option_len, device=device)
@@ -140,7 +166,7 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     steps = (first.unsqueeze(1) + last[:each]).repeat(1, candidates)
     positions = torch.cat([place.expand(examples, room), steps], 1)
     # (places that hold no token of a sequence repeat one, and nothing that is read sees them)
-    positions = positions.clamp_(max=length - 1)
+    positions = positions.clamp_(0, length - 1)
 
     hidden = _hidden(model, ids, positions, _Candidates(room, candidates, each, first.to(torch.int32)))
     width = hidden.shape[-1]
@@ -175,14 +201,30 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, answers: in
         prompt_lengths = torch.full((prompts,), room, dtype=torch.int32, device=device)
     elif prompt_lengths.shape != (prompts,) or prompt_lengths.dtype != torch.int32:
         raise DzError(f"generate: prompt_lengths must be torch.int32 ({prompts},), got {prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
+    if uniform is not None and uniform.shape != (prompts, answers, max_new_tokens):
+        raise DzError(f"generate: uniform must be {(prompts, answers, max_new_tokens)}, got {tuple(uniform.shape)}")
+    _check_model(model)
+    most = getattr(model.config, "max_position_embeddings", None)
+    if most is not None and room + max_new_tokens - 1 > most:  # (an answer's last token is not read again)
+        raise DzError(f"generate: {room} tokens of a prompt and {max_new_tokens} new ones, the model has {most} positions")
+    lengths = prompt_lengths.clamp(1, room)
     if uniform is None:
         uniform = torch.rand(prompts, answers, max_new_tokens, generator=generator, device=device)
-    elif uniform.shape != (prompts, answers, max_new_tokens):
-        raise DzError(f"generate: uniform must be {(prompts, answers, max_new_tokens)}, got {tuple(uniform.shape)}")
-    lengths = prompt_lengths.clamp(1, room)
+    training = model.training
     model.eval()
+    try:
+        return _draw(model, input_ids, max_new_tokens, answers, lengths, uniform, eos_token_id, kv_bits,
+                     dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
+    finally:
+        if training:
+            model.train()
+
+
+def _draw(model, input_ids, max_new_tokens, answers, lengths, uniform, eos_token_id, kv_bits, sampling) -> torch.Tensor:
+    prompts, room = input_ids.shape
+    device = input_ids.device
     with torch.no_grad():
-        layout = _Answers(prompts, answers, max_new_tokens, lengths, kv_bits)
+        layout = _Answers(prompts, answers, room, max_new_tokens, lengths, kv_bits)
         hidden = _hidden(model, input_ids, torch.arange(room, device=device).expand(prompts, room), layout)
         rows = hidden.gather(1, (lengths.long() - 1).view(prompts, 1, 1).expand(prompts, 1, hidden.shape[-1]))
         rows = rows.expand(prompts, answers, rows.shape[-1])
@@ -190,7 +232,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, answers: in
         ended = None
         for t in range(max_new_tokens):
             logits = model.get_output_embeddings()(rows)
-            drawn = sample_tokens(logits, uniform[:, :, t], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            drawn = sample_tokens(logits, uniform[:, :, t], **sampling)
             if eos_token_id is not None:
                 drawn = drawn if ended is None else torch.where(ended, eos_token_id, drawn)
                 ended = drawn == eos_token_id

@@ -150,3 +150,69 @@ def test_logprobs_refuse():
         for lens, n in (([1, 1], 3), ([4, 1], 2), ([0, 1], 2), ([1], 2)):
             with pytest.raises(DzError):
                 S.shared_prompt_logprobs(None, torch.zeros(2, 4, dtype=torch.long), None, lens, n, PAD)
+
+
+def test_prompts_without_a_token_of_their_own(plain):
+    """An option as long as the sequence, and one that reaches into the padding: no answer, and no position outside of the model's."""
+    b = batch(4, 2, 2, [5], 16)
+    b["attention_mask"][:2] = 0
+    b["attention_mask"][0, 11:] = 1  # five tokens, all of the option
+    b["attention_mask"][1, 11:] = 1
+    b["attention_mask"][2:] = 0  # none
+    with torch.no_grad():
+        got = S.shared_prompt_logprobs(tiny("opt"), b["input_ids"], b["attention_mask"], [5] * 4, 2, PAD)
+    assert torch.isnan(got).all()
+
+
+def refused(model, match, **how):
+    ids = torch.randint(2, 211, (2, 12), generator=torch.Generator().manual_seed(3))
+    with pytest.raises(DzError, match=match):
+        S.generate(model, ids, 3, **how)
+    with pytest.raises(DzError, match=match), torch.no_grad():
+        S.shared_prompt_logprobs(model, ids, None, [2, 2], 2, PAD)
+
+
+def other(kind, **how):
+    import transformers
+
+    small = dict(vocab_size=211, hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, intermediate_size=96, head_dim=16,
+                 max_position_embeddings=80, pad_token_id=PAD)
+    return getattr(transformers, kind + "ForCausalLM")(getattr(transformers, kind + "Config")(**small, **how)).eval()
+
+
+def test_models_of_other_attention_are_refused(plain):
+    from transformers import BloomConfig, BloomForCausalLM
+
+    refused(BloomForCausalLM(BloomConfig(vocab_size=211, hidden_size=64, n_layer=2, n_head=4)), "by name")
+    refused(other("Mistral", sliding_window=4), "window")
+    refused(other("Gemma2", final_logit_softcapping=None), "soft cap")
+    refused(other("Gemma2", attn_logit_softcapping=None), "final_logit_softcapping")
+    model = tiny("llama")
+    model.config.num_hidden_layers = 4  # as if a layer mixed tokens in another way
+    refused(model, "3 of 4 layers")
+    model = tiny("llama")
+    model.model.layers[1].self_attn.layer_idx = 0
+    refused(model, "layer_idx")
+
+
+def test_a_window_that_holds_all_tokens_is_none(plain):
+    model = other("Mistral", sliding_window=64)
+    ids = torch.randint(2, 211, (1, 7), generator=torch.Generator().manual_seed(4))
+    assert torch.equal(S.generate(model, ids, 4, temperature=0.0)[0, 0], greedy(model, ids[0], 4))
+
+
+def test_answers_end_with_the_models_positions(plain):
+    model = tiny("opt")  # of 80 positions
+    ids = torch.randint(2, 211, (1, 75), generator=torch.Generator().manual_seed(5))
+    assert S.generate(model, ids, 6, temperature=0.0).shape == (1, 1, 6)
+    with pytest.raises(DzError, match="positions"):
+        S.generate(model, ids, 7, temperature=0.0)
+
+
+def test_a_model_in_training_stays_there(plain):
+    model = tiny("opt")
+    model.train()
+    model.config.dropout = model.config.attention_dropout = 0.0
+    ids = torch.randint(2, 211, (1, 5), generator=torch.Generator().manual_seed(6))
+    S.generate(model, ids, 2, temperature=0.0)
+    assert model.training and all(m.training for m in model.modules())
