@@ -16,6 +16,7 @@ stream are the caller's to order, as with torch's own operators. Calls may be ca
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 from typing import NamedTuple, Optional, Union
 
@@ -74,6 +75,13 @@ def _rows(t: torch.Tensor):
         t = t.clone(memory_format=torch.contiguous_format)
         s = t.stride()[:-1]
     return t, s
+
+
+def _whole(what: str, name: str, x) -> int:
+    try:
+        return operator.index(x)
+    except TypeError:
+        _fail(what, f"{name} must be an integer, got {type(x).__name__}")
 
 
 def _check_operands(what: str, index: int, tensors) -> None:
@@ -253,7 +261,7 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, positions:
     if torch.is_tensor(positions):
         at = _check_int32(what, "positions", positions, shape[:n], index)
     else:
-        position = positions
+        position = _whole(what, "positions", positions)
     if not k.numel():
         return
     if n > 1:
@@ -273,6 +281,7 @@ def cache_read(cache: QuantizedKV, length: int, dtype: torch.dtype, start: int =
     shape = cache.k.shape
     heads, slots, width = shape[n:]
     code = dtype_code(dtype)
+    length, start = _whole(what, "length", length), _whole(what, "start", start)
     if length < 0 or start < 0 or start + length > slots:
         _fail(what, f"slots {start} to {start + length} of {slots}")
     k, v = (torch.empty((*shape[:-2], length, width), dtype=dtype, device=cache.k.device) for _ in range(2))

@@ -7,6 +7,7 @@ device; calls may be captured in a graph.
 """
 from __future__ import annotations
 
+import operator
 from typing import Union
 
 import torch
@@ -20,7 +21,10 @@ MAX_VOCAB = 1 << 20
 def _parameter(what: str, name: str, value, lead, device, dtype):
     """(the number for all rows, the tensor of one for each)"""
     if not torch.is_tensor(value):
-        return value, None
+        try:
+            return (operator.index if dtype == torch.int32 else float)(value), None
+        except (TypeError, ValueError):
+            _fail(what, f"{name} must be a number or a tensor of one for each row, got {value!r}")
     _check_rows(what, name, value, lead, device, (dtype,))
     return 0, _dense(value)
 
