@@ -95,7 +95,7 @@ __device__ __forceinline__ uint32_t own_keys(const Attend& a, uint32_t g, uint32
 __device__ __forceinline__ uint32_t prefix_keys(const Attend& a, uint32_t g) {
   if (!a.prefix_slots) return 0;
   const int32_t l = a.prefix_lengths ? a.prefix_lengths[g] : a.prefix_slots;
-  return __builtin_amdgcn_readfirstlane(l < 0 ? 0 : l > a.prefix_slots ? a.prefix_slots : l);
+  return l < 0 ? 0 : l > a.prefix_slots ? a.prefix_slots : l;
 }
 
 // The rows first + (each set bit) of the workgroup's tile by themselves, one after another. Where they are and what they see
@@ -113,7 +113,7 @@ __device__ __forceinline__ void lone_rows(uint32_t first, uint32_t set) {
   if (!item_of(a, plan, item)) return;
   const uint32_t lane = threadIdx.x & 63, g = item.g, shared = a.heads / a.kv_heads, seq_rows = (uint32_t)a.length * shared;
   const uint32_t row0 = tile_rows_of(plan, item.tile, seq_rows, seq_rows * a.sequences).row0, n0 = row0 / seq_rows;
-  const uint32_t prefix_limit = prefix_keys(a, g), prefix_tiles = (prefix_limit + KT - 1) / KT;
+  const uint32_t prefix_limit = __builtin_amdgcn_readfirstlane(prefix_keys(a, g)), prefix_tiles = (prefix_limit + KT - 1) / KT;
   auto mine = [&](uint32_t tile) { return (BY_KEYS ? tile / WAVES : tile) % item.splits == item.split; };
 #pragma unroll 1
   for (; set; set &= set - 1) {
@@ -136,7 +136,7 @@ __device__ __forceinline__ void lone_rows(uint32_t first, uint32_t set) {
       const uint32_t col = lane + 64 * i;
       if (col >= (uint32_t)a.width) continue;
       if (item.splits > 1) call.partial[to_row * a.width + col] = x.o[i];
-      else to[col] = (Elem)(x.l == 0.f ? 0.f : x.o[i] / x.l);
+      else to[col] = (Elem)(prefix_limit + limit == 0 ? 0.f : x.o[i] / x.l);
     }
   }
 }
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   const TileRows tr = tile_rows_of(plan, item.tile, seq_rows, all_rows);
   const uint32_t row0 = tr.row0, rows = tr.rows;
   const uint32_t n0 = row0 / seq_rows, nseq = (row0 + rows - 1) / seq_rows - n0 + 1;
-  const uint32_t prefix_limit = prefix_keys(a, g);
+  const uint32_t prefix_limit = __builtin_amdgcn_readfirstlane(prefix_keys(a, g));
   // Where a part's keys and values are: the prompt, or one sequence's own.
   struct Source {
     const char *k, *v;
@@ -591,7 +591,8 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
       }
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  // (a query all of whose keys score -inf has no answer: 0 / 0)
+  const float inv = prefix_limit + own_limit == 0 ? 0.f : 1.f / l;
   Elem* to = (Elem*)a.out + (int64_t)g * a.out_s[0] + (int64_t)n_row * a.out_s[1] + (int64_t)h_row * a.out_s[2] + (int64_t)t_row * a.out_s[3];
   typedef Elem Quad __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -628,8 +629,8 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, AttendPlan plan, co
     l = __builtin_fmaf(ms.y, f, l);
     o += x * f;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   const uint32_t gh = item / plan.tiles, row = t.row0 + lane_row, g = gh / a.kv_heads, h = gh % a.kv_heads * shared + row % shared;
+  const float inv = prefix_keys(a, g) + own_keys(a, g, row / seq_rows, row % seq_rows / shared) == 0 ? 0.f : 1.f / l;
   typedef Elem Quad __attribute__((ext_vector_type(4)));
   *(Quad*)((Elem*)a.out + (int64_t)g * a.out_s[0] + (int64_t)(row / seq_rows) * a.out_s[1] + (int64_t)h * a.out_s[2] +
            (int64_t)(row % seq_rows / shared) * a.out_s[3] + col) = Quad{(Elem)(o[0] * inv), (Elem)(o[1] * inv), (Elem)(o[2] * inv), (Elem)(o[3] * inv)};

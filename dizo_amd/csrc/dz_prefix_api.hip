@@ -128,7 +128,7 @@ int32_t plan_of(const dz_attention* x, dz::Attend* a, dz::AttendPlan* plan) {
   DZ_TRY(check_dim(x->prefix_slots, 0, "prefix_slots"));
   if (x->heads % x->kv_heads) return invalid("heads (" + std::to_string(x->heads) + ") is not a multiple of kv_heads (" + std::to_string(x->kv_heads) + ")");
   if (x->width < 8 || x->width > 128 || x->width % 8) return invalid("width must be a multiple of 8 up to 128, got " + std::to_string(x->width));
-  if (!(x->scale > 0.f) || !isfinite(x->scale)) return invalid("scale must be positive and finite");
+  if (!(x->scale > 0.f && x->scale <= 0x1p126f)) return invalid("scale must be positive, 2^126 at most");  // (with log2 e it is finite)
   int64_t rows = 1;
   for (int64_t d : {x->groups, x->sequences, x->heads, x->length}) {
     if (d && rows > kMaxRows / d) return invalid("too many queries: " + std::to_string(kMaxRows) + " at most");

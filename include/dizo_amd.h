@@ -325,7 +325,7 @@ typedef struct dz_attention {
   const int32_t* prefix_lengths; /* (groups), dense; NULL: prefix_slots */
   int64_t groups, sequences, heads, kv_heads, length, width, slots, prefix_slots;
   int32_t dtype;
-  float scale; /* positive and finite */
+  float scale; /* positive, 2^126 at most */
 } dz_attention;
 
 /* `workspace` is device memory (16-byte aligned) of at least the bytes that the

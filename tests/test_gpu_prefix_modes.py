@@ -235,3 +235,58 @@ def test_what_is_not_finite_reaches_those_that_see_it(shape, dtype, bits):
         every = slice(None)
         assert torch.isnan(attend(math.nan, every, own.v)).all()
         assert torch.isnan(attend(math.inf, every, own.k)).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("shape", [
+    (1, 3, 40, 1, 1, 20, 70, 64),   # 40 rows of one token
+    (2, 2, 160, 1, 1, 9, 33, 80),   # 160: two tiles
+    (1, 2, 36, 1, 5, 7, 600, 128),  # tiles that end inside of a token's heads
+], ids=str)
+def test_many_query_heads_of_one_key_head(shape, bits):
+    q, own, pre = inputs(12, "bf16", *shape, bits=bits)
+    check("bf16", q, own, pre)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(1, 3, 2, 1, 2, 30, 0, 72), (1, 2, 2, 2, 40, 60, 0, 64), (1, 3, 2, 1, 2, 30, 1500, 104)], ids=str)
+def test_scores_of_minus_infinity(shape, dtype):
+    q, own, pre = inputs(13, dtype, *shape)
+    q = q.abs() + 0.125
+    prefix = shape[6]
+
+    def is_value(got, v):
+        """Where one key is left, with a score s: its weight is w = 2^x, x what is lost as s log2(e) scale is rounded, and the answer
+        (w v) (1 / w) with three roundings in fp32, of 2^-24 each. Rounded to 16 bits that is v; w is 1 in 16 bits."""
+        v = v.unsqueeze(1).repeat_interleave(shape[2] // shape[3], 0).expand_as(got)
+        return ((got - v).abs() <= (4 * 2.0**-24 if dtype == "fp32" else 0) * v.abs()).all()
+
+    want = P.shared_prefix_attention(q, own, pre)
+    held = own.k[0, 0].clone()
+    own.k[0, 0] = -math.inf
+    if prefix:
+        pre.k[0] = -math.inf
+        assert torch.isnan(P.shared_prefix_attention(q, own, pre)[0, 0]).all()  # 0 / 0
+        pre.k[0, :, 700] = 0.0
+        got = P.shared_prefix_attention(q, own, pre)
+        assert is_value(got[0, 0], pre.v[0, :, 700])
+        return
+    got = P.shared_prefix_attention(q, own, None)
+    assert torch.isnan(got[0, 0]).all()
+    assert torch.equal(got[0, 1:], want[0, 1:])
+    own.k[0, 0, :, 3] = held[:, 3]
+    got = P.shared_prefix_attention(q, own, None)
+    assert is_value(got[0, 0], own.v[0, 0, :, 3])
+
+
+def test_numbers_of_other_types():
+    cache = P.QuantizedKV.empty(2, 1, 8, 16, device=DEV)
+    x = torch.randn(2, 1, 1, 16, device=DEV)
+    P.cache_write(cache, x, x, np.int64(3))
+    assert torch.equal(P.cache_read(cache, np.int32(1), torch.float32, start=np.int64(3)).k, P.cache_read(cache, 1, torch.float32, start=3).k)
+    logits, u = torch.randn(2, 50, device=DEV), torch.rand(2, device=DEV)
+    assert torch.equal(sample_tokens(logits, u, top_k=np.int64(4), temperature=np.float32(0.5)), sample_tokens(logits, u, top_k=4, temperature=0.5))
+    for call in (lambda: P.cache_write(cache, x, x, 1.5), lambda: P.cache_read(cache, 1.0, torch.float32), lambda: P.cache_read(cache, 1, torch.float32, start=None),
+                 lambda: sample_tokens(logits, u, top_k=2.5), lambda: sample_tokens(logits, u, temperature="one"), lambda: sample_tokens(logits, u, top_p=None)):
+        with pytest.raises(DzError, match="must be"):
+            call()
