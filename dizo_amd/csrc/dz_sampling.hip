@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kBins = 2048;
 constexpr int kPowers = 1024;
+constexpr int kBinBits = 5;  // a bin is 2^kBinBits places: 32 bins for each power of two, 48 of which a weight can have
 constexpr int kHeldBytes = 128 * 1024;  // of a row in LDS
 constexpr uint32_t kShortRow = 8192;
 
@@ -34,13 +35,14 @@ struct Shared {
     uint64_t list[kList];
   };
   uint64_t pieces[PIECES];  // sums of a wave's part of a slab
-  double powers[kPowers];  // 2^(i / kPowers)
+  double powers[kPowers];  // 2^(i / kPowers - 2)
   uint64_t wave_sum[kWaves];
   float wave_max[kWaves];
   uint32_t wave_flag[kWaves];
   uint64_t found_before;
   uint64_t cut;
   uint32_t found, low, high, listed;
+  uint32_t edge[2];  // logits between which something lies, as keys
 };
 
 // fp32 numbers as whole ones of the same order. (-0 equals 0.)
@@ -50,7 +52,8 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// Sums up to and with this lane: of 24, 24 and 16 bits each, whose sums over 64 lanes fit 32.
+// Sums up to and with this lane: of 24, 24 and 16 bits each, whose sums over 64 lanes fit 32. SHORT: of numbers up to 2^49 (8 weights),
+// of 24 and 25 bits.
 __device__ __forceinline__ uint32_t wave_scan_part(uint32_t x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // the lane before, of 16
   x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
@@ -60,8 +63,11 @@ __device__ __forceinline__ uint32_t wave_scan_part(uint32_t x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
   return x;
 }
+template <bool SHORT>
 __device__ __forceinline__ uint64_t wave_scan(uint64_t x) {
-  const uint32_t low = wave_scan_part((uint32_t)x & 0xffffff), middle = wave_scan_part((uint32_t)(x >> 24) & 0xffffff), high = wave_scan_part((uint32_t)(x >> 48));
+  const uint32_t low = wave_scan_part((uint32_t)x & 0xffffff);
+  if (SHORT) return low + ((uint64_t)wave_scan_part((uint32_t)(x >> 24)) << 24);
+  const uint32_t middle = wave_scan_part((uint32_t)(x >> 24) & 0xffffff), high = wave_scan_part((uint32_t)(x >> 48));
   return low + ((uint64_t)middle << 24) + ((uint64_t)high << 48);
 }
 
@@ -69,7 +75,7 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t x) {
 template <class Sh>
 __device__ __forceinline__ uint64_t block_scan(Sh& sh, uint64_t x, uint64_t& all) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  x = wave_scan(x);
+  x = wave_scan<false>(x);
   __syncthreads();
   if (lane == 63) sh.wave_sum[wave] = x;
   __syncthreads();
@@ -171,7 +177,7 @@ struct Row {
         if (s0 + i < slabs) {
           if (HELD) held[(s0 + i) * kThreads + threadIdx.x] = e[i];
 #pragma unroll
-          for (int j = 0; j < PER; ++j) f((float)e[i][j]);
+          for (int j = 0; j < PER; j += 2) f((float)e[i][j], (float)e[i][j + 1]);
         }
     }
   }
@@ -219,14 +225,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   const int32_t top_k = temperature == 0 ? 1 : a.top_ks ? a.top_ks[r] : a.top_k;
   const double unit = temperature == 0 ? 1.0 : temperature;
 
-  for (int i = tid; i < kPowers; i += kThreads) sh.powers[i] = exp2(i / (double)kPowers);
+  for (int i = tid; i < kPowers; i += kThreads) sh.powers[i] = exp2(i / (double)kPowers - 2.0);
   for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
   if (tid == 0) sh.listed = 0;
   bool none = !(u >= 0.f && u <= 1.f) || !(temperature == 0 || (temperature >= 0x1p-63 && temperature < 0x1p64)) || top_p != top_p || min_p != min_p;
   float mine = -INFINITY;  // the largest of this thread's
-  row.first([&](float x) {
-    mine = fmaxf(mine, x);
-    none |= x != x;
+  row.first([&](float x, float y) {
+    mine = fmaxf(fmaxf(mine, x), y);
+    none |= __builtin_isunordered(x, y);
   });
   float m = mine;
 #pragma unroll
@@ -255,44 +261,72 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   // place n + f gives 2^(n / 1024 - 2) 2^(f / 1024), by a table, and by Taylor's polynomial (the next term is under 2^-46.6 of
   // it). Places are exact to 2^-38, which moves a weight by 2^-48 of it.
   const int lg = 32 - __clz((a.vocab - 1) | 1), shift = 62 - lg < 46 ? 62 - lg : 46;
+  constexpr double kLn = 0x1.62e42fefa39efp-11;  // ln 2 / 1024
   const double per = kPowers * 1.4426950408889634074 / unit, wide_m = m, most = kPowers * (double)(shift + 2);
   auto place_of = [&](float x) { return fmax(__builtin_fma((double)x - wide_m, per, most), 0.0); };
   auto weight_at = [&](double place) -> uint64_t {
-    constexpr double kLn = 0x1.62e42fefa39efp-11;  // ln 2 / 1024
     const uint32_t n = (uint32_t)place;
     const double f = __builtin_amdgcn_fract(place);
     double p = __builtin_fma(f, kLn * kLn * kLn / 6, kLn * kLn / 2);
     p = __builtin_fma(f, p, kLn) * f;
     const double w = sh.powers[n % kPowers], y = __builtin_fma(w, p, w);
-    const double scaled = __longlong_as_double(__double_as_longlong(y) + ((int64_t)((int32_t)(n / kPowers) - 2) << 52));
+    const double scaled = __hiloint2double(__double2hiint(y) + (int32_t)(n / kPowers << 20), __double2loint(y));
     return (uint64_t)__double_as_longlong(scaled + 0x1p52) & 0xfffffffffffffull;
   };
   auto weight = [&](float x) -> uint64_t { return weight_at(place_of(x)); };
-  // min_p as the place that is reached by what it keeps; the largest is always kept
+  // The least number (as a key) whose place reaches `place`; the largest logit's does. A wave at a time: by the place's inverse, to within a
+// few numbers where their steps are not too small for it, and otherwise in 64ths of what is left.
+  auto least_reaching = [&](double place) -> uint32_t {
+    auto reaches = [&](uint32_t k) { return place_of(of_key(k)) >= place; };
+    uint32_t low = key_of(-INFINITY), high = key_of(m);
+    if (!(place > 0.0)) return low;
+    const uint32_t near = key_of((float)__builtin_fma((place - most) * kLn, unit, wide_m));
+    uint32_t k = near - 32 + lane;
+    uint64_t reached = __ballot(k < low ? false : k > high ? true : reaches(k));
+    if (reached >> 63 && !(reached & 1)) return near - 32 + __builtin_ctzll(reached);
+    while (low < high) {
+      const uint32_t step = (high - low) / 64 + 1;
+      k = lane < (high - low) / step ? low + lane * step : high;
+      reached = __ballot(reaches(k));
+      const uint32_t first = __builtin_ctzll(reached);  // (high reaches it)
+      high = __builtin_amdgcn_readlane(k, first);
+      if (first) low = __builtin_amdgcn_readlane(k, first - 1) + 1;
+      if (!first) break;
+    }
+    return high;
+  };
+  // min_p as the least logit that it keeps; the largest is always kept
   const double least_place = min_p > 0 ? kPowers * (fmin(log2(min_p), 0.0) + (shift + 2)) : 0.0;
 
   auto clear = [&]() {
     for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
   };
   auto add_to = [&](uint32_t bin, uint64_t value) { atomicAdd((unsigned long long*)&sh.bins[bin], (unsigned long long)value); };
-  // Bins by the distance to the largest: 64 a unit of the logits over the temperature, the last one what is further away.
-  const float per_unit = (float)(64.0 / unit);
-  auto bin_of = [&](float x) {
-    const float d = (m - x) * per_unit;
-    return d < (float)(kBins - 1) ? (uint32_t)d : (uint32_t)kBins - 1;
-  };
-  // Logits (above -inf) that `take` takes, one a thread and sorted; the others are 0 (of no order). How many: more than kList if they
-  // do not fit, and nothing then.
+  // Bins by the distance to the largest in places.
+  const uint32_t top_place = (uint32_t)most;
+  auto bin_of = [&](float x) { return (top_place - (uint32_t)place_of(x)) >> kBinBits; };
+  // The least logit of a bin, as a key.
+  auto least_of = [&](uint32_t bin) { return least_reaching((double)top_place - (double)((bin << kBinBits) + (1 << kBinBits) - 1)); };
+  // Logits (above -inf) from `from` to below `below` of an order of `least` or above, one a thread and sorted; the others are 0 (of no
+  // order). How many: more than kList if they do not fit, and nothing then.
   uint64_t e;
   auto weight_of = [&](uint64_t order) -> uint64_t { return order ? weight(of_key((uint32_t)(order >> 32))) : 0; };
-  auto list = [&](auto take) -> uint32_t {
+  auto list = [&](float from, float below, uint64_t least) -> uint32_t {
     __syncthreads();
     if (tid == 0) sh.listed = 0;
     __syncthreads();
-    row.each([&](float x, uint32_t token) {
-      if (take(x, token) && x != -INFINITY) {
+    row.slabs_do([&](uint32_t, const float(&v)[PER], uint32_t token) {
+      bool some = false;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) some |= v[j] >= from && v[j] < below;
+      if (!some) return;  // (nearly all)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (!(v[j] >= from && v[j] < below) || v[j] == -INFINITY) continue;
+        const uint64_t order = order_of(key_of(v[j]), token + j);
+        if (order < least) continue;
         const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kList) sh.list[at] = order_of(key_of(x), token);
+        if (at < kList) sh.list[at] = order;
       }
     });
     __syncthreads();
@@ -312,13 +346,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     const uint32_t bin = sh.found;
     uint64_t before = sh.found_before;
     if (bin == kBins) return least;
-    // (bin_of in as few operations as it takes: nearly all logits lie elsewhere)
-    const float from = (float)bin, to = bin == kBins - 1 ? NAN : (float)(bin + 1);
-    auto in_bin = [&](float x) {
-      const float d = (m - x) * per_unit;
-      return d >= from && !(d >= to);
-    };
-    if (list([&](float x, uint32_t token) { return in_bin(x) && order_of(key_of(x), token) >= least; }) <= kList) {
+    if (wave < 2) {
+      const uint32_t k = wave == 0 ? least_of(bin) : bin ? least_of(bin - 1) : key_of(INFINITY);
+      if (lane == 0) sh.edge[wave] = k;
+    }
+    __syncthreads();
+    const float from = of_key(sh.edge[0]), below = of_key(sh.edge[1]);
+    auto in_bin = [&](float x) { return x >= from && x < below; };
+    if (list(from, below, least) <= kList) {
       uint64_t all;
       const uint64_t v = counts ? e != 0 : weight_of(e), upto = block_scan(sh, v, all);
       if (before + upto - v < target && before + upto >= target) sh.cut = e;
@@ -370,7 +405,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
       uint64_t n = 0;
 #pragma unroll
       for (int j = 0; j < PER; ++j) n += is_equal(v[j], at + j);
-      n = wave_scan(n);
+      n = wave_scan<true>(n);
       if (lane == 63) sh.pieces[s * kWaves + wave] = n;
     });
     __syncthreads();
@@ -381,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
         uint64_t n = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) n += is_equal(v[j], at + j);
-        uint64_t upto = sh.found_before + wave_scan(n) - n;
+        uint64_t upto = sh.found_before + wave_scan<true>(n) - n;
 #pragma unroll
         for (int j = 0; j < PER; ++j)
           if (is_equal(v[j], at + j) && ++upto == nth) sh.cut = order_of(low, at + j);
@@ -390,13 +425,25 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     __syncthreads();
     return sh.cut;
   };
-  // An order as a logit and the token after the last one of those that equal it: what is not below it is compared as it stands.
-  struct Border {
-    float x;
+  // What is not below an order, nor below a logit: of tokens before `end` what reaches `from`, of later ones what reaches `after`.
+  struct Kept {
+    float cut, from, after;
     uint32_t end;
   };
-  auto border_of = [](uint64_t order) { return order ? Border{of_key((uint32_t)(order >> 32)), token_of(order) + 1} : Border{-INFINITY, 0}; };
-  auto not_below = [](const Border& b, float x, uint32_t token) { return x > b.x || (x == b.x && token < b.end); };
+  auto kept_of = [](uint64_t order, float least) {
+    if (!order) return Kept{-INFINITY, least, least, 0};
+    const uint32_t key = (uint32_t)(order >> 32);
+    return Kept{of_key(key), fmaxf(of_key(key), least), fmaxf(of_key(key + 1), least), token_of(order) + 1};
+  };
+  // For a vector of logits, which of them the two are.
+  auto bound = [&](const Kept& k, float(&v)[PER], uint32_t at) {
+    if (at < k.end && at + PER > k.end) {  // (one vector of the row)
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (at + j >= k.end && v[j] == k.cut) v[j] = -INFINITY;
+    }
+    return at < k.end ? k.from : k.after;
+  };
   // What top-p keeps of a sum: whole numbers that have to be reached.
   auto share_of = [&](uint64_t total) -> uint64_t {
     const double share = __builtin_ceil(top_p * (double)total);
@@ -417,8 +464,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
       __syncthreads();
       find(sh, sh.bins, kBins, top_k);
       last_bin = sh.found;
+      const uint32_t k = last_bin < kBins && wave == 0 ? least_of(last_bin) : key_of(-INFINITY);
+      if (tid == 0) sh.edge[0] = k;
+      __syncthreads();
     }
-    const uint32_t n = top_k <= kThreads ? list([&](float x, uint32_t) { return bin_of(x) <= last_bin; }) : kList + 1;
+    const uint32_t n = top_k <= kThreads ? list(of_key(sh.edge[0]), INFINITY, 0) : kList + 1;
     if (n <= kList) {
       // All that matters is in the list, sorted: what is kept is its beginning.
       uint64_t total, sum;
@@ -448,14 +498,23 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     __syncthreads();
   }
   if (top_p < 1.0) {
-    const Border border = border_of(cut);
+    const Kept kept = kept_of(cut, -INFINITY);
     row.slabs_do([&](uint32_t, const float(&v)[PER], uint32_t at) {
-      uint64_t w[PER];
+      float x[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) w[j] = weight(v[j]);
+      for (int j = 0; j < PER; ++j) x[j] = v[j];
+      const float from = bound(kept, x, at);
+      uint64_t w[PER];
+      uint32_t bin[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const double place = place_of(x[j]);
+        w[j] = weight_at(place);
+        bin[j] = (top_place - (uint32_t)place) >> kBinBits;
+      }
 #pragma unroll
       for (int j = 0; j < PER; ++j)
-        if (w[j] && not_below(border, v[j], at + j)) add_to(bin_of(v[j]), w[j]);
+        if (w[j] && x[j] >= from) add_to(bin[j], w[j]);
     });
     __syncthreads();
     uint64_t sum = 0, total;
@@ -465,21 +524,39 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   }
 
   // What is kept of each piece of the row, and the piece and token that u falls on.
-  const Border border = border_of(cut);
-  auto kept = [&](float x, uint32_t token) -> uint64_t {
-    const double place = place_of(x);
-    const uint64_t w = weight_at(place);
-    return place >= least_place && not_below(border, x, token) ? w : 0;
+  if (wave == 0) {
+    const uint32_t k = least_reaching(least_place);
+    if (lane == 0) sh.edge[0] = k;
+  }
+  __syncthreads();
+  const Kept kept = kept_of(cut, of_key(sh.edge[0]));
+  auto kept_weights = [&](const float(&v)[PER], uint32_t at, uint64_t(&w)[PER]) {
+    float x[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = v[j];
+    const float from = bound(kept, x, at);
+    bool some = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      some |= x[j] >= from;
+      w[j] = 0;
+    }
+    if (!some) return;  // (where little is kept, all of most waves')
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t one = weight(x[j]);
+      w[j] = x[j] >= from ? one : 0;
+    }
   };
   const uint32_t pieces = row.slabs * kWaves;
   uint64_t all = 0, sum;
-  __syncthreads();
   row.slabs_do([&](uint32_t s, const float(&v)[PER], uint32_t at) {
-    uint64_t n = 0;
+    uint64_t w[PER], n = 0;
+    kept_weights(v, at, w);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) n += kept(v[j], at + j);
+    for (int j = 0; j < PER; ++j) n += w[j];
     all += n;
-    n = wave_scan(n);
+    n = wave_scan<true>(n);
     if (lane == 63 && s < row.slabs) sh.pieces[s * kWaves + wave] = n;
   });
   block_scan(sh, all, sum);
@@ -489,9 +566,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   if (piece < pieces && wave == piece % kWaves) {
     row.slab(piece / kWaves, [&](const float(&v)[PER], uint32_t at) {
       uint64_t w[PER], n = 0;
+      kept_weights(v, at, w);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) n += w[j] = kept(v[j], at + j);
-      uint64_t before = sh.found_before + wave_scan(n) - n;
+      for (int j = 0; j < PER; ++j) n += w[j];
+      uint64_t before = sh.found_before + wave_scan<true>(n) - n;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         if (before < target && before + w[j] >= target) a.tokens[r] = at + j;
