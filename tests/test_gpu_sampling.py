@@ -95,3 +95,29 @@ def test_frequencies():
     got = sample_tokens(x.expand(n, 5), (torch.arange(n, device=DEV) + 0.5) / n)
     p = torch.softmax(x.double(), 0) * n
     assert ((torch.bincount(got, minlength=5).double() - p).abs() <= 1).all()
+
+
+@pytest.mark.parametrize("how", [dict(top_p=0.3), dict(top_p=0.75, top_k=1500), dict(min_p=0.03), dict(top_k=700), dict(top_k=1200, top_p=0.5)], ids=str)
+def test_logits_around_zero_where_numbers_lie_close(how):
+    """A row's largest is 1 and nearly all of the others are within 1e-5 of 0: a bin's end is 1 - (32 n + 31) T ln 2 / 1024, at 0 to
+    within 1e-16 by the temperature, where fp32 has more numbers than a search of the nearest ones covers."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(8)
+    e = torch.rand(4, 3001, generator=g, device=DEV) * 35 - 40
+    x = torch.pow(10.0, e) * torch.where(torch.rand(4, 3001, generator=g, device=DEV) < 0.5, -1.0, 1.0)
+    x[:, ::5] = 0.0
+    x[:, 17] = 1.0
+    u = torch.tensor([0.1, 0.4, 0.7, 0.95], device=DEV)
+    for n in (3, 10, 11):
+        check(x, u, temperature=1024 / ((32 * n + 31) * math.log(2)), **how)
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e-3, 1e4, 1e19, 3e38])
+@pytest.mark.parametrize("how", [dict(), dict(top_p=0.6), dict(top_k=40, top_p=0.9), dict(top_k=2000), dict(min_p=0.2)], ids=str)
+def test_logits_of_any_size(scale, how):
+    x, u = rows_of(9, 4, 2500, "fp32", std=1.0)
+    x = (x / 5).clamp(-1, 1) * scale
+    for t in (0.05, 1.0, 30.0):
+        if 2.0**-63 <= t * scale < 2.0**64:
+            check(x, u, temperature=t * scale, **how)
+    check(x[:1], u[:1], temperature=1.0, **how)  # all alike, or one alone
