@@ -672,7 +672,10 @@ hipError_t launch_typed(const Attend& a, const AttendPlan& p, void* workspace, h
 AttendPlan attend_plan(int dtype, const Attend& a) {
   const int64_t shared = a.heads / a.kv_heads, seq_rows = a.length * shared, heads = (int64_t)a.groups * a.kv_heads;
   AttendPlan p{};
-  p.by_keys = seq_rows <= 32;
+  // Waves that take keys for themselves: sequences of up to 16 rows (32 x 16 rows after 1,000 keys, fp16 heads of 128: 81 us, shared tiles
+  // 85; the other way round from 24 rows on: 30 and 26); of up to 32 where the tiles are one round of workgroups at most (32 x 32 rows of
+  // four query heads, 300 keys: 10.6 us, shared tiles 18).
+  p.by_keys = seq_rows <= 16 || (seq_rows <= 32 && heads * a.sequences <= 512);
   const int64_t most = p.by_keys ? 32 : 128;
   if (seq_rows <= most) {
     p.tile_rows = (int32_t)(most / seq_rows * seq_rows);
@@ -690,8 +693,14 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
   p.items = (int32_t)items;
   p.per = (p.items + 7) / 8;
   // An XCD's 32 compute units run `slots` workgroups at a time. Items beyond a multiple of that would leave most of them idle for as long as
-  // one takes: as many parts of them as fill the slots once. A part has 256 keys or more.
-  const int slots = 32 * (p.by_keys && dtype == 0 && a.width > 64 ? 1 : 2);
+  // one takes: as many parts of them as fill the slots once (64 single tokens after 2,048 keys: 31 us, whole items 49; 128 tokens after
+  // 8,192: 46 and 162). A part has 256 keys or more (one token after 500: 12.6 us in two parts, 11.6 whole). Shared
+  // tiles of 16-bit operands keep a compute unit's matrix units busy by one workgroup, and a part's sums are 128 rows that are written
+  // and read again: one a compute unit (a causal 1,000: 31 us, two 40; 8 x 60 tokens after 1,000: 30 and 35). fp32 and codes
+  // that are converted on the way take two (16 x 60 tokens after 3,000, fp32: 106 us, one 131; 32 x 61 after 2,048 from
+  // codes 225 and 243).
+  const bool alone = p.by_keys ? dtype == 0 && a.width > 64 : dtype != 0 && !a.bytes;
+  const int slots = alone ? 32 : 64;
   const int64_t seqs = p.tile_rows > seq_rows ? p.tile_rows / seq_rows : 1, keys = a.prefix_slots + seqs * a.slots;
   const int rest = p.per % slots;
   const int64_t fit = rest ? slots / rest : 1, cap = keys / 256;

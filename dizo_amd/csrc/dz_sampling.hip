@@ -20,7 +20,6 @@ constexpr int kBins = 2048;
 constexpr int kPowers = 1024;
 constexpr int kBinBits = 5;  // a bin is 2^kBinBits places: 32 bins for each power of two, 48 of which a weight can have
 constexpr int kHeldBytes = 128 * 1024;  // of a row in LDS
-constexpr uint32_t kShortRow = 8192;
 
 // The order of logits: a logit's key, and its token from the last on. Larger first, equal ones by token.
 __device__ __forceinline__ uint32_t token_of(uint64_t low) { return ~(uint32_t)low; }
@@ -587,11 +586,15 @@ hipError_t launch_held(const SampleRows& a, hipStream_t st) {
   sample_kernel<T, true, THREADS><<<a.nrows, THREADS, bytes, st>>>(a);
   return hipGetLastError();
 }
-// Short rows leave most of 1,024 threads without a vector: 2,000 rows of 1,000 fp16 logits take 16 us, not 66.
+// Threads by the row: 1,024 where its LDS leaves room for one workgroup a compute unit; 512 where two find room (512 x 16,384 bf16, top-p:
+// 28 us, 1,024 threads 40; at 32,000 65 and 64); 256 for rows of up to 4,096 where there are many (2,000 x 4,096: 35 us, 512 threads 42;
+// 256 x 4,096: 13.8 and 12.7) and of up to 2,048.
 template <class T>
 hipError_t launch_typed(const SampleRows& a, hipStream_t st) {
-  if (a.vocab <= kShortRow) return launch_held<T, 256>(a, st);
-  if (a.vocab <= (uint32_t)(kHeldBytes / 16 * T::kPer16)) return launch_held<T, 1024>(a, st);
+  const uint32_t bytes = a.vocab * (16 / T::kPer16);
+  if (a.vocab <= (a.nrows > 512 ? 4096u : 2048u)) return launch_held<T, 256>(a, st);
+  if (bytes <= 48 * 1024) return launch_held<T, 512>(a, st);
+  if (bytes <= kHeldBytes) return launch_held<T, 1024>(a, st);
   sample_kernel<T, false, 1024><<<a.nrows, 1024, 0, st>>>(a);
   return hipGetLastError();
 }

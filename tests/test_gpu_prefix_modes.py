@@ -21,7 +21,11 @@ DEV = "cuda"
 @pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("shape", [
     (1, 1, 523, 523, 1, 2, 700, 16),   # 66 items an XCD: 64 at a time, and two in two parts each
-    (1, 1, 131, 131, 33, 33, 1100, 24),  # the same of larger tiles: 17 items, in three parts
+    (1, 1, 131, 131, 33, 33, 1100, 24),  # 17 larger tiles an XCD
+    (1, 1, 9, 9, 33, 33, 1100, 24),    # 2, in four parts
+    (1, 2, 270, 270, 40, 50, 600, 40),  # 34, of which two are in two parts
+    (2, 3, 4, 2, 12, 20, 600, 64),     # 24 rows a sequence: waves take keys for themselves
+    (1, 1, 520, 520, 24, 24, 40, 16),  # the same where shared tiles are taken
     (2, 66, 4, 4, 1, 20, 300, 64),     # several tiles of sequences, with keys of their own
     (1, 2, 8, 2, 40, 77, 513, 128),    # 160 rows a sequence
 ], ids=str)
