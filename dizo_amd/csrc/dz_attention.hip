@@ -8,6 +8,17 @@
 // sequence that the tile touches, in tiles of their own. The prompt is read once for all of the tile's rows; a sequence's own
 // keys are scored against the whole tile and masked for the rows of others, which costs products that the
 // matrix units have to spare: a tile of single tokens waits for its own keys from memory.
+//
+// What bounds it, and what it measured (one MI355X; the floor: bytes at a large copy's 4.96 TB/s, or products at a large
+// library product's 1,358 TFLOP/s in bf16):
+//   single tokens   their keys from memory: 64 answers after 2,048 keys, 295 MB, 53 us (5.5 TB/s) and 6 to join; floor 60
+//   the same, 8 bit conversions next to the loads: 28 us and 6 to join; floor 15
+//   candidates      the way through one workgroup (lengths, then keys, scores, values, the waves' sums), twice: 640 tiles for 512
+//                   places: 20 us; floor 8
+//   prompts         one causal sequence of 4,096, 40 heads of 128: 222 us, 770 TFLOP/s; the products alone reach 1,030 under the power limit
+//                   in this order (scores, weights, values by one wave)
+// A lane holds one query: scores are taken as K Q^T and results as V^T P^T, so that maxima, sums and weights stay in the
+// lane (two lanes a query) and weights are the second product's operand as they are. Values are read from LDS transposed.
 #include "dz_attention.h"
 #include "dz_lds.h"
 
@@ -18,7 +29,8 @@ namespace {
 enum Store {
   kOperands,   // elements, loaded straight to LDS
   kConverted,  // elements that were codes: loaded to registers and converted once for all waves
-  kCodes,      // codes, loaded straight to LDS and converted by the wave that takes keys for itself; widths of whole chunks
+  kCodes,      // codes, loaded straight to LDS and converted by the wave that takes keys for itself; widths of whole chunks (32 single tokens
+               // after 6,000 keys: 30 us, through registers 37; waves that share keys would convert each code four times)
 };
 
 // The sums of a row by themselves, key by key: a lane takes a key's score, and then a column or two of the values. For rows
@@ -155,7 +167,7 @@ struct Shape {
   static constexpr int SLABS = BY_KEYS ? WAVES : 1;
   static constexpr int PV = (QS + 1) / 2;  // products of 32 columns of values
   // Tiles in LDS. Waves that take keys for themselves have one each: the other waves' loads are on their way meanwhile, and
-  // twice as many of them find room.
+  // twice as many of them find room (candidates fp16: 20 us, with two tiles 28).
   static constexpr int STAGES = BY_KEYS && STORE != kCodes ? 1 : 2;
   // workgroups that a compute unit's LDS holds
   static constexpr int RESIDENT = SLABS * STAGES * 2 * TILE > 72 * 1024 ? 1 : 2;

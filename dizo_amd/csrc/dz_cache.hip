@@ -5,6 +5,9 @@
 // nearest e4m3 number to x / 2^e (ties to even). A power of two moves nothing but exponents: x / 2^e and code 2^e are
 // exact, so the only rounding is the code's, of half a unit of 3 bits (2^-4 of the value; 2^-10 2^e below 2^-6 2^e), and an
 // arbitrary scale would save none of it.
+//
+// Bound by memory: 2,048 tokens of 40 heads of 128 written in 15 us (63 MB; 12.7 at a large copy's 4.96 TB/s), 64 x 300 read in
+// 82 us (591 MB, 7.2 TB/s with what the caches hold); one token of 64 sequences 3.5 us, a launch.
 #include "dz_prefix.h"
 #include "dz_token_math.h"
 
@@ -128,7 +131,8 @@ __global__ __launch_bounds__(kThreads) void cache_kernel(CacheRows a) {
 template <class T, bool READ, int LANES>
 void launch_lanes(const CacheRows& a, hipStream_t st) {
   const uint32_t rows = (uint32_t)a.batch * a.length * a.heads, each = kThreads / LANES;
-  // four rows a thread where that leaves two workgroups a compute unit
+  // four rows a thread where that leaves two workgroups a compute unit (64 x 300 tokens of 40 heads of 64 written: 59 us, one row a thread 76;
+  // 64 tokens: one row a thread 3.0 us, four 4.5)
   if (rows >= 4 * each * 256) cache_kernel<T, READ, LANES, 4><<<dim3((rows + 4 * each - 1) / (4 * each), 2), kThreads, 0, st>>>(a);
   else cache_kernel<T, READ, LANES, 1><<<dim3((rows + each - 1) / each, 2), kThreads, 0, st>>>(a);
 }

@@ -10,6 +10,12 @@
 // of 50,000 borders would give another token in one of a few thousand rows. Weights are computed in 64 bits and
 // kept as whole numbers of 2^-46 (2^-42 for the largest vocabularies, so that a row's sum fits 64 bits): sums are exact in any
 // order, and a token of less weight than half of that, which one number of 2^24 could hardly reach, is not drawn.
+//
+// A workgroup takes a row. The row is read once and held in LDS (512 x 32,003 fp32: 65 us, read again for each pass 71), then gone through:
+// sums of weights by bins of their distance to the largest (top-p), the logits of the bin that the cut lies in, sorted; and sums of what is
+// kept by pieces of the row. Top-k sorts the few logits that can matter and needs none of that. What bounds it: the vector
+// units (weights in 64 bits: about 20 operations each, twice a logit), then the chain of phases: 17 us for one row of 50,272
+// with top-k, 65 for 512 x 32,003 with top-p, two rounds of rows; a read of the logits alone would take 13.
 #include "dz_sampling.h"
 #include "dz_token_math.h"
 
