@@ -400,7 +400,9 @@ class ZOTrainerMixin:
             self.zo_journal = ZOJournal.for_params(self.named_parameters_to_optim, args.zo_eps, projected)
             if args.enhanced:
                 self.dizo_trainer.dizo.journal = self.zo_journal
-        self._hook = model.register_forward_pre_hook(lambda m, a: self.zo_flush())
+        # (the layers under the head, too: dizo_amd.shared_prompt calls them by themselves)
+        self._hooks = [m.register_forward_pre_hook(lambda m, a: self.zo_flush())
+                       for m in {id(m): m for m in (model, getattr(model, "base_model", model))}.values()]
 
     def _get_learning_rate(self) -> float:
         return self.lr_scheduler.get_last_lr()[0]
@@ -597,9 +599,9 @@ class ZOTrainerMixin:
             self._zo_tabs = None
         if getattr(self, "dizo_trainer", None) is not None:
             self.dizo_trainer.close()
-        if getattr(self, "_hook", None) is not None:
-            self._hook.remove()
-            self._hook = None
+        for hook in getattr(self, "_hooks", ()):
+            hook.remove()
+        self._hooks = []
 
 
 def _anchor_copy(model: torch.nn.Module, exclude_list: Sequence[str]) -> torch.nn.Module:

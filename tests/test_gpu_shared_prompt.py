@@ -85,3 +85,27 @@ def test_generate_is_repeatable_and_takes_a_generator():
     ids = torch.randint(2, 211, (1, 7), generator=torch.Generator().manual_seed(6)).to(DEV)
     runs = [S.generate(model, ids, 9, answers=40, generator=torch.Generator(DEV).manual_seed(3), kv_bits=8) for _ in range(2)]
     assert torch.equal(*runs) and runs[0].min() >= 0 and runs[0].max() < 211
+
+
+def test_answers_between_steps_are_the_updated_weights():
+    """A step that leaves its update for the next perturbation: answers and scores read the weights with it."""
+    gen = torch.Generator().manual_seed(5)
+    ids = torch.randint(4, 60, (2, 7), generator=gen).to(DEV)
+    seen = {}
+    for fuse in (False, True):
+        np.random.seed(4)
+        model = build_opt("opt-tiny", torch.float32, DEV)
+        b = make_batch(4, SHAPES["opt-tiny"].vocab, gen=gen.manual_seed(3), device=DEV)
+        tr = ZOTrainer(model, ZOArguments(learning_rate=1e-2, zo_eps=0.5, max_steps=10, zo_fuse_restore=fuse, zo_fuse_next_perturb=fuse))
+        tr.training_step(b)
+        assert (tr._pending_update is not None) == fuse
+        answers = S.generate(model, ids, 8, temperature=0.0)
+        assert tr._pending_update is None
+        tr.training_step(b)
+        with torch.no_grad():
+            scores = S.shared_prompt_logprobs(model, ids, None, [2, 2], 1, model.config.pad_token_id)
+        assert tr._pending_update is None
+        tr.zo_close()
+        seen[fuse] = answers, scores
+    assert torch.equal(seen[False][0], seen[True][0])
+    assert torch.equal(seen[False][1], seen[True][1])
