@@ -13,8 +13,7 @@
 // library product's 1,358 TFLOP/s in bf16):
 //   single tokens   their keys from memory: 64 answers after 2,048 keys, 295 MB, 53 us (5.5 TB/s) and 6 to join; floor 60
 //   the same, 8 bit conversions next to the loads: 28 us and 6 to join; floor 15
-//   candidates      the way through one workgroup (lengths, then keys, scores, values, the waves' sums), twice: 640 tiles for 512
-//                   places: 20 us; floor 8
+//   candidates      the way through one workgroup (lengths, then keys, scores, values, the waves' sums): 14 us; floor 8
 //   prompts         one causal sequence of 4,096, 40 heads of 128: 222 us, 770 TFLOP/s; the products alone reach 1,030 under the power limit
 //                   in this order (scores, weights, values by one wave)
 // A lane holds one query: scores are taken as K Q^T and results as V^T P^T, so that maxima, sums and weights stay in the
@@ -153,13 +152,14 @@ __device__ __forceinline__ void lone_rows(uint32_t first, uint32_t set) {
   }
 }
 
-// QS: sixteenths of the width, rounded up to 4, 5, 6 or 8.
-template <class T, int QS, bool BY_KEYS, Store STORE>
+// QS: sixteenths of the width, rounded up to 4, 5, 6 or 8. BY_KEYS: WAVES waves take keys for themselves; otherwise four share them.
+template <class T, int QS, bool BY_KEYS, Store STORE, int OF_WAVES>
 struct Shape {
   static constexpr bool kWide = std::is_same_v<T, TypeF32>;
   static constexpr int CH = STORE == kCodes ? QS : kWide ? 4 * QS : 2 * QS;  // chunks of 16 bytes a row
   static constexpr int STEPS = STORE == kCodes ? (QS + 1) / 2 * 2 : QS;        // products along the width
-  static constexpr int WAVES = 4;
+  static constexpr int WAVES = OF_WAVES;
+  static_assert(BY_KEYS || WAVES == 4, "shared tiles");
   static constexpr int KT = BY_KEYS || kWide ? 32 : 64;    // keys of a tile
   static constexpr int ROWS = BY_KEYS ? 32 : 32 * WAVES;  // most rows of a workgroup
   static constexpr int TILE = KT * CH * 16;                // bytes of a tile's keys, or of its values
@@ -167,18 +167,18 @@ struct Shape {
   static constexpr int SLABS = BY_KEYS ? WAVES : 1;
   static constexpr int PV = (QS + 1) / 2;  // products of 32 columns of values
   // Tiles in LDS. Waves that take keys for themselves have one each: the other waves' loads are on their way meanwhile, and
-  // twice as many of them find room (candidates fp16: 20 us, with two tiles 28).
+  // twice as many of them find room (candidates fp16 by four waves: 20 us, with two tiles 28).
   static constexpr int STAGES = BY_KEYS && STORE != kCodes ? 1 : 2;
-  // workgroups that a compute unit's LDS holds
-  static constexpr int RESIDENT = SLABS * STAGES * 2 * TILE > 72 * 1024 ? 1 : 2;
+  // workgroups that a compute unit's LDS and registers hold: eight waves, or four with more than half of the LDS
+  static constexpr int RESIDENT = (4 * SLABS / WAVES * STAGES * 2 * TILE > 72 * 1024 ? 4 : 8) / WAVES;
 };
 
-template <class T, int QS, bool BY_KEYS, Store STORE, int THREADS = 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES,
-          int RESIDENT = Shape<T, QS, BY_KEYS, STORE>::RESIDENT>
+template <class T, int QS, bool BY_KEYS, Store STORE, int OF_WAVES, int THREADS = 64 * OF_WAVES,
+          int RESIDENT = Shape<T, QS, BY_KEYS, STORE, OF_WAVES>::RESIDENT>
 __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void attend_kernel(Call call) {
   const Attend& a = call.a;
   const AttendPlan& plan = call.plan;
-  using S = Shape<T, QS, BY_KEYS, STORE>;
+  using S = Shape<T, QS, BY_KEYS, STORE, OF_WAVES>;
   using Elem = typename T::Elem;
   using Frag = typename Op<T>::Frag;
   // Weights of codes carry their row's power of two, which may leave the range of fp16: those are bf16 (and codes are bf16 numbers).
@@ -648,19 +648,25 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, AttendPlan plan, co
            (int64_t)(row % seq_rows / shared) * a.out_s[3] + col) = Quad{(Elem)(o[0] * inv), (Elem)(o[1] * inv), (Elem)(o[2] * inv), (Elem)(o[3] * inv)};
 }
 
-template <class T, int QS, bool BY_KEYS, Store STORE>
+template <class T, int QS, bool BY_KEYS, Store STORE, int WAVES>
 void launch_one(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {
-  attend_kernel<T, QS, BY_KEYS, STORE><<<8 * (p.whole + p.tail * p.splits), 64 * Shape<T, QS, BY_KEYS, STORE>::WAVES, 0, st>>>(Call{a, p, partial, ms});
+  attend_kernel<T, QS, BY_KEYS, STORE, WAVES><<<8 * (p.whole + p.tail * p.splits), 64 * WAVES, 0, st>>>(Call{a, p, partial, ms});
+}
+template <class T, int QS, Store STORE>
+void launch_by_keys(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {
+  if (p.waves == 1) launch_one<T, QS, true, STORE, 1>(a, p, partial, ms, st);
+  else if (p.waves == 2) launch_one<T, QS, true, STORE, 2>(a, p, partial, ms, st);
+  else launch_one<T, QS, true, STORE, 4>(a, p, partial, ms, st);
 }
 template <class T, int QS>
 void launch_qs(const Attend& a, const AttendPlan& p, float* partial, float2* ms, hipStream_t st) {
   if (p.by_keys) {
-    if (!a.bytes) launch_one<T, QS, true, kOperands>(a, p, partial, ms, st);
-    else if (a.whole_chunks) launch_one<T, QS, true, kCodes>(a, p, partial, ms, st);
-    else launch_one<T, QS, true, kConverted>(a, p, partial, ms, st);
+    if (!a.bytes) launch_by_keys<T, QS, kOperands>(a, p, partial, ms, st);
+    else if (a.whole_chunks) launch_by_keys<T, QS, kCodes>(a, p, partial, ms, st);
+    else launch_by_keys<T, QS, kConverted>(a, p, partial, ms, st);
   } else {
-    if (!a.bytes) launch_one<T, QS, false, kOperands>(a, p, partial, ms, st);
-    else launch_one<T, QS, false, kConverted>(a, p, partial, ms, st);
+    if (!a.bytes) launch_one<T, QS, false, kOperands, 4>(a, p, partial, ms, st);
+    else launch_one<T, QS, false, kConverted, 4>(a, p, partial, ms, st);
   }
 }
 template <class T>
@@ -685,9 +691,9 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
   const int64_t shared = a.heads / a.kv_heads, seq_rows = a.length * shared, heads = (int64_t)a.groups * a.kv_heads;
   AttendPlan p{};
   // Waves that take keys for themselves: sequences of up to 16 rows (32 x 16 rows after 1,000 keys, fp16 heads of 128: 81 us, shared tiles
-  // 85; the other way round from 24 rows on: 30 and 26); of up to 32 where the tiles are one round of workgroups at most (32 x 32 rows of
-  // four query heads, 300 keys: 10.6 us, shared tiles 18).
-  p.by_keys = seq_rows <= 16 || (seq_rows <= 32 && heads * a.sequences <= 512);
+  // 85); of up to 32 where there are few tiles (32 x 32 rows of four query heads, 300 keys: 10.6 us, shared tiles 18) or few
+  // keys (64 x 24 causal: 15 us, 27); many tiles of many keys are shared (32 x 32 rows after 1,000: 91 us, the other way 101).
+  p.by_keys = seq_rows <= 16 || (seq_rows <= 32 && (heads * a.sequences <= 512 || a.prefix_slots + a.slots < 1000));
   const int64_t most = p.by_keys ? 32 : 128;
   if (seq_rows <= most) {
     p.tile_rows = (int32_t)(most / seq_rows * seq_rows);
@@ -711,9 +717,15 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
   // and read again: one a compute unit (a causal 1,000: 31 us, two 40; 8 x 60 tokens after 1,000: 30 and 35). fp32 and codes
   // that are converted on the way take two (16 x 60 tokens after 3,000, fp32: 106 us, one 131; 32 x 61 after 2,048 from
   // codes 225 and 243).
-  const bool alone = p.by_keys ? dtype == 0 && a.width > 64 : dtype != 0 && !a.bytes;
-  const int slots = alone ? 32 : 64;
   const int64_t seqs = p.tile_rows > seq_rows ? p.tile_rows / seq_rows : 1, keys = a.prefix_slots + seqs * a.slots;
+  // Of the 256 waves that an XCD holds (wide fp32 heads: 128), an item of few keys takes as many as let all items run at once: a second round
+  // begins again with lengths and first keys (32 x 6 rows after 122 keys, 640 items: two waves 13.8 us, four 20.6, one 15.4; 64 x 12
+  // causal, 2,048 items: one wave 9.6, four 28.7). Many keys are worth four (512 single tokens after 2,000: 374 us, two 392).
+  const int held = p.by_keys && dtype == 0 && a.width > 64 ? 128 : 256;
+  p.waves = 4;
+  if (p.by_keys && keys < 1024)
+    while (p.waves > 1 && p.per * p.waves > held) p.waves /= 2;
+  const int slots = p.by_keys ? held / p.waves : dtype != 0 && !a.bytes ? 32 : 64;
   const int rest = p.per % slots;
   const int64_t fit = rest ? slots / rest : 1, cap = keys / 256;
   p.splits = (int32_t)(fit < cap ? fit : cap);

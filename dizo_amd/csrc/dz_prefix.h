@@ -36,6 +36,7 @@ struct Attend {
 // after another: first `whole` of them, a workgroup each, then `tail`, of which `splits` workgroups each take a part of the keys.
 struct AttendPlan {
   bool by_keys;  // a workgroup's waves share its rows and take keys in turn; else they share keys
+  int32_t waves;  // of a workgroup
   int32_t tile_rows, tiles;
   int32_t items, per, whole, tail, splits;
 };

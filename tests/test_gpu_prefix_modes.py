@@ -25,7 +25,10 @@ DEV = "cuda"
     (1, 1, 9, 9, 33, 33, 1100, 24),    # 2, in four parts
     (1, 2, 270, 270, 40, 50, 600, 40),  # 34, of which two are in two parts
     (2, 3, 4, 2, 12, 20, 600, 64),     # 24 rows a sequence: waves take keys for themselves
-    (1, 1, 520, 520, 24, 24, 40, 16),  # the same where shared tiles are taken
+    (1, 1, 520, 520, 24, 24, 40, 16),  # the same, two waves an item
+    (1, 1, 1100, 1100, 20, 20, 30, 24),  # one wave an item
+    (1, 1, 2060, 2060, 1, 2, 700, 16),  # the same, 258 an XCD: 256 at a time, and two in two parts each
+    (1, 1, 520, 520, 24, 24, 1000, 16),  # many keys: shared tiles
     (2, 66, 4, 4, 1, 20, 300, 64),     # several tiles of sequences, with keys of their own
     (1, 2, 8, 2, 40, 77, 513, 128),    # 160 rows a sequence
 ], ids=str)
@@ -212,6 +215,8 @@ def test_offsets_past_32_bits():
     (1, 2, 2, 1, 70, 90, 65, 80),    # tiles of 128 rows of one
     (1, 40, 1, 1, 1, 3, 0, 16),      # 32 sequences in a tile
     (1, 3, 2, 1, 2, 30, 1500, 104),  # a prompt in several parts
+    (1, 2, 600, 600, 2, 6, 20, 16),  # two waves an item
+    (1, 2, 1100, 1100, 2, 6, 20, 80),  # one
 ], ids=str)
 def test_what_is_not_finite_reaches_those_that_see_it(shape, dtype, bits):
     q, own, pre = inputs(10, dtype, *shape, bits=bits)
