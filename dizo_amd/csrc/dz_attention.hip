@@ -690,10 +690,17 @@ hipError_t launch_typed(const Attend& a, const AttendPlan& p, void* workspace, h
 AttendPlan attend_plan(int dtype, const Attend& a) {
   const int64_t shared = a.heads / a.kv_heads, seq_rows = a.length * shared, heads = (int64_t)a.groups * a.kv_heads;
   AttendPlan p{};
-  // Waves that take keys for themselves: sequences of up to 16 rows (32 x 16 rows after 1,000 keys, fp16 heads of 128: 81 us, shared tiles
-  // 85); of up to 32 where there are few tiles (32 x 32 rows of four query heads, 300 keys: 10.6 us, shared tiles 18) or few
-  // keys (64 x 24 causal: 15 us, 27); many tiles of many keys are shared (32 x 32 rows after 1,000: 91 us, the other way 101).
-  p.by_keys = seq_rows <= 16 || (seq_rows <= 32 && (heads * a.sequences <= 512 || a.prefix_slots + a.slots < 1000));
+  // Waves that take keys for themselves, 32 rows a workgroup, or tiles of 128 rows that share keys. The first reads keys four times as often for
+  // the same rows, and leaves fewer rows empty and more workgroups to run. Sequences of
+  //   up to 16 rows: the first (32 x 16 rows after 1,000 keys, fp16 heads of 128: 81 us, shared 85);
+  //   up to 96 rows, in no more than one round of workgroups, or after few keys: the first (34 heads of 40 rows after 5,066 keys: fp32 92 us,
+  //   shared 164; 32 x 40 rows after 122, bf16: 29 and 29, after 600: 71 and 56; fp32 after 600: 309 and 412);
+  //   more: the second (one sequence of 128 rows after 5,066: 37 and 35; fp32 211 and 169).
+  // Codes are converted by each wave for itself in the first, without a stop in registers before: of wide heads it is the faster one
+  // throughout (a causal 2,048 of 40 heads of 128: 104 us, shared 164; heads of 80, 16 x 256: 33 and 31).
+  const int64_t keys_of_one = a.prefix_slots + a.slots, own_tiles = heads * a.sequences * ((seq_rows + 31) / 32);
+  const int64_t few_keys = seq_rows <= 32 || dtype == 0 || a.bytes ? 1000 : 256;
+  p.by_keys = seq_rows <= 16 || (a.bytes && a.width >= 96 && a.width % 16 == 0) || (seq_rows <= 96 && (own_tiles <= 512 || keys_of_one < few_keys));
   const int64_t most = p.by_keys ? 32 : 128;
   if (seq_rows <= most) {
     p.tile_rows = (int32_t)(most / seq_rows * seq_rows);

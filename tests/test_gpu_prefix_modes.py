@@ -29,6 +29,10 @@ DEV = "cuda"
     (1, 1, 1100, 1100, 20, 20, 30, 24),  # one wave an item
     (1, 1, 2060, 2060, 1, 2, 700, 16),  # the same, 258 an XCD: 256 at a time, and two in two parts each
     (1, 1, 520, 520, 24, 24, 1000, 16),  # many keys: shared tiles
+    (1, 3, 100, 100, 40, 50, 1000, 24),  # shared tiles of three sequences
+    (1, 2, 2, 1, 60, 70, 300, 104),    # shared tiles of wide heads
+    (1, 2, 4, 2, 40, 60, 100, 64),     # 80 rows in tiles of 32
+    (1, 1, 2, 2, 300, 310, 20, 112),   # codes of wide heads in tiles of 32, 16 bits in shared ones
     (2, 66, 4, 4, 1, 20, 300, 64),     # several tiles of sequences, with keys of their own
     (1, 2, 8, 2, 40, 77, 513, 128),    # 160 rows a sequence
 ], ids=str)
