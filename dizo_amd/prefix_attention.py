@@ -21,6 +21,7 @@ import struct
 from typing import NamedTuple, Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .table import dtype_code
@@ -91,7 +92,8 @@ def _check_operands(what: str, index: int, tensors) -> None:
             _fail(what, f"tensors on cuda:{index} and {t.device}")
         if grad and t.requires_grad:
             _fail(what, "nothing is recorded by autograd: call it under torch.no_grad(), or detach the operands")
-    _no_tangents(what, *tensors)
+    if forward_ad._current_level >= 0:
+        _no_tangents(what, *tensors)
 
 
 def _check_store(what: str, name: str, kv, shape, dtype, index: int) -> bool:
@@ -208,8 +210,6 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
 def _one_lead(what: str, t: torch.Tensor, n: int):
     """t's strides of (batch, unused, ...) with its first n dimensions taken as one."""
     s = t.stride()
-    if n == 1:
-        return s[0], 0, s[1], s[2]
     if n == 0:
         return 0, 0, s[0], s[1]
     shape = t.shape
@@ -224,15 +224,20 @@ def _cache_fields(what: str, cache):
     if not isinstance(cache, QuantizedKV):
         _fail(what, f"the cache must be a QuantizedKV, got {type(cache).__name__}")
     k, v, k_scale, v_scale = cache
-    if not k.is_cuda:
+    index = k.get_device()
+    if index < 0:
         _fail(what, f"the cache must live on a GPU, got {k.device}")
     shape = k.shape
     n = len(shape) - 3
     if n < 0:
         _fail(what, f"the cache must be (..., heads, slots, width), got {tuple(shape)}")
-    _check_store(what, "cache", cache, shape, None, k.get_device())
-    if k.stride(-1) != 1 or v.stride(-1) != 1:
+    _check_store(what, "cache", cache, shape, None, index)
+    ks, vs, kss, vss = k.stride(), v.stride(), k_scale.stride(), v_scale.stride()
+    if ks[-1] != 1 or vs[-1] != 1:
         _fail(what, "the width of the cache must be contiguous")
+    if n == 1:
+        return shape[0], 1, (k.data_ptr(), v.data_ptr(), ks[0], 0, ks[1], ks[2], vs[0], 0, vs[1], vs[2], k_scale.data_ptr(), v_scale.data_ptr(),
+                             kss[0], 0, kss[1], kss[2], vss[0], 0, vss[1], vss[2])
     batch = 1
     for x in shape[:n]:
         batch *= x
@@ -284,9 +289,10 @@ def cache_read(cache: QuantizedKV, length: int, dtype: torch.dtype, start: int =
     length, start = _whole(what, "length", length), _whole(what, "start", start)
     if length < 0 or start < 0 or start + length > slots:
         _fail(what, f"slots {start} to {start + length} of {slots}")
-    k, v = (torch.empty((*shape[:-2], length, width), dtype=dtype, device=cache.k.device) for _ in range(2))
+    shape, device = (*shape[:-2], length, width), cache.k.device
+    k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     if k.numel():
         s = (heads * length * width, 0, length * width, width)
-        _call(k.device, "dz_cache_read", _KEYS_VALUES.pack(*fields), _KEYS_VALUES.pack(k.data_ptr(), v.data_ptr(), *s, *s, *_NO_SCALES), code,
+        _call(device, "dz_cache_read", _KEYS_VALUES.pack(*fields), _KEYS_VALUES.pack(k.data_ptr(), v.data_ptr(), *s, *s, *_NO_SCALES), code,
               batch, heads, length, width, slots, start)
     return KV(k, v)
