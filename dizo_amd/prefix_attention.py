@@ -65,17 +65,20 @@ _NO_SCALES = (0,) * 10
 
 
 def _rows(t: torch.Tensor):
-    """(t, its strides but for the width's) where the kernels can read t: the width contiguous, rows at multiples of 16 bytes
-    (codes: 8), slots near enough; otherwise those of a copy."""
-    *s, last = t.stride()
-    es = t.element_size()
-    low = t.data_ptr()
-    for x in s:
-        low |= x * es
-    if last != 1 or low & (7 if es == 1 else 15) or s[-1] >= MAX_SLOT_STRIDE:
+    """(t of four or five dimensions, its strides but for the width's) where the kernels can read t: the width contiguous,
+    rows at multiples of 16 bytes (codes: 8), slots near enough; otherwise those of a copy."""
+    s = t.stride()
+    es = t.element_size()  # (a power of two)
+    if len(s) == 5:
+        a, b, c, step, last = s
+        low = t.data_ptr() | (a | b | c | step) * es
+    else:
+        a, b, step, last = s
+        low = t.data_ptr() | (a | b | step) * es
+    if last != 1 or low & (7 if es == 1 else 15) or step >= MAX_SLOT_STRIDE:
         t = t.clone(memory_format=torch.contiguous_format)
-        s = t.stride()[:-1]
-    return t, s
+        s = t.stride()
+    return t, s[:-1]
 
 
 def _whole(what: str, name: str, x) -> int:
