@@ -303,3 +303,20 @@ def test_numbers_of_other_types():
                  lambda: sample_tokens(logits, u, top_k=2.5), lambda: sample_tokens(logits, u, temperature="one"), lambda: sample_tokens(logits, u, top_p=None)):
         with pytest.raises(DzError, match="must be"):
             call()
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 1, 3, 40, 300, 128), (1, 1, 4, 2, 80, 100, 70, 112), (2, 20, 16, 16, 2, 9, 33, 64)], ids=str)
+def test_codes_whose_rows_start_at_multiples_of_8_bytes(shape):
+    q, own, pre = inputs(14, "bf16", *shape, bits=8)
+    width = shape[-1]
+
+    def moved(x):
+        """The same codes 8 bytes into rows of 16 more."""
+        to = torch.zeros(*x.shape[:-1], width + 16, dtype=torch.uint8, device=DEV)
+        to[..., 8:8 + width] = x.view(torch.uint8)
+        return to.view(P.CODES)[..., 8:8 + width]
+
+    own8, pre8 = (P.QuantizedKV(moved(s.k), moved(s.v), s.k_scale, s.v_scale) for s in (own, pre))
+    assert own8.k.data_ptr() % 16 == 8
+    check("bf16", q, own8, pre8)
+    check("bf16", q, own8, pre)
