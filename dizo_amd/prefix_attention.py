@@ -211,15 +211,20 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
 
 
 def _one_lead(what: str, t: torch.Tensor, n: int):
-    """t's strides of (batch, unused, ...) with its first n dimensions taken as one."""
+    """t's strides of (batch, unused, ...) with its first n dimensions taken as one: the batch's is that of the innermost
+    of them that has more than one, and each further one steps over all of those inside of it."""
     s = t.stride()
-    if n == 0:
-        return 0, 0, s[0], s[1]
     shape = t.shape
-    for i in range(n - 1):
-        if shape[i] != 1 and s[i] != s[i + 1] * shape[i + 1]:
+    lead = span = None  # the batch's stride, and what the next dimension has to step over
+    for i in range(n - 1, -1, -1):
+        if shape[i] == 1:
+            continue
+        if lead is None:
+            lead = span = s[i]
+        elif s[i] != span:
             _fail(what, "the cache's leading dimensions must be one by their strides")
-    return s[n - 1], 0, s[n], s[n + 1]
+        span *= shape[i]
+    return lead or 0, 0, s[n], s[n + 1]
 
 
 def _cache_fields(what: str, cache):
