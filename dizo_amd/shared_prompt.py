@@ -8,11 +8,11 @@ sampling.
                             once, its keys and values are kept once for all of its answers, in the model's dtype or in
                             8 bits, and each answer keeps its own
 
-Both run the model's own layers, OPT's, LLaMA's or others that call the attention HF registers by name, with one of this
+Both run the model's own layers, OPT's, LLaMA's or others of MODELS, which call the attention HF registers by name, with one of this
 module's in its place (in the model's config, for as long as a forward takes: one call at a time for a model): a forward gets
-one row for each prompt, and the attention is told where things lie by the keyword argument dz_shared. Attention with a
-window, a soft cap or sinks, layers that mix tokens in another way, and heads whose logits are scaled or capped are
-refused. Nothing is recorded by autograd.
+one row for each prompt, and the attention is told where things lie by the keyword argument dz_shared. Other models,
+attention with a window, a soft cap or sinks, layers that mix tokens in another way, and heads that do more than multiply by the
+output embedding are refused. Nothing is recorded by autograd.
 """
 from __future__ import annotations
 
@@ -101,10 +101,22 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, dro
     return dz_shared.attend(layer, query, key, value, scale), None
 
 
+# Types of models (config.model_type) that are no more than layers of the attention above, one for each of config.num_hidden_layers, and
+# an output embedding: nothing else mixes tokens, and nothing lies between the last hidden states and the head, or behind it.
+MODELS = frozenset("""apertus arcee bitnet cwm ernie4_5 ernie4_5_moe exaone4 gemma gemma2 gemma3_text glm glm4 glm4_moe gpt2 gpt_bigcode gpt_neox
+    granite granitemoe granitemoeshared helium hyperclovax llama minimax_m2 ministral mistral mixtral olmo olmo2 olmo3 olmoe opt persimmon phi phi3
+    phimoe qwen2 qwen2_moe qwen3 qwen3_moe seed_oss smollm3 starcoder2""".split())
+
+
 def _check_model(model) -> None:
     config = model.config
     if not getattr(model, "_supports_attention_backend", False):
         raise DzError(f"shared_prompt: {type(model).__name__} does not call an attention that HF registers by name")
+    if getattr(config, "model_type", None) not in MODELS:
+        raise DzError(f"shared_prompt: {type(model).__name__} is not one of the models whose head and layers are known: {', '.join(sorted(MODELS))}")
+    head, base = model.get_output_embeddings(), model.base_model
+    if not isinstance(head, torch.nn.Module) or base is model or any(m is not head and m is not base for m in model.children()):
+        raise DzError(f"shared_prompt: {type(model).__name__} has more than its layers and an output embedding")
     for name in ("final_logit_softcapping", "logit_scale", "logits_scaling", "output_multiplier_scale"):
         if getattr(config, name, None) not in (None, 1, 1.0):
             raise DzError(f"shared_prompt: a model with {name}")
