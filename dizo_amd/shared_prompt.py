@@ -108,7 +108,8 @@ MODELS = frozenset("""apertus arcee bitnet cwm ernie4_5 ernie4_5_moe exaone4 gem
     phimoe qwen2 qwen2_moe qwen3 qwen3_moe seed_oss smollm3 starcoder2""".split())
 
 
-def _check_model(model) -> None:
+def _check_model(model, tokens: int) -> None:
+    """Whether the model's answers to sequences of up to `tokens` are what its layers and output embedding give here."""
     config = model.config
     if not getattr(model, "_supports_attention_backend", False):
         raise DzError(f"shared_prompt: {type(model).__name__} does not call an attention that HF registers by name")
@@ -120,6 +121,11 @@ def _check_model(model) -> None:
     for name in ("final_logit_softcapping", "logit_scale", "logits_scaling", "output_multiplier_scale"):
         if getattr(config, name, None) not in (None, 1, 1.0):
             raise DzError(f"shared_prompt: a model with {name}")
+    # (some models have a window in their masks only, which the attention is not told of)
+    for name in ("sliding_window", "attention_chunk_size"):
+        window = getattr(config, name, None)
+        if window is not None and window < tokens:
+            raise DzError(f"shared_prompt: attention with a window of {window} of {tokens} tokens ({name})")
 
 
 def _hidden(model, input_ids: torch.Tensor, position_ids: torch.Tensor, layout) -> torch.Tensor:
@@ -158,7 +164,7 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     sequences, length = input_ids.shape
     if candidates < 1 or sequences % candidates or len(option_len) != sequences or not 1 <= min(option_len) <= max(option_len) < length:
         raise DzError(f"shared_prompt_logprobs: {sequences} sequences of {length} tokens, {candidates} candidates each, option_len {list(option_len)[:8]}")
-    _check_model(model)
+    _check_model(model, length)
     device, examples, most = input_ids.device, sequences // candidates, max(option_len)
     room, each = length - min(option_len), most - 1
     options = torch.as_tensor(option_len, device=device)
@@ -215,7 +221,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, answers: in
         raise DzError(f"generate: prompt_lengths must be torch.int32 ({prompts},), got {prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
     if uniform is not None and uniform.shape != (prompts, answers, max_new_tokens):
         raise DzError(f"generate: uniform must be {(prompts, answers, max_new_tokens)}, got {tuple(uniform.shape)}")
-    _check_model(model)
+    _check_model(model, room + max_new_tokens)
     most = getattr(model.config, "max_position_embeddings", None)
     if most is not None and room + max_new_tokens - 1 > most:  # (an answer's last token is not read again)
         raise DzError(f"generate: {room} tokens of a prompt and {max_new_tokens} new ones, the model has {most} positions")

@@ -73,3 +73,27 @@ def test_a_head_of_several_parts_is_refused(plain):  # noqa: F811
     scores = transformers.OPTForSequenceClassification(model_of("opt").config).eval()
     with pytest.raises(DzError, match="output embedding"):
         S.generate(scores, ids, 2)
+
+
+@pytest.mark.parametrize("how", [{}, dict(layer_types=["sliding_attention", "full_attention"], use_sliding_window=True), dict(layer_types=["full_attention"] * 2),
+                                 dict(layer_types=["sliding_attention"] * 2, use_sliding_window=True)], ids=str)
+@pytest.mark.parametrize("kind", sorted(S.MODELS))
+def test_windows_are_refused_where_they_are_less_than_all_tokens(kind, how, plain):  # noqa: F811
+    model = model_of(kind, sliding_window=4, **how)
+    ids = torch.randint(2, 211, (1, 9), generator=torch.Generator().manual_seed(1))
+    try:
+        assert same(model, batch(*BATCHES[0]))
+    except DzError as e:
+        assert "window" in str(e)
+    try:
+        assert torch.equal(S.generate(model, ids, 6, temperature=0.0)[0, 0], greedy(model, ids[0], 6))
+    except DzError as e:
+        assert "window" in str(e)
+
+
+def test_a_window_of_the_masks_alone_is_refused(plain):  # noqa: F811
+    ids = torch.randint(2, 211, (1, 9), generator=torch.Generator().manual_seed(1))
+    with pytest.raises(DzError, match="window of 4 of 15 tokens"):
+        S.generate(model_of("phimoe", sliding_window=4), ids, 6)
+    model = model_of("phimoe", sliding_window=15)
+    assert torch.equal(S.generate(model, ids, 6, temperature=0.0)[0, 0], greedy(model, ids[0], 6))
