@@ -124,7 +124,7 @@ def _check_model(model, tokens: int) -> None:
     # (some models have a window in their masks only, which the attention is not told of)
     for name in ("sliding_window", "attention_chunk_size"):
         window = getattr(config, name, None)
-        if window is not None and window < tokens:
+        if window and window < tokens:  # (0: none)
             raise DzError(f"shared_prompt: attention with a window of {window} of {tokens} tokens ({name})")
 
 
