@@ -108,6 +108,11 @@ MODELS = frozenset("""apertus arcee bitnet cwm ernie4_5 ernie4_5_moe exaone4 gem
     phimoe qwen2 qwen2_moe qwen3 qwen3_moe seed_oss smollm3 starcoder2""".split())
 
 
+# Of these, the ones that learn a vector for each position and count the padding on a sequence's left, too, where they are given no
+# positions. (The others take positions from the mask, or nothing but the distance between two tokens matters to them.)
+COUNT_PADS = frozenset(("gpt2", "gpt_bigcode"))
+
+
 def _check_model(model, tokens: int) -> None:
     """Whether the model's answers to sequences of up to `tokens` are what its layers and output embedding give here."""
     config = model.config
@@ -157,7 +162,8 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     (attention_mask 0), that differ in their last option_len tokens only.
 
     option_len: integers on the host, at least 1. Tokens that equal pad_id are left out, as there. Examples whose
-    sequences do not share their prompt give NaN. (A sequence's last token predicts nothing that is read and is not
+    sequences do not share their prompt give NaN, and so do those of a model that counts padding (COUNT_PADS) whose sequences
+    have their prompt in other places. (A sequence's last token predicts nothing that is read and is not
     computed, so that candidates of one token cost nothing beyond the prompt.)"""
     if torch.is_grad_enabled():
         raise DzError("shared_prompt_logprobs: nothing is recorded by autograd, call it under torch.no_grad()")
@@ -178,11 +184,16 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     prompts = input_ids.gather(1, from_pads).view(examples, candidates, room)
     inside = place < first.view(examples, 1, 1)
     same = ((prompts == prompts[:, :1]) | ~inside).all(-1) & (prompt_len == prompt_len[:, :1]) & (prompt_len > 0)
+    before = 0  # a prompt's first position
+    if model.config.model_type in COUNT_PADS:
+        places = pads.view(examples, candidates)
+        same &= places == places[:, :1]
+        before = places[:, :1]
     last = torch.arange(most, device=device)
     targets = input_ids.gather(1, (length - options.unsqueeze(1) + last).clamp_(max=length - 1))  # (sequences, most)
     ids = torch.cat([prompts[:, 0], targets[:, :each].reshape(examples, candidates * each)], 1)
     steps = (first.unsqueeze(1) + last[:each]).repeat(1, candidates)
-    positions = torch.cat([place.expand(examples, room), steps], 1)
+    positions = torch.cat([place.expand(examples, room), steps], 1) + before
     # (places that hold no token of a sequence repeat one, and nothing that is read sees them)
     positions = positions.clamp_(0, length - 1)
 

@@ -55,6 +55,22 @@ def test_prompts_of_one_length(kind, plain):  # noqa: F811
     assert torch.equal(S.generate(model, ids, 6, temperature=0.0)[0, 0], greedy(model, ids[0], 6))
 
 
+@pytest.mark.parametrize("kind", sorted(S.MODELS))
+def test_prompts_of_several_lengths(kind, plain):  # noqa: F811
+    model = model_of(kind)
+    assert same(model, batch(*BATCHES[1]))
+    if kind not in S.COUNT_PADS:
+        assert same(model, batch(*BATCHES[2]))
+
+
+@pytest.mark.parametrize("kind", sorted(S.COUNT_PADS))
+def test_prompts_in_other_places_of_models_that_count_padding(kind, plain):  # noqa: F811
+    b = batch(*BATCHES[2])  # candidates of 2 and 4 tokens: their prompts start two places apart
+    with torch.no_grad():
+        got = S.shared_prompt_logprobs(model_of(kind), b["input_ids"], b["attention_mask"], b["option_len"].tolist(), 2, PAD)
+    assert torch.equal(torch.isnan(got), torch.tensor([False, True] * 3))
+
+
 @pytest.mark.parametrize("kind", ["bert", "roberta", "roberta-prelayernorm", "xlm-roberta", "data2vec-text", "modernbert-decoder"])
 def test_models_whose_head_is_more_than_an_embedding_are_refused(kind, plain):  # noqa: F811
     model = model_of(kind)
