@@ -155,6 +155,46 @@ def _hidden(model, input_ids: torch.Tensor, position_ids: torch.Tensor, layout) 
     return hidden
 
 
+class _Prompts:
+    """Where the prompts of a batch of candidates lie: sequences of [padding | prompt | option]."""
+
+    def __init__(self, model, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], option_len, candidates: int):
+        sequences, length = input_ids.shape
+        device, examples = input_ids.device, sequences // candidates
+        self.options = torch.as_tensor(option_len, device=device)
+        columns = torch.arange(length, device=device)
+        if attention_mask is None:
+            self.pads, padded_left = torch.zeros_like(self.options), True
+        else:
+            there = attention_mask != 0
+            self.pads = length - there.sum(1)
+            padded_left = (there == (columns >= self.pads.unsqueeze(1))).all(1).view(examples, candidates)
+        self.length = (length - self.pads - self.options).view(examples, candidates)
+        self.first = self.length[:, 0]
+        self.room = length - min(option_len)
+        self.place = columns[:self.room]
+        from_pads = (self.pads.unsqueeze(1) + self.place).clamp_(max=length - 1)
+        self.tokens = input_ids.gather(1, from_pads).view(examples, candidates, self.room)  # prompts from their first token on
+        # Of each sequence: whether its prompt lies as its example's first, and whether it has the same tokens there.
+        self.placed = (self.length == self.length[:, :1]) & (self.length > 0) & padded_left
+        self.before = 0  # a prompt's first position
+        if model.config.model_type in COUNT_PADS:
+            pads = self.pads.view(examples, candidates)
+            self.placed &= pads == pads[:, :1]
+            self.before = pads[:, :1]
+        self.alike = ((self.tokens == self.tokens[:, :1]) | (self.place >= self.first.view(examples, 1, 1))).all(-1)
+
+
+def shares_prompts(model, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], option_len, candidates: int, *,
+                   tokens: bool = True) -> bool:
+    """Whether the candidates of each example of a batch, as shared_prompt_logprobs takes it, have one prompt: in the same
+    places and (unless tokens is False) with the same tokens. The host waits for the answer."""
+    if attention_mask is not None and attention_mask.shape != input_ids.shape:
+        return False
+    p = _Prompts(model, input_ids, attention_mask, option_len, candidates)
+    return bool((p.placed & p.alike if tokens else p.placed).all())
+
+
 def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], option_len, candidates: int,
                            pad_id: Optional[int]) -> torch.Tensor:
     """The mean log probability of each sequence's last option_len tokens, (sequences,) in the logits' dtype: what
@@ -172,28 +212,16 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
         raise DzError(f"shared_prompt_logprobs: {sequences} sequences of {length} tokens, {candidates} candidates each, option_len {list(option_len)[:8]}")
     _check_model(model, length)
     device, examples, most = input_ids.device, sequences // candidates, max(option_len)
-    room, each = length - min(option_len), most - 1
-    options = torch.as_tensor(option_len, device=device)
-    pads = torch.zeros_like(options) if attention_mask is None else length - attention_mask.to(torch.int64).sum(1)
-    prompt_len = (length - pads - options).view(examples, candidates)
-    first = prompt_len[:, 0]
+    each = most - 1
+    p = _Prompts(model, input_ids, attention_mask, option_len, candidates)
+    options, room, place, first, same = p.options, p.room, p.place, p.first, p.placed & p.alike
 
-    # prompts from their first token on, then what each candidate adds to them
-    place = torch.arange(room, device=device)
-    from_pads = (pads.unsqueeze(1) + place).clamp_(max=length - 1)
-    prompts = input_ids.gather(1, from_pads).view(examples, candidates, room)
-    inside = place < first.view(examples, 1, 1)
-    same = ((prompts == prompts[:, :1]) | ~inside).all(-1) & (prompt_len == prompt_len[:, :1]) & (prompt_len > 0)
-    before = 0  # a prompt's first position
-    if model.config.model_type in COUNT_PADS:
-        places = pads.view(examples, candidates)
-        same &= places == places[:, :1]
-        before = places[:, :1]
+    # prompts, then what each candidate adds to them
     last = torch.arange(most, device=device)
     targets = input_ids.gather(1, (length - options.unsqueeze(1) + last).clamp_(max=length - 1))  # (sequences, most)
-    ids = torch.cat([prompts[:, 0], targets[:, :each].reshape(examples, candidates * each)], 1)
+    ids = torch.cat([p.tokens[:, 0], targets[:, :each].reshape(examples, candidates * each)], 1)
     steps = (first.unsqueeze(1) + last[:each]).repeat(1, candidates)
-    positions = torch.cat([place.expand(examples, room), steps], 1) + before
+    positions = torch.cat([place.expand(examples, room), steps], 1) + p.before
     # (places that hold no token of a sequence repeat one, and nothing that is read sees them)
     positions = positions.clamp_(0, length - 1)
 

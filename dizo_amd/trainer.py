@@ -95,7 +95,9 @@ class ZOArguments:
     # build-specific: compute the prompt that an example's candidates share
     # once instead of once for each (dizo_amd.shared_prompt): the forwards of
     # the classification loss get one row per example. The loss agrees to
-    # rounding; batches that have another form run as they do otherwise
+    # rounding; batches that have another form run as they do otherwise, and
+    # so do those whose candidates do not have one prompt (cut from the left,
+    # say). The host looks at each batch's prompts before its forward
     zo_shared_prompt: bool = False
     # build-specific: run each OPT decoder layer's fc1 + ReLU as one GEMM with
     # a ReLU epilogue, and its k/v/q projections as one GEMM over a [k; v; q]
@@ -240,24 +242,29 @@ def option_len_loss(model, build_graph: bool, input_ids=None, labels=None, optio
     arithmetic is the same; the LM-head GEMM has fewer rows, so the logits,
     and with them the loss, can differ from the full-logit ones by rounding.
     Shared prompt (``model.dz_shared_prompt``, without an autograd graph and with
-    return_dict): where every example has the same number of candidates, each
-    example's prompt is computed once (dizo_amd.shared_prompt); the loss agrees
-    to rounding, and is NaN where an example's candidates have other prompts.
+    return_dict): where every example has the same number of candidates, with
+    one prompt, each example's prompt is computed once (dizo_amd.shared_prompt);
+    the loss agrees to rounding. Other batches run whole sequences; only where
+    dz_shared_prompt is True and nothing but the tokens of prompts of one length
+    differ is the loss NaN ("or whole", which the trainer sets, runs those too).
 
     With the option head and return_dict falsy the logits returned are the
     window's. dz_window = 0 asks for the full logits without looking at
     option_len (a captured graph decides the window on the host beforehand).
     """
-    if (getattr(model, "dz_shared_prompt", False) and not build_graph and return_dict and dz_window is None
+    shared = getattr(model, "dz_shared_prompt", False)
+    if (shared and not build_graph and return_dict and dz_window is None
             and labels is not None and option_len is not None and num_options is not None and set(kwargs) <= {"attention_mask"}):
         lens, nopt = host_ints(option_len), host_ints(num_options)
         if (all(x == nopt[0] for x in nopt) and input_ids.shape[0] % nopt[0] == 0 and len(lens) == input_ids.shape[0]
                 and 0 < min(lens) <= max(lens) < input_ids.shape[1]):
-            from .shared_prompt import shared_prompt_logprobs
+            from .shared_prompt import shared_prompt_logprobs, shares_prompts
 
-            with torch.no_grad():
-                selected = shared_prompt_logprobs(model, input_ids, kwargs.get("attention_mask"), lens, nopt[0], model.config.pad_token_id)
-                return SimpleNamespace(loss=_candidates_loss(selected, labels, nopt))
+            mask = kwargs.get("attention_mask")
+            if shares_prompts(model, input_ids, mask, lens, nopt[0], tokens=shared is not True):
+                with torch.no_grad():
+                    selected = shared_prompt_logprobs(model, input_ids, mask, lens, nopt[0], model.config.pad_token_id)
+                    return SimpleNamespace(loss=_candidates_loss(selected, labels, nopt))
     kwargs.setdefault("use_cache", False)
     window = dz_window
     if (window is None and labels is not None and option_len is not None and num_options is not None
@@ -391,7 +398,7 @@ class ZOTrainerMixin:
         self._pending_update = None   # (seed, eps, g, lr): restore + update of zo_update
         self.kernel_timer = None
         model.dz_option_head = bool(getattr(args, "zo_option_head", False))
-        model.dz_shared_prompt = bool(getattr(args, "zo_shared_prompt", False))
+        model.dz_shared_prompt = "or whole" if getattr(args, "zo_shared_prompt", False) else False
         self.zo_journal = None
         if getattr(args, "zo_journal", False):
             from .checkpoint import ZOJournal
