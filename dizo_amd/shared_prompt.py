@@ -9,13 +9,15 @@ sampling.
                             8 bits, and each answer keeps its own
 
 Both run the model's own layers, OPT's, LLaMA's or others of MODELS, which call the attention HF registers by name, with one of this
-module's in its place (in the model's config, for as long as a forward takes: one call at a time for a model): a forward gets
+module's in its place (in the model's config, for as long as a forward takes: one call at a time for a model, a second one is refused): a forward gets
 one row for each prompt, and the attention is told where things lie by the keyword argument dz_shared. Other models,
 attention with a window, a soft cap or sinks, layers that mix tokens in another way, and heads that do more than multiply by the
 output embedding are refused. Nothing is recorded by autograd.
 """
 from __future__ import annotations
 
+import contextlib
+import threading
 from typing import Optional, Union
 
 import torch
@@ -26,6 +28,24 @@ from .sampling import sample_tokens
 
 ATTN_IMPL = "dizo_shared_prompt"
 _registered = False
+_lock = threading.Lock()
+_running = set()  # the configs (by id, while a call holds them) whose attention is exchanged
+
+
+@contextlib.contextmanager
+def _alone(model):
+    """One call at a time for a model, or for models of one config: a second one would put the first one's attention back as the
+    model's own, and take it out of evaluation in the middle of an answer."""
+    config = model.config
+    with _lock:
+        if id(config) in _running or config._attn_implementation == ATTN_IMPL:
+            raise DzError(f"shared_prompt: another call of this {type(model).__name__} is not through")
+        _running.add(id(config))
+    try:
+        yield
+    finally:
+        with _lock:
+            _running.discard(id(config))
 
 
 class _Candidates:
@@ -225,7 +245,8 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     # (places that hold no token of a sequence repeat one, and nothing that is read sees them)
     positions = positions.clamp_(0, length - 1)
 
-    hidden = _hidden(model, ids, positions, _Candidates(room, candidates, each, first.to(torch.int32)))
+    with _alone(model):
+        hidden = _hidden(model, ids, positions, _Candidates(room, candidates, each, first.to(torch.int32)))
     width = hidden.shape[-1]
     ends = hidden.gather(1, (first - 1).clamp(min=0).view(examples, 1, 1).expand(examples, 1, width))
     rows = torch.cat([ends.unsqueeze(1).expand(examples, candidates, 1, width), hidden[:, room:].view(examples, candidates, each, width)], 2)
@@ -267,14 +288,15 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, answers: in
     lengths = prompt_lengths.clamp(1, room)
     if uniform is None:
         uniform = torch.rand(prompts, answers, max_new_tokens, generator=generator, device=device)
-    training = model.training
-    model.eval()
-    try:
-        return _draw(model, input_ids, max_new_tokens, answers, lengths, uniform, eos_token_id, kv_bits,
-                     dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
-    finally:
-        if training:
-            model.train()
+    with _alone(model):
+        training = [m for m in model.modules() if m.training]
+        model.eval()
+        try:
+            return _draw(model, input_ids, max_new_tokens, answers, lengths, uniform, eos_token_id, kv_bits,
+                         dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
+        finally:
+            for m in training:
+                m.training = True
 
 
 def _draw(model, input_ids, max_new_tokens, answers, lengths, uniform, eos_token_id, kv_bits, sampling) -> torch.Tensor:
