@@ -227,13 +227,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
   const float u = a.uniform[r];
   const double temperature = a.temperatures ? a.temperatures[r] : a.temperature;
   const double top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p = a.min_ps ? a.min_ps[r] : a.min_p;
-  const int32_t top_k = temperature == 0 ? 1 : a.top_ks ? a.top_ks[r] : a.top_k;
+  const int32_t row_k = a.top_ks ? a.top_ks[r] : a.top_k, top_k = temperature == 0 ? 1 : row_k;
   const double unit = temperature == 0 ? 1.0 : temperature;
 
   for (int i = tid; i < kPowers; i += kThreads) sh.powers[i] = exp2(i / (double)kPowers - 2.0);
   for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
   if (tid == 0) sh.listed = 0;
-  bool none = !(u >= 0.f && u <= 1.f) || !(temperature == 0 || (temperature >= 0x1p-63 && temperature < 0x1p64)) || top_p != top_p || min_p != min_p;
+  bool none = !(u >= 0.f && u <= 1.f) || !(temperature == 0 || (temperature >= 0x1p-63 && temperature < 0x1p64)) || row_k < 0 ||
+              !(top_p >= 0 && top_p <= 1) || !(min_p >= 0 && min_p <= 1);
   float mine = -INFINITY;  // the largest of this thread's
   row.first([&](float x, float y) {
     mine = fmaxf(fmaxf(mine, x), y);
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleRows a) {
     return high;
   };
   // min_p as the least logit that it keeps; the largest is always kept
-  const double least_place = min_p > 0 ? kPowers * (fmin(log2(min_p), 0.0) + (shift + 2)) : 0.0;
+  const double least_place = min_p > 0 ? kPowers * (log2(min_p) + (shift + 2)) : 0.0;
 
   auto clear = [&]() {
     for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;

@@ -352,7 +352,7 @@ int32_t dz_cache_read(const dz_keys_values* cache, const dz_keys_values* kv, int
  * elements, logits_stride apart), drawn by uniform[r] (0 to 1) from softmax(logits_r /
  * temperature) restricted to its top_k largest (0: no limit; equal logits by
  * token), of these to the fewest, largest first, that hold top_p of their
- * probability (1 or more: all), and of these to those of at least min_p times the
+ * probability (1: all), and of these to those of at least min_p times the
  * largest one's: the first token up to which the sum of what is left exceeds uniform[r]
  * of the whole. Weights are kept as whole numbers of 2^-46 of the largest (2^-42 for
  * the longest rows), so that results do not depend on an order. Temperature 0
