@@ -184,6 +184,12 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   // Weights of codes carry their row's power of two, which may leave the range of fp16: those are bf16 (and codes are bf16 numbers).
   using TV = std::conditional_t<STORE == kCodes && std::is_same_v<T, TypeF16>, TypeBF16, T>;
   using FragV = typename Op<TV>::Frag;
+  // Weights are 2^(s + kBias - m), where m trails the row's largest score by kLag at most: sums change their scale a few times, and not
+  // with each tile. fp16 weights are taken up to 2^15 that way, so that they have all of their bits down to 2^-25 of the row's largest, and
+  // what rounds to 0 is below 2^-36 of it: 2^24 keys of that lose 2^-12 (with the largest at 1, 2^20 keys of 2^-26 would be lost
+  // whole, 1.6 % of the result). bf16 has fp32's range.
+  constexpr bool kHalf = std::is_same_v<TV, TypeF16>;
+  constexpr float kBias = kHalf ? 11.f : 0.f, kLag = kHalf ? 4.f : 8.f;
   constexpr int CH = S::CH, KT = S::KT, NK = KT / 32;
   constexpr bool BYTES = STORE != kOperands;
   __shared__ __attribute__((aligned(256))) char lds[S::SLABS][S::STAGES][2][S::TILE];
@@ -454,8 +460,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
     top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * c;
-    // Weights may exceed 1 by 2^8 before their maximum is taken up: sums change their scale a few times, and not with each tile.
-    if (__any(top > m + 8.f)) {
+    if (__any(top > m + kLag)) {
       const float m2 = fmaxf(m, top);
       const float f = m2 == -INFINITY ? 1.f : exp2_hw(m - m2);
       m = m2;
@@ -463,7 +468,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
 #pragma unroll
       for (int d = 0; d < S::PV; ++d) o[d] *= f;
     }
-    const float mm = m == -INFINITY ? 0.f : m;
+    const float mm = m == -INFINITY ? 0.f : m - kBias;
     // Weights of 16 keys at a time (those of 8 a lane), each next to the products with the 16 before: their values are read one such
     // group ahead.
     FragV w[GROUPS];
@@ -542,6 +547,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     }
   }
   l = both_halves(l, [](float x, float y) { return x + y; });
+  m -= kBias;  // what the sums are relative to
 
   if constexpr (BY_KEYS) {
     // The waves' sums against the largest of their maxima.
