@@ -181,14 +181,15 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   using S = Shape<T, QS, BY_KEYS, STORE, OF_WAVES>;
   using Elem = typename T::Elem;
   using Frag = typename Op<T>::Frag;
-  // Weights of codes carry their row's power of two, which may leave the range of fp16: those are bf16 (and codes are bf16 numbers).
+  // Weights of codes carry their row's power of two, which may leave the range of fp16: those are bf16 (and codes are bf16 numbers), for
+  // fp16 results two of them, the nearest one and the nearest to what that leaves: 2^-16 of a weight at most.
   using TV = std::conditional_t<STORE == kCodes && std::is_same_v<T, TypeF16>, TypeBF16, T>;
   using FragV = typename Op<TV>::Frag;
   // Weights are 2^(s + kBias - m), where m trails the row's largest score by kLag at most: sums change their scale a few times, and not
   // with each tile. fp16 weights are taken up to 2^15 that way, so that they have all of their bits down to 2^-25 of the row's largest, and
   // what rounds to 0 is below 2^-36 of it: 2^24 keys of that lose 2^-12 (with the largest at 1, 2^20 keys of 2^-26 would be lost
   // whole, 1.6 % of the result). bf16 has fp32's range.
-  constexpr bool kHalf = std::is_same_v<TV, TypeF16>;
+  constexpr bool kHalf = std::is_same_v<TV, TypeF16>, kTwo = std::is_same_v<T, TypeF16> && !kHalf;
   constexpr float kBias = kHalf ? 11.f : 0.f, kLag = kHalf ? 4.f : 8.f;
   constexpr int CH = S::CH, KT = S::KT, NK = KT / 32;
   constexpr bool BYTES = STORE != kOperands;
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     const float mm = m == -INFINITY ? 0.f : m - kBias;
     // Weights of 16 keys at a time (those of 8 a lane), each next to the products with the 16 before: their values are read one such
     // group ahead.
-    FragV w[GROUPS];
+    FragV w[GROUPS], rest[kTwo ? GROUPS : 1];
     auto weights = [&](int g) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -484,6 +485,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
           l += e;
           if (STORE == kCodes) e *= power[r];
           w[g][4 * b + r] = (typename TV::Elem)e;
+          if constexpr (kTwo) rest[g][4 * b + r] = (typename TV::Elem)(e - (float)w[g][4 * b + r]);
         }
       }
     };
@@ -493,8 +495,11 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
       if (g + 1 < GROUPS) read_group(g + 1);
 #pragma unroll
       for (int d = 0; d < S::PV; ++d) {
-        if constexpr (STORE == kCodes) o[d] = Op<TV>::mma(Op<TV>::widen8(values[g % 2][d], 1.f), w[g], o[d]);
-        else o[d] = Op<TV>::mma(values[g % 2][d], w[g], o[d]);
+        if constexpr (STORE == kCodes) {
+          const FragV v = Op<TV>::widen8(values[g % 2][d], 1.f);
+          o[d] = Op<TV>::mma(v, w[g], o[d]);
+          if constexpr (kTwo) o[d] = Op<TV>::mma(v, rest[g], o[d]);
+        } else o[d] = Op<TV>::mma(values[g % 2][d], w[g], o[d]);
       }
       if (g + 1 < GROUPS) weights(g + 1);
       if (!S::kWide) __builtin_amdgcn_sched_barrier(0);

@@ -307,9 +307,9 @@ typedef struct dz_keys_values {
  * multiple of 8 up to 128. Lengths and positions outside their ranges are taken
  * as the nearest in it. What slots hold that a query does not see, infinities
  * and NaN too, does not matter to it. Products and sums are fp32; weights are
- * rounded to `dtype` (of an 8-bit store: at least to bf16) before they multiply
- * values, as their sum is taken before: bf16 ones by 2^-8 of each at most, fp16 ones by
- * 2^-11 of each and 2^-36 of the query's largest. Both stores are of
+ * rounded to `dtype`, or less, before they multiply values, as their sum is taken
+ * before: for bf16 by 2^-8 of each at most, for fp16 by 2^-11 of each and 2^-36 of the
+ * query's largest. Both stores are of
  * `dtype`, or both 8-bit, whose values are taken in `dtype`. `out` may not
  * overlap an input. Rows whose sums are NaN are taken again by themselves, key
  * by key: right, and slow where there are many. Replaces, for

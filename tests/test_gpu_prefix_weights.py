@@ -6,7 +6,7 @@ import torch
 
 from dizo_amd import prefix_attention as P
 from oracle import prefix as O
-from test_gpu_prefix_attention import DT, HALF_STEP, bound, stored, values
+from test_gpu_prefix_attention import DT, bound, inputs, stored, values
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -35,4 +35,23 @@ def test_a_key_above_many_others(dtype, bits, length, keys, nats, width):
     most = bound(dtype, out, spread, reach, keys, width, bits) + (keys * 2.0**-36 * float(v.max()) if dtype == "fp16" else 0.0)
     assert (most < out / 4).all() or math.exp(nats) * 64 > keys  # it says something
     far = (got - out).abs()
+    assert (far <= most).all(), f"{float((far / most).max())} times the bound"
+
+
+@pytest.mark.parametrize("shape", [
+    (2, 3, 4, 2, 1, 7, 5, 128),      # codes in whole chunks of 16, by waves with keys for themselves
+    (1, 9, 3, 3, 2, 33, 100, 80),
+    (1, 2, 2, 1, 50, 70, 129, 96),
+    (1, 2, 2, 1, 40, 70, 3000, 64),  # prompts in several parts
+    (2, 3, 4, 2, 1, 7, 5, 120),      # half a chunk at the end
+    (1, 2, 2, 1, 100, 130, 129, 64),  # tiles that waves share
+], ids=str)
+@pytest.mark.parametrize("std", [1.0, 4.0])
+def test_fp16_queries_keep_their_bits_beside_8_bit_stores(shape, std):
+    """However the codes lie: fp16's half step for the weights, and not bf16's."""
+    q, own, pre = inputs(sum(shape), "fp16", *shape, bits=8, std=std)
+    got = P.shared_prefix_attention(q, own, pre).cpu().double()
+    out, spread, reach = O.attend(q, values(own), values(pre), None, None, shape[-1] ** -0.5)
+    far = (got - out).abs()
+    most = bound("fp16", out, spread, reach, shape[5] + shape[6], shape[-1], 16)
     assert (far <= most).all(), f"{float((far / most).max())} times the bound"
