@@ -32,9 +32,10 @@ enum Store {
                // after 6,000 keys: 30 us, through registers 37; waves that share keys would convert each code four times)
 };
 
-// The sums of a row by themselves, key by key: a lane takes a key's score, and then a column or two of the values. For rows
-// whose sums came out as NaN: a product with a weight of 0 is NaN where the value is infinite or NaN, so that one such value reaches
-// all rows that its tile was scored against. Here a row meets the keys that it sees and no others.
+// A row by itself, key by key: a lane takes a key's score, and then a column or two of the values. For rows whose sums are not finite:
+// a product with a weight of 0 is NaN where the value is infinite or NaN, so that one such value reaches all rows that its tile was
+// scored against, and sums of values near fp32's limits may leave it where their mean does not. Here a row meets the keys that it
+// sees and no others, and o is the mean of the values so far.
 template <class T, bool BYTES>
 struct LoneRow {
   using Elem = typename T::Elem;
@@ -65,20 +66,19 @@ struct LoneRow {
     }
     float top = s;
     for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
-    if (top > m) {
-      const float f = exp2_hw(m - top);
-      m = top;
-      l *= f;
-      o[0] *= f;
-      o[1] *= f;
-    }
-    const float e = s == -INFINITY ? 0.f : exp2_hw(s - m);
+    top = fmaxf(top, m);
+    const float e = s == -INFINITY ? 0.f : exp2_hw(s - top);
     float sum = e;
     for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-    l += sum;
+    const float before = l == 0.f ? 0.f : l * exp2_hw(m - top);
+    m = top;
+    l = before + sum;
+    const float part = l == 0.f ? 0.f : 1.f / l;
+    o[0] *= before * part;
+    o[1] *= before * part;
 #pragma unroll 1
     for (uint32_t key = k0; key < k1; ++key) {
-      const float w = __shfl(e, key - k0);
+      const float w = __shfl(e, key - k0) * part;
       const int64_t at = from(kv.v_s, key), power_at = BYTES ? from(kv.v_scale_s, key) : 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -141,13 +141,14 @@ __device__ __forceinline__ void lone_rows(uint32_t first, uint32_t set) {
     for (uint32_t i = 0; i * KT < limit && !done; ++i)
       if (mine(begin + i)) done = x.keys(a, a.own, g, n, item.hk, i * KT, min((i + 1) * KT, limit));
     const uint64_t to_row = item.splits > 1 ? partial_row(plan, item, lane_row) : 0;
-    if (item.splits > 1 && lane == 0) call.partial_ms[to_row] = float2{x.m, x.l};
+    // (a mean: a sum of weights of 1 relative to 2^m of them all)
+    if (item.splits > 1 && lane == 0) call.partial_ms[to_row] = x.l == 0.f ? float2{-INFINITY, 0.f} : float2{x.m + log2_hw(x.l), 1.f};
     Elem* to = (Elem*)a.out + (int64_t)g * a.out_s[0] + (int64_t)n * a.out_s[1] + (int64_t)h * a.out_s[2] + (int64_t)t * a.out_s[3];
     for (int i = 0; i < 2; ++i) {
       const uint32_t col = lane + 64 * i;
       if (col >= (uint32_t)a.width) continue;
       if (item.splits > 1) call.partial[to_row * a.width + col] = x.o[i];
-      else to[col] = (Elem)(prefix_limit + limit == 0 ? 0.f : x.o[i] / x.l);
+      else to[col] = (Elem)(prefix_limit + limit == 0 ? 0.f : x.l == 0.f ? NAN : x.o[i]);
     }
   }
 }
@@ -592,15 +593,15 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
         for (int r = 0; r < 4; ++r) o[d][4 * b + r] += x[r];
       }
   }
-  bool nan = false;
+  bool finite = true;
 #pragma unroll
   for (int d = 0; d < S::PV; ++d)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) nan |= o[d][j] != o[d][j];  // (columns past the width are finite, or the row's first ones again)
-  const uint64_t nan_lanes = __ballot(live && nan);
-  uint32_t nan_rows = (uint32_t)nan_lanes | (uint32_t)(nan_lanes >> 32);
-  if (nan_rows) lone_rows<T, BY_KEYS, BYTES, KT, S::WAVES>(BY_KEYS ? 0 : wave * 32, nan_rows);
-  if (!live || nan_rows >> (lane & 31) & 1) return;
+    for (int j = 0; j < 16; ++j) finite &= fabsf(o[d][j]) < INFINITY;  // (columns past the width are finite, or the row's first ones again)
+  const uint64_t lone_lanes = __ballot(live && !finite);
+  const uint32_t lone = (uint32_t)lone_lanes | (uint32_t)(lone_lanes >> 32);
+  if (lone) lone_rows<T, BY_KEYS, BYTES, KT, S::WAVES>(BY_KEYS ? 0 : wave * 32, lone);
+  if (!live || lone >> (lane & 31) & 1) return;
   if (splits > 1) {
     const uint64_t to_row = partial_row(plan, item, lane_row);
     if (half == 0) call.partial_ms[to_row] = float2{m, l};
@@ -643,14 +644,23 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, AttendPlan plan, co
   for (int i = 0; i < plan.splits; ++i) m = fmaxf(m, partial_ms[from + (uint64_t)i * plan.tile_rows].x);
   float l = 0.f;
   f32x4 o = f32x4(0.f);
-#pragma unroll 4
-  for (int i = 0; i < plan.splits; ++i) {
+  auto add = [&](int i) {
     const uint64_t at = from + (uint64_t)i * plan.tile_rows;
     const float2 ms = partial_ms[at];
     const f32x4 x = *(const f32x4*)(partial + at * a.width + col);
     const float f = ms.x == -INFINITY ? 0.f : exp2_hw(ms.x - m);  // (saw no key)
     l = __builtin_fmaf(ms.y, f, l);
     o += x * f;
+  };
+#pragma unroll 4
+  for (int i = 0; i < plan.splits; ++i) add(i);
+  const f32x4 nothing = o - o;
+  if (nothing[0] + nothing[1] + nothing[2] + nothing[3] != 0.f) {  // not finite: the sums of up to 64 finite parts are, as 2^-8 of themselves
+    m += 8.f;
+    l = 0.f;
+    o = f32x4(0.f);
+#pragma unroll 1
+    for (int i = 0; i < plan.splits; ++i) add(i);
   }
   const uint32_t gh = item / plan.tiles, row = t.row0 + lane_row, g = gh / a.kv_heads, h = gh % a.kv_heads * shared + row % shared;
   const float inv = prefix_keys(a, g) + own_keys(a, g, row / seq_rows, row % seq_rows / shared) == 0 ? 0.f : 1.f / l;

@@ -311,8 +311,8 @@ typedef struct dz_keys_values {
  * before: for bf16 by 2^-8 of each at most, for fp16 by 2^-11 of each and 2^-36 of the
  * query's largest. Both stores are of
  * `dtype`, or both 8-bit, whose values are taken in `dtype`. `out` may not
- * overlap an input. Rows whose sums are NaN are taken again by themselves, key
- * by key: right, and slow where there are many. Replaces, for
+ * overlap an input. Rows whose sums are not finite are taken again by themselves,
+ * key by key: right, and slow where there are many. Replaces, for
  * candidates that share a prompt, the attention of the forwards in
  * trainer.py:1524-1542, which repeats it for each. */
 typedef struct dz_attention {
