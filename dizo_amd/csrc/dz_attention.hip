@@ -32,6 +32,11 @@ enum Store {
                // after 6,000 keys: 30 us, through registers 37; waves that share keys would convert each code four times)
 };
 
+// What an e8m0 scale stands for: 2^(s - 127), 0 being fp32's subnormal one, and NaN for 255. (The conversions of codes take s << 23 for that.)
+__device__ __forceinline__ float power_of(uint32_t s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
+}
+
 // A row by itself, key by key: a lane takes a key's score, and then a column or two of the values. For rows whose sums are not finite:
 // a product with a weight of 0 is NaN where the value is infinite or NaN, so that one such value reaches all rows that its tile was
 // scored against, and sums of values near fp32's limits may leave it where their mean does not. Here a row meets the keys that it
@@ -44,7 +49,7 @@ struct LoneRow {
   uint32_t lane = threadIdx.x & 63;
 
   __device__ static float value(const void* x, const uint8_t* power, int64_t at, int64_t power_at) {
-    if constexpr (BYTES) return __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)x)[at], 0) * __uint_as_float((uint32_t)power[power_at] << 23);
+    if constexpr (BYTES) return __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)x)[at], 0) * power_of(power[power_at]);
     return (float)((const Elem*)x)[at];
   }
   // Keys k0 ... k1 - 1, 64 at most; true when the answer is NaN whatever follows.
@@ -191,7 +196,8 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
   // what rounds to 0 is below 2^-36 of it: 2^24 keys of that lose 2^-12 (with the largest at 1, 2^20 keys of 2^-26 would be lost
   // whole, 1.6 % of the result). bf16 has fp32's range.
   constexpr bool kHalf = std::is_same_v<TV, TypeF16>, kTwo = std::is_same_v<T, TypeF16> && !kHalf;
-  constexpr float kBias = kHalf ? 11.f : 0.f, kLag = kHalf ? 4.f : 8.f;
+  // Those of codes times powers of two are taken 2^16 higher, to have bits left at 2^-127, the least power there is.
+  constexpr float kBias = kHalf ? 11.f : STORE == kCodes ? 16.f : 0.f, kLag = kHalf ? 4.f : 8.f;
   constexpr int CH = S::CH, KT = S::KT, NK = KT / 32;
   constexpr bool BYTES = STORE != kOperands;
   __shared__ __attribute__((aligned(256))) char lds[S::SLABS][S::STAGES][2][S::TILE];
@@ -370,7 +376,7 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
     const char* vt = slab[stage][1];
     f32x16 s[NK];
     if constexpr (STORE == kCodes) {
-      if (half == 0) powers[wave][lane] = __uint_as_float((uint32_t)pow.v << 23);
+      if (half == 0) powers[wave][lane] = power_of(pow.v);
       const float power = __uint_as_float((uint32_t)pow.k << 23);
       const uint32_t r = lane & 31;
       s[0] = f32x16(0.f);
