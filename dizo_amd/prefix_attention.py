@@ -258,8 +258,9 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, positions:
     number for all sequences, or int32 (...), one for each (tokens that fall outside of the cache are left out then).
 
     A row (one token's head) is kept as code * 2^e: e the least, from -100, that leaves nothing above 448, and codes
-    rounded to the nearest e4m3 number, ties to even. fp16 numbers beyond 61440 are kept as that. A row with an infinity
-    or a NaN becomes NaN."""
+    rounded to the nearest e4m3 number, ties to even (e = 0 for a row of zeros). Numbers beyond 240 * 2^8 (fp16) or
+    240 * 2^120 (the others), the last before a power of two that the type does not have, are kept as that. A row with an
+    infinity or a NaN becomes NaN."""
     what = "cache_write"
     batch, n, fields = _cache_fields(what, cache)
     shape, got = cache.k.shape, k.shape

@@ -339,9 +339,9 @@ int32_t dz_shared_prefix_attention(const dz_attention* a, void* workspace, int64
  * strides: batch, unused, head, token) into an 8-bit store (batch, unused, head,
  * slot) from slot positions[b] on (NULL: `position` for all). Tokens that fall outside
  * of the store's slots are left out. A row (one token's head) is kept as code
- * 2^e, with e the least (from -100) that leaves nothing above 448 and codes rounded to
- * nearest even. fp16 numbers above 61440 are kept as that. A row with an infinity or
- * NaN becomes NaN. dz_cache_read gives code 2^e in `dtype`, of slots
+ * 2^e, with e the least (from -100; 0 for a row of zeros) that leaves nothing above 448
+ * and codes rounded to nearest even. Numbers beyond 240 2^8 (fp16) or 240 2^120 (the
+ * others) are kept as that. A row with an infinity or NaN becomes NaN. dz_cache_read gives code 2^e in `dtype`, of slots
  * position .. position + length - 1. */
 int32_t dz_cache_write(const dz_keys_values* kv, const dz_keys_values* cache, int32_t dtype, int64_t batch, int64_t heads,
                        int64_t length, int64_t width, int64_t slots, const int32_t* positions, int64_t position,

@@ -95,3 +95,22 @@ def test_reading_scales_of_every_kind(dtype):
     for got in P.cache_read(cache, 256, DT[dtype]):
         got = got.cpu()
         assert ((got == want) | (torch.isnan(got) & torch.isnan(want))).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_the_largest_numbers_are_kept(dtype):
+    """The nearest code of a number above 248 2^120 stands for 2^128, which is none of fp32 or bf16."""
+    top = torch.finfo(DT[dtype]).max
+    k = torch.ones(1, 9, 16, dtype=DT[dtype], device=DEV)
+    for i, x in enumerate((1.0, 0.99, 0.98, 0.97, 0.9375, 0.93, 0.9, 0.875, 0.5)):
+        k[0, i, 3] = x * top
+        k[0, i, 4] = -x * top
+    cache = P.QuantizedKV.empty(1, 9, 16, device=DEV)
+    P.cache_write(cache, k, -k, 0)
+    got = P.cache_read(cache, 9, DT[dtype])
+    most = 240.0 * 2.0 ** (8 if dtype == "fp16" else 120)
+    kept = k.cpu().double().clamp(-most, most)
+    far = (got.k.cpu().double() - kept).abs()
+    # half a step of a code: 2^-4 of the value, or 2^-10 of 2^e
+    assert (far <= torch.maximum(kept.abs() * 2.0**-4, torch.tensor(2.0**-10 * most / 240, dtype=torch.float64))).all()
+    assert torch.equal(got.v, -got.k) and torch.isfinite(got.k).all()
