@@ -168,6 +168,15 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
             _fail(what, "one of own and prefix is an 8-bit store and the other is not")
     positions = _check_int32(what, "positions", positions, (groups, sequences), index)
     prefix_lengths = _check_int32(what, "prefix_lengths", prefix_lengths, (groups,), index)
+    if scale is None:
+        scale = width ** -0.5 if width else 1.0
+    else:
+        try:
+            scale = float(scale)
+        except (TypeError, ValueError, OverflowError):
+            _fail(what, f"scale must be a number, got {scale!r}")
+        if not 0.0 < scale <= 2.0**126:
+            _fail(what, f"scale must be positive, 2^126 at most, got {scale}")
     if out is None:
         out = torch.empty_like(q)
         if out.stride(-1) != 1 or width * out.element_size() % 16:
@@ -197,8 +206,7 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
             prefix_f = (*prefix_f[:10], prefix[2].data_ptr(), prefix[3].data_ptr(), a, 0, b, c, d, 0, e, f)
     args = _ATTENTION.pack(q.data_ptr(), out.data_ptr(), *qs, *out.stride()[:4], *own_f, *prefix_f,
                            0 if positions is None else positions.data_ptr(), 0 if prefix_lengths is None else prefix_lengths.data_ptr(),
-                           groups, sequences, heads, kv_heads, length, width, slots, prefix_slots, code,
-                           width ** -0.5 if scale is None else scale)
+                           groups, sequences, heads, kv_heads, length, width, slots, prefix_slots, code, scale)
     need = C.c_int64()
     L.call("dz_shared_prefix_attention_workspace", args, C.byref(need))
     need = need.value
@@ -278,6 +286,8 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, positions:
         position = _whole(what, "positions", positions)
     if not k.numel():
         return
+    if at is None and not 0 <= position <= slots - length:
+        _fail(what, f"tokens {position} to {position + length} do not fit {slots} slots")
     if n > 1:
         k, v = k.flatten(0, n - 1), v.flatten(0, n - 1)
     elif n == 0:

@@ -23,7 +23,7 @@ def _parameter(what: str, name: str, value, lead, device, dtype):
     if not torch.is_tensor(value):
         try:
             return (operator.index if dtype == torch.int32 else float)(value), None
-        except (TypeError, ValueError):
+        except (TypeError, ValueError, OverflowError):
             _fail(what, f"{name} must be a number or a tensor of one for each row, got {value!r}")
     _check_rows(what, name, value, lead, device, (dtype,))
     return 0, _dense(value)
