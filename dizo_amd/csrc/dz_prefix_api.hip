@@ -76,6 +76,37 @@ int32_t check_distinct(const int64_t (&dims)[4], const int64_t* strides, int64_t
 
 bool overlap(const Extent& a, const Extent& b) { return a.first < b.end && b.first < a.end; }
 
+// Whether two tensors of the same dimensions, by strides in bytes, share none. They lie apart, or their outer dimensions have the same
+// strides, and what lies inside of these is apart and fits into the least of them: rows of keys and values in turn, or
+// codes with their scales behind them.
+bool apart(const int64_t (&dims)[4], const Extent& a, const int64_t* a_strides, const Extent& b, const int64_t* b_strides) {
+  if (!overlap(a, b)) return true;
+  int order[4], n = 0;  // the largest stride first, dimensions of one element aside
+  for (int i = 0; i < 4; ++i) {
+    if (dims[i] == 1) continue;
+    int at = n++;
+    for (; at > 0 && a_strides[order[at - 1]] < a_strides[i]; --at) order[at] = order[at - 1];
+    order[at] = i;
+  }
+  int64_t a_size = (int64_t)(a.end - a.first), b_size = (int64_t)(b.end - b.first);
+  const int64_t off = (int64_t)(b.first - a.first);
+  for (int outer = 0; outer < n; ++outer) {
+    const int64_t stride = a_strides[order[outer]], steps = dims[order[outer]] - 1;
+    if (b_strides[order[outer]] != stride) return false;
+    a_size -= steps * stride;
+    b_size -= steps * stride;
+    if (off < a_size && -off < b_size) continue;
+    int64_t span = (off + b_size > a_size ? off + b_size : a_size) - (off < 0 ? off : 0);
+    bool fits = true;
+    for (int i = outer; i >= 0 && fits; --i) {
+      fits = a_strides[order[i]] >= span;
+      span += (dims[order[i]] - 1) * a_strides[order[i]];
+    }
+    if (fits) return true;
+  }
+  return false;
+}
+
 #define DZ_TRY(expr)             \
   do {                           \
     const int32_t rc_ = (expr);  \
@@ -186,14 +217,16 @@ int32_t cache_call(const dz_keys_values* kv, const dz_keys_values* cache, int32_
     return invalid("tokens " + std::to_string(position) + " to " + std::to_string(position + length) + " do not fit " + std::to_string(slots) + " slots");
   if (!rows) return DZ_OK;
   const int64_t es = size_of(dtype), in_dims[4] = {batch, 1, heads, length}, dims[4] = {batch, 1, heads, slots};
-  Extent x[2], c[4];
+  Extent x[2], c[4], at{};
   DZ_TRY(check_tensor(kv->k, es, in_dims, kv->k_strides, width, 16, "k", x));
   DZ_TRY(check_tensor(kv->v, es, in_dims, kv->v_strides, width, 16, "v", x + 1));
   if (!cache->k_scales || !cache->v_scales) return invalid("cache scales are NULL");
   DZ_TRY(check_store(*cache, dtype, true, dims, width, "cache", c));
   if (positions) {
     const int64_t all[4] = {1, 1, 1, batch}, dense[4] = {0, 0, 0, 1};
-    DZ_TRY(check_tensor(positions, 4, all, dense, 1, 4, "positions", nullptr));
+    DZ_TRY(check_tensor(positions, 4, all, dense, 1, 4, "positions", &at));
+    for (const Extent& f : c)
+      if (overlap(at, f)) return invalid("the cache overlaps positions");
   }
   if (read) {
     DZ_TRY(check_distinct(in_dims, kv->k_strides, width, "k"));
@@ -204,6 +237,10 @@ int32_t cache_call(const dz_keys_values* kv, const dz_keys_values* cache, int32_
     DZ_TRY(check_distinct(dims, cache->v_strides, width, "cache values"));
     DZ_TRY(check_distinct(dims, cache->k_scale_strides, 1, "cache key scales"));
     DZ_TRY(check_distinct(dims, cache->v_scale_strides, 1, "cache value scales"));
+    const int64_t* const strides[4] = {cache->k_strides, cache->v_strides, cache->k_scale_strides, cache->v_scale_strides};
+    for (int i = 0; i < 4; ++i)
+      for (int j = i + 1; j < 4; ++j)
+        if (!apart(dims, c[i], strides[i], c[j], strides[j])) return invalid("the cache's keys, values or scales overlap");
   }
   for (const Extent& e : x)
     for (const Extent& f : c)
@@ -270,18 +307,26 @@ int32_t dz_shared_prefix_attention(const dz_attention* x, void* workspace, int64
   const int64_t dense[4] = {0, 0, 0, 1};
   if (x->positions) {
     const int64_t n[4] = {1, 1, 1, x->groups * x->sequences};
-    DZ_TRY(check_tensor(x->positions, 4, n, dense, 1, 4, "positions", nullptr));
+    Extent at;
+    DZ_TRY(check_tensor(x->positions, 4, n, dense, 1, 4, "positions", &at));
+    if (overlap(out, at)) return invalid("out overlaps positions");
   }
   if (x->prefix_lengths) {
     const int64_t n[4] = {1, 1, 1, x->groups};
-    DZ_TRY(check_tensor(x->prefix_lengths, 4, n, dense, 1, 4, "prefix_lengths", nullptr));
+    Extent at;
+    DZ_TRY(check_tensor(x->prefix_lengths, 4, n, dense, 1, 4, "prefix_lengths", &at));
+    if (overlap(out, at)) return invalid("out overlaps prefix_lengths");
   }
   const int64_t need = dz::attend_workspace(a, plan);
   if (workspace_bytes < need)
     return invalid("workspace of " + std::to_string(workspace_bytes) + " bytes: " + std::to_string(need) + " are needed");
   if (need) {
     const int64_t n[4] = {1, 1, 1, (need + 15) / 16};
-    DZ_TRY(check_tensor(workspace, 16, n, dense, 1, 16, "workspace", nullptr));
+    Extent work;
+    DZ_TRY(check_tensor(workspace, 16, n, dense, 1, 16, "workspace", &work));
+    if (overlap(work, q) || overlap(work, out)) return invalid("workspace overlaps q or out");
+    for (const Extent& e : in)
+      if (overlap(work, e)) return invalid("workspace overlaps keys or values");
   }
   a.q = x->q;
   a.out = x->out;
@@ -319,13 +364,17 @@ int32_t dz_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_
   if (!min_ps && !(min_p >= 0 && min_p <= 1)) return invalid("min_p must be 0 to 1");
   if (!rows) return DZ_OK;
   const int64_t es = size_of(dtype), n[4] = {1, 1, 1, rows}, dense[4] = {0, 0, 0, 1}, strides[4] = {0, 0, 0, logits_stride};
-  DZ_TRY(check_tensor(logits, es, n, strides, vocab, es, "logits", nullptr));
-  DZ_TRY(check_tensor(uniform, 4, n, dense, 1, 4, "uniform", nullptr));
-  if (temperatures) DZ_TRY(check_tensor(temperatures, 4, n, dense, 1, 4, "temperatures", nullptr));
-  if (top_ks) DZ_TRY(check_tensor(top_ks, 4, n, dense, 1, 4, "top_ks", nullptr));
-  if (top_ps) DZ_TRY(check_tensor(top_ps, 4, n, dense, 1, 4, "top_ps", nullptr));
-  if (min_ps) DZ_TRY(check_tensor(min_ps, 4, n, dense, 1, 4, "min_ps", nullptr));
-  DZ_TRY(check_tensor(tokens, 8, n, dense, 1, 8, "tokens", nullptr));
+  const struct {
+    const void* p;
+    const char* what;
+  } of_row[] = {{uniform, "uniform"}, {temperatures, "temperatures"}, {top_ks, "top_ks"}, {top_ps, "top_ps"}, {min_ps, "min_ps"}};
+  Extent in[6] = {}, out;
+  DZ_TRY(check_tensor(logits, es, n, strides, vocab, es, "logits", in + 5));
+  for (int i = 0; i < 5; ++i)
+    if (i == 0 || of_row[i].p) DZ_TRY(check_tensor(of_row[i].p, 4, n, dense, 1, 4, of_row[i].what, in + i));
+  DZ_TRY(check_tensor(tokens, 8, n, dense, 1, 8, "tokens", &out));
+  for (const Extent& e : in)
+    if (overlap(out, e)) return invalid("tokens overlap an input");
   dz::SampleRows a{};
   a.logits = logits;
   a.stride = logits_stride;

@@ -341,7 +341,8 @@ int32_t dz_shared_prefix_attention(const dz_attention* a, void* workspace, int64
  * of the store's slots are left out. A row (one token's head) is kept as code
  * 2^e, with e the least (from -100; 0 for a row of zeros) that leaves nothing above 448
  * and codes rounded to nearest even. Numbers beyond 240 2^8 (fp16) or 240 2^120 (the
- * others) are kept as that. A row with an infinity or NaN becomes NaN. dz_cache_read gives code 2^e in `dtype`, of slots
+ * others) are kept as that. A row with an infinity or NaN becomes NaN. The store's four
+ * parts may lie among each other, but share no byte. dz_cache_read gives code 2^e in `dtype`, of slots
  * position .. position + length - 1. */
 int32_t dz_cache_write(const dz_keys_values* kv, const dz_keys_values* cache, int32_t dtype, int64_t batch, int64_t heads,
                        int64_t length, int64_t width, int64_t slots, const int32_t* positions, int64_t position,
@@ -360,8 +361,8 @@ int32_t dz_cache_read(const dz_keys_values* cache, const dz_keys_values* kv, int
  * takes the largest logit. Temperatures are 0, or from 2^-63 up to 2^64. Each
  * parameter may be given per row (a pointer that is not NULL). Rows with a
  * NaN, or nothing above -inf, or whose parameters are NaN or out of range, give -1;
- * logits of +inf share the whole. Replaces the sampling of
- * model.generate in trainer.py:1544-1568. */
+ * logits of +inf share the whole. `tokens` may not overlap an input. Replaces the
+ * sampling of model.generate in trainer.py:1544-1568. */
 int32_t dz_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t logits_stride,
                          const float* uniform, double temperature, int32_t top_k, double top_p, double min_p,
                          const float* temperatures, const int32_t* top_ks, const float* top_ps, const float* min_ps,
