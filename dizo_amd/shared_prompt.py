@@ -151,6 +151,15 @@ def _check_model(model, tokens: int) -> None:
         window = getattr(config, name, None)
         if window and window < tokens:  # (0: none)
             raise DzError(f"shared_prompt: attention with a window of {window} of {tokens} tokens ({name})")
+    # (rotations that change with the longest sequence of a forward, past a length)
+    for name in ("rope_parameters", "rope_scaling"):
+        rope = getattr(config, name, None)
+        for r in (rope, *rope.values()) if isinstance(rope, dict) else ():  # (some have one for each type of layer)
+            if isinstance(r, dict) and r.get("rope_type", r.get("type")) in ("dynamic", "longrope"):
+                most = [n for n in (r.get("original_max_position_embeddings"), getattr(config, "original_max_position_embeddings", None),
+                                    getattr(config, "max_position_embeddings", None)) if n]
+                if not most or tokens > min(most):
+                    raise DzError(f"shared_prompt: rotations that go by a sequence's length ({r.get('rope_type', r.get('type'))}), past that of {most}")
 
 
 def _hidden(model, input_ids: torch.Tensor, position_ids: torch.Tensor, layout) -> torch.Tensor:

@@ -113,3 +113,26 @@ def test_a_window_of_the_masks_alone_is_refused(plain):  # noqa: F811
         S.generate(model_of("phimoe", sliding_window=4), ids, 6)
     model = model_of("phimoe", sliding_window=15)
     assert torch.equal(S.generate(model, ids, 6, temperature=0.0)[0, 0], greedy(model, ids[0], 6))
+
+
+@pytest.mark.parametrize("kind, rope, how", [
+    ("llama", dict(rope_type="dynamic", factor=4.0), {}),
+    ("llama", dict(rope_type="longrope", factor=4.0, short_factor=[1.0] * 8, long_factor=[4.0] * 8, original_max_position_embeddings=16), dict(max_position_embeddings=64)),
+    ("phi3", dict(rope_type="longrope", short_factor=[1.0] * 8, long_factor=[4.0] * 8, original_max_position_embeddings=16),
+     dict(max_position_embeddings=64, original_max_position_embeddings=16)),
+], ids=["dynamic", "longrope", "phi3"])
+def test_rotations_that_change_with_the_length_are_refused_past_it(kind, rope, how, plain):  # noqa: F811
+    """Past 16 tokens a whole forward's rotations are others than those of a forward of the prompt, or of fewer tokens."""
+    make = lambda: model_of(kind, **{"max_position_embeddings": 16, **how}, rope_parameters=dict(rope, rope_theta=100.0))  # noqa: E731
+    assert same(make(), batch(7, 1, 2, [2], 16))
+    with pytest.raises(DzError, match="rotations"):
+        losses(make(), batch(7, 1, 2, [2], 17))
+    ids = torch.randint(2, 211, (1, 12), generator=torch.Generator().manual_seed(1))
+    assert torch.equal(S.generate(make(), ids, 4, temperature=0.0)[0, 0], greedy(make(), ids[0], 4))
+    with pytest.raises(DzError, match="rotations"):
+        S.generate(make(), ids, 5, temperature=0.0)
+
+
+def test_rotations_of_other_scalings(plain):  # noqa: F811
+    model = model_of("llama", rope_parameters=dict(rope_type="yarn", factor=4.0, rope_theta=100.0, original_max_position_embeddings=10), max_position_embeddings=40)
+    assert same(model, batch(*BATCHES[2]))
