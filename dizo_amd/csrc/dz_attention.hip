@@ -11,10 +11,11 @@
 //
 // What bounds it, and what it measured (one MI355X; the floor: bytes at a large copy's 4.96 TB/s, or products at a large
 // library product's 1,358 TFLOP/s in bf16):
-//   single tokens   their keys from memory: 64 answers after 2,048 keys, 295 MB, 53 us (5.5 TB/s) and 6 to join; floor 60
-//   the same, 8 bit conversions next to the loads: 28 us and 6 to join; floor 15
+//   single tokens   their keys from memory: 64 answers of up to 256 tokens after 2,048 keys, 40 heads of 128, 295 MB, 53 us (5.5 TB/s) and 6
+//                   to join; floor 60
+//   the same, 8 bit conversions next to the loads: 2 x 32 answers after 6,000, 8 key heads of 32, 28 us and 6 to join; floor 15
 //   candidates      the way through one workgroup (lengths, then keys, scores, values, the waves' sums): 14 us; floor 8
-//   prompts         one causal sequence of 4,096, 40 heads of 128: 222 us, 770 TFLOP/s; the products alone reach 1,030 under the power limit
+//   prompts         one causal sequence of 4,096, 40 heads of 128: 220 us, 780 TFLOP/s; the products alone reach 1,030 under the power limit
 //                   in this order (scores, weights, values by one wave)
 // A lane holds one query: scores are taken as K Q^T and results as V^T P^T, so that maxima, sums and weights stay in the
 // lane (two lanes a query) and weights are the second product's operand as they are. Values are read from LDS transposed.
@@ -724,7 +725,7 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
   //   shared 164; 32 x 40 rows after 122, bf16: 29 and 29, after 600: 71 and 56; fp32 after 600: 309 and 412);
   //   more: the second (one sequence of 128 rows after 5,066: 37 and 35; fp32 211 and 169).
   // Codes are converted by each wave for itself in the first, without a stop in registers before: of wide heads it is the faster one
-  // throughout (a causal 2,048 of 40 heads of 128: 104 us, shared 164; heads of 80, 16 x 256: 33 and 31).
+  // throughout (a causal 2,048 of 40 heads of 128: 95 us in bf16 and 109 in fp16, shared 164; heads of 80, 16 x 256: 33 and 31).
   const int64_t keys_of_one = a.prefix_slots + a.slots, own_tiles = heads * a.sequences * ((seq_rows + 31) / 32);
   const int64_t few_keys = seq_rows <= 32 || dtype == 0 || a.bytes ? 1000 : 256;
   p.by_keys = seq_rows <= 16 || (a.bytes && a.width >= 96 && a.width % 16 == 0) || (seq_rows <= 96 && (own_tiles <= 512 || keys_of_one < few_keys));
@@ -745,10 +746,11 @@ AttendPlan attend_plan(int dtype, const Attend& a) {
   p.items = (int32_t)items;
   p.per = (p.items + 7) / 8;
   // An XCD's 32 compute units run `slots` workgroups at a time. Items beyond a multiple of that would leave most of them idle for as long as
-  // one takes: as many parts of them as fill the slots once (64 single tokens after 2,048 keys: 31 us, whole items 49; 128 tokens after
-  // 8,192: 46 and 162). A part has 256 keys or more (one token after 500: 12.6 us in two parts, 11.6 whole). Shared
-  // tiles of 16-bit operands keep a compute unit's matrix units busy by one workgroup, and a part's sums are 128 rows that are written
-  // and read again: one a compute unit (a causal 1,000: 31 us, two 40; 8 x 60 tokens after 1,000: 30 and 35). fp32 and codes
+  // one takes: as many parts of them as fill the slots once (40 heads of 128, fp16, keys that the caches hold: 64 single tokens after
+  // 2,048 keys 26 us, whole items 38; 128 tokens after 8,192: 47 and 164). A part has 256 keys or more (one token after 500: 12.6 us in two
+  // parts, 11.6 whole). Shared tiles of 16-bit operands keep a compute unit's matrix units busy by one workgroup, and a part's sums are 128
+  // rows that are written and read again: one a compute unit (128 tokens after 8,192: 47 us, two 50; a causal 1,000 of 40 heads of 128: 39
+  // and 40; 8 x 60 tokens after 1,000: 30 and 35). fp32 and codes
   // that are converted on the way take two (16 x 60 tokens after 3,000, fp32: 106 us, one 131; 32 x 61 after 2,048 from
   // codes 225 and 243).
   const int64_t seqs = p.tile_rows > seq_rows ? p.tile_rows / seq_rows : 1, keys = a.prefix_slots + seqs * a.slots;

@@ -140,8 +140,10 @@ def shared_prefix_attention(q: torch.Tensor, own: Union[KV, QuantizedKV, None], 
 
     Stores are KV, of q's dtype, or both QuantizedKV. heads is a multiple of kv_heads, the width a multiple of 8 up to
     128; scale (default: width ** -0.5) is positive. Products and sums are fp32, and weights are rounded to q's dtype,
-    or less, before they multiply values (for bf16 by 2^-8 of each at most, for fp16 by 2^-11 of each and 2^-36 of the largest). The result is laid out like q unless `out` is given. Tensors whose rows do not
-    start at multiples of 16 bytes (codes: 8) are copied first, `out` has to fit."""
+    or less, before they multiply values (for bf16 by 2^-8 of each at most, for fp16 by 2^-11 of each and 2^-36 of the
+    largest). The result is laid out like q unless `out` is given. The same call gives the same bits; one of other sizes,
+    which is cut for the card in another way, may differ in the last ones. Tensors whose rows do not start at multiples of 16
+    bytes (codes: 8) are copied first, `out` has to fit."""
     what = "shared_prefix_attention"
     if not q.is_cuda:
         _fail(what, f"q must live on a GPU, got {q.device}")

@@ -309,11 +309,12 @@ typedef struct dz_keys_values {
  * and NaN too, does not matter to it. Products and sums are fp32; weights are
  * rounded to `dtype`, or less, before they multiply values, as their sum is taken
  * before: for bf16 by 2^-8 of each at most, for fp16 by 2^-11 of each and 2^-36 of the
- * query's largest. Both stores are of
- * `dtype`, or both 8-bit, whose values are taken in `dtype`. `out` may not
- * overlap an input. Rows whose sums are not finite are taken again by themselves,
- * key by key: right, and slow where there are many. Replaces, for
- * candidates that share a prompt, the attention of the forwards in
+ * query's largest. Both stores are of `dtype`, or both 8-bit, whose keys and values are
+ * taken in `dtype` (values also as they are). `out` may not overlap an input. Rows whose
+ * sums are not finite are taken again by themselves, key by key: right, and slow where
+ * there are many. The same call gives the same bits; one of other sizes, which is cut
+ * for the card in another way, may differ in the last ones. Replaces, for candidates
+ * that share a prompt, the attention of the forwards in
  * trainer.py:1524-1542, which repeats it for each. */
 typedef struct dz_attention {
   const void* q;
@@ -342,8 +343,8 @@ int32_t dz_shared_prefix_attention(const dz_attention* a, void* workspace, int64
  * 2^e, with e the least (from -100; 0 for a row of zeros) that leaves nothing above 448
  * and codes rounded to nearest even. Numbers beyond 240 2^8 (fp16) or 240 2^120 (the
  * others) are kept as that. A row with an infinity or NaN becomes NaN. The store's four
- * parts may lie among each other, but share no byte. dz_cache_read gives code 2^e in `dtype`, of slots
- * position .. position + length - 1. */
+ * parts may lie among each other, but share no byte. dz_cache_read gives code 2^e in
+ * `dtype`, of slots position .. position + length - 1. */
 int32_t dz_cache_write(const dz_keys_values* kv, const dz_keys_values* cache, int32_t dtype, int64_t batch, int64_t heads,
                        int64_t length, int64_t width, int64_t slots, const int32_t* positions, int64_t position,
                        void* stream);
