@@ -123,14 +123,15 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, dro
 
 # Types of models (config.model_type) that are no more than layers of the attention above, one for each of config.num_hidden_layers, and
 # an output embedding: nothing else mixes tokens, and nothing lies between the last hidden states and the head, or behind it.
-MODELS = frozenset("""apertus arcee bitnet cwm ernie4_5 ernie4_5_moe exaone4 gemma gemma2 gemma3_text glm glm4 glm4_moe gpt2 gpt_bigcode gpt_neox
-    granite granitemoe granitemoeshared helium hyperclovax llama minimax_m2 ministral mistral mixtral olmo olmo2 olmo3 olmoe opt persimmon phi phi3
-    phimoe qwen2 qwen2_moe qwen3 qwen3_moe seed_oss smollm3 starcoder2""".split())
+MODELS = frozenset("""afmoe apertus arcee aria_text bitnet ctrl cwm ernie4_5 ernie4_5_moe exaone4 exaone_moe flex_olmo gemma gemma2
+    gemma3_text glm glm4 glm4_moe gpt2 gpt_bigcode gpt_neox granite granitemoe granitemoeshared helium hunyuan_v1_dense hunyuan_v1_moe hy_v3
+    hyperclovax jais2 jetmoe laguna llama mellum minimax_m2 ministral ministral3 mistral mixtral olmo olmo2 olmo3 olmoe opt persimmon phi
+    phi3 phimoe qwen2 qwen2_moe qwen3 qwen3_moe seed_oss smollm3 solar_open starcoder2""".split())
 
 
-# Of these, the ones that learn a vector for each position and count the padding on a sequence's left, too, where they are given no
-# positions. (The others take positions from the mask, or nothing but the distance between two tokens matters to them.)
-COUNT_PADS = frozenset(("gpt2", "gpt_bigcode"))
+# Of these, the ones to which more than the distance between two tokens matters (a vector for each position, or a norm of rotated keys
+# by channel) and that count the padding on a sequence's left, too, where they are given no positions. (OPT takes positions from the mask.)
+COUNT_PADS = frozenset(("ctrl", "gpt2", "gpt_bigcode", "hunyuan_v1_dense", "hunyuan_v1_moe"))
 
 
 def _check_model(model, tokens: int) -> None:

@@ -21,6 +21,11 @@ OF_TYPE = {
     "qwen3_moe": dict(num_experts=4, num_experts_per_tok=2, moe_intermediate_size=32),
     "ernie4_5_moe": dict(moe_num_experts=4, moe_k=2, moe_intermediate_size=32, moe_layer_start_index=0),
     "glm4_moe": dict(n_routed_experts=4, num_experts_per_tok=2, moe_intermediate_size=32, n_group=1, topk_group=1, first_k_dense_replace=1),
+    "jetmoe": dict(num_local_experts=4, num_experts_per_tok=2, kv_channels=16), "flex_olmo": dict(num_experts=4, num_experts_per_tok=2),
+    "hunyuan_v1_moe": dict(num_experts=4, moe_topk=2), "aria_text": dict(moe_num_experts=4, moe_topk=2),
+    "solar_open": dict(n_routed_experts=4, num_experts_per_tok=2, moe_intermediate_size=32, n_group=1, topk_group=1),
+    "exaone_moe": dict(num_experts=4, num_experts_per_tok=2, moe_intermediate_size=32, n_group=1, topk_group=1),
+    **{kind: dict(num_experts=4, num_experts_per_tok=2, moe_intermediate_size=32) for kind in ("afmoe", "hy_v3", "laguna", "mellum")},
     "gemma2": dict(final_logit_softcapping=None, attn_logit_softcapping=None),
 }
 
