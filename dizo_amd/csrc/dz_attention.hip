@@ -600,11 +600,12 @@ __global__ __launch_bounds__(THREADS, (THREADS * RESIDENT + 255) / 256) void att
         for (int r = 0; r < 4; ++r) o[d][4 * b + r] += x[r];
       }
   }
-  bool finite = true;
+  float zero = 0.f;  // NaN where a sum is not finite (columns past the width are, or are the row's first ones again)
 #pragma unroll
   for (int d = 0; d < S::PV; ++d)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) finite &= fabsf(o[d][j]) < INFINITY;  // (columns past the width are finite, or the row's first ones again)
+    for (int j = 0; j < 16; ++j) zero = __builtin_fmaf(o[d][j], 0.f, zero);
+  const bool finite = zero == 0.f;
   const uint64_t lone_lanes = __ballot(live && !finite);
   const uint32_t lone = (uint32_t)lone_lanes | (uint32_t)(lone_lanes >> 32);
   if (lone) lone_rows<T, BY_KEYS, BYTES, KT, S::WAVES>(BY_KEYS ? 0 : wave * 32, lone);
