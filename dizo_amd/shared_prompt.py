@@ -134,8 +134,9 @@ MODELS = frozenset("""afmoe apertus arcee aria_text bitnet ctrl cwm ernie4_5 ern
 COUNT_PADS = frozenset(("ctrl", "gpt2", "gpt_bigcode", "hunyuan_v1_dense", "hunyuan_v1_moe"))
 
 
-def _check_model(model, tokens: int) -> None:
-    """Whether the model's answers to sequences of up to `tokens` are what its layers and output embedding give here."""
+def _check_model(model, tokens: int, seen: int) -> None:
+    """Whether the model's answers to sequences of up to `tokens`, of which one of those that are read sees `seen`, are what its layers
+    and output embedding give here."""
     config = model.config
     if not getattr(model, "_supports_attention_backend", False):
         raise DzError(f"shared_prompt: {type(model).__name__} does not call an attention that HF registers by name")
@@ -150,8 +151,8 @@ def _check_model(model, tokens: int) -> None:
     # (some models have a window in their masks only, which the attention is not told of)
     for name in ("sliding_window", "attention_chunk_size"):
         window = getattr(config, name, None)
-        if window and window < tokens:  # (0: none)
-            raise DzError(f"shared_prompt: attention with a window of {window} of {tokens} tokens ({name})")
+        if window and window < seen:  # (0: none)
+            raise DzError(f"shared_prompt: attention with a window of {window} of {seen} tokens ({name})")
     # (rotations that change with the longest sequence of a forward, past a length)
     for name in ("rope_parameters", "rope_scaling"):
         rope = getattr(config, name, None)
@@ -240,7 +241,7 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     sequences, length = input_ids.shape
     if candidates < 1 or sequences % candidates or len(option_len) != sequences or not 1 <= min(option_len) <= max(option_len) < length:
         raise DzError(f"shared_prompt_logprobs: {sequences} sequences of {length} tokens, {candidates} candidates each, option_len {list(option_len)[:8]}")
-    _check_model(model, length)
+    _check_model(model, length, length - 1)  # (the last token predicts nothing)
     device, examples, most = input_ids.device, sequences // candidates, max(option_len)
     each = most - 1
     p = _Prompts(model, input_ids, attention_mask, option_len, candidates)
@@ -291,7 +292,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, answers: in
         raise DzError(f"generate: prompt_lengths must be torch.int32 ({prompts},), got {prompt_lengths.dtype} {tuple(prompt_lengths.shape)}")
     if uniform is not None and uniform.shape != (prompts, answers, max_new_tokens):
         raise DzError(f"generate: uniform must be {(prompts, answers, max_new_tokens)}, got {tuple(uniform.shape)}")
-    _check_model(model, room + max_new_tokens)
+    _check_model(model, room + max_new_tokens, room + max_new_tokens)
     most = getattr(model.config, "max_position_embeddings", None)
     if most is not None and room + max_new_tokens - 1 > most:  # (an answer's last token is not read again)
         raise DzError(f"generate: {room} tokens of a prompt and {max_new_tokens} new ones, the model has {most} positions")

@@ -141,3 +141,10 @@ def test_rotations_that_change_with_the_length_are_refused_past_it(kind, rope, h
 def test_rotations_of_other_scalings(plain):  # noqa: F811
     model = model_of("llama", rope_parameters=dict(rope_type="yarn", factor=4.0, rope_theta=100.0, original_max_position_embeddings=10), max_position_embeddings=40)
     assert same(model, batch(*BATCHES[2]))
+
+
+@pytest.mark.parametrize("kind", ["mistral", "phimoe"])
+def test_a_window_of_all_tokens_that_are_read_is_none(kind, plain):  # noqa: F811
+    assert same(model_of(kind, sliding_window=15), batch(7, 1, 2, [2], 16))  # the last token's logits are not
+    with pytest.raises(DzError, match="window"):
+        losses(model_of(kind, sliding_window=14), batch(7, 1, 2, [2], 16))
