@@ -241,6 +241,8 @@ def shared_prompt_logprobs(model, input_ids: torch.Tensor, attention_mask: Optio
     sequences, length = input_ids.shape
     if candidates < 1 or sequences % candidates or len(option_len) != sequences or not 1 <= min(option_len) <= max(option_len) < length:
         raise DzError(f"shared_prompt_logprobs: {sequences} sequences of {length} tokens, {candidates} candidates each, option_len {list(option_len)[:8]}")
+    if attention_mask is not None and attention_mask.shape != input_ids.shape:
+        raise DzError(f"shared_prompt_logprobs: attention_mask must be {tuple(input_ids.shape)}, got {tuple(attention_mask.shape)}")
     _check_model(model, length, length - 1)  # (the last token predicts nothing)
     device, examples, most = input_ids.device, sequences // candidates, max(option_len)
     each = most - 1

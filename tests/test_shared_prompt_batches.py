@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from dizo_amd import shared_prompt as S
+from dizo_amd._lib import DzError
 from dizo_amd.trainer import ZOArguments, ZOTrainer, forward_wrap_with_option_len
 from test_shared_prompt import PAD, batch, plain, tiny  # noqa: F401
 from test_shared_prompt_models import model_of
@@ -95,3 +96,10 @@ def test_the_trainers_option_takes_any_batch(plain):  # noqa: F811
         seen[shared] = float(trainer.zo_forward(model, b))
         trainer.zo_close()
     assert seen[False] == seen[True]
+
+
+@pytest.mark.parametrize("shape", [(4, 1, 16, 16), (4, 15), (16,)])
+def test_a_mask_of_another_shape_is_refused(shape):
+    b = batch(4, 2, 2, [2, 3], 16)
+    with pytest.raises(DzError, match="attention_mask"), torch.no_grad():
+        S.shared_prompt_logprobs(tiny("opt"), b["input_ids"], torch.ones(shape), b["option_len"].tolist(), 2, PAD)
